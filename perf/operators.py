@@ -199,7 +199,7 @@ def prepare(case, seed):
     if own:
         from deepptmpred_amd import layers
         s["plan"] = layers.AttentionPlan(rows, keys, heads=h, kv_heads=hk, head_dim=d, window=(case["left"], case["right"]),
-                                         sinks=case["sinks"], q_positions=pos if case["few"] > 1 else None)
+                                         sinks=case["sinks"], q_positions=pos if case["few"] > 1 else None, training=case["kind"] == "train")
     return s
 
 
