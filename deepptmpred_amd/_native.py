@@ -37,6 +37,8 @@ EXPORTS = (
     "dptm_trainer_profile_begin", "dptm_trainer_profile_end", "dptm_trainer_loss_buffer", "dptm_trainer_proba_buffer", "dptm_trainer_stream",
     "dptm_trainer_stage_loss", "dptm_trainer_lanes",
     "dptm_trainer_last_error", "dptm_trainer_set_allreduce", "dptm_sasa", "dptm_sasa_last_error",
+    "dptm_attention_plan", "dptm_attention_workspace", "dptm_attention_forward", "dptm_attention_backward",
+    "dptm_qk_norm_rope_forward", "dptm_qk_norm_rope_workspace", "dptm_qk_norm_rope_backward", "dptm_layer_last_error",
 )
 
 # int (*dptm_allreduce_fn)(void* user, float* buf, int64_t count, void* stream)
@@ -83,6 +85,25 @@ class TrainOpts(C.Structure):
         ("rate_tb", C.c_float), ("rate_dense", C.c_float), ("n_global", C.c_int64),
         ("n_pos_global", C.c_int64), ("l2", C.c_float), ("l2_scale", C.c_float),
     ]
+
+
+class Rows(C.Structure):
+    """dptm_rows: a device tensor [rows][heads][head_dim], strides in elements."""
+    _fields_ = [("data", C.c_void_p), ("rows", C.c_int64), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = [("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("window_left", C.c_int32),
+                ("window_right", C.c_int32), ("sinks", C.c_int32), ("training", C.c_int32)]
+
+
+class AttentionBias(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("buckets", C.c_void_p), ("n_buckets", C.c_int32), ("max_distance", C.c_int32)]
+
+
+class NormRopeDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("head_dim", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("rows", C.c_int64), ("n_positions", C.c_int32), ("interleaved", C.c_int32), ("eps", C.c_float)]
 
 
 _lib: Optional[C.CDLL] = None
@@ -207,6 +228,24 @@ def load_library() -> C.CDLL:
     lib.dptm_sasa.argtypes = [vp, vp, i64, C.c_double, vp, C.c_int32, C.c_int32, vp]
     lib.dptm_sasa_last_error.restype = C.c_char_p
     lib.dptm_sasa_last_error.argtypes = []
+    i32, sz, f32, rp, bp = C.c_int32, C.c_size_t, C.c_float, C.POINTER(Rows), C.POINTER(AttentionBias)
+    lib.dptm_attention_plan.restype = C.c_int64
+    lib.dptm_attention_plan.argtypes = [C.POINTER(AttentionDesc), vp, vp, vp, i64, vp, i64]
+    lib.dptm_attention_workspace.restype = C.c_int64
+    lib.dptm_attention_workspace.argtypes = [vp, i32, i32]
+    lib.dptm_attention_forward.restype = C.c_int
+    lib.dptm_attention_forward.argtypes = [vp, vp, i32, rp, rp, rp, rp, vp, f32, bp, vp, sz, i32, vp]
+    lib.dptm_attention_backward.restype = C.c_int
+    lib.dptm_attention_backward.argtypes = [vp, vp, i32, rp, rp, rp, rp, rp, vp, f32, bp, rp, rp, rp, vp, vp, sz, i32, vp]
+    nd = C.POINTER(NormRopeDesc)
+    lib.dptm_qk_norm_rope_forward.restype = C.c_int
+    lib.dptm_qk_norm_rope_forward.argtypes = [nd, rp, rp, vp, vp, vp, vp, vp, rp, rp, i32, vp]
+    lib.dptm_qk_norm_rope_workspace.restype = C.c_int64
+    lib.dptm_qk_norm_rope_workspace.argtypes = [nd]
+    lib.dptm_qk_norm_rope_backward.restype = C.c_int
+    lib.dptm_qk_norm_rope_backward.argtypes = [nd, rp, rp, rp, rp, vp, vp, vp, vp, vp, rp, rp, vp, vp, vp, sz, i32, vp]
+    lib.dptm_layer_last_error.restype = C.c_char_p
+    lib.dptm_layer_last_error.argtypes = []
     _lib = lib
     return lib
 

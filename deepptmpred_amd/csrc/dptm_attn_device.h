@@ -1,0 +1,251 @@
+// Device helpers of the attention kernels: operand fragments of the 32x32 matrix instructions for the three element
+// types, tiles in LDS, visibility of a pair, and the product that keeps non-finite operands out of hidden pairs.
+//
+// Layout.  v_mfma_f32_32x32x16 leaves D[row][col] with col = lane % 32 and row = 8 (r / 4) + 4 (lane / 32) + r % 4 for
+// register r.  Taken as S^T = K Q^T a lane holds one query's scores of 16 keys, so row sums and maxima are in-lane but for
+// one exchange between the half-waves, and registers 8s..8s+7 ARE the B operand of the next product (contraction over
+// the keys 16 s + {4h..4h+3, 8+4h..8+4h+3}), whose order within a step is free as long as the A operand uses it too.
+// Products chain register to register; the A operand of the second product is read from LDS transposed.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "dptm_layers.h"
+
+namespace dptm {
+
+typedef float f32x16_a __attribute__((ext_vector_type(16)));
+typedef short s16x4_a __attribute__((ext_vector_type(4)));
+typedef short s16x8_a __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4_a __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kMinusInf = -__builtin_inff();
+
+template <typename T> struct Elem;
+template <> struct Elem<__bf16> {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 v4 __attribute__((ext_vector_type(4)));
+    static constexpr unsigned kExp = 0x7f80;
+};
+template <> struct Elem<_Float16> {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 v4 __attribute__((ext_vector_type(4)));
+    static constexpr unsigned kExp = 0x7c00;
+};
+template <> struct Elem<float> {
+    typedef float v8 __attribute__((ext_vector_type(8)));
+    typedef float v4 __attribute__((ext_vector_type(4)));
+};
+template <typename T> using V8 = typename Elem<T>::v8;
+template <typename T> using V4 = typename Elem<T>::v4;
+
+// one step of 16 along the contraction; lane: index lane % 32, contraction elements 8 (lane / 32) .. +7.  In fp32 the step is
+// eight 32x32x2 instructions, element e of both operands in the e-th.
+__device__ __forceinline__ void mma(f32x16_a& c, const V8<__bf16>& a, const V8<__bf16>& b) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16_a& c, const V8<_Float16>& a, const V8<_Float16>& b) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16_a& c, const V8<float>& a, const V8<float>& b) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ V8<T> pack8(const f32x16_a& x, int s) {   // registers 8s..8s+7
+    V8<T> r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = (T)x[8 * s + e];
+    return r;
+}
+
+// ---- a tile of rows in LDS: 16-byte chunks, chunk index XORed with a function of the row so that both the row reads
+// ---- (32 rows, one chunk) and the transposed reads (8 rows, four chunks) spread over the banks
+template <typename T, int D>
+struct Tile {
+    static constexpr int kChunks = D * (int)sizeof(T) / 16;   // of a row
+    __device__ static __forceinline__ int swz(int row) {
+        if constexpr (kChunks >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+        else if constexpr (kChunks == 8) return ((row >> 1 & 1) << 2) | (row >> 2 & 3);
+        else if constexpr (kChunks == 4) return row >> 2 & 3;
+        else return row >> 3 & 1;
+    }
+    // A or B operand with the row on the lane: contraction elements 16 step + 8h ..
+    __device__ static __forceinline__ V8<T> row_frag(const char* t, int row, int step, int h) {
+        const char* p = t + row * (kChunks * 16);
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const V8<T>*>(p + (((2 * step + h) ^ swz(row)) << 4));
+        } else {
+            const V4<T> lo = *reinterpret_cast<const V4<T>*>(p + (((4 * step + 2 * h) ^ swz(row)) << 4));
+            const V4<T> hi = *reinterpret_cast<const V4<T>*>(p + (((4 * step + 2 * h + 1) ^ swz(row)) << 4));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    // A operand with the column 32 dt + lane % 32 on the lane: contraction rows row0 + {4h..4h+3, 8+4h..8+4h+3}.
+    // 16-bit types: each group of 16 lanes hands in 4 rows x 16 columns and takes a column of 4 (ds_read_b64_tr_b16).
+    // Head dimension 16 has half a tile of columns: the other lanes repeat them, and their results are not used.
+    __device__ static __forceinline__ V8<T> col_frag(const char* t, int row0, int dt, int lane) {
+        const int h = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            const int q = lane & 15;
+            const int col = 32 * dt + (D >= 32 ? (lane & 16) : 0) + 4 * (q & 3);
+            s16x4_a r[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int row = row0 + 8 * i + 4 * h + (q >> 2);
+                const char* p = t + row * (kChunks * 16) + (((col >> 3) ^ swz(row)) << 4) + (col & 7) * 2;
+                r[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_a*)(p));
+            }
+            return __builtin_bit_cast(V8<T>, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const int col = (32 * dt + (lane & 31)) & (D - 1);
+            V8<T> f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int row = row0 + 8 * (e >> 2) + 4 * h + (e & 3);
+                f[e] = *reinterpret_cast<const float*>(t + row * (kChunks * 16) + (((col >> 2) ^ swz(row)) << 4) + (col & 3) * 4);
+            }
+            return f;
+        }
+    }
+};
+
+// ROWS rows of a strided tensor on the way to LDS through registers; rows from `valid` on become zeros
+template <typename T, int D, int ROWS, int NT>
+struct Stage {
+    static constexpr int kChunks = Tile<T, D>::kChunks;
+    static constexpr int kAll = ROWS * kChunks, kMine = (kAll + NT - 1) / NT;
+    u32x4_a r[kMine];
+    __device__ __forceinline__ void load(const char* base, int64_t row_bytes, int valid, int tid) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int c = tid + i * NT, row = c / kChunks;
+            r[i] = u32x4_a{0, 0, 0, 0};
+            if (row < valid && (kAll % NT == 0 || c < kAll))
+                r[i] = *reinterpret_cast<const u32x4_a*>(base + row * row_bytes + (c % kChunks) * 16);
+        }
+    }
+    __device__ __forceinline__ void store(char* t, int tid) const {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int c = tid + i * NT, row = c / kChunks;
+            if (kAll % NT == 0 || c < kAll)
+                *reinterpret_cast<u32x4_a*>(t + row * (kChunks * 16) + (((c % kChunks) ^ Tile<T, D>::swz(row)) << 4)) = r[i];
+        }
+    }
+};
+
+// operand straight from memory: row on the lane
+template <typename T>
+__device__ __forceinline__ V8<T> global_frag(const char* row, int step, int h) {
+    if constexpr (sizeof(T) == 2) {
+        return *reinterpret_cast<const V8<T>*>(row + (2 * step + h) * 16);
+    } else {
+        const V4<T> lo = *reinterpret_cast<const V4<T>*>(row + (4 * step + 2 * h) * 16);
+        const V4<T> hi = *reinterpret_cast<const V4<T>*>(row + (4 * step + 2 * h + 1) * 16);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
+__device__ __forceinline__ float half_other(float v) { return __shfl_xor(v, 32); }
+__device__ __forceinline__ float half_max(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+    for (int m = 16; m; m >>= 1) v = min(v, __shfl_xor(v, m));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+    for (int m = 16; m; m >>= 1) v = max(v, __shfl_xor(v, m));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// key index of register r of a 32-key score tile, without the 4h
+__device__ __forceinline__ constexpr int reg_row(int r) { return 8 * (r >> 2) + (r & 3); }
+
+// pair of a query and a key `far` = key - position behind it: within the window, or one of the first keys.  Without short
+// circuits, so that a mask is compares and selects: as branches it is slow, and hipcc 7.2 has dropped the select of a
+// score register whose condition it had turned into control flow.
+struct Window { int left, right, sinks; };
+__device__ __forceinline__ bool visible(const Window& w, int far, int key) {
+    return (far <= w.right) & ((far >= -w.left) | (key < w.sinks));
+}
+// all pairs of positions [pmin, pmax] and keys [j0, j1): every one visible / none visible
+__device__ __forceinline__ bool all_visible(const Window& w, int pmin, int pmax, int j0, int j1) {
+    return j1 - 1 - pmin <= w.right && (j0 - pmax >= -w.left || j1 <= w.sinks);
+}
+__device__ __forceinline__ bool none_visible(const Window& w, int pmin, int pmax, int j0, int j1) {
+    return j0 - pmax > w.right || (j1 - 1 - pmin < -w.left && j0 >= w.sinks);
+}
+
+// ---- products over tiles that hold hidden pairs: the hidden pair's weight is 0, but 0 * inf and 0 * NaN are NaN, so
+// ---- non-finite elements of the A operand are taken out of the product and given back to the lanes with a weight alone
+template <typename T>
+__device__ __forceinline__ bool not_finite(T x) {
+    if constexpr (sizeof(T) == 2) return (__builtin_bit_cast(unsigned short, x) & Elem<T>::kExp) == Elem<T>::kExp;
+    else return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
+}
+template <typename T>
+__device__ __forceinline__ void mma_guarded(f32x16_a& c, V8<T> a, const V8<T>& b) {
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bad |= not_finite(a[e]);
+    if (__ballot(bad) == 0) {
+        mma(c, a, b);
+        return;
+    }
+    V8<T> fine, sign, any, has;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float x = (float)a[e];
+        const bool nf = not_finite(a[e]);
+        fine[e] = nf ? (T)0.f : a[e];
+        sign[e] = (T)(nf ? (x > 0.f ? 1.f : x < 0.f ? -1.f : 0.f) : 0.f);
+        any[e] = (T)(nf ? 1.f : 0.f);
+        has[e] = (T)((float)b[e] != 0.f ? 1.f : 0.f);
+    }
+    mma(c, fine, b);
+    f32x16_a n, m;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) n[r] = m[r] = 0.f;
+    mma(n, sign, has);
+    mma(m, any, has);
+    // only infinities of one sign: that infinity (weights of the forward pass are positive); anything else: NaN
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        if (m[r] > 0.f) c[r] += n[r] == m[r] ? __builtin_inff() : n[r] == -m[r] ? -__builtin_inff() : __builtin_nanf("");
+}
+
+// ---- relative position bias in LDS: value per distance in units of log2, one head.  Entries at or below -2^100 hide their
+// ---- pairs, so that a table of the type's lowest value works as a mask does
+template <typename T>
+__device__ __forceinline__ void load_bias(float* lds, const BiasArgs& b, int heads, int head, int tid, int nt) {
+    const T* table = static_cast<const T*>(b.table);
+    for (int i = tid; i < 2 * b.reach + 1; i += nt) {
+        const int k = min(max(b.buckets[i], 0), b.n_buckets - 1);
+        const float v = (float)table[(int64_t)k * heads + head];
+        lds[i] = v <= -0x1p100f ? kMinusInf : v * kLog2e;
+    }
+}
+
+// blocks of one key head's tiles on one XCD, which has an L2 of its own: block b runs on XCD b % 8, and each XCD takes a
+// contiguous piece of the (head-major) order
+__device__ __forceinline__ int xcd_order(int b, int n) {
+    const int per = n >> 3, rest = n & 7, x = b & 7, i = b >> 3;
+    return x * per + min(x, rest) + i;
+}
+
+__device__ __forceinline__ int row_position(const int* plan, int has_pos, int pos_at, int pos0, int q0, int i) {
+    return has_pos ? plan[pos_at + q0 + i] : pos0 + i;
+}
+
+}  // namespace dptm

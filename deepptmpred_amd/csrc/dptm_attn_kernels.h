@@ -1,0 +1,397 @@
+// Attention over packed sequences: forward kernels (dptm_attn_device.h explains the layout the products use).
+//
+//   visible(i, j): 0 <= j < keys of i's sequence, j - p_i <= right, and (j - p_i >= -left or j < sinks)
+//   s_ij = scale q_i . k_j + bias(j - p_i);  lse_i = log sum_j exp s_ij;  out_i = sum_j exp(s_ij - lse_i) v_j
+//
+// One pass over the keys with a running maximum m and sum l per query, in units of log2 and in 32 bits.  The weights are
+// rounded to the tensors' type for the second product (fp32: not at all), l sums them unrounded.
+#pragma once
+#include "dptm_attn_device.h"
+
+namespace dptm {
+namespace {
+
+// float16 weights are kept 2^10 times larger than exp2(s - m): a weight of 2^-24 of the largest is then still a normal number.
+// The maximum that the weights refer to is only moved when a score passes it by more than 2^kLazy, so the largest
+// weight is 2^(kShift + kLazy): 2^14 in float16, whose largest number is 65504.
+template <typename T> constexpr float kShift = sizeof(T) == 2 && Elem<T>::kExp == 0x7c00 ? 10.f : 0.f;
+template <> constexpr float kShift<float> = 0.f;
+constexpr float kLazy = 4.f;
+
+template <typename T> constexpr int kKeysPerTile = sizeof(T) == 2 ? 64 : 32;
+
+// what a wavefront knows of its 32 queries
+struct Rows {
+    int pos, pmin, pmax;
+};
+
+// scores of 32 NK keys -> weights (in place), running maximum and sum, accumulators moved to the new maximum
+template <typename T, int NK, int DT, bool BIAS>
+__device__ __forceinline__ void softmax_step(f32x16_a (&s)[NK], f32x16_a (&acc)[DT], float& m, float& l, float c, const Rows& w,
+                                             const Window& win, int j0, int j1, bool full, const float* bias, int reach, int h) {
+    if constexpr (BIAS) {
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            const int a = j0 + 32 * k, z = a + 31;
+            if (a - w.pmax >= reach || z - w.pmin <= -reach) {   // one value for the whole tile
+                const float b = bias[a - w.pmax >= reach ? 2 * reach : 0];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[k][r] = fmaf(s[k][r], c, b);
+            } else {
+                const int far0 = a + 4 * h - w.pos + reach;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[k][r] = fmaf(s[k][r], c, bias[min(max(far0 + reg_row(r), 0), 2 * reach)]);
+            }
+        }
+    }
+    if (!full) {
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int j = j0 + 32 * k + 4 * h + reg_row(r);
+                s[k][r] = ((j < j1) & visible(win, j - w.pos, j)) ? s[k][r] : kMinusInf;
+            }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[k][r]);
+    mx = half_max(mx);
+    if constexpr (!BIAS) mx *= c;
+    const bool grow = mx > m + kLazy || (m == kMinusInf && mx > m);
+    if (__ballot(grow)) {
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m - mx) : 1.f;
+        m = grow ? mx : m;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+    }
+    const float ref = (m == kMinusInf ? 0.f : m) - kShift<T>;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float p = __builtin_amdgcn_exp2f(BIAS ? s[k][r] - ref : fmaf(s[k][r], c, -ref));
+            s[k][r] = p;
+            sum += p;
+        }
+    l += sum;
+}
+
+// acc += V^T P^T over 32 NK keys of a tile in LDS
+template <typename T, int D, int NK, int DT>
+__device__ __forceinline__ void weighted_values(f32x16_a (&acc)[DT], const f32x16_a (&p)[NK], const char* vt, bool full, int lane) {
+    if (full) {
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const V8<T> b = pack8<T>(p[k], s);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) mma(acc[d], Tile<T, D>::col_frag(vt, 32 * k + 16 * s, d, lane), b);
+            }
+    } else {
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const V8<T> b = pack8<T>(p[k], s);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) mma_guarded<T>(acc[d], Tile<T, D>::col_frag(vt, 32 * k + 16 * s, d, lane), b);
+            }
+    }
+}
+
+__device__ __forceinline__ Rows rows_of(const AttnArgs& a, int q0, int pos0, int first, int last, int mine) {
+    Rows w;
+    if (a.has_pos) {
+        w.pos = a.plan[a.pos_at + q0 + mine];
+        w.pmin = wave_min(w.pos);
+        w.pmax = wave_max(w.pos);
+    } else {
+        w.pos = pos0 + mine;
+        w.pmin = pos0 + first;
+        w.pmax = pos0 + last;
+    }
+    return w;
+}
+
+// ---- many queries: NW wavefronts of 32 queries share tiles of keys and values in LDS (two buffers, one barrier a tile)
+template <typename T, int D, int NW, bool BIAS>
+__global__ __launch_bounds__(NW * 64) void attn_fwd_wide_kernel(AttnArgs a) {
+    constexpr int kBK = kKeysPerTile<T>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
+    constexpr int kBytes = kBK * D * (int)sizeof(T);
+    extern __shared__ char smem[];
+    float* bias = reinterpret_cast<float*>(smem + 4 * kBytes);
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int id = xcd_order(blockIdx.x, gridDim.x);
+    const int head = id / a.n_items;
+    const QItem it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[id - head * a.n_items];
+    const Window win{a.left, a.right, a.sinks};
+    const float c = a.scale * kLog2e;
+
+    const int first = min(32 * w, it.nq - 1), last = min(32 * w + 31, it.nq - 1);
+    const bool active = 32 * w < it.nq;
+    const int row = 32 * w + (lane & 31), rowc = min(row, it.nq - 1);
+    const Rows rw = rows_of(a, it.q0, it.pos0, first, last, rowc);
+    const char* qrow = static_cast<const char*>(a.q.p) + (((int64_t)it.q0 + rowc) * a.q.row + (int64_t)head * a.q.head) * (int)sizeof(T);
+    V8<T> q[ST];
+#pragma unroll
+    for (int s = 0; s < ST; ++s) q[s] = global_frag<T>(qrow, s, h);
+
+    const int hk = head / a.group;
+    const char* kbase = static_cast<const char*>(a.k.p) + ((int64_t)it.k0 * a.k.row + (int64_t)hk * a.k.head) * (int)sizeof(T);
+    const char* vbase = static_cast<const char*>(a.v.p) + ((int64_t)it.k0 * a.v.row + (int64_t)hk * a.v.head) * (int)sizeof(T);
+    const int64_t kstep = a.k.row * (int)sizeof(T), vstep = a.v.row * (int)sizeof(T);
+    const int ns = (it.sink_end + kBK - 1) / kBK, n = ns + (it.ke - it.kb + kBK - 1) / kBK;
+
+    Stage<T, D, kBK, NW * 64> sk, sv;
+    auto fetch = [&](int t) {
+        const int j0 = t < ns ? t * kBK : it.kb + (t - ns) * kBK, j1 = t < ns ? it.sink_end : it.ke;
+        sk.load(kbase + j0 * kstep, kstep, j1 - j0, tid);
+        sv.load(vbase + j0 * vstep, vstep, j1 - j0, tid);
+    };
+    f32x16_a acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+    float m = kMinusInf, l = 0.f;
+
+    if (n > 0) fetch(0);
+    if constexpr (BIAS) load_bias<T>(bias, a.bias, a.heads, head, tid, NW * 64);
+    if (n > 0) {
+        sk.store(smem, tid);
+        sv.store(smem + 2 * kBytes, tid);
+    }
+    __syncthreads();
+    for (int t = 0; t < n; ++t) {
+        if (t + 1 < n) fetch(t + 1);
+        const char* kt = smem + (t & 1) * kBytes;
+        const char* vt = smem + (2 + (t & 1)) * kBytes;
+        const int j0 = t < ns ? t * kBK : it.kb + (t - ns) * kBK, j1 = min(j0 + kBK, t < ns ? it.sink_end : it.ke);
+        if (active && !none_visible(win, rw.pmin, rw.pmax, j0, j1)) {
+            const bool full = j1 - j0 == kBK && all_visible(win, rw.pmin, rw.pmax, j0, j1);
+            f32x16_a s[NK];
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[k][r] = 0.f;
+#pragma unroll
+                for (int st = 0; st < ST; ++st) mma(s[k], Tile<T, D>::row_frag(kt, 32 * k + (lane & 31), st, h), q[st]);
+            }
+            softmax_step<T, NK, DT, BIAS>(s, acc, m, l, c, rw, win, j0, j1, full, bias, a.bias.reach, h);
+            weighted_values<T, D, NK, DT>(acc, s, vt, full, lane);
+        }
+        if (t + 1 < n) {
+            sk.store(smem + ((t + 1) & 1) * kBytes, tid);
+            sv.store(smem + (2 + ((t + 1) & 1)) * kBytes, tid);
+        }
+        __syncthreads();
+    }
+    if (row < it.nq) {
+        l = half_sum(l);
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        T* o = static_cast<T*>(a.out.p) + ((int64_t)it.q0 + row) * a.out.row + (int64_t)head * a.out.head;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int g = 0; g < (D >= 32 ? 4 : 2); ++g) {
+                V4<T> x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = (T)(acc[d][4 * g + e] * inv);
+                *reinterpret_cast<V4<T>*>(o + 32 * d + 8 * g + 4 * h) = x;
+            }
+        if (h == 0) a.lse[(int64_t)head * a.q_rows + it.q0 + row] = m == kMinusInf ? kMinusInf : (m - kShift<T> + __log2f(l)) * kLn2;
+    }
+}
+
+// ---- few queries: the four wavefronts of a workgroup hold the SAME 32 queries and take every fourth tile of 32 keys, and a
+// ---- long range of keys is cut over workgroups as well; the parts meet in LDS, those of several workgroups in attn_join_kernel
+template <typename T, int D, bool BIAS>
+__global__ __launch_bounds__(256) void attn_fwd_split_kernel(AttnArgs a) {
+    constexpr int NW = 4, DT = D >= 32 ? D / 32 : 1, ST = D / 16, kPad = D + 4;
+    constexpr int kBytes = 32 * D * (int)sizeof(T);
+    extern __shared__ char smem[];
+    float* ml = reinterpret_cast<float*>(smem);                 // [NW][32][2]
+    float* bias = ml + NW * 64;
+    char* tiles = smem + (NW * 64 + (BIAS ? ((2 * a.bias.reach + 1 + 3) & ~3) : 0)) * 4;
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int id = xcd_order(blockIdx.x, gridDim.x);
+    const int head = id / a.n_items;
+    const QItem it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[id - head * a.n_items];
+    const Window win{a.left, a.right, a.sinks};
+    const float c = a.scale * kLog2e;
+    const int row = lane & 31, rowc = min(row, it.nq - 1);
+    const Rows rw = rows_of(a, it.q0, it.pos0, 0, it.nq - 1, rowc);
+    const char* qrow = static_cast<const char*>(a.q.p) + (((int64_t)it.q0 + rowc) * a.q.row + (int64_t)head * a.q.head) * (int)sizeof(T);
+    V8<T> q[ST];
+#pragma unroll
+    for (int s = 0; s < ST; ++s) q[s] = global_frag<T>(qrow, s, h);
+    const int hk = head / a.group;
+    const char* kbase = static_cast<const char*>(a.k.p) + ((int64_t)it.k0 * a.k.row + (int64_t)hk * a.k.head) * (int)sizeof(T);
+    const char* vbase = static_cast<const char*>(a.v.p) + ((int64_t)it.k0 * a.v.row + (int64_t)hk * a.v.head) * (int)sizeof(T);
+    const int64_t kstep = a.k.row * (int)sizeof(T), vstep = a.v.row * (int)sizeof(T);
+    const int ns = (it.sink_end + 31) / 32, n = ns + (it.ke - it.kb + 31) / 32;
+    if constexpr (BIAS) {
+        load_bias<T>(bias, a.bias, a.heads, head, tid, 256);
+        __syncthreads();
+    }
+    V8<T> kf[ST];
+    Stage<T, D, 32, 64> sv;
+    char* vt = tiles + w * kBytes;
+    auto fetch = [&](int t) {
+        const int j0 = t < ns ? t * 32 : it.kb + (t - ns) * 32, j1 = t < ns ? it.sink_end : it.ke;
+        const char* krow = kbase + min(j0 + (lane & 31), j1 - 1) * kstep;
+#pragma unroll
+        for (int s = 0; s < ST; ++s) kf[s] = global_frag<T>(krow, s, h);
+        sv.load(vbase + j0 * vstep, vstep, j1 - j0, lane);
+    };
+    f32x16_a acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+    float m = kMinusInf, l = 0.f;
+    if (w < n) fetch(w);
+    for (int t = w; t < n; t += NW) {
+        const int j0 = t < ns ? t * 32 : it.kb + (t - ns) * 32, j1 = min(j0 + 32, t < ns ? it.sink_end : it.ke);
+        f32x16_a s[1];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+#pragma unroll
+        for (int st = 0; st < ST; ++st) mma(s[0], kf[st], q[st]);
+        __builtin_amdgcn_wave_barrier();
+        sv.store(vt, lane);
+        if (t + NW < n) fetch(t + NW);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const bool full = j1 - j0 == 32 && all_visible(win, rw.pmin, rw.pmax, j0, j1);
+        softmax_step<T, 1, DT, BIAS>(s, acc, m, l, c, rw, win, j0, j1, full, bias, a.bias.reach, h);
+        weighted_values<T, D, 1, DT>(acc, s, vt, full, lane);
+    }
+    l = half_sum(l);
+    if (h == 0) {
+        ml[(w * 32 + lane) * 2] = m;
+        ml[(w * 32 + lane) * 2 + 1] = l;
+    }
+    __syncthreads();
+    float top = kMinusInf;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) top = fmaxf(top, ml[(i * 32 + (lane & 31)) * 2]);
+    const float f = m == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    float* o = reinterpret_cast<float*>(tiles);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int g = 0; g < (D >= 32 ? 4 : 2); ++g) {
+            V4<float> x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = acc[d][4 * g + e] * f;
+            *reinterpret_cast<V4<float>*>(o + (w * 32 + (lane & 31)) * kPad + 32 * d + 8 * g + 4 * h) = x;
+        }
+    __syncthreads();
+    for (int i = tid; i < 32 * (D / 4); i += 256) {
+        const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+        if (r >= it.nq) break;
+        float t = kMinusInf, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) t = fmaxf(t, ml[(k * 32 + r) * 2]);
+#pragma unroll
+        for (int k = 0; k < NW; ++k) {
+            const float mk = ml[(k * 32 + r) * 2];
+            sum += mk == kMinusInf ? 0.f : ml[(k * 32 + r) * 2 + 1] * __builtin_amdgcn_exp2f(mk - t);
+        }
+        V4<float> x = *reinterpret_cast<V4<float>*>(o + r * kPad + d);
+#pragma unroll
+        for (int k = 1; k < NW; ++k) x += *reinterpret_cast<V4<float>*>(o + (k * 32 + r) * kPad + d);
+        if (it.slot < 0) {
+            const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+            V4<T> y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * inv);
+            *reinterpret_cast<V4<T>*>(static_cast<T*>(a.out.p) + ((int64_t)it.q0 + r) * a.out.row + (int64_t)head * a.out.head + d) = y;
+            if (d == 0) a.lse[(int64_t)head * a.q_rows + it.q0 + r] = t == kMinusInf ? kMinusInf : (t - kShift<T> + __log2f(sum)) * kLn2;
+        } else {
+            const int64_t at = ((int64_t)it.slot * a.heads + head) * 32 + r;
+            *reinterpret_cast<V4<float>*>(a.part_o + at * D + d) = x;
+            if (d == 0) {
+                a.part_ml[at * 2] = t;
+                a.part_ml[at * 2 + 1] = sum;
+            }
+        }
+    }
+}
+
+// the parts of one tile of rows from several workgroups, one thread for four columns
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int n_join, int join_at) {
+    const int head = blockIdx.x / n_join;
+    const Join jn = reinterpret_cast<const Join*>(a.plan + join_at)[blockIdx.x - head * n_join];
+    for (int i = threadIdx.x; i < 32 * (D / 4); i += 256) {
+        const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+        if (r >= jn.n) break;
+        float m = kMinusInf, l = 0.f;
+        V4<float> x{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < jn.slots; ++k) {
+            const int64_t at = ((int64_t)(jn.slot0 + k) * a.heads + head) * 32 + r;
+            const float mk = a.part_ml[at * 2], lk = a.part_ml[at * 2 + 1];
+            const V4<float> xk = *reinterpret_cast<const V4<float>*>(a.part_o + at * D + d);
+            const float top = fmaxf(m, mk);
+            const float f0 = m == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(m - top);
+            const float f1 = mk == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(mk - top);
+            m = top;
+            l = l * f0 + lk * f1;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = x[e] * f0 + xk[e] * f1;
+        }
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        V4<T> y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * inv);
+        *reinterpret_cast<V4<T>*>(static_cast<T*>(a.out.p) + ((int64_t)jn.row0 + r) * a.out.row + (int64_t)head * a.out.head + d) = y;
+        if (d == 0) a.lse[(int64_t)head * a.q_rows + jn.row0 + r] = m == kMinusInf ? kMinusInf : (m - kShift<T> + __log2f(l)) * kLn2;
+    }
+}
+
+template <typename K>
+hipError_t lds_room(K kernel, size_t bytes) {
+    return bytes > 65536 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)
+                         : hipSuccess;
+}
+template <typename K, typename... A>
+hipError_t start(K kernel, int64_t blocks, int threads, size_t lds, hipStream_t s, const A&... args) {
+    if (blocks == 0) return hipSuccess;
+    const hipError_t e = lds_room(kernel, lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, s, args...);
+    return hipGetLastError();
+}
+inline size_t bias_floats(const AttnArgs& a) { return a.bias.table ? (size_t)((2 * a.bias.reach + 1 + 3) & ~3) : 0; }
+
+template <typename T, int D>
+hipError_t forward_dim(const AttnArgs& a, int mode, hipStream_t s) {
+    const int64_t blocks = (int64_t)a.n_items * a.heads;
+    if (mode == kSplitKeys) {
+        const size_t v = 4 * 32 * D * sizeof(T), o = 4 * 32 * (D + 4) * 4;
+        const size_t lds = (4 * 64 + bias_floats(a)) * 4 + (v > o ? v : o);
+        return a.bias.table ? start(attn_fwd_split_kernel<T, D, true>, blocks, 256, lds, s, a)
+                            : start(attn_fwd_split_kernel<T, D, false>, blocks, 256, lds, s, a);
+    }
+    const size_t lds = 4 * kKeysPerTile<T> * D * sizeof(T) + bias_floats(a) * 4;
+    if (mode == kWide64)
+        return a.bias.table ? start(attn_fwd_wide_kernel<T, D, 2, true>, blocks, 128, lds, s, a)
+                            : start(attn_fwd_wide_kernel<T, D, 2, false>, blocks, 128, lds, s, a);
+    return a.bias.table ? start(attn_fwd_wide_kernel<T, D, 4, true>, blocks, 256, lds, s, a)
+                        : start(attn_fwd_wide_kernel<T, D, 4, false>, blocks, 256, lds, s, a);
+}
+
+}  // namespace
+}  // namespace dptm

@@ -1,0 +1,554 @@
+// Entry points of the layer operators: argument checks, the attention plan, launches.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <exception>
+#include <new>
+#include <string>
+#include <vector>
+
+#include "../../include/dptm.h"
+#include "dptm_layers.h"
+
+using namespace dptm;
+
+namespace {
+
+thread_local std::string g_lerr;
+
+int fail(int code, const std::string& msg) {
+    g_lerr = msg;
+    return code;
+}
+
+// An exception must not leave an extern "C" function: the handlers of the entry points land here.
+int on_exception(const char* where) noexcept {
+    int code = DPTM_EHIP;
+    try {
+        try {
+            throw;
+        } catch (const std::bad_alloc&) {
+            code = DPTM_ENOMEM;
+            g_lerr = std::string(where) + ": out of host memory";
+        } catch (const std::exception& e) {
+            g_lerr = std::string(where) + ": " + e.what();
+        } catch (...) {
+            g_lerr = std::string(where) + ": unknown C++ exception";
+        }
+    } catch (...) {
+    }
+    return code;
+}
+
+// the caller's current device comes back when the call returns
+struct OnDevice {
+    int before = -1;
+    bool ok = false;
+    explicit OnDevice(int device) {
+        if (hipGetDevice(&before) != hipSuccess) before = -1;
+        ok = before == device || hipSetDevice(device) == hipSuccess;
+    }
+    ~OnDevice() {
+        int now = -1;
+        if (before >= 0 && hipGetDevice(&now) == hipSuccess && now != before) (void)hipSetDevice(before);
+    }
+};
+
+bool good_dim(int d) { return d == 16 || d == 32 || d == 64 || d == 128; }
+int size_of(int dtype) { return dtype == DPTM_PREC_F32 ? 4 : 2; }
+bool good_type(int t) { return t == DPTM_PREC_F32 || t == DPTM_PREC_BF16 || t == DPTM_PREC_F16; }
+
+// A tensor [rows][heads][dim] whose kernels fetch 16-byte vectors; `written`: rows and heads may not overlap.
+int check_rows(const char* who, const char* name, const dptm_rows* t, int64_t rows, int heads, int dim, int dtype, bool written,
+               Strided* out) {
+    const std::string at = std::string(who) + ": " + name;
+    if (!t) return fail(DPTM_EINVAL, at + " is NULL");
+    if (rows == 0) {
+        *out = Strided{nullptr, 0, 0};
+        return DPTM_OK;
+    }
+    const int size = size_of(dtype);
+    if (!t->data) return fail(DPTM_EINVAL, at + ": NULL buffer");
+    if (t->rows < rows) return fail(DPTM_EINVAL, at + " has " + std::to_string(t->rows) + " rows, the call needs " + std::to_string(rows));
+    if ((reinterpret_cast<uintptr_t>(t->data) & 15) || (t->row_stride * size) % 16 || (t->head_stride * size) % 16)
+        return fail(DPTM_EINVAL, at + ": address and strides must be multiples of 16 bytes");
+    if (t->row_stride < 0 || t->head_stride < 0) return fail(DPTM_EINVAL, at + ": negative stride");
+    if (t->row_stride > (int64_t(1) << 40) || t->head_stride > (int64_t(1) << 40)) return fail(DPTM_EINVAL, at + ": stride too large");
+    if (written) {
+        const bool rows_outside = (heads == 1 || t->head_stride >= dim) && (rows == 1 || t->row_stride >= (heads - 1) * t->head_stride + dim);
+        const bool heads_outside = (rows == 1 || t->row_stride >= dim) && (heads == 1 || t->head_stride >= (rows - 1) * t->row_stride + dim);
+        if (!rows_outside && !heads_outside) return fail(DPTM_EINVAL, at + ": rows or heads of a written tensor overlap");
+    }
+    *out = Strided{t->data, t->row_stride, t->head_stride};
+    return DPTM_OK;
+}
+
+constexpr int kGroups = 1024;   // workgroups that fill the card four times over
+
+int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+uint32_t header_sum(const int32_t* p) {
+    uint32_t h = 2166136261u;
+    for (int i = 0; i < kPlanHeader; ++i)
+        if (i != kPlanCheck) h = (h ^ (uint32_t)p[i]) * 16777619u;
+    return h;
+}
+
+struct Seq { int q0, nq, k0, nk, pos0, tile0; };
+
+struct PlanMaker {
+    int left, right, sinks;
+    const int32_t* pos;      // packed, NULL: row i of a sequence stands at i + nk - nq
+    std::vector<Seq> seqs;
+    std::vector<int> bounds;   // smallest and largest position of every 32 rows, where `pos` is given
+
+    void span(const Seq& s, int first, int n, int* lo, int* hi) const {
+        if (!pos) {
+            *lo = s.pos0 + first;
+            *hi = s.pos0 + first + n - 1;
+            return;
+        }
+        *lo = kFar, *hi = -kFar;
+        for (int i = 0; i < n; ++i) {
+            const int p = pos[s.q0 + first + i];
+            *lo = std::min(*lo, p), *hi = std::max(*hi, p);
+        }
+    }
+    // rows [first, first + n) of a sequence and the keys some of them see
+    QItem q_item(const Seq& s, int first, int n) const {
+        int lo, hi;
+        span(s, first, n, &lo, &hi);
+        QItem it{s.q0 + first, n, s.k0, s.pos0 + first, 0, 0, 0, -1};
+        it.ke = (int)std::max<int64_t>(0, std::min<int64_t>(s.nk, (int64_t)hi + right + 1));
+        it.kb = (int)std::min<int64_t>(it.ke, std::max<int64_t>(0, (int64_t)lo - left));
+        it.sink_end = std::min(std::min(sinks, it.kb), it.ke);
+        return it;
+    }
+    static int64_t keys(const QItem& it) { return (int64_t)it.ke - it.kb + it.sink_end; }
+    std::vector<QItem> q_items(int tile) const {
+        std::vector<QItem> all;
+        for (const Seq& s : seqs)
+            for (int i = 0; i < s.nq; i += tile) all.push_back(q_item(s, i, std::min(tile, s.nq - i)));
+        return all;
+    }
+    // the rows [qb, qe) that see some of the keys [j0, j1)
+    void q_range(const Seq& s, int j0, int j1, int* qb, int* qe) const {
+        auto sees = [&](int lo, int hi) {
+            return (int64_t)hi + right >= j0 && ((int64_t)lo - left <= j1 - 1 || j0 < sinks);
+        };
+        *qb = *qe = 0;
+        if (!pos) {
+            // positions grow with the row: rows from the first whose window reaches j0 to the last whose window still holds j1 - 1
+            const int64_t b = std::max<int64_t>(0, (int64_t)j0 - right - s.pos0);
+            const int64_t e = j0 < sinks ? s.nq : std::min<int64_t>(s.nq, (int64_t)j1 + left - s.pos0);
+            if (b < e) *qb = (int)(b / 32 * 32), *qe = (int)e;
+            return;
+        }
+        bool any = false;
+        for (int i = 0; i < s.nq; i += 32)
+            if (sees(bounds[2 * (s.tile0 + i / 32)], bounds[2 * (s.tile0 + i / 32) + 1])) {
+                if (!any) *qb = i;
+                any = true;
+                *qe = std::min(i + 32, s.nq);
+            }
+    }
+};
+
+int make_plan(const dptm_attention_desc& d, const int32_t* q_len, const int32_t* k_len, const int32_t* q_pos, int64_t n_seqs,
+              std::vector<int32_t>& words) {
+    const char* who = "dptm_attention_plan: ";
+    PlanMaker m;
+    m.left = d.window_left < 0 ? kFar : std::min(d.window_left, kFar);
+    m.right = d.window_right < 0 ? kFar : std::min(d.window_right, kFar);
+    m.sinks = std::min(d.sinks, kFar);
+    m.pos = q_pos;
+    int64_t q0 = 0, k0 = 0;
+    for (int64_t b = 0; b < n_seqs; ++b) {
+        const int nq = q_len[b], nk = k_len ? k_len[b] : q_len[b];
+        if (nq < 0 || nk < 0 || nq >= kFar || nk >= kFar)
+            return fail(DPTM_EINVAL, std::string(who) + "length of sequence " + std::to_string(b) + " is outside 0..2^29-1");
+        m.seqs.push_back(Seq{(int)q0, nq, (int)k0, nk, nk - nq, (int)(m.bounds.size() / 2)});
+        if (q_pos)
+            for (int i = 0; i < nq; i += 32) {
+                int lo = kFar, hi = -kFar;
+                for (int r = i; r < std::min(i + 32, nq); ++r) {
+                    const int p = q_pos[q0 + r];
+                    if (p <= -kFar || p >= kFar) return fail(DPTM_EINVAL, std::string(who) + "a position is outside -2^29..2^29");
+                    lo = std::min(lo, p), hi = std::max(hi, p);
+                }
+                m.bounds.push_back(lo);
+                m.bounds.push_back(hi);
+            }
+        q0 += nq, k0 += nk;
+        if (q0 > INT32_MAX || k0 > INT32_MAX) return fail(DPTM_EINVAL, std::string(who) + "more than 2^31-1 rows");
+    }
+    int64_t t32 = 0, t64 = 0, t128 = 0;
+    for (const Seq& s : m.seqs) t32 += up(s.nq, 32) / 32, t64 += up(s.nq, 64) / 64, t128 += up(s.nq, 128) / 128;
+
+    // Forward.  Tiles of 128 rows while they fill the card twice and waste little; of 64 below; workgroups that split the
+    // keys of 32 rows where even those leave processors idle, or no sequence has more rows than one wavefront takes.
+    int mode = kWide128;
+    if (t64 * d.heads < 256 || t32 == t64) mode = kSplitKeys;
+    else if (t128 * d.heads < 512 || t64 * 64 * 5 < t128 * 128 * 4) mode = kWide64;
+    std::vector<QItem> fwd = m.q_items(mode == kWide128 ? 128 : mode == kWide64 ? 64 : 32);
+    std::vector<Join> joins;
+    int slots = 0;
+    if (mode == kSplitKeys) {
+        int64_t total = 0;
+        for (const QItem& it : fwd) total += m.keys(it);
+        // keys of a workgroup: at least two tiles of each of its four wavefronts, and no more parts than fill the card
+        const int64_t chunk = std::max<int64_t>(256, up((total * d.heads + kGroups - 1) / kGroups, 128));
+        std::vector<QItem> cut;
+        for (const QItem& it : fwd) {
+            const int64_t n = it.ke - it.kb, parts = std::max<int64_t>(1, (n + chunk - 1) / chunk);
+            if (parts == 1) {
+                cut.push_back(it);
+                continue;
+            }
+            const int64_t each = up((n + parts - 1) / parts, 32);
+            Join j{it.q0, it.nq, slots, 0};
+            for (int64_t b = it.kb; b < it.ke; b += each) {
+                QItem p = it;
+                p.kb = (int)b, p.ke = (int)std::min<int64_t>(it.ke, b + each);
+                if (b != it.kb) p.sink_end = 0;
+                p.slot = slots++;
+                ++j.slots;
+                cut.push_back(p);
+            }
+            joins.push_back(j);
+        }
+        fwd.swap(cut);
+    }
+    auto heavy = [](const QItem& a, const QItem& b) { return PlanMaker::keys(a) > PlanMaker::keys(b); };
+    std::stable_sort(fwd.begin(), fwd.end(), heavy);
+
+    // Backward.  dq as the forward pass without splitting; dk, dv by tiles of keys, the range of rows cut where there
+    // are few tiles, or where a tile (the first keys of a window with sinks) sees far more rows than the others.
+    std::vector<QItem> dq;
+    std::vector<KItem> dkv;
+    std::vector<Join> dkv_joins;
+    int dq_waves = 4, dkv_waves = 4, dkv_slots = 0;
+    if (d.training) {
+        if (t128 * d.heads < 512 || t64 * 64 * 5 < t128 * 128 * 4) dq_waves = 2;
+        dq = m.q_items(32 * dq_waves);
+        std::stable_sort(dq.begin(), dq.end(), heavy);
+        int64_t k64 = 0, k128 = 0;
+        for (const Seq& s : m.seqs) k64 += up(s.nk, 64) / 64, k128 += up(s.nk, 128) / 128;
+        if (k128 * d.kv_heads < 512 || k64 * 64 * 5 < k128 * 128 * 4) dkv_waves = 2;
+        const int tile = 32 * dkv_waves;
+        int64_t total = 0;
+        for (const Seq& s : m.seqs)
+            for (int j = 0; j < s.nk; j += tile) {
+                KItem it{s.k0 + j, std::min(tile, s.nk - j), j, s.q0, 0, 0, s.pos0, -1, s.tile0, s.nq, {0, 0}};
+                m.q_range(s, j, j + it.nk, &it.qb, &it.qe);
+                dkv.push_back(it);
+                total += it.qe - it.qb;
+            }
+        const int64_t n = (int64_t)dkv.size();
+        if (n) {
+            const int64_t chunk = n * d.kv_heads >= kGroups ? std::max<int64_t>(1024, up(2 * total / n, 64))
+                                                            : std::max<int64_t>(128, up((total * d.kv_heads + kGroups - 1) / kGroups, 64));
+            std::vector<KItem> cut;
+            for (const KItem& it : dkv) {
+                const int64_t rows = it.qe - it.qb, parts = std::max<int64_t>(1, (rows + chunk - 1) / chunk);
+                if (parts == 1) {
+                    cut.push_back(it);
+                    continue;
+                }
+                const int64_t each = up((rows + parts - 1) / parts, 64);
+                Join j{it.k0, it.nk, dkv_slots, 0};
+                for (int64_t b = it.qb; b < it.qe; b += each) {
+                    KItem p = it;
+                    p.qb = (int)b, p.qe = (int)std::min<int64_t>(it.qe, b + each);
+                    p.slot = dkv_slots++;
+                    ++j.slots;
+                    cut.push_back(p);
+                }
+                dkv_joins.push_back(j);
+            }
+            dkv.swap(cut);
+            std::stable_sort(dkv.begin(), dkv.end(), [](const KItem& a, const KItem& b) { return a.qe - a.qb > b.qe - b.qb; });
+        }
+    }
+    const int64_t most = (int64_t(1) << 31) - 1;
+    if ((int64_t)fwd.size() * d.heads > most || (int64_t)dq.size() * d.heads > most || (int64_t)dkv.size() * d.kv_heads > most)
+        return fail(DPTM_EINVAL, std::string(who) + "too many tiles for one launch");
+
+    words.assign(kPlanHeader, 0);
+    auto append = [&](const void* p, size_t bytes) {
+        const int at = (int)words.size();
+        words.resize(words.size() + bytes / 4);
+        if (bytes) memcpy(words.data() + at, p, bytes);
+        return at;
+    };
+    const int fwd_at = append(fwd.data(), fwd.size() * sizeof(QItem));
+    const int join_at = append(joins.data(), joins.size() * sizeof(Join));
+    const int dq_at = append(dq.data(), dq.size() * sizeof(QItem));
+    const int dkv_at = append(dkv.data(), dkv.size() * sizeof(KItem));
+    const int dkv_join_at = append(dkv_joins.data(), dkv_joins.size() * sizeof(Join));
+    const int pos_at = append(q_pos, q_pos ? (size_t)q0 * 4 : 0);
+    const int tiles_at = append(m.bounds.data(), m.bounds.size() * 4);
+    if (words.size() > (size_t)INT32_MAX) return fail(DPTM_EINVAL, std::string(who) + "plan too large");
+    int32_t* p = words.data();
+    p[kPlanMagicAt] = kPlanMagic, p[kPlanWords] = (int32_t)words.size();
+    p[kPlanHeads] = d.heads, p[kPlanKvHeads] = d.kv_heads, p[kPlanHeadDim] = d.head_dim;
+    p[kPlanLeft] = m.left, p[kPlanRight] = m.right, p[kPlanSinks] = m.sinks;
+    p[kPlanSeqs] = (int32_t)n_seqs, p[kPlanQRows] = (int32_t)q0, p[kPlanKRows] = (int32_t)k0;
+    p[kPlanMode] = mode, p[kPlanFwd] = (int32_t)fwd.size(), p[kPlanFwdAt] = fwd_at, p[kPlanSlots] = slots;
+    p[kPlanJoin] = (int32_t)joins.size(), p[kPlanJoinAt] = join_at;
+    p[kPlanDq] = (int32_t)dq.size(), p[kPlanDqAt] = dq_at, p[kPlanDqWaves] = d.training ? dq_waves : 0;
+    p[kPlanDkv] = (int32_t)dkv.size(), p[kPlanDkvAt] = dkv_at, p[kPlanDkvWaves] = dkv_waves, p[kPlanDkvSlots] = dkv_slots;
+    p[kPlanDkvJoin] = (int32_t)dkv_joins.size(), p[kPlanDkvJoinAt] = dkv_join_at;
+    p[kPlanHasPos] = q_pos ? 1 : 0, p[kPlanPosAt] = pos_at;
+    p[kPlanTiles] = (int32_t)(m.bounds.size() / 2), p[kPlanTilesAt] = tiles_at;
+    p[kPlanCheck] = (int32_t)header_sum(p);
+    return DPTM_OK;
+}
+
+int check_plan(const char* who, const int32_t* plan, const int32_t* plan_dev) {
+    if (!plan || !plan_dev) return fail(DPTM_EINVAL, std::string(who) + ": NULL plan");
+    if (plan[kPlanMagicAt] != kPlanMagic || plan[kPlanCheck] != (int32_t)header_sum(plan))
+        return fail(DPTM_EINVAL, std::string(who) + ": not a plan of dptm_attention_plan");
+    return DPTM_OK;
+}
+
+// byte sizes of the workspace's parts, each rounded up to 256
+struct Work { size_t fwd_o, fwd_ml, delta, dkv, bias; };
+Work work_of(const int32_t* p, int n_buckets) {
+    Work w;
+    const size_t dim = p[kPlanHeadDim], heads = p[kPlanHeads], kv = p[kPlanKvHeads];
+    w.fwd_o = up((size_t)p[kPlanSlots] * heads * 32 * dim * 4, 256);
+    w.fwd_ml = up((size_t)p[kPlanSlots] * heads * 32 * 2 * 4, 256);
+    w.delta = up(heads * (size_t)p[kPlanQRows] * 4, 256);
+    w.dkv = up((size_t)p[kPlanDkvSlots] * kv * 2 * 32 * (size_t)p[kPlanDkvWaves] * dim * 4, 256);
+    w.bias = up(heads * (size_t)p[kPlanDq] * (size_t)n_buckets * 4, 256);
+    return w;
+}
+
+constexpr int kMaxBuckets = 64, kMaxReach = 1024;
+
+int check_bias(const char* who, const dptm_attention_bias* b, BiasArgs* out) {
+    *out = BiasArgs{nullptr, nullptr, 0, 0};
+    if (!b) return DPTM_OK;
+    if (!b->table || !b->buckets) return fail(DPTM_EINVAL, std::string(who) + ": bias without table or buckets");
+    if (b->n_buckets < 1 || b->n_buckets > kMaxBuckets) return fail(DPTM_EINVAL, std::string(who) + ": 1 to 64 buckets are supported");
+    if (b->max_distance < 0 || b->max_distance > kMaxReach)
+        return fail(DPTM_EINVAL, std::string(who) + ": a largest distance of 0 to 1024 is supported");
+    if (reinterpret_cast<uintptr_t>(b->buckets) & 3) return fail(DPTM_EINVAL, std::string(who) + ": buckets must be 4-byte aligned");
+    *out = BiasArgs{b->table, b->buckets, b->n_buckets, b->max_distance};
+    return DPTM_OK;
+}
+
+int check_common(const char* who, int dtype, float scale, const void* ws, size_t have, size_t need) {
+    if (!good_type(dtype)) return fail(DPTM_EINVAL, std::string(who) + ": dtype must be DPTM_PREC_F32, _BF16 or _F16");
+    if (!(scale > 0.f) || !std::isfinite(scale)) return fail(DPTM_EINVAL, std::string(who) + ": scale must be positive and finite");
+    if (need && (!ws || have < need))
+        return fail(DPTM_EINVAL, std::string(who) + ": workspace of " + std::to_string(need) + " bytes needed, " + std::to_string(ws ? have : 0) + " given");
+    if (need && (reinterpret_cast<uintptr_t>(ws) & 255)) return fail(DPTM_EINVAL, std::string(who) + ": workspace must be 256-byte aligned");
+    return DPTM_OK;
+}
+
+AttnArgs common_args(const int32_t* p, const int32_t* dev, float scale) {
+    AttnArgs a{};
+    a.plan = dev;
+    a.scale = scale;
+    a.heads = p[kPlanHeads];
+    a.group = p[kPlanHeads] / p[kPlanKvHeads];
+    a.left = p[kPlanLeft], a.right = p[kPlanRight], a.sinks = p[kPlanSinks];
+    a.q_rows = p[kPlanQRows];
+    a.has_pos = p[kPlanHasPos], a.pos_at = p[kPlanPosAt], a.tiles_at = p[kPlanTilesAt];
+    return a;
+}
+
+int hip_result(const char* who, hipError_t e) {
+    return e == hipSuccess ? DPTM_OK : fail(DPTM_EHIP, std::string(who) + ": " + hipGetErrorString(e));
+}
+
+#define BY_TYPE(F, ...) (dtype == DPTM_PREC_BF16 ? F##_bf16(__VA_ARGS__) : dtype == DPTM_PREC_F16 ? F##_f16(__VA_ARGS__) : F##_f32(__VA_ARGS__))
+#define OK_OR_RETURN(x)            \
+    do {                           \
+        const int rc_ = (x);       \
+        if (rc_) return rc_;       \
+    } while (0)
+
+}  // namespace
+
+extern "C" {
+
+const char* dptm_layer_last_error(void) { return g_lerr.c_str(); }
+
+int64_t dptm_attention_plan(const dptm_attention_desc* d, const int32_t* q_len, const int32_t* k_len, const int32_t* q_pos,
+                            int64_t n_seqs, int32_t* plan, int64_t capacity) try {
+    const char* who = "dptm_attention_plan: ";
+    if (!d) return fail(DPTM_EINVAL, std::string(who) + "NULL description");
+    if (d->heads < 1 || d->kv_heads < 1 || d->heads > 4096 || d->heads % d->kv_heads)
+        return fail(DPTM_EINVAL, std::string(who) + "heads must be 1..4096 and a multiple of kv_heads");
+    if (!good_dim(d->head_dim)) return fail(DPTM_EINVAL, std::string(who) + "head_dim must be 16, 32, 64 or 128");
+    if (d->sinks < 0) return fail(DPTM_EINVAL, std::string(who) + "negative number of first tokens");
+    if (n_seqs < 0 || n_seqs > INT32_MAX || (n_seqs > 0 && !q_len)) return fail(DPTM_EINVAL, std::string(who) + "bad sequence lengths");
+    if (capacity < 0 || (capacity > 0 && !plan)) return fail(DPTM_EINVAL, std::string(who) + "NULL plan");
+    std::vector<int32_t> words;
+    OK_OR_RETURN(make_plan(*d, q_len, k_len, q_pos, n_seqs, words));
+    if ((int64_t)words.size() <= capacity) memcpy(plan, words.data(), words.size() * 4);
+    return (int64_t)words.size();
+} catch (...) {
+    return on_exception("dptm_attention_plan");
+}
+
+int64_t dptm_attention_workspace(const int32_t* plan, int32_t n_buckets, int32_t backward) try {
+    OK_OR_RETURN(check_plan("dptm_attention_workspace", plan, plan));
+    if (n_buckets < 0 || n_buckets > kMaxBuckets) return fail(DPTM_EINVAL, "dptm_attention_workspace: 0 to 64 buckets are supported");
+    const Work w = work_of(plan, n_buckets);
+    return (int64_t)(backward ? w.delta + w.dkv + w.bias : w.fwd_o + w.fwd_ml);
+} catch (...) {
+    return on_exception("dptm_attention_workspace");
+}
+
+int dptm_attention_forward(const int32_t* plan, const int32_t* plan_dev, int32_t dtype, const dptm_rows* q, const dptm_rows* k,
+                           const dptm_rows* v, const dptm_rows* out, float* lse, float scale, const dptm_attention_bias* bias,
+                           void* workspace, size_t workspace_bytes, int32_t device, void* stream) try {
+    const char* who = "dptm_attention_forward";
+    OK_OR_RETURN(check_plan(who, plan, plan_dev));
+    const Work w = work_of(plan, 0);
+    OK_OR_RETURN(check_common(who, dtype, scale, workspace, workspace_bytes, w.fwd_o + w.fwd_ml));
+    const int heads = plan[kPlanHeads], kv = plan[kPlanKvHeads], dim = plan[kPlanHeadDim];
+    const int64_t nq = plan[kPlanQRows], nk = plan[kPlanKRows];
+    AttnArgs a = common_args(plan, plan_dev, scale);
+    OK_OR_RETURN(check_rows(who, "q", q, nq, heads, dim, dtype, false, &a.q));
+    OK_OR_RETURN(check_rows(who, "k", k, nk, kv, dim, dtype, false, &a.k));
+    OK_OR_RETURN(check_rows(who, "v", v, nk, kv, dim, dtype, false, &a.v));
+    OK_OR_RETURN(check_rows(who, "out", out, nq, heads, dim, dtype, true, &a.out));
+    OK_OR_RETURN(check_bias(who, bias, &a.bias));
+    if (nq == 0) return DPTM_OK;
+    if (!lse || (reinterpret_cast<uintptr_t>(lse) & 3)) return fail(DPTM_EINVAL, std::string(who) + ": lse is NULL or misaligned");
+    a.lse = lse;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.fwd_o);
+    a.n_items = plan[kPlanFwd], a.items_at = plan[kPlanFwdAt];
+    const OnDevice on(device);
+    if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    OK_OR_RETURN(hip_result(who, BY_TYPE(attn_forward, a, dim, plan[kPlanMode], s)));
+    return hip_result(who, BY_TYPE(attn_join, a, dim, plan[kPlanJoin], plan[kPlanJoinAt], s));
+} catch (...) {
+    return on_exception("dptm_attention_forward");
+}
+
+int dptm_attention_backward(const int32_t* plan, const int32_t* plan_dev, int32_t dtype, const dptm_rows* dout, const dptm_rows* q,
+                            const dptm_rows* k, const dptm_rows* v, const dptm_rows* out, const float* lse, float scale,
+                            const dptm_attention_bias* bias, const dptm_rows* dq, const dptm_rows* dk, const dptm_rows* dv,
+                            void* dtable, void* workspace, size_t workspace_bytes, int32_t device, void* stream) try {
+    const char* who = "dptm_attention_backward";
+    OK_OR_RETURN(check_plan(who, plan, plan_dev));
+    if (!plan[kPlanDqWaves]) return fail(DPTM_EINVAL, std::string(who) + ": the plan was made without training");
+    AttnArgs a = common_args(plan, plan_dev, scale);
+    OK_OR_RETURN(check_bias(who, bias, &a.bias));
+    const Work w = work_of(plan, a.bias.n_buckets);
+    OK_OR_RETURN(check_common(who, dtype, scale, workspace, workspace_bytes, w.delta + w.dkv + w.bias));
+    const int heads = plan[kPlanHeads], kv = plan[kPlanKvHeads], dim = plan[kPlanHeadDim];
+    const int64_t nq = plan[kPlanQRows], nk = plan[kPlanKRows];
+    OK_OR_RETURN(check_rows(who, "dout", dout, nq, heads, dim, dtype, false, &a.dout));
+    OK_OR_RETURN(check_rows(who, "q", q, nq, heads, dim, dtype, false, &a.q));
+    OK_OR_RETURN(check_rows(who, "k", k, nk, kv, dim, dtype, false, &a.k));
+    OK_OR_RETURN(check_rows(who, "v", v, nk, kv, dim, dtype, false, &a.v));
+    OK_OR_RETURN(check_rows(who, "out", out, nq, heads, dim, dtype, false, &a.out));
+    OK_OR_RETURN(check_rows(who, "dq", dq, nq, heads, dim, dtype, true, &a.dq));
+    OK_OR_RETURN(check_rows(who, "dk", dk, nk, kv, dim, dtype, true, &a.dk));
+    OK_OR_RETURN(check_rows(who, "dv", dv, nk, kv, dim, dtype, true, &a.dv));
+    if (nq && (!lse || (reinterpret_cast<uintptr_t>(lse) & 3))) return fail(DPTM_EINVAL, std::string(who) + ": lse is NULL or misaligned");
+    if (bias && !dtable) return fail(DPTM_EINVAL, std::string(who) + ": bias without a buffer for its gradient");
+    a.lse = const_cast<float*>(lse);
+    a.delta = static_cast<float*>(workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.delta);
+    a.part_bias = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.delta + w.dkv);
+    a.dtable = dtable;
+    const OnDevice on(device);
+    if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    a.n_items = plan[kPlanDq], a.items_at = plan[kPlanDqAt];
+    OK_OR_RETURN(hip_result(who, BY_TYPE(attn_dq, a, dim, plan[kPlanDqWaves], s)));
+    if (bias) OK_OR_RETURN(hip_result(who, BY_TYPE(attn_dtable, a, plan[kPlanDq], s)));
+    a.n_items = plan[kPlanDkv], a.items_at = plan[kPlanDkvAt];
+    OK_OR_RETURN(hip_result(who, BY_TYPE(attn_dkv, a, dim, plan[kPlanDkvWaves], s)));
+    return hip_result(who, BY_TYPE(attn_dkv_join, a, dim, plan[kPlanDkvJoin], plan[kPlanDkvJoinAt], 32 * plan[kPlanDkvWaves], s));
+} catch (...) {
+    return on_exception("dptm_attention_backward");
+}
+
+static int norm_rope_args(const char* who, const dptm_norm_rope_desc* d, const dptm_rows* q, const dptm_rows* k, const float* q_gain,
+                          const float* k_gain, const float* cosv, const float* sinv, const int32_t* positions, NormRopeArgs* a) {
+    if (!d) return fail(DPTM_EINVAL, std::string(who) + ": NULL description");
+    if (!good_type(d->dtype)) return fail(DPTM_EINVAL, std::string(who) + ": dtype must be DPTM_PREC_F32, _BF16 or _F16");
+    if (!good_dim(d->head_dim)) return fail(DPTM_EINVAL, std::string(who) + ": head_dim must be 16, 32, 64 or 128");
+    if (d->heads < 0 || d->kv_heads < 0 || d->heads + d->kv_heads < 1 || d->heads > 4096 || d->kv_heads > 4096)
+        return fail(DPTM_EINVAL, std::string(who) + ": 0 to 4096 heads each, at least one in all");
+    if (d->rows < 0 || d->rows > (int64_t(1) << 31) - 1) return fail(DPTM_EINVAL, std::string(who) + ": bad row count");
+    if (!(d->eps >= 0.f) || !std::isfinite(d->eps)) return fail(DPTM_EINVAL, std::string(who) + ": eps must be finite and not negative");
+    if (d->n_positions < 0) return fail(DPTM_EINVAL, std::string(who) + ": negative number of positions");
+    // every row's heads, D / 16 lanes each, in blocks of 256 threads: the grid stays below 2^31
+    if (d->rows * (d->heads + d->kv_heads) * (d->head_dim / 16) / 256 >= (int64_t(1) << 31) - 1)
+        return fail(DPTM_EINVAL, std::string(who) + ": too many rows for one launch");
+    if (d->rows && (!cosv || !sinv || (reinterpret_cast<uintptr_t>(cosv) & 15) || (reinterpret_cast<uintptr_t>(sinv) & 15)))
+        return fail(DPTM_EINVAL, std::string(who) + ": cos / sin are NULL or not 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(positions) & 3) || (reinterpret_cast<uintptr_t>(q_gain) & 3) || (reinterpret_cast<uintptr_t>(k_gain) & 3))
+        return fail(DPTM_EINVAL, std::string(who) + ": positions and gains must be 4-byte aligned");
+    *a = NormRopeArgs{};
+    OK_OR_RETURN(check_rows(who, "q", q, d->heads ? d->rows : 0, d->heads, d->head_dim, d->dtype, false, &a->x[0]));
+    OK_OR_RETURN(check_rows(who, "k", k, d->kv_heads ? d->rows : 0, d->kv_heads, d->head_dim, d->dtype, false, &a->x[1]));
+    a->heads[0] = d->heads, a->heads[1] = d->kv_heads;
+    a->gain[0] = q_gain, a->gain[1] = k_gain;
+    a->cosv = cosv, a->sinv = sinv, a->positions = positions;
+    a->rows = d->rows, a->n_pos = d->n_positions, a->dim = d->head_dim, a->interleaved = d->interleaved ? 1 : 0, a->eps = d->eps;
+    return DPTM_OK;
+}
+
+int dptm_qk_norm_rope_forward(const dptm_norm_rope_desc* d, const dptm_rows* q, const dptm_rows* k, const float* q_gain,
+                              const float* k_gain, const float* cosv, const float* sinv, const int32_t* positions,
+                              const dptm_rows* q_out, const dptm_rows* k_out, int32_t device, void* stream) try {
+    const char* who = "dptm_qk_norm_rope_forward";
+    NormRopeArgs a;
+    OK_OR_RETURN(norm_rope_args(who, d, q, k, q_gain, k_gain, cosv, sinv, positions, &a));
+    OK_OR_RETURN(check_rows(who, "q_out", q_out, d->heads ? d->rows : 0, d->heads, d->head_dim, d->dtype, true, &a.y[0]));
+    OK_OR_RETURN(check_rows(who, "k_out", k_out, d->kv_heads ? d->rows : 0, d->kv_heads, d->head_dim, d->dtype, true, &a.y[1]));
+    if (d->rows == 0) return DPTM_OK;
+    const OnDevice on(device);
+    if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
+    return hip_result(who, norm_rope_forward(a, d->dtype, static_cast<hipStream_t>(stream)));
+} catch (...) {
+    return on_exception("dptm_qk_norm_rope_forward");
+}
+
+int64_t dptm_qk_norm_rope_workspace(const dptm_norm_rope_desc* d) {
+    if (!d || !good_dim(d->head_dim) || d->rows < 0 || d->heads < 0 || d->kv_heads < 0) return fail(DPTM_EINVAL, "dptm_qk_norm_rope_workspace: bad sizes");
+    return (int64_t)norm_rope_blocks(d->rows, d->heads + d->kv_heads, d->head_dim) * d->head_dim * 2 * 4;
+}
+
+int dptm_qk_norm_rope_backward(const dptm_norm_rope_desc* d, const dptm_rows* dq_out, const dptm_rows* dk_out, const dptm_rows* q,
+                               const dptm_rows* k, const float* q_gain, const float* k_gain, const float* cosv, const float* sinv,
+                               const int32_t* positions, const dptm_rows* dq, const dptm_rows* dk, float* dq_gain, float* dk_gain,
+                               void* workspace, size_t workspace_bytes, int32_t device, void* stream) try {
+    const char* who = "dptm_qk_norm_rope_backward";
+    NormRopeArgs a;
+    OK_OR_RETURN(norm_rope_args(who, d, q, k, q_gain, k_gain, cosv, sinv, positions, &a));
+    const int64_t rq = d->heads ? d->rows : 0, rk = d->kv_heads ? d->rows : 0;
+    OK_OR_RETURN(check_rows(who, "dq_out", dq_out, rq, d->heads, d->head_dim, d->dtype, false, &a.dy[0]));
+    OK_OR_RETURN(check_rows(who, "dk_out", dk_out, rk, d->kv_heads, d->head_dim, d->dtype, false, &a.dy[1]));
+    OK_OR_RETURN(check_rows(who, "dq", dq, rq, d->heads, d->head_dim, d->dtype, true, &a.dx[0]));
+    OK_OR_RETURN(check_rows(who, "dk", dk, rk, d->kv_heads, d->head_dim, d->dtype, true, &a.dx[1]));
+    if ((q_gain && !dq_gain) || (k_gain && !dk_gain)) return fail(DPTM_EINVAL, std::string(who) + ": gain without a buffer for its gradient");
+    const int64_t half = dptm_qk_norm_rope_workspace(d) / 2;
+    if ((q_gain || k_gain) && (!workspace || workspace_bytes < (size_t)half * 2 || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+        return fail(DPTM_EINVAL, std::string(who) + ": workspace of " + std::to_string(half * 2) + " bytes, 256-byte aligned, needed");
+    a.part[0] = static_cast<float*>(workspace);
+    a.part[1] = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + half) : nullptr;
+    a.dgain[0] = dq_gain, a.dgain[1] = dk_gain;
+    const OnDevice on(device);
+    if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
+    return hip_result(who, norm_rope_backward(a, d->dtype, static_cast<hipStream_t>(stream)));
+} catch (...) {
+    return on_exception("dptm_qk_norm_rope_backward");
+}
+
+}  // extern "C"

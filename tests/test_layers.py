@@ -1,0 +1,272 @@
+"""Layer operators without a GPU: the attention plan covers what it has to, tables are what they say, bad calls are refused."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from deepptmpred_amd import _native, layers  # noqa: E402
+from oracle import layers_ref as R  # noqa: E402
+
+Q_ITEM, K_ITEM, JOIN = 8, 12, 4
+
+
+def see(q_lens, k_lens, window, sinks, pos):
+    """Visible pairs of packed rows and packed keys."""
+    m = np.zeros((sum(q_lens), sum(k_lens)), bool)
+    q0 = k0 = 0
+    for a, b in zip(q_lens, k_lens):
+        p, j = pos[q0:q0 + a][:, None], np.arange(b)[None]
+        v = np.ones((a, b), bool)
+        if window[1] >= 0:
+            v &= j <= p + window[1]
+        if window[0] >= 0:
+            v &= (j >= p - window[0]) | (j < sinks)
+        m[q0:q0 + a, k0:k0 + b] = v
+        q0, k0 = q0 + a, k0 + b
+    return m
+
+
+BATCHES = [([], []), ([0], [0]), ([1], [1]), ([5, 0, 200], [5, 0, 200]), ([1, 1, 1], [700, 0, 3000]), ([40, 3], [10, 500]),
+           ([129, 64, 1], [129, 64, 1]), ([53], [2000])]
+
+
+@pytest.mark.parametrize("q_lens,k_lens", BATCHES)
+@pytest.mark.parametrize("window,sinks", [((-1, -1), 0), ((-1, 0), 0), ((20, 7), 3), ((0, 0), 40), ((5, -1), 2), ((300, 0), 130)])
+@pytest.mark.parametrize("heads", [1, 64])
+@pytest.mark.parametrize("given", [False, True])
+def test_plan_covers_every_visible_pair_once(q_lens, k_lens, window, sinks, heads, given):
+    rng = np.random.default_rng(sum(k_lens) + sinks)
+    pos = np.concatenate([rng.integers(-3, b + 3, a) for a, b in zip(q_lens, k_lens)] or [np.zeros(0)]).astype(np.int32) if given else None
+    plan = layers.AttentionPlan(q_lens, k_lens, heads=heads, head_dim=32, window=window, sinks=sinks, q_positions=pos, device=None)
+    w = plan.words
+    p = pos if given else R.default_positions(q_lens, k_lens)
+    m = see(q_lens, k_lens, window, sinks, p)
+    starts = {}
+    q0 = k0 = 0
+    for a, b in zip(q_lens, k_lens):
+        for i in range(a):
+            starts[q0 + i] = (k0, b)
+        q0, k0 = q0 + a, k0 + b
+    # forward and dq: every row's visible keys lie in the ranges of its items, each once; parts are joined
+    for at, n, tile in ((w[13], w[12], (128, 64, 32)[w[11]]), (w[18], w[17], 32 * w[19])):
+        count = np.zeros(m.shape, np.int64)
+        slots = []
+        for it in w[at:at + Q_ITEM * n].reshape(-1, Q_ITEM):
+            first, nq, ks, pos0, kb, ke, sink_end, slot = (int(v) for v in it)
+            assert 1 <= nq <= tile
+            for r in range(first, first + nq):
+                base, length = starts[r]
+                assert ks == base and 0 <= kb <= ke <= length and 0 <= sink_end <= kb
+                if not given:
+                    assert p[r] == pos0 + r - first
+                count[r, ks + kb:ks + ke] += 1
+                count[r, ks:ks + sink_end] += 1
+            if slot >= 0:
+                slots.append(slot)
+        assert count.max(initial=0) <= 1 and not (m & (count == 0)).any()
+        rows = np.zeros(len(m), np.int64)
+        for it in w[at:at + Q_ITEM * n].reshape(-1, Q_ITEM):
+            if it[7] < 0:
+                rows[it[0]:it[0] + it[1]] += 1
+        if at == w[13]:
+            joined = []
+            for first, nq, slot0, k in w[w[16]:w[16] + JOIN * w[15]].reshape(-1, JOIN):
+                rows[first:first + nq] += 1
+                joined += list(range(slot0, slot0 + k))
+            assert sorted(slots) == sorted(joined) == list(range(w[14]))
+        assert (rows == 1).all()
+    # dk, dv: the other way round
+    count = np.zeros(m.shape, np.int64)
+    keys = np.zeros(m.shape[1], np.int64)
+    slots = []
+    for it in w[w[21]:w[21] + K_ITEM * w[20]].reshape(-1, K_ITEM):
+        first, nk, j0, q0, qb, qe, pos0, slot, tile0, nseq = (int(v) for v in it[:10])
+        assert 1 <= nk <= 32 * w[22] and qb % 32 == 0 and 0 <= qb <= qe <= nseq
+        count[q0 + qb:q0 + qe, first:first + nk] += 1
+        if slot < 0:
+            keys[first:first + nk] += 1
+        else:
+            slots.append(slot)
+        if given:
+            for i in range(qb, qe, 32):
+                lo, hi = w[w[29] + 2 * (tile0 + i // 32)], w[w[29] + 2 * (tile0 + i // 32) + 1]
+                assert lo == p[q0 + i:q0 + min(i + 32, nseq)].min() and hi == p[q0 + i:q0 + min(i + 32, nseq)].max()
+    joined = []
+    for first, nk, slot0, k in w[w[25]:w[25] + JOIN * w[24]].reshape(-1, JOIN):
+        keys[first:first + nk] += 1
+        joined += list(range(slot0, slot0 + k))
+    assert sorted(slots) == sorted(joined) == list(range(w[23]))
+    assert (keys == 1).all() and count.max(initial=0) <= 1 and not (m & (count == 0)).any()
+
+
+def test_long_sequences_split_evenly():
+    """One long sequence under a window with first tokens: no tile of keys keeps a range of rows far longer than the others'."""
+    plan = layers.AttentionPlan([16001], heads=8, head_dim=64, window=(512, 512), sinks=1, device=None)
+    w = plan.words
+    rows = [int(it[5] - it[4]) for it in w[w[21]:w[21] + K_ITEM * w[20]].reshape(-1, K_ITEM)]
+    assert max(rows) <= 4 * np.median(rows)
+
+
+def test_relative_buckets():
+    m = layers.relative_buckets(32, 128, device=None)
+    assert m.dtype == np.int32 and m.shape == (257,)
+    at = lambda d: int(m[128 + d])  # noqa: E731
+    assert [at(-d) for d in range(9)] == list(range(9)) and [at(d) for d in range(1, 9)] == list(range(17, 25))
+    assert at(0) == 0 and at(-128) == 15 and at(128) == 31
+    # 8 (128 / 8)^(k / 8) = 8 2^(k / 2): borders at 11.3, 16, 22.6, 32, 45.3, 64, 90.5
+    assert [at(-d) for d in (11, 12, 15, 16, 22, 23, 31, 32, 45, 46, 63, 64, 90, 91)] == [8, 9, 9, 10, 10, 11, 11, 12, 12, 13, 13, 14, 14, 15]
+    b = layers.relative_buckets(8, 20, False, device=None)
+    assert (b[20:] == 0).all() and b[0] == 7 and (np.diff(b) <= 0).all() and set(b) == set(range(8))
+    for bad in ((3, 9, True), (2, 9, True), (66, 128, True), (32, 8, True), (32, 1025, True), (1, 9, False)):
+        with pytest.raises(ValueError):
+            layers.relative_buckets(*bad, device=None)
+
+
+def test_rotary_table():
+    cos, sin = layers.rotary_table(5000, 64, device="cpu")
+    assert cos.shape == sin.shape == (5000, 32) and cos.dtype == torch.float32
+    a = 4999 * 10000.0 ** (-2 * 7 / 64)
+    assert abs(float(cos[4999, 7]) - np.cos(a)) < 1e-7 and abs(float(sin[4999, 7]) - np.sin(a)) < 1e-7
+    with pytest.raises(ValueError):
+        layers.rotary_table(10, 7, device="cpu")
+
+
+def test_plan_refusals():
+    ok = dict(heads=4, head_dim=64, device=None)
+    for bad, more in (([5], dict(head_dim=48)), ([5], dict(heads=4, kv_heads=3)), ([5], dict(heads=0)), ([5], dict(sinks=-1)),
+                      ([-1], {}), ([2 ** 29], {}), ([2 ** 28] * 8 + [7] * 2, {}), ([5], dict(q_positions=[0, 1, 2])),
+                      ([2], dict(q_positions=[0, 2 ** 29])), ([5], dict(k_lens=[5, 5])), ([[5]], {}), ([5.5], {}),
+                      ([2 ** 40], {}), ([5], dict(heads=5000))):
+        with pytest.raises(ValueError):
+            layers.AttentionPlan(bad, **{**ok, **more})
+    assert layers.AttentionPlan([], **ok).q_rows == 0
+
+
+def rows_of(n, heads, dim, at=1 << 20, size=2):
+    return _native.Rows(at, n, heads * dim, dim)
+
+
+def test_c_calls_are_refused_before_anything_runs():
+    """Bad sizes, strides, addresses and plans come back as DPTM_EINVAL: none of these addresses is ever touched."""
+    lib = _native.load_library()
+    plan = layers.AttentionPlan([10], heads=2, head_dim=64, device=None)
+    P, ref = plan.words.ctypes.data, C.byref
+    good = rows_of(10, 2, 64)
+
+    def forward(plan_host=P, dtype=1, q=good, k=good, v=good, out=good, lse=1 << 20, scale=0.1, bias=None, ws=None, ws_bytes=0, dev=0):
+        return lib.dptm_attention_forward(plan_host, P, dtype, None if q is None else ref(q), ref(k), ref(v), ref(out), lse, scale,
+                                          None if bias is None else ref(bias), ws, ws_bytes, dev, None)
+
+    def says(rc, text):
+        assert rc == _native.DPTM_EINVAL and text in lib.dptm_layer_last_error().decode(), lib.dptm_layer_last_error()
+
+    need = lib.dptm_attention_workspace(P, 0, 0)
+    ws = dict(ws=1 << 20, ws_bytes=need)
+    says(forward(plan_host=None, **ws), "NULL plan")
+    other = plan.words.copy()
+    other[12] += 1
+    says(forward(plan_host=other.ctypes.data, **ws), "not a plan")
+    says(forward(dtype=3, **ws), "dtype")
+    says(forward(scale=0.0, **ws), "scale")
+    says(forward(scale=-1.0, **ws), "scale")
+    says(forward(scale=float("nan"), **ws), "scale")
+    says(forward(q=None, **ws), "q is NULL")
+    says(forward(q=_native.Rows(None, 10, 128, 64), **ws), "NULL buffer")
+    says(forward(k=rows_of(9, 2, 64), **ws), "k has 9 rows")
+    says(forward(v=rows_of(10, 2, 64, at=(1 << 20) + 8), **ws), "16 bytes")
+    says(forward(q=_native.Rows(1 << 20, 10, 132, 64), **ws), "16 bytes")
+    says(forward(q=_native.Rows(1 << 20, 10, -128, 64), **ws), "negative")
+    says(forward(out=_native.Rows(1 << 20, 10, 64, 64), **ws), "overlap")
+    says(forward(out=_native.Rows(1 << 20, 10, 128, 0), **ws), "overlap")
+    says(forward(lse=None, **ws), "lse")
+    if need:
+        says(forward(), "workspace")
+        says(forward(ws=(1 << 20) + 16, ws_bytes=need), "256-byte")
+    for n, far in ((0, 5), (65, 5), (8, -1), (8, 1025)):
+        says(forward(bias=_native.AttentionBias(1 << 20, 1 << 20, n, far), **ws), "supported")
+    says(forward(bias=_native.AttentionBias(None, 1 << 20, 8, 9), **ws), "without")
+
+    def backward(plan_host=P, dq=good, dk=good, bias=None, dtable=None, ws=1 << 20, ws_bytes=1 << 30, lse=1 << 20):
+        return lib.dptm_attention_backward(plan_host, P, 1, *[ref(good)] * 5, lse, 0.1, None if bias is None else ref(bias), ref(dq),
+                                           ref(dk), ref(good), dtable, ws, ws_bytes, 0, None)
+
+    says(backward(ws_bytes=16), "workspace")
+    says(backward(dq=_native.Rows(1 << 20, 10, 128, 0)), "overlap")
+    says(backward(dk=rows_of(3, 2, 64)), "dk has 3 rows")
+    says(backward(bias=_native.AttentionBias(1 << 20, 1 << 20, 8, 9)), "gradient")
+    says(backward(lse=None), "lse")
+    fwd_only = layers.AttentionPlan([10], heads=2, head_dim=64, training=False, device=None)
+    says(backward(plan_host=fwd_only.words.ctypes.data), "without training")
+    assert lib.dptm_attention_workspace(None, 0, 0) == _native.DPTM_EINVAL
+    assert lib.dptm_attention_workspace(P, 65, 0) == _native.DPTM_EINVAL
+    assert lib.dptm_attention_plan(None, None, None, None, 0, None, 0) == _native.DPTM_EINVAL
+
+
+def test_c_norm_calls_are_refused_before_anything_runs():
+    lib = _native.load_library()
+    ref, good = C.byref, rows_of(10, 2, 64)
+    tab = 1 << 20
+
+    def call(q=good, out=good, cos=tab, gain=tab, positions=None, **d):
+        desc = _native.NormRopeDesc(**{**dict(dtype=1, head_dim=64, heads=2, kv_heads=2, rows=10, n_positions=10, interleaved=0, eps=1e-6), **d})
+        return lib.dptm_qk_norm_rope_forward(ref(desc), ref(q), ref(good), gain, gain, cos, tab, positions, ref(out), ref(good), 0, None)
+
+    for bad, text in ((dict(dtype=7), "dtype"), (dict(head_dim=24), "head_dim"), (dict(heads=-1), "heads"),
+                      (dict(heads=0, kv_heads=0), "heads"), (dict(rows=-1), "row"), (dict(eps=-1.0), "eps"),
+                      (dict(eps=float("nan")), "eps"), (dict(n_positions=-1), "positions"), (dict(cos=None), "cos"),
+                      (dict(cos=tab + 4), "16-byte"), (dict(gain=tab + 2), "aligned"), (dict(positions=tab + 2), "aligned"),
+                      (dict(q=rows_of(9, 2, 64)), "rows"), (dict(out=_native.Rows(tab, 10, 128, 0)), "overlap"),
+                      (dict(rows=2 ** 31), "row")):
+        rc = call(**bad)
+        assert rc == _native.DPTM_EINVAL and text in lib.dptm_layer_last_error().decode(), (text, lib.dptm_layer_last_error())
+    desc = _native.NormRopeDesc(1, 64, 2, 2, 10, 10, 0, 1e-6)
+    rc = lib.dptm_qk_norm_rope_backward(ref(desc), *[ref(good)] * 4, tab, tab, tab, tab, None, ref(good), ref(good), None, tab, tab, 1 << 20, 0, None)
+    assert rc == _native.DPTM_EINVAL and b"gradient" in lib.dptm_layer_last_error()
+    rc = lib.dptm_qk_norm_rope_backward(ref(desc), *[ref(good)] * 4, tab, tab, tab, tab, None, ref(good), ref(good), tab, tab, None, 0, 0, None)
+    assert rc == _native.DPTM_EINVAL and b"workspace" in lib.dptm_layer_last_error()
+
+
+def test_python_refusals():
+    plan = layers.AttentionPlan([4], heads=2, head_dim=16, device=None)
+    t = torch.zeros(4, 2, 16)
+    for bad in ((t, t, t), (t.double(), t, t), (np.zeros((4, 2, 16), np.float32), t, t)):
+        with pytest.raises(ValueError):
+            layers.attention(*bad, plan)
+    with pytest.raises(ValueError):
+        layers.qk_norm_rope(t, t, torch.zeros(4, 8), torch.zeros(4, 8))
+    with pytest.raises(ValueError):
+        layers.qk_norm_rope(t, t[:3], torch.zeros(4, 8), torch.zeros(4, 8))
+
+
+@pytest.mark.parametrize("window,sinks,buckets", [((-1, -1), 0, False), ((3, 1), 2, True), ((2, 0), 0, True)])
+def test_the_restated_gradients_are_the_differences_of_the_forward_pass(window, sinks, buckets):
+    rng = np.random.default_rng(4)
+    q_lens, k_lens = [5, 3, 1], [7, 3, 0]
+    x = {"q": rng.normal(size=(9, 4, 6)), "k": rng.normal(size=(10, 2, 6)), "v": rng.normal(size=(10, 2, 6)), "table": rng.normal(size=(4, 4))}
+    of = np.array([0, 1, 2, 3, 3]) if buckets else None
+    w = rng.normal(size=(9, 4, 6))
+
+    def loss(y, dout=None):
+        return R.attention(y["q"], y["k"], y["v"], q_lens, k_lens, window, sinks, None, None, y["table"] if buckets else None, of, dout)
+
+    r = loss(x, w)
+    for n, g in (("q", "dq"), ("k", "dk"), ("v", "dv")) + ((("table", "dtable"),) if buckets else ()):
+        d = rng.normal(size=x[n].shape)
+        up, down = {**x, n: x[n] + 1e-6 * d}, {**x, n: x[n] - 1e-6 * d}
+        slope = ((loss(up)["out"][0] - loss(down)["out"][0]) * w).sum() / 2e-6
+        assert abs(slope - (r[g][0] * d).sum()) < 1e-6, n
+    cos, sin = np.cos(rng.normal(size=(9, 3))), np.sin(rng.normal(size=(9, 3)))
+    gain = rng.normal(size=6)
+    for inter in (False, True):
+        for gn in (gain, None):
+            f = lambda y, dy=None, gg=gn: R.qk_norm_rope(y, gg, cos, sin, np.arange(9), 1e-3, inter, dy)  # noqa: E731
+            r = f(x["q"], w)
+            d = rng.normal(size=x["q"].shape)
+            slope = ((f(x["q"] + 1e-6 * d)["y"][0] - f(x["q"] - 1e-6 * d)["y"][0]) * w).sum() / 2e-6
+            assert abs(slope - (r["dx"][0] * d).sum()) < 1e-6
+            if gn is not None:
+                d = rng.normal(size=6)
+                slope = ((f(x["q"], None, gn + 1e-6 * d)["y"][0] - f(x["q"], None, gn - 1e-6 * d)["y"][0]) * w).sum() / 2e-6
+                assert abs(slope - (r["dgain"][0] * d).sum()) < 1e-6
