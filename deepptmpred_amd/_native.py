@@ -97,13 +97,23 @@ class AttentionDesc(C.Structure):
                 ("window_right", C.c_int32), ("sinks", C.c_int32), ("training", C.c_int32)]
 
 
-class AttentionBias(C.Structure):
-    _fields_ = [("table", C.c_void_p), ("buckets", C.c_void_p), ("n_buckets", C.c_int32), ("max_distance", C.c_int32)]
+class AttentionArgs(C.Structure):
+    """dptm_attention_args (include/dptm.h)."""
+    _fields_ = [("plan", C.c_void_p), ("plan_dev", C.c_void_p), ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows),
+                ("lse", C.c_void_p), ("table", C.c_void_p), ("buckets", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p), ("dout", Rows), ("dq", Rows), ("dk", Rows), ("dv", Rows),
+                ("dtable", C.c_void_p), ("dtype", C.c_int32), ("device", C.c_int32), ("n_buckets", C.c_int32),
+                ("max_distance", C.c_int32), ("scale", C.c_float)]
 
 
-class NormRopeDesc(C.Structure):
-    _fields_ = [("dtype", C.c_int32), ("head_dim", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
-                ("rows", C.c_int64), ("n_positions", C.c_int32), ("interleaved", C.c_int32), ("eps", C.c_float)]
+class NormRopeArgs(C.Structure):
+    """dptm_norm_rope_args (include/dptm.h)."""
+    _fields_ = [("q", Rows), ("k", Rows), ("q_out", Rows), ("k_out", Rows), ("q_gain", C.c_void_p), ("k_gain", C.c_void_p),
+                ("cosv", C.c_void_p), ("sinv", C.c_void_p), ("positions", C.c_void_p), ("stream", C.c_void_p), ("dq_out", Rows),
+                ("dk_out", Rows), ("dq", Rows), ("dk", Rows), ("dq_gain", C.c_void_p), ("dk_gain", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("rows", C.c_int64), ("dtype", C.c_int32),
+                ("device", C.c_int32), ("head_dim", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("n_positions", C.c_int32), ("interleaved", C.c_int32), ("eps", C.c_float)]
 
 
 _lib: Optional[C.CDLL] = None
@@ -228,22 +238,16 @@ def load_library() -> C.CDLL:
     lib.dptm_sasa.argtypes = [vp, vp, i64, C.c_double, vp, C.c_int32, C.c_int32, vp]
     lib.dptm_sasa_last_error.restype = C.c_char_p
     lib.dptm_sasa_last_error.argtypes = []
-    i32, sz, f32, rp, bp = C.c_int32, C.c_size_t, C.c_float, C.POINTER(Rows), C.POINTER(AttentionBias)
     lib.dptm_attention_plan.restype = C.c_int64
     lib.dptm_attention_plan.argtypes = [C.POINTER(AttentionDesc), vp, vp, vp, i64, vp, i64]
     lib.dptm_attention_workspace.restype = C.c_int64
-    lib.dptm_attention_workspace.argtypes = [vp, i32, i32]
-    lib.dptm_attention_forward.restype = C.c_int
-    lib.dptm_attention_forward.argtypes = [vp, vp, i32, rp, rp, rp, rp, vp, f32, bp, vp, sz, i32, vp]
-    lib.dptm_attention_backward.restype = C.c_int
-    lib.dptm_attention_backward.argtypes = [vp, vp, i32, rp, rp, rp, rp, rp, vp, f32, bp, rp, rp, rp, vp, vp, sz, i32, vp]
-    nd = C.POINTER(NormRopeDesc)
-    lib.dptm_qk_norm_rope_forward.restype = C.c_int
-    lib.dptm_qk_norm_rope_forward.argtypes = [nd, rp, rp, vp, vp, vp, vp, vp, rp, rp, i32, vp]
+    lib.dptm_attention_workspace.argtypes = [vp, C.c_int32, C.c_int32, C.c_int32]
     lib.dptm_qk_norm_rope_workspace.restype = C.c_int64
-    lib.dptm_qk_norm_rope_workspace.argtypes = [nd]
-    lib.dptm_qk_norm_rope_backward.restype = C.c_int
-    lib.dptm_qk_norm_rope_backward.argtypes = [nd, rp, rp, rp, rp, vp, vp, vp, vp, vp, rp, rp, vp, vp, vp, sz, i32, vp]
+    for f in (lib.dptm_attention_forward, lib.dptm_attention_backward, lib.dptm_qk_norm_rope_forward,
+              lib.dptm_qk_norm_rope_workspace, lib.dptm_qk_norm_rope_backward):
+        f.argtypes = [vp]                # the address of an argument block (layers.py packs it)
+    for f in (lib.dptm_attention_forward, lib.dptm_attention_backward, lib.dptm_qk_norm_rope_forward, lib.dptm_qk_norm_rope_backward):
+        f.restype = C.c_int
     lib.dptm_layer_last_error.restype = C.c_char_p
     lib.dptm_layer_last_error.argtypes = []
     _lib = lib

@@ -179,6 +179,16 @@ struct Window { int left, right, sinks; };
 __device__ __forceinline__ bool visible(const Window& w, int far, int key) {
     return (far <= w.right) & ((far >= -w.left) | (key < w.sinks));
 }
+// The same for the 16 keys of a lane's score registers: register r is visible if reg_row(r) - lo < n unsigned, or
+// reg_row(r) < first.  Three or four instructions an element.
+struct LaneMask { int lo, n, first; };
+__device__ __forceinline__ LaneMask lane_mask(const Window& w, int pos, int key0, int key_end) {
+    const int lo = pos - w.left - key0, hi = min(pos + w.right, key_end - 1) - key0;
+    return LaneMask{lo, max(hi - lo + 1, 0), min(w.sinks - key0, hi + 1)};
+}
+__device__ __forceinline__ bool sees(const LaneMask& m, int c) {
+    return ((unsigned)(c - m.lo) < (unsigned)m.n) | (c < m.first);
+}
 // all pairs of positions [pmin, pmax] and keys [j0, j1): every one visible / none visible
 __device__ __forceinline__ bool all_visible(const Window& w, int pmin, int pmax, int j0, int j1) {
     return j1 - 1 - pmin <= w.right && (j0 - pmax >= -w.left || j1 <= w.sinks);
@@ -187,53 +197,43 @@ __device__ __forceinline__ bool none_visible(const Window& w, int pmin, int pmax
     return j0 - pmax > w.right || (j1 - 1 - pmin < -w.left && j0 >= w.sinks);
 }
 
-// ---- products over tiles that hold hidden pairs: the hidden pair's weight is 0, but 0 * inf and 0 * NaN are NaN, so
-// ---- non-finite elements of the A operand are taken out of the product and given back to the lanes with a weight alone
+// A hidden pair's weight is 0, but 0 * inf and 0 * NaN are NaN.  Wavefronts that meet a tile with hidden pairs look whether its
+// rows hold such an element (tile_not_finite), and those that found one do their rows over at the end, pair by pair.
 template <typename T>
 __device__ __forceinline__ bool not_finite(T x) {
     if constexpr (sizeof(T) == 2) return (__builtin_bit_cast(unsigned short, x) & Elem<T>::kExp) == Elem<T>::kExp;
     else return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
 }
-template <typename T>
-__device__ __forceinline__ void mma_guarded(f32x16_a& c, V8<T> a, const V8<T>& b) {
+template <typename T, int D, int ROWS>
+__device__ __forceinline__ bool tile_not_finite(const char* t, int row0, int lane) {
     bool bad = false;
+    const char* p = t + row0 * (Tile<T, D>::kChunks * 16);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) bad |= not_finite(a[e]);
-    if (__ballot(bad) == 0) {
-        mma(c, a, b);
-        return;
+    for (int i = 0; i < (ROWS * Tile<T, D>::kChunks + 63) / 64; ++i) {
+        const int c = i * 64 + lane;
+        if (ROWS * Tile<T, D>::kChunks % 64 && c >= ROWS * Tile<T, D>::kChunks) break;
+        typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+        const vec x = *reinterpret_cast<const vec*>(p + c * 16);
+#pragma unroll
+        for (int e = 0; e < 16 / (int)sizeof(T); ++e) bad |= not_finite(x[e]);
     }
-    V8<T> fine, sign, any, has;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float x = (float)a[e];
-        const bool nf = not_finite(a[e]);
-        fine[e] = nf ? (T)0.f : a[e];
-        sign[e] = (T)(nf ? (x > 0.f ? 1.f : x < 0.f ? -1.f : 0.f) : 0.f);
-        any[e] = (T)(nf ? 1.f : 0.f);
-        has[e] = (T)((float)b[e] != 0.f ? 1.f : 0.f);
-    }
-    mma(c, fine, b);
-    f32x16_a n, m;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) n[r] = m[r] = 0.f;
-    mma(n, sign, has);
-    mma(m, any, has);
-    // only infinities of one sign: that infinity (weights of the forward pass are positive); anything else: NaN
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-        if (m[r] > 0.f) c[r] += n[r] == m[r] ? __builtin_inff() : n[r] == -m[r] ? -__builtin_inff() : __builtin_nanf("");
+    return __ballot(bad) != 0;
 }
-
 // ---- relative position bias in LDS: value per distance in units of log2, one head.  Entries at or below -2^100 hide their
 // ---- pairs, so that a table of the type's lowest value works as a mask does
+// The table goes on for 31 distances on either side with the last value: a lane clamps the distance of its first key of a
+// tile alone (bias_at), and the others lie behind it.
+constexpr int kBiasPad = 31;
+__host__ __device__ inline int bias_room(int reach) { return (2 * reach + 1 + 2 * kBiasPad + 3) & ~3; }   // floats
+__device__ __forceinline__ int bias_at(int far, int reach) { return min(max(far, -reach - kBiasPad), reach) + reach + kBiasPad; }
+__device__ __forceinline__ float bias_value(float v) { return v <= -0x1p100f ? kMinusInf : v * kLog2e; }
 template <typename T>
 __device__ __forceinline__ void load_bias(float* lds, const BiasArgs& b, int heads, int head, int tid, int nt) {
     const T* table = static_cast<const T*>(b.table);
-    for (int i = tid; i < 2 * b.reach + 1; i += nt) {
-        const int k = min(max(b.buckets[i], 0), b.n_buckets - 1);
+    for (int i = tid; i < 2 * b.reach + 1 + 2 * kBiasPad; i += nt) {
+        const int k = min(max(b.buckets[min(max(i - kBiasPad, 0), 2 * b.reach)], 0), b.n_buckets - 1);
         const float v = (float)table[(int64_t)k * heads + head];
-        lds[i] = v <= -0x1p100f ? kMinusInf : v * kLog2e;
+        lds[i] = bias_value(v);
     }
 }
 

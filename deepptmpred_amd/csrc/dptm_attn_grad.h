@@ -16,17 +16,51 @@ namespace {
 // weight of an empty row (lse = -inf) is 0 everywhere: its reference is +inf
 __device__ __forceinline__ float lse_log2(float lse) { return lse == kMinusInf ? __builtin_inff() : lse * kLog2e; }
 
-template <typename T, int D, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
-    constexpr int kBK = kKeysPerTile<T>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
+// A wavefront's rows of dq once more, pair by pair (see tile_not_finite).
+template <typename T, int D, int DT, bool BIAS>
+DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, int item, const T* q, const T* g, int hk, int pos, float ref, float delta, const float* bias, int h) {
+    const QItem& it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[item];
+    const Window win{a.left, a.right, a.sinks};
+#pragma unroll 1
+    for (int i = 0; i < 16 * DT; ++i) acc[i] = 0.f;
+    for (int j = 0; j < it.ke; ++j) {
+        if (j >= it.sink_end && j < it.kb) continue;
+        const T* k = row_ptr<T>(a.k, (int64_t)it.k0 + j, hk);
+        float s = dot_rows<T, D>(q, k) * (a.scale * kLog2e);
+        if constexpr (BIAS) s += bias[bias_at(j - pos, a.bias.reach)];
+        const float ds = __builtin_amdgcn_exp2f(s - ref) * (dot_rows<T, D>(g, row_ptr<T>(a.v, (int64_t)it.k0 + j, hk)) - delta);
+        const bool see = visible(win, j - pos, j);
+#pragma unroll 1
+        for (int i = 0; i < 16 * DT; ++i) acc[i] += see ? (float)(T)ds * (float)k[reg_col<D>(i >> 4, i & 15, h)] : 0.f;
+    }
+}
+
+// Bias gradient, in the kernel that owns queries.  Far tiles (one bucket) are summed in a register.  In a near one the
+// wavefront's rows stand at consecutive positions, so that equal distances are the diagonals of its 32 x 32 dS: it goes to LDS
+// with zeros between its rows, lane l adds diagonal l up (32 reads at a fixed stride, no bank twice) and keeps the
+// sum by distance; what distances share a bucket is left to attn_dtable_kernel.  Adding every element into its bucket by LDS
+// atomics instead took 773 us of a 48-protein batch where this takes a fraction.  POS: rows at positions from a
+// list; each lane then adds into a column of its own per bucket, and no order but the program's enters either.
+constexpr int kShear = 32 * 64 + 32;   // floats: 32 zeros, then 32 rows of 32 values and 32 zeros
+template <bool POS> __host__ __device__ inline int dq_lds_floats(int waves, int n_buckets, int reach) {
+    return POS ? waves * n_buckets * 64 + (bias_room(reach) + 3) / 4 : waves * (kShear + ((2 * reach + 1 + 2 * kFarPad + 3) & ~3));
+}
+
+template <typename T, int D, int NW, bool BIAS, bool POS>
+__global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
+    constexpr int kBK = kKeysPerTile<T, D>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
     constexpr int kBytes = kBK * D * (int)sizeof(T);
     extern __shared__ char smem[];
     float* bias = reinterpret_cast<float*>(smem + 4 * kBytes);
     const int reach = a.bias.reach, nb = a.bias.n_buckets;
-    float* bins = bias + (BIAS ? ((2 * reach + 1 + 3) & ~3) : 0);                        // [NW][nb][64]
-    unsigned char* bucket = reinterpret_cast<unsigned char*>(bins + (BIAS ? NW * nb * 64 : 0));
+    const int words = 2 * reach + 1 + 2 * kFarPad, room = (words + 3) & ~3;
+    float* more = bias + (BIAS ? bias_room(reach) : 0);
+    unsigned char* bucket = reinterpret_cast<unsigned char*>(more + NW * nb * 64);   // POS
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    float* shear = more + w * kShear;                     // not POS
+    float* sums = more + NW * kShear + w * room;          // by distance, from -reach - kFarPad
+    float* bins = more + w * nb * 64;                     // POS: [nb][64]
     const int id = xcd_order(blockIdx.x, gridDim.x);
     const int head = id / a.n_items, item = id - head * a.n_items;
     const QItem it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[item];
@@ -38,27 +72,26 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
     const int row = 32 * w + (lane & 31), rowc = min(row, it.nq - 1);
     const Rows rw = rows_of(a, it.q0, it.pos0, first, last, rowc);
     const int64_t qr = (int64_t)it.q0 + rowc;
-    const char* qrow = static_cast<const char*>(a.q.p) + (qr * a.q.row + (int64_t)head * a.q.head) * (int)sizeof(T);
-    const char* grow = static_cast<const char*>(a.dout.p) + (qr * a.dout.row + (int64_t)head * a.dout.head) * (int)sizeof(T);
-    const char* orow = static_cast<const char*>(a.out.p) + (qr * a.out.row + (int64_t)head * a.out.head) * (int)sizeof(T);
+    const T* qrow = row_ptr<T>(a.q, qr, head);
+    const T* grow = row_ptr<T>(a.dout, qr, head);
+    const T* orow = row_ptr<T>(a.out, qr, head);
     V8<T> q[ST], g[ST];
     float delta = 0.f;
 #pragma unroll
     for (int s = 0; s < ST; ++s) {
-        q[s] = global_frag<T>(qrow, s, h);
-        g[s] = global_frag<T>(grow, s, h);
-        const V8<T> o = global_frag<T>(orow, s, h);
+        q[s] = global_frag<T>(reinterpret_cast<const char*>(qrow), s, h);
+        g[s] = global_frag<T>(reinterpret_cast<const char*>(grow), s, h);
+        const V8<T> o = global_frag<T>(reinterpret_cast<const char*>(orow), s, h);
 #pragma unroll
         for (int e = 0; e < 8; ++e) delta = fmaf((float)g[s][e], (float)o[e], delta);
     }
     delta = half_sum(delta);
-    const float lse = a.lse[(int64_t)head * a.q_rows + qr];
-    const float ref = lse_log2(lse);
+    const float ref = lse_log2(a.lse[(int64_t)head * a.q_rows + qr]);
     if (h == 0 && row < it.nq) a.delta[(int64_t)head * a.q_rows + qr] = delta;
 
     const int hk = head / a.group;
-    const char* kbase = static_cast<const char*>(a.k.p) + ((int64_t)it.k0 * a.k.row + (int64_t)hk * a.k.head) * (int)sizeof(T);
-    const char* vbase = static_cast<const char*>(a.v.p) + ((int64_t)it.k0 * a.v.row + (int64_t)hk * a.v.head) * (int)sizeof(T);
+    const char* kbase = reinterpret_cast<const char*>(row_ptr<T>(a.k, it.k0, hk));
+    const char* vbase = reinterpret_cast<const char*>(row_ptr<T>(a.v, it.k0, hk));
     const int64_t kstep = a.k.row * (int)sizeof(T), vstep = a.v.row * (int)sizeof(T);
     const int ns = (it.sink_end + kBK - 1) / kBK, n = ns + (it.ke - it.kb + kBK - 1) / kBK;
     Stage<T, D, kBK, NW * 64> sk, sv;
@@ -72,11 +105,16 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+    bool over = false;
+    float below = 0.f, above = 0.f;     // dS of distances up to -reach, from reach on
     if (n > 0) fetch(0);
     if constexpr (BIAS) {
         load_bias<T>(bias, a.bias, a.heads, head, tid, NW * 64);
-        for (int i = tid; i < NW * nb * 64; i += NW * 64) bins[i] = 0.f;
-        for (int i = tid; i < 2 * reach + 1; i += NW * 64) bucket[i] = (unsigned char)min(max(a.bias.buckets[i], 0), nb - 1);
+        const int floats = POS ? NW * nb * 64 : NW * (kShear + room);
+        for (int i = tid; i < floats; i += NW * 64) more[i] = 0.f;
+        if constexpr (POS)
+            for (int i = tid; i < bias_room(reach); i += NW * 64)
+                bucket[i] = (unsigned char)min(max(a.bias.buckets[min(max(i - kBiasPad, 0), 2 * reach)], 0), nb - 1);
     }
     if (n > 0) {
         sk.store(smem, tid);
@@ -101,16 +139,16 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
                     mma(s, Tile<T, D>::row_frag(kt, 32 * k + (lane & 31), st, h), q[st]);
                     mma(p, Tile<T, D>::row_frag(vt, 32 * k + (lane & 31), st, h), g[st]);
                 }
-                const bool one = a0 - rw.pmax >= reach || a0 + 31 - rw.pmin <= -reach;   // one bucket for the whole tile
-                const int far0 = a0 + 4 * h - rw.pos + reach;
+                const bool is_above = a0 - rw.pmax >= reach, is_below = a0 + 31 - rw.pmin <= -reach;   // one bucket for the tile
+                const int at = BIAS ? bias_at(a0 + 4 * h - rw.pos, reach) : 0;
                 if constexpr (BIAS) {
-                    if (one) {
-                        const float b = bias[a0 - rw.pmax >= reach ? 2 * reach : 0];
+                    if (is_above | is_below) {
+                        const float b = bias[is_above ? 2 * reach + kBiasPad : 0];
 #pragma unroll
                         for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, b);
                     } else {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, bias[min(max(far0 + reg_row(r), 0), 2 * reach)]);
+                        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, bias[at + reg_row(r)]);
                     }
                 }
 #pragma unroll
@@ -119,40 +157,53 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
                     s[r] = __builtin_amdgcn_exp2f(x) * (p[r] - delta);
                 }
                 if (!full) {
+                    const LaneMask lm = lane_mask(win, rw.pos, a0 + 4 * h, j1);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int j = a0 + 4 * h + reg_row(r);
-                        s[r] = ((j < j1) & visible(win, j - rw.pos, j)) ? s[r] : 0.f;
-                    }
+                    for (int r = 0; r < 16; ++r) s[r] = sees(lm, reg_row(r)) ? s[r] : 0.f;
+                    over |= tile_not_finite<T, D, 32>(kt, 32 * k, lane);
                 }
                 if constexpr (BIAS) {
-                    // a lane adds into a column of its own: no two threads meet, and the order is the program's
-                    float* mine = bins + w * nb * 64 + lane;
-                    const bool counts = row < it.nq;
-                    if (one) {
+                    
+                    if (is_above | is_below) {
                         float sum = 0.f;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) sum += s[r];
-                        const int b = bucket[a0 - rw.pmax >= reach ? 2 * reach : 0];
-                        if (counts) __hip_atomic_fetch_add(mine + b * 64, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                    } else if (counts) {
+                        sum = row < it.nq ? sum : 0.f;
+                        above += is_above ? sum : 0.f;
+                        below += is_above ? 0.f : sum;
+                    } else if constexpr (POS) {
+                        if (row < it.nq) {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int b = bucket[min(max(far0 + reg_row(r), 0), 2 * reach)];
-                            __hip_atomic_fetch_add(mine + b * 64, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                            for (int r = 0; r < 16; ++r)
+                                __hip_atomic_fetch_add(bins + bucket[at + reg_row(r)] * 64 + lane, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                         }
+                    } else {
+                        float* mine = shear + 32 + (lane & 31) * 64 + 4 * h;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            V4<float> y;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) y[e] = row < it.nq ? s[4 * x + e] : 0.f;
+                            *reinterpret_cast<V4<float>*>(mine + 8 * x) = y;
+                        }
+                        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                        __builtin_amdgcn_wave_barrier();
+                        // lane l: key - row = l - 31, which is the distance a0 + l - 31 - (position of row 0)
+                        const float* from = shear + 32 + lane - 31;
+                        float sum = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sum += from[i * 65];
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        __builtin_amdgcn_wave_barrier();
+                        const int dist = a0 + lane - 31 - (it.pos0 + 32 * w) + reach + kFarPad;
+                        if (lane < 63) sums[dist] += sum;
                     }
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const V8<T> b = pack8<T>(s, x);
-                    if (full) {
 #pragma unroll
-                        for (int d = 0; d < DT; ++d) mma(acc[d], Tile<T, D>::col_frag(kt, 32 * k + 16 * x, d, lane), b);
-                    } else {
-#pragma unroll
-                        for (int d = 0; d < DT; ++d) mma_guarded<T>(acc[d], Tile<T, D>::col_frag(kt, 32 * k + 16 * x, d, lane), b);
-                    }
+                    for (int d = 0; d < DT; ++d) mma(acc[d], Tile<T, D>::col_frag(kt, 32 * k + 16 * x, d, lane), b);
                 }
             }
         }
@@ -162,8 +213,13 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
         }
         __syncthreads();
     }
+    if (over) {
+        float t[16 * DT];
+        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, item, qrow, grow, hk, rw.pos, ref, delta, bias, h);
+        take<DT>(acc, t);
+    }
     if (row < it.nq) {
-        T* o = static_cast<T*>(a.dq.p) + ((int64_t)it.q0 + row) * a.dq.row + (int64_t)head * a.dq.head;
+        T* o = const_cast<T*>(row_ptr<T>(a.dq, (int64_t)it.q0 + row, head));
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -175,36 +231,107 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
             }
     }
     if constexpr (BIAS) {
-        for (int b = w; b < nb; b += NW) {
-            float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < NW; ++i) sum += bins[(i * nb + b) * 64 + lane];
+        for (int k = 32; k; k >>= 1) {
+            above += __shfl_xor(above, k);
+            below += __shfl_xor(below, k);
+        }
+        if constexpr (POS) {
+            if (lane == 0) {
+                bins[bucket[2 * reach + kBiasPad] * 64] += above;
+                bins[bucket[0] * 64] += below;
+            }
+            __syncthreads();
+            for (int b = w; b < nb; b += NW) {
+                float sum = 0.f;
 #pragma unroll
-            for (int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
-            if (lane == 0) a.part_bias[((int64_t)head * a.n_items + item) * nb + b] = sum;
+                for (int i = 0; i < NW; ++i) sum += more[(i * nb + b) * 64 + lane];
+#pragma unroll
+                for (int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
+                if (lane == 0) a.part_bias[((int64_t)head * a.n_items + item) * nb + b] = sum;
+            }
+        } else {
+            if (lane == 0) {
+                sums[words - 1] += above;
+                sums[0] += below;
+            }
+            __syncthreads();
+            const float* all = more + NW * kShear;
+            for (int i = tid; i < words; i += NW * 64) {
+                float sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < NW; ++k) sum += all[k * room + i];
+                a.part_bias[((int64_t)head * a.n_items + item) * words + i] = sum;
+            }
         }
     }
 }
 
-// dtable[b][head] from the tiles' sums, in 64 bits and in a fixed order
+// dtable[b][head] from the tiles' sums, in 64 bits and in a fixed order: sixteen wavefronts take tiles, their lanes distances
 template <typename T>
-__global__ __launch_bounds__(256) void attn_dtable_kernel(const float* part, int n_items, int nb, int heads, T* dtable) {
-    __shared__ double sums[256];
-    const int b = blockIdx.x % nb, head = blockIdx.x / nb;
+__global__ __launch_bounds__(1024) void attn_dtable_kernel(AttnArgs a, int n_items) {
+    __shared__ double part[16];
+    const int nb = a.bias.n_buckets, reach = a.bias.reach, b = blockIdx.x % nb, head = blockIdx.x / nb;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     double x = 0.0;
-    for (int i = threadIdx.x; i < n_items; i += 256) x += (double)part[((int64_t)head * n_items + i) * nb + b];
-    sums[threadIdx.x] = x;
-    __syncthreads();
-    for (int k = 128; k; k >>= 1) {
-        if ((int)threadIdx.x < k) sums[threadIdx.x] += sums[threadIdx.x + k];
-        __syncthreads();
+    if (a.has_pos) {
+        for (int i = threadIdx.x; i < n_items; i += 1024) x += (double)a.part_bias[((int64_t)head * n_items + i) * nb + b];
+    } else {
+        const int words = 2 * reach + 1 + 2 * kFarPad;
+        for (int i = lane; i < words; i += 64) {
+            const int of = min(max(a.bias.buckets[min(max(i - kFarPad, 0), 2 * reach)], 0), nb - 1);
+            if (of != b) continue;
+            const float* p = a.part_bias + (int64_t)head * n_items * words + i;
+#pragma unroll 4
+            for (int k = w; k < n_items; k += 16) x += (double)p[(int64_t)k * words];
+        }
     }
-    if (threadIdx.x == 0) dtable[(int64_t)b * heads + head] = (T)(float)sums[0];
+    for (int k = 32; k; k >>= 1) x += __shfl_xor(x, k);
+    if (lane == 0) part[w] = x;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < 16; ++k) x += part[k];
+        static_cast<T*>(a.dtable)[(int64_t)b * a.heads + head] = (T)(float)x;
+    }
 }
 
+// A wavefront's keys of dk and dv once more, pair by pair (see tile_not_finite).
+template <typename T, int D, int DT, bool BIAS>
+DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int item, const T* k, const T* v, int hk, int j, int h) {
+    const KItem& it = reinterpret_cast<const KItem*>(a.plan + a.items_at)[item];
+    const Window win{a.left, a.right, a.sinks};
+    const float c = a.scale * kLog2e;
+#pragma unroll 1
+    for (int i = 0; i < 16 * DT; ++i) dk[i] = dv[i] = 0.f;
+    for (int head = hk * a.group; head < (hk + 1) * a.group; ++head)
+        for (int i = it.qb; i < it.qe; ++i) {
+            const int64_t row = (int64_t)it.q0 + i;
+            const int pos = row_position(a.plan, a.has_pos, a.pos_at, it.pos0, it.q0, i);
+            const T* q = row_ptr<T>(a.q, row, head);
+            const T* g = row_ptr<T>(a.dout, row, head);
+            float s = dot_rows<T, D>(q, k) * c;
+            if constexpr (BIAS) {
+                const int at = min(max(a.bias.buckets[min(max(j - pos, -a.bias.reach), a.bias.reach) + a.bias.reach], 0), a.bias.n_buckets - 1);
+                s += bias_value((float)static_cast<const T*>(a.bias.table)[(int64_t)at * a.heads + head]);
+            }
+            const float p = __builtin_amdgcn_exp2f(s - lse_log2(a.lse[(int64_t)head * a.q_rows + row]));
+            const float ds = p * (dot_rows<T, D>(g, v) - a.delta[(int64_t)head * a.q_rows + row]);
+            const bool see = visible(win, j - pos, j);
+#pragma unroll 1
+            for (int x = 0; x < 16 * DT; ++x) {
+                const int col = reg_col<D>(x >> 4, x & 15, h);
+                dk[x] += see ? (float)(T)ds * (float)q[col] : 0.f;
+                dv[x] += see ? (float)(T)p * (float)g[col] : 0.f;
+            }
+        }
+}
+
+// rows of a tile of queries: fewer where a wavefront's own keys and sums take the registers
+template <typename T, int D> constexpr int kRowsPerTile = sizeof(T) == 2 && D <= 64 ? 64 : 32;
+
 template <typename T, int D, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
-    constexpr int kBQ = kKeysPerTile<T>, NQ = kBQ / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
+__global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
+    constexpr int kBQ = kRowsPerTile<T, D>, NQ = kBQ / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
     constexpr int kBytes = kBQ * D * (int)sizeof(T);
     extern __shared__ char smem[];
     float* rowref = reinterpret_cast<float*>(smem + 4 * kBytes);   // [2][kBQ] each
@@ -224,42 +351,38 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
     const int key = 32 * w + (lane & 31), keyc = min(key, it.nk - 1);
     const int j = it.j0 + key;                                      // index in the sequence
     const int j0 = it.j0 + 32 * w, j1 = it.j0 + min(32 * w + 32, it.nk);
-    const int64_t kr = (int64_t)it.k0 + keyc;
-    const char* krow = static_cast<const char*>(a.k.p) + (kr * a.k.row + (int64_t)hk * a.k.head) * (int)sizeof(T);
-    const char* vrow = static_cast<const char*>(a.v.p) + (kr * a.v.row + (int64_t)hk * a.v.head) * (int)sizeof(T);
+    const T* krow = row_ptr<T>(a.k, (int64_t)it.k0 + keyc, hk);
+    const T* vrow = row_ptr<T>(a.v, (int64_t)it.k0 + keyc, hk);
     V8<T> kf[ST], vf[ST];
 #pragma unroll
     for (int s = 0; s < ST; ++s) {
-        kf[s] = global_frag<T>(krow, s, h);
-        vf[s] = global_frag<T>(vrow, s, h);
+        kf[s] = global_frag<T>(reinterpret_cast<const char*>(krow), s, h);
+        vf[s] = global_frag<T>(reinterpret_cast<const char*>(vrow), s, h);
     }
     f32x16_a dk[DT], dv[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
+    bool over = false;
 
-    const int nt = (it.qe - it.qb + kBQ - 1) / kBQ, n = nt * a.group;
+    const int nt = (it.qe - it.qb + kBQ - 1) / kBQ;
     const int64_t qstep = a.q.row * (int)sizeof(T), gstep = a.dout.row * (int)sizeof(T);
     Stage<T, D, kBQ, NW * 64> sq, sg;
     float nref = 0.f, ndelta = 0.f;
     int npos = 0;
-    auto fetch = [&](int step) {
-        const int g = step / nt, head = hk * a.group + g, i0 = it.qb + (step - g * nt) * kBQ;
+    auto fetch = [&](int head, int t) {
+        const int i0 = it.qb + t * kBQ;
         const int64_t r0 = (int64_t)it.q0 + i0;
         const int valid = it.qe - i0;
-        sq.load(static_cast<const char*>(a.q.p) + (r0 * a.q.row + (int64_t)head * a.q.head) * (int)sizeof(T), qstep, valid, tid);
-        sg.load(static_cast<const char*>(a.dout.p) + (r0 * a.dout.row + (int64_t)head * a.dout.head) * (int)sizeof(T), gstep, valid, tid);
+        sq.load(reinterpret_cast<const char*>(row_ptr<T>(a.q, r0, head)), qstep, valid, tid);
+        sg.load(reinterpret_cast<const char*>(row_ptr<T>(a.dout, r0, head)), gstep, valid, tid);
         if (tid < kBQ) {
-            nref = __builtin_inff();
-            ndelta = 0.f;
-            npos = 0;
-            if (tid < valid) {
-                const int64_t at = (int64_t)head * a.q_rows + r0 + tid;
-                nref = lse_log2(a.lse[at]);
-                ndelta = a.delta[at];
-                npos = row_position(a.plan, a.has_pos, a.pos_at, it.pos0 + i0, it.q0 + i0, tid);
-            }
+            const int64_t at = (int64_t)head * a.q_rows + r0 + min(tid, valid - 1);
+            // rows behind the last weigh nothing: their reference is +inf
+            nref = tid < valid ? lse_log2(a.lse[at]) : __builtin_inff();
+            ndelta = tid < valid ? a.delta[at] : 0.f;
+            npos = a.has_pos ? a.plan[a.pos_at + it.q0 + i0 + min(tid, valid - 1)] : 0;
         }
     };
     auto put = [&](int buf) {
@@ -271,98 +394,109 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
             rowpos[buf * kBQ + tid] = npos;
         }
     };
-    if (n > 0) {
-        fetch(0);
-        if constexpr (BIAS) load_bias<T>(bias, a.bias, a.heads, hk * a.group, tid, NW * 64);
+    for (int head = hk * a.group; head < (hk + 1) * a.group && nt > 0; ++head) {
+        fetch(head, 0);
+        if constexpr (BIAS) load_bias<T>(bias, a.bias, a.heads, head, tid, NW * 64);
         put(0);
-    }
-    __syncthreads();
-    for (int t = 0; t < n; ++t) {
-        if (t + 1 < n) fetch(t + 1);
-        const int buf = t & 1, g = t / nt, i0 = it.qb + (t - g * nt) * kBQ;
-        const char* qt = smem + buf * kBytes;
-        const char* gt = smem + (2 + buf) * kBytes;
-#pragma unroll
-        for (int u = 0; u < NQ; ++u) {
-            const int r0 = i0 + 32 * u;
-            if (!active || r0 >= it.qe) continue;
-            int pmin, pmax;
-            if (a.has_pos) {
-                pmin = a.plan[a.tiles_at + 2 * (it.tile0 + (r0 >> 5))];
-                pmax = a.plan[a.tiles_at + 2 * (it.tile0 + (r0 >> 5)) + 1];
-            } else {
-                pmin = it.pos0 + r0;
-                pmax = it.pos0 + min(r0 + 31, it.nseq - 1);
-            }
-            if (none_visible(win, pmin, pmax, j0, j1)) continue;
-            // rows behind the last weigh nothing by their reference of +inf
-            const bool full = all_visible(win, pmin, pmax, j0, j0 + 32);
-            f32x16_a s, p;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = p[r] = 0.f;
-#pragma unroll
-            for (int st = 0; st < ST; ++st) {
-                mma(s, Tile<T, D>::row_frag(qt, 32 * u + (lane & 31), st, h), kf[st]);
-                mma(p, Tile<T, D>::row_frag(gt, 32 * u + (lane & 31), st, h), vf[st]);
-            }
-            const float* ref = rowref + buf * kBQ + 32 * u + 4 * h;
-            const float* del = rowdelta + buf * kBQ + 32 * u + 4 * h;
-            const int* pos = rowpos + buf * kBQ + 32 * u + 4 * h;
-            if constexpr (BIAS) {
-                if (j0 - pmax >= reach || j0 + 31 - pmin <= -reach) {
-                    const float b = bias[j0 - pmax >= reach ? 2 * reach : 0];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, b);
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, bias[min(max(j - pos[reg_row(r)] + reach, 0), 2 * reach)]);
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float x = BIAS ? s[r] - ref[reg_row(r)] : fmaf(s[r], c, -ref[reg_row(r)]);
-                s[r] = __builtin_amdgcn_exp2f(x);
-            }
-            if (!full) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = visible(win, j - pos[reg_row(r)], j) ? s[r] : 0.f;
-            }
-            // dS of a hidden pair is 0 whatever its operands hold
-#pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] = full ? s[r] * (p[r] - del[reg_row(r)]) : s[r] == 0.f ? 0.f : s[r] * (p[r] - del[reg_row(r)]);
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const V8<T> pw = pack8<T>(s, x), ps = pack8<T>(p, x);
-                if (full) {
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        mma(dv[d], Tile<T, D>::col_frag(gt, 32 * u + 16 * x, d, lane), pw);
-                        mma(dk[d], Tile<T, D>::col_frag(qt, 32 * u + 16 * x, d, lane), ps);
-                    }
-                } else {
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        mma_guarded<T>(dv[d], Tile<T, D>::col_frag(gt, 32 * u + 16 * x, d, lane), pw);
-                        mma_guarded<T>(dk[d], Tile<T, D>::col_frag(qt, 32 * u + 16 * x, d, lane), ps);
-                    }
-                }
-            }
-        }
-        if (t + 1 < n) {
-            put((t + 1) & 1);
-            if constexpr (BIAS) {
-                if ((t + 1) / nt != g) {     // the next query head's bias, once nobody reads this one's
-                    __syncthreads();
-                    load_bias<T>(bias, a.bias, a.heads, hk * a.group + g + 1, tid, NW * 64);
-                }
-            }
-        }
         __syncthreads();
+        for (int t = 0; t < nt; ++t) {
+            if (t + 1 < nt) fetch(head, t + 1);
+            const int buf = t & 1, i0 = it.qb + t * kBQ;
+            const char* qt = smem + buf * kBytes;
+            const char* gt = smem + (2 + buf) * kBytes;
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) {
+                const int r0 = i0 + 32 * u;
+                int pmin = 0, pmax = 0;
+                if (a.has_pos) {
+                    if (r0 < it.qe) {
+                        pmin = a.plan[a.tiles_at + 2 * (it.tile0 + (r0 >> 5))];
+                        pmax = a.plan[a.tiles_at + 2 * (it.tile0 + (r0 >> 5)) + 1];
+                    }
+                } else {
+                    pmin = it.pos0 + r0;
+                    pmax = it.pos0 + min(r0 + 31, it.nseq - 1);
+                }
+                if (active && r0 < it.qe && !none_visible(win, pmin, pmax, j0, j1)) {
+                    const bool full = all_visible(win, pmin, pmax, j0, j0 + 32);
+                    f32x16_a s, p;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = p[r] = 0.f;
+#pragma unroll
+                    for (int st = 0; st < ST; ++st) {
+                        mma(s, Tile<T, D>::row_frag(qt, 32 * u + (lane & 31), st, h), kf[st]);
+                        mma(p, Tile<T, D>::row_frag(gt, 32 * u + (lane & 31), st, h), vf[st]);
+                    }
+                    const float* ref = rowref + buf * kBQ + 32 * u + 4 * h;
+                    const float* del = rowdelta + buf * kBQ + 32 * u + 4 * h;
+                    const int* pos = rowpos + buf * kBQ + 32 * u + 4 * h;
+                    const int far = j - (it.pos0 + r0 + 4 * h);      // to the row of register 0, where the plan lists no positions
+                    if constexpr (BIAS) {
+                        const bool is_above = j0 - pmax >= reach, is_below = j0 + 31 - pmin <= -reach;
+                        if (is_above | is_below) {
+                            const float b = bias[is_above ? 2 * reach + kBiasPad : 0];
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, b);
+                        } else if (a.has_pos) {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, bias[bias_at(j - pos[reg_row(r)], reach)]);
+                        } else {
+                            const float* b = bias + bias_at(far - kBiasPad, reach) + kBiasPad;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, b[-reg_row(r)]);
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float x = BIAS ? s[r] - ref[reg_row(r)] : fmaf(s[r], c, -ref[reg_row(r)]);
+                        s[r] = __builtin_amdgcn_exp2f(x);
+                        p[r] = s[r] * (p[r] - del[reg_row(r)]);
+                    }
+                    if (!full) {
+                        if (a.has_pos) {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                const bool see = visible(win, j - pos[reg_row(r)], j);
+                                s[r] = see ? s[r] : 0.f;
+                                p[r] = see ? p[r] : 0.f;
+                            }
+                        } else {
+                            // row c is seen if far - c <= right and far - c >= -left, or the key is one of the first
+                            const int lo = far - win.right, hi = j < win.sinks ? kFar : far + win.left, m = max(hi - lo + 1, 0);
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                const bool see = (unsigned)(reg_row(r) - lo) < (unsigned)m;
+                                s[r] = see ? s[r] : 0.f;
+                                p[r] = see ? p[r] : 0.f;
+                            }
+                        }
+                        over = over || tile_not_finite<T, D, 32>(qt, 32 * u, lane) || tile_not_finite<T, D, 32>(gt, 32 * u, lane);
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const V8<T> pw = pack8<T>(s, x), ps = pack8<T>(p, x);
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) {
+                            mma(dv[d], Tile<T, D>::col_frag(gt, 32 * u + 16 * x, d, lane), pw);
+                            mma(dk[d], Tile<T, D>::col_frag(qt, 32 * u + 16 * x, d, lane), ps);
+                        }
+                    }
+                }
+            }
+            if (t + 1 < nt) put((t + 1) & 1);
+            __syncthreads();
+        }
+    }
+    if (over) {
+        float x[16 * DT], y[16 * DT];
+        dkv_by_pairs<T, D, DT, BIAS>(kernel_args(), x, y, id - hk * a.n_items, krow, vrow, hk, j, h);
+        take<DT>(dk, x);
+        take<DT>(dv, y);
     }
     if (key < it.nk) {
         if (it.slot < 0) {
-            T* ok = static_cast<T*>(a.dk.p) + ((int64_t)it.k0 + key) * a.dk.row + (int64_t)hk * a.dk.head;
-            T* ov = static_cast<T*>(a.dv.p) + ((int64_t)it.k0 + key) * a.dv.row + (int64_t)hk * a.dv.head;
+            T* ok = const_cast<T*>(row_ptr<T>(a.dk, (int64_t)it.k0 + key, hk));
+            T* ov = const_cast<T*>(row_ptr<T>(a.dv, (int64_t)it.k0 + key, hk));
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -396,39 +530,41 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
     }
 }
 
-// dk, dv of a tile of keys from the parts of several workgroups (grid.y: keys and values)
+// dk, dv of a tile of keys from the parts of several workgroups (grid.y: keys and values, and groups of eight rows)
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_dkv_join_kernel(AttnArgs a, int n_join, int join_at, int tile_keys) {
-    const int kvh = a.heads / a.group;
-    const int hk = blockIdx.x / n_join;
+__global__ __launch_bounds__(kJoinRows * (D / 4)) void attn_dkv_join_kernel(AttnArgs a, int n_join, int join_at, int tile_keys) {
+    const int kvh = a.heads / a.group, hk = blockIdx.x / n_join, which = blockIdx.y & 1;
     const Join jn = reinterpret_cast<const Join*>(a.plan + join_at)[blockIdx.x - hk * n_join];
-    const Strided& to = blockIdx.y ? a.dv : a.dk;
-    for (int i = threadIdx.x; i < jn.n * (D / 4); i += 256) {
-        const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-        V4<float> x{0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < jn.slots; ++k)
-            x += *reinterpret_cast<const V4<float>*>(a.part_o + ((((int64_t)(jn.slot0 + k) * kvh + hk) * 2 + blockIdx.y) * tile_keys + r) * D + d);
-        V4<T> y;
+    const int r = (blockIdx.y >> 1) * kJoinRows + threadIdx.x / (D / 4), d = (threadIdx.x % (D / 4)) * 4;
+    if (r >= jn.n) return;
+    V4<float> x{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int k = 0; k < jn.slots; ++k)
+        x += *reinterpret_cast<const V4<float>*>(a.part_o + ((((int64_t)(jn.slot0 + k) * kvh + hk) * 2 + which) * tile_keys + r) * D + d);
+    V4<T> y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (T)x[e];
-        *reinterpret_cast<V4<T>*>(static_cast<T*>(to.p) + ((int64_t)jn.row0 + r) * to.row + (int64_t)hk * to.head + d) = y;
-    }
+    for (int e = 0; e < 4; ++e) y[e] = (T)x[e];
+    *reinterpret_cast<V4<T>*>(const_cast<T*>(row_ptr<T>(which ? a.dv : a.dk, (int64_t)jn.row0 + r, hk)) + d) = y;
 }
 
+template <typename T, int D, int NW>
+hipError_t dq_waves(const AttnArgs& a, hipStream_t s) {
+    const int64_t blocks = (int64_t)a.n_items * a.heads;
+    const size_t lds = 4 * kKeysPerTile<T, D> * D * sizeof(T) + bias_floats(a) * 4;
+    if (!a.bias.table) return start(attn_dq_kernel<T, D, NW, false, false>, blocks, NW * 64, lds, s, a);
+    if (a.has_pos)
+        return start(attn_dq_kernel<T, D, NW, true, true>, blocks, NW * 64, lds + 4 * dq_lds_floats<true>(NW, a.bias.n_buckets, a.bias.reach), s, a);
+    return start(attn_dq_kernel<T, D, NW, true, false>, blocks, NW * 64, lds + 4 * dq_lds_floats<false>(NW, a.bias.n_buckets, a.bias.reach), s, a);
+}
 template <typename T, int D>
 hipError_t dq_dim(const AttnArgs& a, int waves, hipStream_t s) {
-    const int64_t blocks = (int64_t)a.n_items * a.heads;
-    size_t lds = 4 * kKeysPerTile<T> * D * sizeof(T);
-    if (a.bias.table) lds += bias_floats(a) * 4 + (size_t)waves * a.bias.n_buckets * 64 * 4 + bias_floats(a);
-    if (waves == 2)
-        return a.bias.table ? start(attn_dq_kernel<T, D, 2, true>, blocks, 128, lds, s, a) : start(attn_dq_kernel<T, D, 2, false>, blocks, 128, lds, s, a);
-    return a.bias.table ? start(attn_dq_kernel<T, D, 4, true>, blocks, 256, lds, s, a) : start(attn_dq_kernel<T, D, 4, false>, blocks, 256, lds, s, a);
+    return waves == 2 ? dq_waves<T, D, 2>(a, s) : dq_waves<T, D, 4>(a, s);
 }
 
 template <typename T, int D>
 hipError_t dkv_dim(const AttnArgs& a, int waves, hipStream_t s) {
     const int64_t blocks = (int64_t)a.n_items * (a.heads / a.group);
-    const size_t lds = 4 * kKeysPerTile<T> * D * sizeof(T) + 6 * kKeysPerTile<T> * 4 + bias_floats(a) * 4;
+    const size_t lds = 4 * kRowsPerTile<T, D> * D * sizeof(T) + 6 * kRowsPerTile<T, D> * 4 + bias_floats(a) * 4;
     if (waves == 2)
         return a.bias.table ? start(attn_dkv_kernel<T, D, 2, true>, blocks, 128, lds, s, a) : start(attn_dkv_kernel<T, D, 2, false>, blocks, 128, lds, s, a);
     return a.bias.table ? start(attn_dkv_kernel<T, D, 4, true>, blocks, 256, lds, s, a) : start(attn_dkv_kernel<T, D, 4, false>, blocks, 256, lds, s, a);
@@ -437,7 +573,8 @@ hipError_t dkv_dim(const AttnArgs& a, int waves, hipStream_t s) {
 template <typename T, int D>
 hipError_t dkv_join_dim(const AttnArgs& a, int n_join, int join_at, int tile_keys, hipStream_t s) {
     if (n_join == 0) return hipSuccess;
-    hipLaunchKernelGGL((attn_dkv_join_kernel<T, D>), dim3((unsigned)n_join * (a.heads / a.group), 2), dim3(256), 0, s, a, n_join, join_at, tile_keys);
+    hipLaunchKernelGGL((attn_dkv_join_kernel<T, D>), dim3((unsigned)n_join * (a.heads / a.group), 2 * (tile_keys / kJoinRows)),
+                       dim3(kJoinRows * (D / 4)), 0, s, a, n_join, join_at, tile_keys);
     return hipGetLastError();
 }
 
@@ -457,18 +594,11 @@ hipError_t dkv_join_dim(const AttnArgs& a, int n_join, int join_at, int tile_key
     hipError_t attn_forward_##NAME(const AttnArgs& a, int dim, int mode, hipStream_t s) { return DPTM_ATTN_BY_DIM(forward_dim, a, mode, s); } \
     hipError_t attn_dq_##NAME(const AttnArgs& a, int dim, int waves, hipStream_t s) { return DPTM_ATTN_BY_DIM(dq_dim, a, waves, s); }         \
     hipError_t attn_dkv_##NAME(const AttnArgs& a, int dim, int waves, hipStream_t s) { return DPTM_ATTN_BY_DIM(dkv_dim, a, waves, s); }       \
-    hipError_t attn_join_##NAME(const AttnArgs& a, int dim, int n, int at, hipStream_t s) {                                \
-        const int64_t blocks = (int64_t)n * a.heads;                                                                       \
-        return dim == 16 ? start(attn_join_kernel<E, 16>, blocks, 256, 0, s, a, n, at)                                     \
-             : dim == 32 ? start(attn_join_kernel<E, 32>, blocks, 256, 0, s, a, n, at)                                     \
-             : dim == 64 ? start(attn_join_kernel<E, 64>, blocks, 256, 0, s, a, n, at)                                     \
-                         : start(attn_join_kernel<E, 128>, blocks, 256, 0, s, a, n, at);                                   \
-    }                                                                                                                      \
+    hipError_t attn_join_##NAME(const AttnArgs& a, int dim, int n, int at, hipStream_t s) { return DPTM_ATTN_BY_DIM(join_dim, a, n, at, s); } \
     hipError_t attn_dkv_join_##NAME(const AttnArgs& a, int dim, int n, int at, int keys, hipStream_t s) {                  \
         return DPTM_ATTN_BY_DIM(dkv_join_dim, a, n, at, keys, s);                                                          \
     }                                                                                                                      \
     hipError_t attn_dtable_##NAME(const AttnArgs& a, int n_items, hipStream_t s) {                                         \
-        return start(attn_dtable_kernel<E>, (int64_t)a.bias.n_buckets * a.heads, 256, 0, s, (const float*)a.part_bias, n_items, \
-                     a.bias.n_buckets, a.heads, static_cast<E*>(a.dtable));                                                \
+        return start(attn_dtable_kernel<E>, (int64_t)a.bias.n_buckets * a.heads, 1024, 0, s, a, n_items);                  \
     }                                                                                                                      \
     }

@@ -18,7 +18,8 @@ template <typename T> constexpr float kShift = sizeof(T) == 2 && Elem<T>::kExp =
 template <> constexpr float kShift<float> = 0.f;
 constexpr float kLazy = 4.f;
 
-template <typename T> constexpr int kKeysPerTile = sizeof(T) == 2 ? 64 : 32;
+// keys of a tile in LDS: 64 where the registers that carry the next tile allow it
+template <typename T, int D> constexpr int kKeysPerTile = sizeof(T) == 2 && D <= 64 ? 64 : 32;
 
 // what a wavefront knows of its 32 queries
 struct Rows {
@@ -34,24 +35,23 @@ __device__ __forceinline__ void softmax_step(f32x16_a (&s)[NK], f32x16_a (&acc)[
         for (int k = 0; k < NK; ++k) {
             const int a = j0 + 32 * k, z = a + 31;
             if (a - w.pmax >= reach || z - w.pmin <= -reach) {   // one value for the whole tile
-                const float b = bias[a - w.pmax >= reach ? 2 * reach : 0];
+                const float b = bias[a - w.pmax >= reach ? 2 * reach + kBiasPad : 0];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[k][r] = fmaf(s[k][r], c, b);
             } else {
-                const int far0 = a + 4 * h - w.pos + reach;
+                const float* b = bias + bias_at(a + 4 * h - w.pos, reach);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[k][r] = fmaf(s[k][r], c, bias[min(max(far0 + reg_row(r), 0), 2 * reach)]);
+                for (int r = 0; r < 16; ++r) s[k][r] = fmaf(s[k][r], c, b[reg_row(r)]);
             }
         }
     }
     if (!full) {
 #pragma unroll
-        for (int k = 0; k < NK; ++k)
+        for (int k = 0; k < NK; ++k) {
+            const LaneMask lm = lane_mask(win, w.pos, j0 + 32 * k + 4 * h, j1);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int j = j0 + 32 * k + 4 * h + reg_row(r);
-                s[k][r] = ((j < j1) & visible(win, j - w.pos, j)) ? s[k][r] : kMinusInf;
-            }
+            for (int r = 0; r < 16; ++r) s[k][r] = sees(lm, reg_row(r)) ? s[k][r] : kMinusInf;
+        }
     }
     float mx = s[0][0];
 #pragma unroll
@@ -85,26 +85,79 @@ __device__ __forceinline__ void softmax_step(f32x16_a (&s)[NK], f32x16_a (&acc)[
 
 // acc += V^T P^T over 32 NK keys of a tile in LDS
 template <typename T, int D, int NK, int DT>
-__device__ __forceinline__ void weighted_values(f32x16_a (&acc)[DT], const f32x16_a (&p)[NK], const char* vt, bool full, int lane) {
-    if (full) {
+__device__ __forceinline__ void weighted_values(f32x16_a (&acc)[DT], const f32x16_a (&p)[NK], const char* vt, int lane) {
 #pragma unroll
-        for (int k = 0; k < NK; ++k)
+    for (int k = 0; k < NK; ++k)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const V8<T> b = pack8<T>(p[k], s);
+        for (int s = 0; s < 2; ++s) {
+            const V8<T> b = pack8<T>(p[k], s);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) mma(acc[d], Tile<T, D>::col_frag(vt, 32 * k + 16 * s, d, lane), b);
-            }
-    } else {
+            for (int d = 0; d < DT; ++d) mma(acc[d], Tile<T, D>::col_frag(vt, 32 * k + 16 * s, d, lane), b);
+        }
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_ptr(const Strided& t, int64_t row, int head) {
+    return static_cast<const T*>(t.p) + row * t.row + (int64_t)head * t.head;
+}
+template <typename T, int D>
+__device__ __forceinline__ float dot_rows(const T* a, const T* b) {
+    float s = 0.f;
+    for (int d = 0; d < D; d += 8) {
+        const V8<T> x = *reinterpret_cast<const V8<T>*>(a + d), y = *reinterpret_cast<const V8<T>*>(b + d);
 #pragma unroll
-        for (int k = 0; k < NK; ++k)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const V8<T> b = pack8<T>(p[k], s);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) mma_guarded<T>(acc[d], Tile<T, D>::col_frag(vt, 32 * k + 16 * s, d, lane), b);
-            }
+        for (int e = 0; e < 8; ++e) s = fmaf((float)x[e], (float)y[e], s);
     }
+    return s;
+}
+// column of the head that accumulator register r of tile d holds in half-wave h (head dimension 16: half a tile)
+template <int D> __device__ __forceinline__ int reg_col(int d, int r, int h) { return (32 * d + reg_row(r) + 4 * h) & (D - 1); }
+
+// The functions that do rows over are out of line and keep their sums in private memory: such rows are rare, and the kernels
+// that call them shall not pay with registers.  They are handed the kernel's arguments where the launch put them, because a
+// reference to the kernel's copy would move that into private memory too.
+__device__ __forceinline__ const AttnArgs& kernel_args() {
+    return *(const AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+}
+#define DPTM_COLD __device__ __attribute__((noinline))
+
+// The rows of a wavefront once more, pair by pair: hidden pairs do not enter.  For tiles `first`, `first + every`, ... of `keys` keys.
+template <typename T, int D, int DT, bool BIAS>
+DPTM_COLD void forward_by_pairs(const AttnArgs& a, float* acc, float* ml, int item, const T* q, int hk, int pos, int first, int every, int keys,
+                                const float* bias, int h) {
+    const QItem& it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[item];
+    const Window win{a.left, a.right, a.sinks};
+    const float c = a.scale * kLog2e;
+    const int ns = (it.sink_end + keys - 1) / keys, n = ns + (it.ke - it.kb + keys - 1) / keys;
+#pragma unroll 1
+    for (int i = 0; i < 16 * DT; ++i) acc[i] = 0.f;
+    float m = kMinusInf, l = 0.f;
+    for (int t = first; t < n; t += every) {
+        const int j0 = t < ns ? t * keys : it.kb + (t - ns) * keys, j1 = min(j0 + keys, t < ns ? it.sink_end : it.ke);
+        for (int j = j0; j < j1; ++j) {
+            float s = dot_rows<T, D>(q, row_ptr<T>(a.k, (int64_t)it.k0 + j, hk)) * c;
+            if constexpr (BIAS) s += bias[bias_at(j - pos, a.bias.reach)];
+            s = visible(win, j - pos, j) ? s : kMinusInf;
+            const float top = fmaxf(m, s), f = m == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(m - top);
+            const float p = s == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(s - top + kShift<T>);
+            m = top;
+            l = l * f + p;
+            const T* v = row_ptr<T>(a.v, (int64_t)it.k0 + j, hk);
+#pragma unroll 1
+            for (int i = 0; i < 16 * DT; ++i)
+                acc[i] = acc[i] * f + (s == kMinusInf ? 0.f : (float)(T)p * (float)v[reg_col<D>(i >> 4, i & 15, h)]);
+        }
+    }
+    ml[0] = m;
+    ml[1] = h ? 0.f : l;      // the caller adds the halves
+}
+// accumulators <-> what the functions above leave
+template <int DT>
+__device__ __forceinline__ void take(f32x16_a (&acc)[DT], const float* from) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] = from[16 * d + r];
 }
 
 __device__ __forceinline__ Rows rows_of(const AttnArgs& a, int q0, int pos0, int first, int last, int mine) {
@@ -123,8 +176,8 @@ __device__ __forceinline__ Rows rows_of(const AttnArgs& a, int q0, int pos0, int
 
 // ---- many queries: NW wavefronts of 32 queries share tiles of keys and values in LDS (two buffers, one barrier a tile)
 template <typename T, int D, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64) void attn_fwd_wide_kernel(AttnArgs a) {
-    constexpr int kBK = kKeysPerTile<T>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
+__global__ __launch_bounds__(NW * 64, 2) void attn_fwd_wide_kernel(AttnArgs a) {
+    constexpr int kBK = kKeysPerTile<T, D>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
     constexpr int kBytes = kBK * D * (int)sizeof(T);
     extern __shared__ char smem[];
     float* bias = reinterpret_cast<float*>(smem + 4 * kBytes);
@@ -163,6 +216,7 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_wide_kernel(AttnArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
     float m = kMinusInf, l = 0.f;
+    bool over = false;
 
     if (n > 0) fetch(0);
     if constexpr (BIAS) load_bias<T>(bias, a.bias, a.heads, head, tid, NW * 64);
@@ -187,13 +241,21 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_wide_kernel(AttnArgs a) {
                 for (int st = 0; st < ST; ++st) mma(s[k], Tile<T, D>::row_frag(kt, 32 * k + (lane & 31), st, h), q[st]);
             }
             softmax_step<T, NK, DT, BIAS>(s, acc, m, l, c, rw, win, j0, j1, full, bias, a.bias.reach, h);
-            weighted_values<T, D, NK, DT>(acc, s, vt, full, lane);
+            weighted_values<T, D, NK, DT>(acc, s, vt, lane);
+            if (!full) over |= tile_not_finite<T, D, kBK>(vt, 0, lane);
         }
         if (t + 1 < n) {
             sk.store(smem + ((t + 1) & 1) * kBytes, tid);
             sv.store(smem + (2 + ((t + 1) & 1)) * kBytes, tid);
         }
         __syncthreads();
+    }
+    if (over) {
+        float t[16 * DT], ml[2];
+        forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, ml, id - head * a.n_items, row_ptr<T>(a.q, (int64_t)it.q0 + rowc, head), hk, rw.pos, 0, 1, kBK,
+                                         bias, h);
+        take<DT>(acc, t);
+        m = ml[0], l = ml[1];
     }
     if (row < it.nq) {
         l = half_sum(l);
@@ -212,38 +274,36 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_wide_kernel(AttnArgs a) {
     }
 }
 
-// ---- few queries: the four wavefronts of a workgroup hold the SAME 32 queries and take every fourth tile of 32 keys, and a
-// ---- long range of keys is cut over workgroups as well; the parts meet in LDS, those of several workgroups in attn_join_kernel
+// ---- few queries: the four wavefronts of a workgroup hold the SAME 32 rows and take every fourth tile of 32 keys, and a long
+// ---- range of keys is cut over workgroups as well; the parts meet in LDS, those of several workgroups in attn_join_kernel.
+// ---- A row is a query of one of `pack` heads that share their keys, so that keys are read once for all of them
 template <typename T, int D, bool BIAS>
-__global__ __launch_bounds__(256) void attn_fwd_split_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void attn_fwd_split_kernel(AttnArgs a) {
     constexpr int NW = 4, DT = D >= 32 ? D / 32 : 1, ST = D / 16, kPad = D + 4;
     constexpr int kBytes = 32 * D * (int)sizeof(T);
     extern __shared__ char smem[];
     float* ml = reinterpret_cast<float*>(smem);                 // [NW][32][2]
-    float* bias = ml + NW * 64;
-    char* tiles = smem + (NW * 64 + (BIAS ? ((2 * a.bias.reach + 1 + 3) & ~3) : 0)) * 4;
+    float* bias = ml + NW * 64;                                 // [pack][bias_room]
+    const int room = BIAS ? bias_room(a.bias.reach) : 0;
+    char* tiles = smem + (NW * 64 + a.pack * room) * 4;
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int id = xcd_order(blockIdx.x, gridDim.x);
-    const int head = id / a.n_items;
-    const QItem it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[id - head * a.n_items];
+    const int pack = a.pack, head0 = id / a.n_items * pack;
+    const QItem it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[id - id / a.n_items * a.n_items];
     const Window win{a.left, a.right, a.sinks};
     const float c = a.scale * kLog2e;
-    const int row = lane & 31, rowc = min(row, it.nq - 1);
-    const Rows rw = rows_of(a, it.q0, it.pos0, 0, it.nq - 1, rowc);
-    const char* qrow = static_cast<const char*>(a.q.p) + (((int64_t)it.q0 + rowc) * a.q.row + (int64_t)head * a.q.head) * (int)sizeof(T);
+    const int rows = it.nq * pack, row = min(lane & 31, rows - 1), query = row / pack, head = head0 + row - query * pack;
+    const Rows rw = rows_of(a, it.q0, it.pos0, 0, it.nq - 1, query);
+    const T* qrow = row_ptr<T>(a.q, (int64_t)it.q0 + query, head);
     V8<T> q[ST];
 #pragma unroll
-    for (int s = 0; s < ST; ++s) q[s] = global_frag<T>(qrow, s, h);
-    const int hk = head / a.group;
-    const char* kbase = static_cast<const char*>(a.k.p) + ((int64_t)it.k0 * a.k.row + (int64_t)hk * a.k.head) * (int)sizeof(T);
-    const char* vbase = static_cast<const char*>(a.v.p) + ((int64_t)it.k0 * a.v.row + (int64_t)hk * a.v.head) * (int)sizeof(T);
+    for (int s = 0; s < ST; ++s) q[s] = global_frag<T>(reinterpret_cast<const char*>(qrow), s, h);
+    const int hk = head0 / a.group;
+    const char* kbase = reinterpret_cast<const char*>(row_ptr<T>(a.k, it.k0, hk));
+    const char* vbase = reinterpret_cast<const char*>(row_ptr<T>(a.v, it.k0, hk));
     const int64_t kstep = a.k.row * (int)sizeof(T), vstep = a.v.row * (int)sizeof(T);
     const int ns = (it.sink_end + 31) / 32, n = ns + (it.ke - it.kb + 31) / 32;
-    if constexpr (BIAS) {
-        load_bias<T>(bias, a.bias, a.heads, head, tid, 256);
-        __syncthreads();
-    }
     V8<T> kf[ST];
     Stage<T, D, 32, 64> sv;
     char* vt = tiles + w * kBytes;
@@ -254,13 +314,19 @@ __global__ __launch_bounds__(256) void attn_fwd_split_kernel(AttnArgs a) {
         for (int s = 0; s < ST; ++s) kf[s] = global_frag<T>(krow, s, h);
         sv.load(vbase + j0 * vstep, vstep, j1 - j0, lane);
     };
+    if (w < n) fetch(w);
+    if constexpr (BIAS) {
+        for (int p = 0; p < pack; ++p) load_bias<T>(bias + p * room, a.bias, a.heads, head0 + p, tid, 256);
+        __syncthreads();
+        bias += (head - head0) * room;
+    }
     f32x16_a acc[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
     float m = kMinusInf, l = 0.f;
-    if (w < n) fetch(w);
+    bool over = false;
     for (int t = w; t < n; t += NW) {
         const int j0 = t < ns ? t * 32 : it.kb + (t - ns) * 32, j1 = min(j0 + 32, t < ns ? it.sink_end : it.ke);
         f32x16_a s[1];
@@ -275,7 +341,14 @@ __global__ __launch_bounds__(256) void attn_fwd_split_kernel(AttnArgs a) {
         __builtin_amdgcn_wave_barrier();
         const bool full = j1 - j0 == 32 && all_visible(win, rw.pmin, rw.pmax, j0, j1);
         softmax_step<T, 1, DT, BIAS>(s, acc, m, l, c, rw, win, j0, j1, full, bias, a.bias.reach, h);
-        weighted_values<T, D, 1, DT>(acc, s, vt, full, lane);
+        weighted_values<T, D, 1, DT>(acc, s, vt, lane);
+        if (!full) over |= tile_not_finite<T, D, 32>(vt, 0, lane);
+    }
+    if (over) {
+        float t[16 * DT], x[2];
+        forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, x, id - id / a.n_items * a.n_items, qrow, hk, rw.pos, w, NW, 32, bias, h);
+        take<DT>(acc, t);
+        m = x[0], l = x[1];
     }
     l = half_sum(l);
     if (h == 0) {
@@ -298,9 +371,8 @@ __global__ __launch_bounds__(256) void attn_fwd_split_kernel(AttnArgs a) {
             *reinterpret_cast<V4<float>*>(o + (w * 32 + (lane & 31)) * kPad + 32 * d + 8 * g + 4 * h) = x;
         }
     __syncthreads();
-    for (int i = tid; i < 32 * (D / 4); i += 256) {
-        const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-        if (r >= it.nq) break;
+    for (int i = tid; i < rows * (D / 4); i += 256) {
+        const int r = i / (D / 4), d = (i % (D / 4)) * 4, qi = r / pack, hd = head0 + r - qi * pack;
         float t = kMinusInf, sum = 0.f;
 #pragma unroll
         for (int k = 0; k < NW; ++k) t = fmaxf(t, ml[(k * 32 + r) * 2]);
@@ -317,10 +389,10 @@ __global__ __launch_bounds__(256) void attn_fwd_split_kernel(AttnArgs a) {
             V4<T> y;
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * inv);
-            *reinterpret_cast<V4<T>*>(static_cast<T*>(a.out.p) + ((int64_t)it.q0 + r) * a.out.row + (int64_t)head * a.out.head + d) = y;
-            if (d == 0) a.lse[(int64_t)head * a.q_rows + it.q0 + r] = t == kMinusInf ? kMinusInf : (t - kShift<T> + __log2f(sum)) * kLn2;
+            *reinterpret_cast<V4<T>*>(const_cast<T*>(row_ptr<T>(a.out, (int64_t)it.q0 + qi, hd)) + d) = y;
+            if (d == 0) a.lse[(int64_t)hd * a.q_rows + it.q0 + qi] = t == kMinusInf ? kMinusInf : (t - kShift<T> + __log2f(sum)) * kLn2;
         } else {
-            const int64_t at = ((int64_t)it.slot * a.heads + head) * 32 + r;
+            const int64_t at = ((int64_t)it.slot * (a.heads / pack) + head0 / pack) * 32 + r;
             *reinterpret_cast<V4<float>*>(a.part_o + at * D + d) = x;
             if (d == 0) {
                 a.part_ml[at * 2] = t;
@@ -330,35 +402,35 @@ __global__ __launch_bounds__(256) void attn_fwd_split_kernel(AttnArgs a) {
     }
 }
 
-// the parts of one tile of rows from several workgroups, one thread for four columns
+// the parts of one tile of rows from several workgroups: eight rows a block, one thread for four columns
+constexpr int kJoinRows = 8;
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int n_join, int join_at) {
-    const int head = blockIdx.x / n_join;
-    const Join jn = reinterpret_cast<const Join*>(a.plan + join_at)[blockIdx.x - head * n_join];
-    for (int i = threadIdx.x; i < 32 * (D / 4); i += 256) {
-        const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-        if (r >= jn.n) break;
-        float m = kMinusInf, l = 0.f;
-        V4<float> x{0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < jn.slots; ++k) {
-            const int64_t at = ((int64_t)(jn.slot0 + k) * a.heads + head) * 32 + r;
-            const float mk = a.part_ml[at * 2], lk = a.part_ml[at * 2 + 1];
-            const V4<float> xk = *reinterpret_cast<const V4<float>*>(a.part_o + at * D + d);
-            const float top = fmaxf(m, mk);
-            const float f0 = m == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(m - top);
-            const float f1 = mk == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(mk - top);
-            m = top;
-            l = l * f0 + lk * f1;
+__global__ __launch_bounds__(kJoinRows * (D / 4)) void attn_join_kernel(AttnArgs a, int n_join, int join_at) {
+    const int hp = blockIdx.x / n_join, pack = a.pack, heads = a.heads / pack;
+    const Join jn = reinterpret_cast<const Join*>(a.plan + join_at)[blockIdx.x - hp * n_join];
+    const int r = blockIdx.y * kJoinRows + threadIdx.x / (D / 4), d = (threadIdx.x % (D / 4)) * 4;
+    if (r >= jn.n * pack) return;
+    const int64_t first = ((int64_t)jn.slot0 * heads + hp) * 32 + r, next = (int64_t)heads * 32;
+    float m = kMinusInf, l = 0.f;
+    for (int k = 0; k < jn.slots; ++k) m = fmaxf(m, a.part_ml[(first + k * next) * 2]);
+    V4<float> x{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int k = 0; k < jn.slots; ++k) {
+        const int64_t at = first + k * next;
+        const float mk = a.part_ml[at * 2], lk = a.part_ml[at * 2 + 1];
+        const V4<float> xk = *reinterpret_cast<const V4<float>*>(a.part_o + at * D + d);
+        const float f = mk == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(mk - m);
+        l += lk * f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = x[e] * f0 + xk[e] * f1;
-        }
-        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-        V4<T> y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * inv);
-        *reinterpret_cast<V4<T>*>(static_cast<T*>(a.out.p) + ((int64_t)jn.row0 + r) * a.out.row + (int64_t)head * a.out.head + d) = y;
-        if (d == 0) a.lse[(int64_t)head * a.q_rows + jn.row0 + r] = m == kMinusInf ? kMinusInf : (m - kShift<T> + __log2f(l)) * kLn2;
+        for (int e = 0; e < 4; ++e) x[e] += xk[e] * f;
     }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    V4<T> y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * inv);
+    const int qi = r / pack, head = hp * pack + r - qi * pack;
+    *reinterpret_cast<V4<T>*>(const_cast<T*>(row_ptr<T>(a.out, (int64_t)jn.row0 + qi, head)) + d) = y;
+    if (d == 0) a.lse[(int64_t)head * a.q_rows + jn.row0 + qi] = m == kMinusInf ? kMinusInf : (m - kShift<T> + __log2f(l)) * kLn2;
 }
 
 template <typename K>
@@ -374,23 +446,32 @@ hipError_t start(K kernel, int64_t blocks, int threads, size_t lds, hipStream_t 
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, s, args...);
     return hipGetLastError();
 }
-inline size_t bias_floats(const AttnArgs& a) { return a.bias.table ? (size_t)((2 * a.bias.reach + 1 + 3) & ~3) : 0; }
+inline size_t bias_floats(const AttnArgs& a) { return a.bias.table ? (size_t)bias_room(a.bias.reach) : 0; }
 
 template <typename T, int D>
 hipError_t forward_dim(const AttnArgs& a, int mode, hipStream_t s) {
-    const int64_t blocks = (int64_t)a.n_items * a.heads;
+    int64_t blocks = (int64_t)a.n_items * a.heads;
     if (mode == kSplitKeys) {
+        blocks /= a.pack;
         const size_t v = 4 * 32 * D * sizeof(T), o = 4 * 32 * (D + 4) * 4;
-        const size_t lds = (4 * 64 + bias_floats(a)) * 4 + (v > o ? v : o);
+        const size_t lds = (4 * 64 + a.pack * bias_floats(a)) * 4 + (v > o ? v : o);
         return a.bias.table ? start(attn_fwd_split_kernel<T, D, true>, blocks, 256, lds, s, a)
                             : start(attn_fwd_split_kernel<T, D, false>, blocks, 256, lds, s, a);
     }
-    const size_t lds = 4 * kKeysPerTile<T> * D * sizeof(T) + bias_floats(a) * 4;
+    const size_t lds = 4 * kKeysPerTile<T, D> * D * sizeof(T) + bias_floats(a) * 4;
     if (mode == kWide64)
         return a.bias.table ? start(attn_fwd_wide_kernel<T, D, 2, true>, blocks, 128, lds, s, a)
                             : start(attn_fwd_wide_kernel<T, D, 2, false>, blocks, 128, lds, s, a);
     return a.bias.table ? start(attn_fwd_wide_kernel<T, D, 4, true>, blocks, 256, lds, s, a)
                         : start(attn_fwd_wide_kernel<T, D, 4, false>, blocks, 256, lds, s, a);
+}
+
+template <typename T, int D>
+hipError_t join_dim(const AttnArgs& a, int n_join, int join_at, hipStream_t s) {
+    if (n_join == 0) return hipSuccess;
+    hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3((unsigned)(n_join * (a.heads / a.pack)), 32 / kJoinRows), dim3(kJoinRows * (D / 4)), 0, s, a,
+                       n_join, join_at);
+    return hipGetLastError();
 }
 
 }  // namespace

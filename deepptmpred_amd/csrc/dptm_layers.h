@@ -12,7 +12,7 @@ enum PlanWord {
     kPlanMagicAt = 0, kPlanWords, kPlanHeads, kPlanKvHeads, kPlanHeadDim, kPlanLeft, kPlanRight, kPlanSinks, kPlanSeqs,
     kPlanQRows, kPlanKRows, kPlanMode, kPlanFwd, kPlanFwdAt, kPlanSlots, kPlanJoin, kPlanJoinAt, kPlanDq, kPlanDqAt,
     kPlanDqWaves, kPlanDkv, kPlanDkvAt, kPlanDkvWaves, kPlanDkvSlots, kPlanDkvJoin, kPlanDkvJoinAt, kPlanHasPos, kPlanPosAt,
-    kPlanTiles, kPlanTilesAt, kPlanCheck, kPlanHeader = 32
+    kPlanTiles, kPlanTilesAt, kPlanPack, kPlanCheck, kPlanHeader = 32
 };
 constexpr int kPlanMagic = 0x31544144;   // "DAT1"
 constexpr int kFar = 1 << 29;            // a window side without limit; lengths and positions stay below it
@@ -54,14 +54,15 @@ struct AttnArgs {
     float* lse;            // [heads][q_rows]
     float* delta;          // [heads][q_rows]
     float* part_o;         // forward partials [slot * heads + h][32][D]; backward: dk | dv partials
-    float* part_ml;        // [slot * heads + h][32][2]
-    float* part_bias;      // [heads][n_dq][n_buckets]
+    float* part_ml;        // the same [32][2]
+    float* part_bias;      // [heads][n_dq][dtable_words]
     void* dtable;          // [n_buckets][heads]
     const int* plan;       // device copy
     BiasArgs bias;
     float scale;           // of the scores
     int heads, group;      // query heads, query heads per key head
-    int left, right, sinks, q_rows, n_items, items_at, has_pos, pos_at, tiles_at, slots;
+    int left, right, sinks, q_rows, n_items, items_at, has_pos, pos_at, tiles_at;
+    int pack;              // heads of a group that share a tile of rows where the keys are split
 };
 
 // one set of launchers per element type; dim is one of 16, 32, 64, 128
@@ -75,6 +76,11 @@ struct AttnArgs {
 DPTM_ATTN_LAUNCHERS(bf16)
 DPTM_ATTN_LAUNCHERS(f16)
 DPTM_ATTN_LAUNCHERS(f32)
+
+// words of a dq tile's sums for the bias gradient: by distance (with 62 on either side, see dptm_attn_grad.h), or by
+// bucket where the plan lists positions
+constexpr int kFarPad = 62;
+inline int dtable_words(int has_pos, int n_buckets, int reach) { return has_pos ? n_buckets : 2 * reach + 1 + 2 * kFarPad; }
 
 struct NormRopeArgs {
     Strided x[2], y[2], dy[2], dx[2];   // q and k

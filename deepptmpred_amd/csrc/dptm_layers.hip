@@ -61,27 +61,26 @@ int size_of(int dtype) { return dtype == DPTM_PREC_F32 ? 4 : 2; }
 bool good_type(int t) { return t == DPTM_PREC_F32 || t == DPTM_PREC_BF16 || t == DPTM_PREC_F16; }
 
 // A tensor [rows][heads][dim] whose kernels fetch 16-byte vectors; `written`: rows and heads may not overlap.
-int check_rows(const char* who, const char* name, const dptm_rows* t, int64_t rows, int heads, int dim, int dtype, bool written,
+int check_rows(const char* who, const char* name, const dptm_rows& t, int64_t rows, int heads, int dim, int dtype, bool written,
                Strided* out) {
-    const std::string at = std::string(who) + ": " + name;
-    if (!t) return fail(DPTM_EINVAL, at + " is NULL");
+    auto at = [&] { return std::string(who) + ": " + name; };
     if (rows == 0) {
         *out = Strided{nullptr, 0, 0};
         return DPTM_OK;
     }
     const int size = size_of(dtype);
-    if (!t->data) return fail(DPTM_EINVAL, at + ": NULL buffer");
-    if (t->rows < rows) return fail(DPTM_EINVAL, at + " has " + std::to_string(t->rows) + " rows, the call needs " + std::to_string(rows));
-    if ((reinterpret_cast<uintptr_t>(t->data) & 15) || (t->row_stride * size) % 16 || (t->head_stride * size) % 16)
-        return fail(DPTM_EINVAL, at + ": address and strides must be multiples of 16 bytes");
-    if (t->row_stride < 0 || t->head_stride < 0) return fail(DPTM_EINVAL, at + ": negative stride");
-    if (t->row_stride > (int64_t(1) << 40) || t->head_stride > (int64_t(1) << 40)) return fail(DPTM_EINVAL, at + ": stride too large");
+    if (!t.data) return fail(DPTM_EINVAL, at() + ": NULL buffer");
+    if (t.rows < rows) return fail(DPTM_EINVAL, at() + " has " + std::to_string(t.rows) + " rows, the call needs " + std::to_string(rows));
+    if ((reinterpret_cast<uintptr_t>(t.data) & 15) || (t.row_stride * size) % 16 || (t.head_stride * size) % 16)
+        return fail(DPTM_EINVAL, at() + ": address and strides must be multiples of 16 bytes");
+    if (t.row_stride < 0 || t.head_stride < 0) return fail(DPTM_EINVAL, at() + ": negative stride");
+    if (t.row_stride > (int64_t(1) << 40) || t.head_stride > (int64_t(1) << 40)) return fail(DPTM_EINVAL, at() + ": stride too large");
     if (written) {
-        const bool rows_outside = (heads == 1 || t->head_stride >= dim) && (rows == 1 || t->row_stride >= (heads - 1) * t->head_stride + dim);
-        const bool heads_outside = (rows == 1 || t->row_stride >= dim) && (heads == 1 || t->head_stride >= (rows - 1) * t->row_stride + dim);
-        if (!rows_outside && !heads_outside) return fail(DPTM_EINVAL, at + ": rows or heads of a written tensor overlap");
+        const bool rows_outside = (heads == 1 || t.head_stride >= dim) && (rows == 1 || t.row_stride >= (heads - 1) * t.head_stride + dim);
+        const bool heads_outside = (rows == 1 || t.row_stride >= dim) && (heads == 1 || t.head_stride >= (rows - 1) * t.row_stride + dim);
+        if (!rows_outside && !heads_outside) return fail(DPTM_EINVAL, at() + ": rows or heads of a written tensor overlap");
     }
-    *out = Strided{t->data, t->row_stride, t->head_stride};
+    *out = Strided{t.data, t.row_stride, t.head_stride};
     return DPTM_OK;
 }
 
@@ -192,14 +191,23 @@ int make_plan(const dptm_attention_desc& d, const int32_t* q_len, const int32_t*
     int mode = kWide128;
     if (t64 * d.heads < 256 || t32 == t64) mode = kSplitKeys;
     else if (t128 * d.heads < 512 || t64 * 64 * 5 < t128 * 128 * 4) mode = kWide64;
-    std::vector<QItem> fwd = m.q_items(mode == kWide128 ? 128 : mode == kWide64 ? 64 : 32);
+    // Where keys are split, a tile's 32 rows are queries of up to eight heads that read the same keys (their bias tables
+    // have to fit LDS together), as many as the longest sequence leaves room for.
+    int pack = 1;
+    if (mode == kSplitKeys) {
+        int longest = 1;
+        for (const Seq& s : m.seqs) longest = std::max(longest, s.nq);
+        for (int p = 2; p <= 8; ++p)
+            if (d.heads / d.kv_heads % p == 0 && p * std::min(longest, 32) <= 32) pack = p;
+    }
+    std::vector<QItem> fwd = m.q_items(mode == kWide128 ? 128 : mode == kWide64 ? 64 : 32 / pack);
     std::vector<Join> joins;
     int slots = 0;
     if (mode == kSplitKeys) {
         int64_t total = 0;
         for (const QItem& it : fwd) total += m.keys(it);
         // keys of a workgroup: at least two tiles of each of its four wavefronts, and no more parts than fill the card
-        const int64_t chunk = std::max<int64_t>(256, up((total * d.heads + kGroups - 1) / kGroups, 128));
+        const int64_t chunk = std::max<int64_t>(256, up((total * (d.heads / pack) + kGroups - 1) / kGroups, 128));
         std::vector<QItem> cut;
         for (const QItem& it : fwd) {
             const int64_t n = it.ke - it.kb, parts = std::max<int64_t>(1, (n + chunk - 1) / chunk);
@@ -303,6 +311,7 @@ int make_plan(const dptm_attention_desc& d, const int32_t* q_len, const int32_t*
     p[kPlanDkvJoin] = (int32_t)dkv_joins.size(), p[kPlanDkvJoinAt] = dkv_join_at;
     p[kPlanHasPos] = q_pos ? 1 : 0, p[kPlanPosAt] = pos_at;
     p[kPlanTiles] = (int32_t)(m.bounds.size() / 2), p[kPlanTilesAt] = tiles_at;
+    p[kPlanPack] = pack;
     p[kPlanCheck] = (int32_t)header_sum(p);
     return DPTM_OK;
 }
@@ -316,33 +325,37 @@ int check_plan(const char* who, const int32_t* plan, const int32_t* plan_dev) {
 
 // byte sizes of the workspace's parts, each rounded up to 256
 struct Work { size_t fwd_o, fwd_ml, delta, dkv, bias; };
-Work work_of(const int32_t* p, int n_buckets) {
+Work work_of(const int32_t* p, int n_buckets, int reach) {
     Work w;
     const size_t dim = p[kPlanHeadDim], heads = p[kPlanHeads], kv = p[kPlanKvHeads];
-    w.fwd_o = up((size_t)p[kPlanSlots] * heads * 32 * dim * 4, 256);
-    w.fwd_ml = up((size_t)p[kPlanSlots] * heads * 32 * 2 * 4, 256);
+    w.fwd_o = up((size_t)p[kPlanSlots] * (heads / p[kPlanPack]) * 32 * dim * 4, 256);
+    w.fwd_ml = up((size_t)p[kPlanSlots] * (heads / p[kPlanPack]) * 32 * 2 * 4, 256);
     w.delta = up(heads * (size_t)p[kPlanQRows] * 4, 256);
     w.dkv = up((size_t)p[kPlanDkvSlots] * kv * 2 * 32 * (size_t)p[kPlanDkvWaves] * dim * 4, 256);
-    w.bias = up(heads * (size_t)p[kPlanDq] * (size_t)n_buckets * 4, 256);
+    w.bias = up(heads * (size_t)p[kPlanDq] * (size_t)(n_buckets ? dtable_words(p[kPlanHasPos], n_buckets, reach) : 0) * 4, 256);
     return w;
 }
 
 constexpr int kMaxBuckets = 64, kMaxReach = 1024;
 
-int check_bias(const char* who, const dptm_attention_bias* b, BiasArgs* out) {
+int check_bias(const char* who, const dptm_attention_args& x, BiasArgs* out) {
     *out = BiasArgs{nullptr, nullptr, 0, 0};
-    if (!b) return DPTM_OK;
-    if (!b->table || !b->buckets) return fail(DPTM_EINVAL, std::string(who) + ": bias without table or buckets");
-    if (b->n_buckets < 1 || b->n_buckets > kMaxBuckets) return fail(DPTM_EINVAL, std::string(who) + ": 1 to 64 buckets are supported");
-    if (b->max_distance < 0 || b->max_distance > kMaxReach)
+    if (!x.table && !x.buckets) return DPTM_OK;
+    if (!x.table || !x.buckets) return fail(DPTM_EINVAL, std::string(who) + ": table and buckets go together");
+    if (x.n_buckets < 1 || x.n_buckets > kMaxBuckets) return fail(DPTM_EINVAL, std::string(who) + ": 1 to 64 buckets are supported");
+    if (x.max_distance < 0 || x.max_distance > kMaxReach)
         return fail(DPTM_EINVAL, std::string(who) + ": a largest distance of 0 to 1024 is supported");
-    if (reinterpret_cast<uintptr_t>(b->buckets) & 3) return fail(DPTM_EINVAL, std::string(who) + ": buckets must be 4-byte aligned");
-    *out = BiasArgs{b->table, b->buckets, b->n_buckets, b->max_distance};
+    if ((reinterpret_cast<uintptr_t>(x.buckets) & 3) || (reinterpret_cast<uintptr_t>(x.table) & 3 & (size_of(x.dtype) - 1)))
+        return fail(DPTM_EINVAL, std::string(who) + ": table and buckets must be aligned to their elements");
+    *out = BiasArgs{x.table, x.buckets, x.n_buckets, x.max_distance};
     return DPTM_OK;
 }
 
-int check_common(const char* who, int dtype, float scale, const void* ws, size_t have, size_t need) {
-    if (!good_type(dtype)) return fail(DPTM_EINVAL, std::string(who) + ": dtype must be DPTM_PREC_F32, _BF16 or _F16");
+int check_common(const char* who, const dptm_attention_args& x, size_t need) {
+    const float scale = x.scale;
+    const void* ws = x.workspace;
+    const size_t have = x.workspace_bytes;
+    if (!good_type(x.dtype)) return fail(DPTM_EINVAL, std::string(who) + ": dtype must be DPTM_PREC_F32, _BF16 or _F16");
     if (!(scale > 0.f) || !std::isfinite(scale)) return fail(DPTM_EINVAL, std::string(who) + ": scale must be positive and finite");
     if (need && (!ws || have < need))
         return fail(DPTM_EINVAL, std::string(who) + ": workspace of " + std::to_string(need) + " bytes needed, " + std::to_string(ws ? have : 0) + " given");
@@ -358,6 +371,7 @@ AttnArgs common_args(const int32_t* p, const int32_t* dev, float scale) {
     a.group = p[kPlanHeads] / p[kPlanKvHeads];
     a.left = p[kPlanLeft], a.right = p[kPlanRight], a.sinks = p[kPlanSinks];
     a.q_rows = p[kPlanQRows];
+    a.pack = p[kPlanPack];
     a.has_pos = p[kPlanHasPos], a.pos_at = p[kPlanPosAt], a.tiles_at = p[kPlanTilesAt];
     return a;
 }
@@ -397,79 +411,83 @@ int64_t dptm_attention_plan(const dptm_attention_desc* d, const int32_t* q_len, 
     return on_exception("dptm_attention_plan");
 }
 
-int64_t dptm_attention_workspace(const int32_t* plan, int32_t n_buckets, int32_t backward) try {
+int64_t dptm_attention_workspace(const int32_t* plan, int32_t n_buckets, int32_t max_distance, int32_t backward) try {
     OK_OR_RETURN(check_plan("dptm_attention_workspace", plan, plan));
     if (n_buckets < 0 || n_buckets > kMaxBuckets) return fail(DPTM_EINVAL, "dptm_attention_workspace: 0 to 64 buckets are supported");
-    const Work w = work_of(plan, n_buckets);
+    if (max_distance < 0 || max_distance > kMaxReach)
+        return fail(DPTM_EINVAL, "dptm_attention_workspace: a largest distance of 0 to 1024 is supported");
+    const Work w = work_of(plan, n_buckets, max_distance);
     return (int64_t)(backward ? w.delta + w.dkv + w.bias : w.fwd_o + w.fwd_ml);
 } catch (...) {
     return on_exception("dptm_attention_workspace");
 }
 
-int dptm_attention_forward(const int32_t* plan, const int32_t* plan_dev, int32_t dtype, const dptm_rows* q, const dptm_rows* k,
-                           const dptm_rows* v, const dptm_rows* out, float* lse, float scale, const dptm_attention_bias* bias,
-                           void* workspace, size_t workspace_bytes, int32_t device, void* stream) try {
+int dptm_attention_forward(const dptm_attention_args* args) try {
     const char* who = "dptm_attention_forward";
-    OK_OR_RETURN(check_plan(who, plan, plan_dev));
-    const Work w = work_of(plan, 0);
-    OK_OR_RETURN(check_common(who, dtype, scale, workspace, workspace_bytes, w.fwd_o + w.fwd_ml));
-    const int heads = plan[kPlanHeads], kv = plan[kPlanKvHeads], dim = plan[kPlanHeadDim];
+    if (!args) return fail(DPTM_EINVAL, std::string(who) + ": NULL arguments");
+    const dptm_attention_args& x = *args;
+    const int32_t* plan = x.plan;
+    OK_OR_RETURN(check_plan(who, plan, x.plan_dev));
+    const Work w = work_of(plan, 0, 0);
+    OK_OR_RETURN(check_common(who, x, w.fwd_o + w.fwd_ml));
+    const int heads = plan[kPlanHeads], kv = plan[kPlanKvHeads], dim = plan[kPlanHeadDim], dtype = x.dtype;
     const int64_t nq = plan[kPlanQRows], nk = plan[kPlanKRows];
-    AttnArgs a = common_args(plan, plan_dev, scale);
-    OK_OR_RETURN(check_rows(who, "q", q, nq, heads, dim, dtype, false, &a.q));
-    OK_OR_RETURN(check_rows(who, "k", k, nk, kv, dim, dtype, false, &a.k));
-    OK_OR_RETURN(check_rows(who, "v", v, nk, kv, dim, dtype, false, &a.v));
-    OK_OR_RETURN(check_rows(who, "out", out, nq, heads, dim, dtype, true, &a.out));
-    OK_OR_RETURN(check_bias(who, bias, &a.bias));
+    AttnArgs a = common_args(plan, x.plan_dev, x.scale);
+    OK_OR_RETURN(check_rows(who, "q", x.q, nq, heads, dim, dtype, false, &a.q));
+    OK_OR_RETURN(check_rows(who, "k", x.k, nk, kv, dim, dtype, false, &a.k));
+    OK_OR_RETURN(check_rows(who, "v", x.v, nk, kv, dim, dtype, false, &a.v));
+    OK_OR_RETURN(check_rows(who, "out", x.out, nq, heads, dim, dtype, true, &a.out));
+    OK_OR_RETURN(check_bias(who, x, &a.bias));
     if (nq == 0) return DPTM_OK;
-    if (!lse || (reinterpret_cast<uintptr_t>(lse) & 3)) return fail(DPTM_EINVAL, std::string(who) + ": lse is NULL or misaligned");
-    a.lse = lse;
-    a.part_o = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.fwd_o);
+    if (!x.lse || (reinterpret_cast<uintptr_t>(x.lse) & 3)) return fail(DPTM_EINVAL, std::string(who) + ": lse is NULL or misaligned");
+    a.lse = x.lse;
+    a.part_o = static_cast<float*>(x.workspace);
+    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(x.workspace) + w.fwd_o);
     a.n_items = plan[kPlanFwd], a.items_at = plan[kPlanFwdAt];
-    const OnDevice on(device);
+    const OnDevice on(x.device);
     if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
-    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const hipStream_t s = static_cast<hipStream_t>(x.stream);
     OK_OR_RETURN(hip_result(who, BY_TYPE(attn_forward, a, dim, plan[kPlanMode], s)));
     return hip_result(who, BY_TYPE(attn_join, a, dim, plan[kPlanJoin], plan[kPlanJoinAt], s));
 } catch (...) {
     return on_exception("dptm_attention_forward");
 }
 
-int dptm_attention_backward(const int32_t* plan, const int32_t* plan_dev, int32_t dtype, const dptm_rows* dout, const dptm_rows* q,
-                            const dptm_rows* k, const dptm_rows* v, const dptm_rows* out, const float* lse, float scale,
-                            const dptm_attention_bias* bias, const dptm_rows* dq, const dptm_rows* dk, const dptm_rows* dv,
-                            void* dtable, void* workspace, size_t workspace_bytes, int32_t device, void* stream) try {
+int dptm_attention_backward(const dptm_attention_args* args) try {
     const char* who = "dptm_attention_backward";
-    OK_OR_RETURN(check_plan(who, plan, plan_dev));
+    if (!args) return fail(DPTM_EINVAL, std::string(who) + ": NULL arguments");
+    const dptm_attention_args& x = *args;
+    const int32_t* plan = x.plan;
+    OK_OR_RETURN(check_plan(who, plan, x.plan_dev));
     if (!plan[kPlanDqWaves]) return fail(DPTM_EINVAL, std::string(who) + ": the plan was made without training");
-    AttnArgs a = common_args(plan, plan_dev, scale);
-    OK_OR_RETURN(check_bias(who, bias, &a.bias));
-    const Work w = work_of(plan, a.bias.n_buckets);
-    OK_OR_RETURN(check_common(who, dtype, scale, workspace, workspace_bytes, w.delta + w.dkv + w.bias));
-    const int heads = plan[kPlanHeads], kv = plan[kPlanKvHeads], dim = plan[kPlanHeadDim];
+    AttnArgs a = common_args(plan, x.plan_dev, x.scale);
+    OK_OR_RETURN(check_bias(who, x, &a.bias));
+    const Work w = work_of(plan, a.bias.n_buckets, a.bias.reach);
+    OK_OR_RETURN(check_common(who, x, w.delta + w.dkv + w.bias));
+    const int heads = plan[kPlanHeads], kv = plan[kPlanKvHeads], dim = plan[kPlanHeadDim], dtype = x.dtype;
     const int64_t nq = plan[kPlanQRows], nk = plan[kPlanKRows];
-    OK_OR_RETURN(check_rows(who, "dout", dout, nq, heads, dim, dtype, false, &a.dout));
-    OK_OR_RETURN(check_rows(who, "q", q, nq, heads, dim, dtype, false, &a.q));
-    OK_OR_RETURN(check_rows(who, "k", k, nk, kv, dim, dtype, false, &a.k));
-    OK_OR_RETURN(check_rows(who, "v", v, nk, kv, dim, dtype, false, &a.v));
-    OK_OR_RETURN(check_rows(who, "out", out, nq, heads, dim, dtype, false, &a.out));
-    OK_OR_RETURN(check_rows(who, "dq", dq, nq, heads, dim, dtype, true, &a.dq));
-    OK_OR_RETURN(check_rows(who, "dk", dk, nk, kv, dim, dtype, true, &a.dk));
-    OK_OR_RETURN(check_rows(who, "dv", dv, nk, kv, dim, dtype, true, &a.dv));
-    if (nq && (!lse || (reinterpret_cast<uintptr_t>(lse) & 3))) return fail(DPTM_EINVAL, std::string(who) + ": lse is NULL or misaligned");
-    if (bias && !dtable) return fail(DPTM_EINVAL, std::string(who) + ": bias without a buffer for its gradient");
-    a.lse = const_cast<float*>(lse);
-    a.delta = static_cast<float*>(workspace);
-    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.delta);
-    a.part_bias = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.delta + w.dkv);
-    a.dtable = dtable;
-    const OnDevice on(device);
+    OK_OR_RETURN(check_rows(who, "dout", x.dout, nq, heads, dim, dtype, false, &a.dout));
+    OK_OR_RETURN(check_rows(who, "q", x.q, nq, heads, dim, dtype, false, &a.q));
+    OK_OR_RETURN(check_rows(who, "k", x.k, nk, kv, dim, dtype, false, &a.k));
+    OK_OR_RETURN(check_rows(who, "v", x.v, nk, kv, dim, dtype, false, &a.v));
+    OK_OR_RETURN(check_rows(who, "out", x.out, nq, heads, dim, dtype, false, &a.out));
+    OK_OR_RETURN(check_rows(who, "dq", x.dq, nq, heads, dim, dtype, true, &a.dq));
+    OK_OR_RETURN(check_rows(who, "dk", x.dk, nk, kv, dim, dtype, true, &a.dk));
+    OK_OR_RETURN(check_rows(who, "dv", x.dv, nk, kv, dim, dtype, true, &a.dv));
+    if (nq && (!x.lse || (reinterpret_cast<uintptr_t>(x.lse) & 3))) return fail(DPTM_EINVAL, std::string(who) + ": lse is NULL or misaligned");
+    if (a.bias.table && (!x.dtable || (reinterpret_cast<uintptr_t>(x.dtable) & 3 & (size_of(dtype) - 1))))
+        return fail(DPTM_EINVAL, std::string(who) + ": bias without an aligned buffer for its gradient");
+    a.lse = x.lse;
+    a.delta = static_cast<float*>(x.workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(x.workspace) + w.delta);
+    a.part_bias = reinterpret_cast<float*>(static_cast<char*>(x.workspace) + w.delta + w.dkv);
+    a.dtable = x.dtable;
+    const OnDevice on(x.device);
     if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
-    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const hipStream_t s = static_cast<hipStream_t>(x.stream);
     a.n_items = plan[kPlanDq], a.items_at = plan[kPlanDqAt];
     OK_OR_RETURN(hip_result(who, BY_TYPE(attn_dq, a, dim, plan[kPlanDqWaves], s)));
-    if (bias) OK_OR_RETURN(hip_result(who, BY_TYPE(attn_dtable, a, plan[kPlanDq], s)));
+    if (a.bias.table) OK_OR_RETURN(hip_result(who, BY_TYPE(attn_dtable, a, plan[kPlanDq], s)));
     a.n_items = plan[kPlanDkv], a.items_at = plan[kPlanDkvAt];
     OK_OR_RETURN(hip_result(who, BY_TYPE(attn_dkv, a, dim, plan[kPlanDkvWaves], s)));
     return hip_result(who, BY_TYPE(attn_dkv_join, a, dim, plan[kPlanDkvJoin], plan[kPlanDkvJoinAt], 32 * plan[kPlanDkvWaves], s));
@@ -477,76 +495,72 @@ int dptm_attention_backward(const int32_t* plan, const int32_t* plan_dev, int32_
     return on_exception("dptm_attention_backward");
 }
 
-static int norm_rope_args(const char* who, const dptm_norm_rope_desc* d, const dptm_rows* q, const dptm_rows* k, const float* q_gain,
-                          const float* k_gain, const float* cosv, const float* sinv, const int32_t* positions, NormRopeArgs* a) {
-    if (!d) return fail(DPTM_EINVAL, std::string(who) + ": NULL description");
-    if (!good_type(d->dtype)) return fail(DPTM_EINVAL, std::string(who) + ": dtype must be DPTM_PREC_F32, _BF16 or _F16");
-    if (!good_dim(d->head_dim)) return fail(DPTM_EINVAL, std::string(who) + ": head_dim must be 16, 32, 64 or 128");
-    if (d->heads < 0 || d->kv_heads < 0 || d->heads + d->kv_heads < 1 || d->heads > 4096 || d->kv_heads > 4096)
+static int norm_rope_args(const char* who, const dptm_norm_rope_args* x, NormRopeArgs* a) {
+    if (!x) return fail(DPTM_EINVAL, std::string(who) + ": NULL arguments");
+    if (!good_type(x->dtype)) return fail(DPTM_EINVAL, std::string(who) + ": dtype must be DPTM_PREC_F32, _BF16 or _F16");
+    if (!good_dim(x->head_dim)) return fail(DPTM_EINVAL, std::string(who) + ": head_dim must be 16, 32, 64 or 128");
+    if (x->heads < 0 || x->kv_heads < 0 || x->heads + x->kv_heads < 1 || x->heads > 4096 || x->kv_heads > 4096)
         return fail(DPTM_EINVAL, std::string(who) + ": 0 to 4096 heads each, at least one in all");
-    if (d->rows < 0 || d->rows > (int64_t(1) << 31) - 1) return fail(DPTM_EINVAL, std::string(who) + ": bad row count");
-    if (!(d->eps >= 0.f) || !std::isfinite(d->eps)) return fail(DPTM_EINVAL, std::string(who) + ": eps must be finite and not negative");
-    if (d->n_positions < 0) return fail(DPTM_EINVAL, std::string(who) + ": negative number of positions");
+    if (x->rows < 0 || x->rows > (int64_t(1) << 31) - 1) return fail(DPTM_EINVAL, std::string(who) + ": bad row count");
+    if (!(x->eps >= 0.f) || !std::isfinite(x->eps)) return fail(DPTM_EINVAL, std::string(who) + ": eps must be finite and not negative");
+    if (x->n_positions < 0) return fail(DPTM_EINVAL, std::string(who) + ": negative number of positions");
     // every row's heads, D / 16 lanes each, in blocks of 256 threads: the grid stays below 2^31
-    if (d->rows * (d->heads + d->kv_heads) * (d->head_dim / 16) / 256 >= (int64_t(1) << 31) - 1)
+    if (x->rows * (x->heads + x->kv_heads) * (x->head_dim / 16) / 256 >= (int64_t(1) << 31) - 1)
         return fail(DPTM_EINVAL, std::string(who) + ": too many rows for one launch");
-    if (d->rows && (!cosv || !sinv || (reinterpret_cast<uintptr_t>(cosv) & 15) || (reinterpret_cast<uintptr_t>(sinv) & 15)))
+    if (x->rows && (!x->cosv || !x->sinv || (reinterpret_cast<uintptr_t>(x->cosv) & 15) || (reinterpret_cast<uintptr_t>(x->sinv) & 15)))
         return fail(DPTM_EINVAL, std::string(who) + ": cos / sin are NULL or not 16-byte aligned");
-    if ((reinterpret_cast<uintptr_t>(positions) & 3) || (reinterpret_cast<uintptr_t>(q_gain) & 3) || (reinterpret_cast<uintptr_t>(k_gain) & 3))
-        return fail(DPTM_EINVAL, std::string(who) + ": positions and gains must be 4-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(x->positions) & 3) || (reinterpret_cast<uintptr_t>(x->q_gain) & 15) || (reinterpret_cast<uintptr_t>(x->k_gain) & 15))
+        return fail(DPTM_EINVAL, std::string(who) + ": positions must be 4-byte and gains 16-byte aligned");
     *a = NormRopeArgs{};
-    OK_OR_RETURN(check_rows(who, "q", q, d->heads ? d->rows : 0, d->heads, d->head_dim, d->dtype, false, &a->x[0]));
-    OK_OR_RETURN(check_rows(who, "k", k, d->kv_heads ? d->rows : 0, d->kv_heads, d->head_dim, d->dtype, false, &a->x[1]));
-    a->heads[0] = d->heads, a->heads[1] = d->kv_heads;
-    a->gain[0] = q_gain, a->gain[1] = k_gain;
-    a->cosv = cosv, a->sinv = sinv, a->positions = positions;
-    a->rows = d->rows, a->n_pos = d->n_positions, a->dim = d->head_dim, a->interleaved = d->interleaved ? 1 : 0, a->eps = d->eps;
+    OK_OR_RETURN(check_rows(who, "q", x->q, x->heads ? x->rows : 0, x->heads, x->head_dim, x->dtype, false, &a->x[0]));
+    OK_OR_RETURN(check_rows(who, "k", x->k, x->kv_heads ? x->rows : 0, x->kv_heads, x->head_dim, x->dtype, false, &a->x[1]));
+    a->heads[0] = x->heads, a->heads[1] = x->kv_heads;
+    a->gain[0] = x->q_gain, a->gain[1] = x->k_gain;
+    a->cosv = x->cosv, a->sinv = x->sinv, a->positions = x->positions;
+    a->rows = x->rows, a->n_pos = x->n_positions, a->dim = x->head_dim, a->interleaved = x->interleaved ? 1 : 0, a->eps = x->eps;
     return DPTM_OK;
 }
 
-int dptm_qk_norm_rope_forward(const dptm_norm_rope_desc* d, const dptm_rows* q, const dptm_rows* k, const float* q_gain,
-                              const float* k_gain, const float* cosv, const float* sinv, const int32_t* positions,
-                              const dptm_rows* q_out, const dptm_rows* k_out, int32_t device, void* stream) try {
+int dptm_qk_norm_rope_forward(const dptm_norm_rope_args* x) try {
     const char* who = "dptm_qk_norm_rope_forward";
     NormRopeArgs a;
-    OK_OR_RETURN(norm_rope_args(who, d, q, k, q_gain, k_gain, cosv, sinv, positions, &a));
-    OK_OR_RETURN(check_rows(who, "q_out", q_out, d->heads ? d->rows : 0, d->heads, d->head_dim, d->dtype, true, &a.y[0]));
-    OK_OR_RETURN(check_rows(who, "k_out", k_out, d->kv_heads ? d->rows : 0, d->kv_heads, d->head_dim, d->dtype, true, &a.y[1]));
-    if (d->rows == 0) return DPTM_OK;
-    const OnDevice on(device);
+    OK_OR_RETURN(norm_rope_args(who, x, &a));
+    OK_OR_RETURN(check_rows(who, "q_out", x->q_out, x->heads ? x->rows : 0, x->heads, x->head_dim, x->dtype, true, &a.y[0]));
+    OK_OR_RETURN(check_rows(who, "k_out", x->k_out, x->kv_heads ? x->rows : 0, x->kv_heads, x->head_dim, x->dtype, true, &a.y[1]));
+    if (x->rows == 0) return DPTM_OK;
+    const OnDevice on(x->device);
     if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
-    return hip_result(who, norm_rope_forward(a, d->dtype, static_cast<hipStream_t>(stream)));
+    return hip_result(who, norm_rope_forward(a, x->dtype, static_cast<hipStream_t>(x->stream)));
 } catch (...) {
     return on_exception("dptm_qk_norm_rope_forward");
 }
 
-int64_t dptm_qk_norm_rope_workspace(const dptm_norm_rope_desc* d) {
-    if (!d || !good_dim(d->head_dim) || d->rows < 0 || d->heads < 0 || d->kv_heads < 0) return fail(DPTM_EINVAL, "dptm_qk_norm_rope_workspace: bad sizes");
-    return (int64_t)norm_rope_blocks(d->rows, d->heads + d->kv_heads, d->head_dim) * d->head_dim * 2 * 4;
+int64_t dptm_qk_norm_rope_workspace(const dptm_norm_rope_args* x) {
+    if (!x || !good_dim(x->head_dim) || x->rows < 0 || x->heads < 0 || x->kv_heads < 0)
+        return fail(DPTM_EINVAL, "dptm_qk_norm_rope_workspace: bad sizes");
+    return (int64_t)norm_rope_blocks(x->rows, x->heads + x->kv_heads, x->head_dim) * x->head_dim * 2 * 4;
 }
 
-int dptm_qk_norm_rope_backward(const dptm_norm_rope_desc* d, const dptm_rows* dq_out, const dptm_rows* dk_out, const dptm_rows* q,
-                               const dptm_rows* k, const float* q_gain, const float* k_gain, const float* cosv, const float* sinv,
-                               const int32_t* positions, const dptm_rows* dq, const dptm_rows* dk, float* dq_gain, float* dk_gain,
-                               void* workspace, size_t workspace_bytes, int32_t device, void* stream) try {
+int dptm_qk_norm_rope_backward(const dptm_norm_rope_args* x) try {
     const char* who = "dptm_qk_norm_rope_backward";
     NormRopeArgs a;
-    OK_OR_RETURN(norm_rope_args(who, d, q, k, q_gain, k_gain, cosv, sinv, positions, &a));
-    const int64_t rq = d->heads ? d->rows : 0, rk = d->kv_heads ? d->rows : 0;
-    OK_OR_RETURN(check_rows(who, "dq_out", dq_out, rq, d->heads, d->head_dim, d->dtype, false, &a.dy[0]));
-    OK_OR_RETURN(check_rows(who, "dk_out", dk_out, rk, d->kv_heads, d->head_dim, d->dtype, false, &a.dy[1]));
-    OK_OR_RETURN(check_rows(who, "dq", dq, rq, d->heads, d->head_dim, d->dtype, true, &a.dx[0]));
-    OK_OR_RETURN(check_rows(who, "dk", dk, rk, d->kv_heads, d->head_dim, d->dtype, true, &a.dx[1]));
-    if ((q_gain && !dq_gain) || (k_gain && !dk_gain)) return fail(DPTM_EINVAL, std::string(who) + ": gain without a buffer for its gradient");
-    const int64_t half = dptm_qk_norm_rope_workspace(d) / 2;
-    if ((q_gain || k_gain) && (!workspace || workspace_bytes < (size_t)half * 2 || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    OK_OR_RETURN(norm_rope_args(who, x, &a));
+    const int64_t rq = x->heads ? x->rows : 0, rk = x->kv_heads ? x->rows : 0;
+    OK_OR_RETURN(check_rows(who, "dq_out", x->dq_out, rq, x->heads, x->head_dim, x->dtype, false, &a.dy[0]));
+    OK_OR_RETURN(check_rows(who, "dk_out", x->dk_out, rk, x->kv_heads, x->head_dim, x->dtype, false, &a.dy[1]));
+    OK_OR_RETURN(check_rows(who, "dq", x->dq, rq, x->heads, x->head_dim, x->dtype, true, &a.dx[0]));
+    OK_OR_RETURN(check_rows(who, "dk", x->dk, rk, x->kv_heads, x->head_dim, x->dtype, true, &a.dx[1]));
+    if ((x->q_gain && !x->dq_gain) || (x->k_gain && !x->dk_gain))
+        return fail(DPTM_EINVAL, std::string(who) + ": gain without a buffer for its gradient");
+    const int64_t half = dptm_qk_norm_rope_workspace(x) / 2;
+    if ((x->q_gain || x->k_gain) && (!x->workspace || x->workspace_bytes < (size_t)half * 2 || (reinterpret_cast<uintptr_t>(x->workspace) & 255)))
         return fail(DPTM_EINVAL, std::string(who) + ": workspace of " + std::to_string(half * 2) + " bytes, 256-byte aligned, needed");
-    a.part[0] = static_cast<float*>(workspace);
-    a.part[1] = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + half) : nullptr;
-    a.dgain[0] = dq_gain, a.dgain[1] = dk_gain;
-    const OnDevice on(device);
+    a.part[0] = static_cast<float*>(x->workspace);
+    a.part[1] = x->workspace ? reinterpret_cast<float*>(static_cast<char*>(x->workspace) + half) : nullptr;
+    a.dgain[0] = x->dq_gain, a.dgain[1] = x->dk_gain;
+    const OnDevice on(x->device);
     if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
-    return hip_result(who, norm_rope_backward(a, d->dtype, static_cast<hipStream_t>(stream)));
+    return hip_result(who, norm_rope_backward(a, x->dtype, static_cast<hipStream_t>(x->stream)));
 } catch (...) {
     return on_exception("dptm_qk_norm_rope_backward");
 }

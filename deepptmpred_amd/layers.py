@@ -17,6 +17,8 @@ records.
 from __future__ import annotations
 
 import ctypes as C
+import struct
+import threading
 from typing import Optional, Sequence, Tuple
 
 import numpy as np
@@ -26,6 +28,30 @@ from . import _native
 
 _TYPES = {torch.float32: _native.PRECISIONS["f32"], torch.bfloat16: _native.PRECISIONS["bf16"],
           torch.float16: _native.PRECISIONS["f16"]}
+
+# The argument blocks of the C calls, packed in one go: a call's cost on the host counts where a protein is short.
+_ROWS = "Qqqq"
+_NO_ROWS = (0, 0, 0, 0)
+_ATTENTION = struct.Struct("@QQ" + 4 * _ROWS + "QQQQQQ" + 4 * _ROWS + "Qiiiif")
+_NORM_ROPE = struct.Struct("@" + 4 * _ROWS + "QQQQQQ" + 4 * _ROWS + "QQQQqiiiiiiif")
+
+
+class _Block(threading.local):
+    """Memory that a call's arguments are packed into, one per thread."""
+
+    def __init__(self):
+        self.attention = C.create_string_buffer(C.sizeof(_native.AttentionArgs))
+        self.attention_at = C.addressof(self.attention)
+        self.norm_rope = C.create_string_buffer(C.sizeof(_native.NormRopeArgs))
+        self.norm_rope_at = C.addressof(self.norm_rope)
+
+
+_block = _Block()
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(device: int) -> int:
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def _check(rc: int, what: str) -> int:
@@ -48,60 +74,69 @@ def _device(device) -> torch.device:
     return device
 
 
-class _Call:
-    """Checks of the tensors of one call, and their C form."""
+def _first(t, what: str):
+    """Type code and GPU of a call's first tensor; the others have to agree."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{what}: expected torch tensors")
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what}: dtype {t.dtype} is not float32, bfloat16 or float16")
+    device = t.get_device()
+    if device < 0:
+        raise ValueError(f"{what}: tensors must be on a GPU")
+    return code, device
 
-    def __init__(self, what: str, first: torch.Tensor, dim: int):
-        self.what, self.dim = what, dim
-        if not isinstance(first, torch.Tensor):
-            raise ValueError(f"{what}: expected torch tensors")
-        if first.dtype not in _TYPES:
-            raise ValueError(f"{what}: dtype {first.dtype} is not float32, bfloat16 or float16")
-        if first.device.type != "cuda":
-            raise ValueError(f"{what}: tensors must be on a GPU")
-        self.dtype, self.device = first.dtype, first.device
 
-    def tensor(self, t, name: str, dtype=None):
-        if not isinstance(t, torch.Tensor):
-            raise ValueError(f"{self.what}: {name} is not a torch tensor")
-        if t.device != self.device:
-            raise ValueError(f"{self.what}: {name} is on {t.device}, not on {self.device}")
-        if t.dtype != (dtype or self.dtype):
-            raise ValueError(f"{self.what}: {name} has dtype {t.dtype}, expected {dtype or self.dtype}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{self.what}: {name} requires grad, and this call does not record; detach it or use no_grad")
-        return t
+def _refuse(t, what: str, name: str, dtype, device: int):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{what}: {name} is not a torch tensor")
+    if t.dtype != dtype:
+        raise ValueError(f"{what}: {name} has dtype {t.dtype}, expected {dtype}")
+    if t.get_device() != device:
+        raise ValueError(f"{what}: {name} is on {t.device}, not on cuda:{device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: {name} requires grad, and this call does not record; detach it or use no_grad")
 
-    def rows(self, t, name: str, heads: int, rows: int) -> _native.Rows:
-        self.tensor(t, name)
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.dim:
-            raise ValueError(f"{self.what}: {name} has shape {tuple(t.shape)}, expected [rows, {heads}, {self.dim}]")
-        if t.shape[0] < rows:
-            raise ValueError(f"{self.what}: {name} has {t.shape[0]} rows, the call needs {rows}")
-        if t.stride(2) != 1 and t.numel():
-            raise ValueError(f"{self.what}: the elements of a head of {name} are not adjacent")
-        # the stride of a dimension of one entry says nothing
-        head = t.stride(1) if heads > 1 else self.dim
-        row = t.stride(0) if t.shape[0] > 1 else heads * self.dim
-        return _native.Rows(t.data_ptr(), t.shape[0], row, head)
 
-    def flat(self, t, name: str, shape, dtype) -> Optional[int]:
-        if t is None:
-            return None
-        self.tensor(t, name, dtype)
-        if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-            raise ValueError(f"{self.what}: {name} must be contiguous of shape {tuple(shape)}, got {tuple(t.shape)}")
-        return t.data_ptr()
+def _rows(t, what: str, name: str, dtype, device: int, heads: int, dim: int, rows: int):
+    """Address, rows and strides of a tensor [rows or more, heads, dim]."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != device or t.requires_grad:
+        _refuse(t, what, name, dtype, device)
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"{what}: {name} has shape {tuple(shape)}, expected [rows, {heads}, {dim}]")
+    n = shape[0]
+    if n < rows:
+        raise ValueError(f"{what}: {name} has {n} rows, the call needs {rows}")
+    row, head, one = t.stride()
+    if one != 1 and n and heads:
+        raise ValueError(f"{what}: the elements of a head of {name} are not adjacent")
+    # the stride of a dimension of one entry says nothing
+    return t.data_ptr(), n, row if n > 1 else heads * dim, head if heads > 1 else dim
 
-    def empty(self, *shape, dtype=None):
-        return torch.empty(shape, dtype=dtype or self.dtype, device=self.device)
 
-    def stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+def _flat(t, what: str, name: str, shape, dtype, device: int) -> int:
+    if t is None:
+        return 0
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != device or t.requires_grad:
+        _refuse(t, what, name, dtype, device)
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be contiguous of shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t.data_ptr()
 
-    def workspace(self, nbytes: int):
-        t = torch.empty(max(0, nbytes), dtype=torch.uint8, device=self.device)
-        return t, (t.data_ptr() if nbytes else None)
+
+def _empty(shape, dtype, device: int):
+    return torch.empty(shape, dtype=dtype, device=_gpu(device))
+
+
+_gpus: dict = {}
+
+
+def _gpu(index: int) -> torch.device:
+    d = _gpus.get(index)
+    if d is None:
+        d = _gpus[index] = torch.device("cuda", index)
+    return d
 
 
 def _lengths(a, name: str) -> np.ndarray:
@@ -155,13 +190,23 @@ class AttentionPlan:
         self.training = bool(training)
         self.device = None if device is None else _device(device)
         self.device_words = None if device is None else torch.from_numpy(self.words).to(self.device)
+        self._at = None if device is None else (self.words.ctypes.data, self.device_words.data_ptr())
+        self._bytes: dict = {}
 
-    def _pair(self, call: _Call):
-        if self.device_words is None:
-            raise ValueError(f"{call.what}: the plan was made for the host only")
-        if self.device != call.device:
-            raise ValueError(f"{call.what}: the plan is on {self.device}, the tensors are on {call.device}")
-        return self.words.ctypes.data, self.device_words.data_ptr()
+    def _words(self, what: str, device: int):
+        """Addresses of the plan's two copies."""
+        if self._at is None:
+            raise ValueError(f"{what}: the plan was made for the host only")
+        if self.device.index != device:
+            raise ValueError(f"{what}: the plan is on {self.device}, the tensors are on cuda:{device}")
+        return self._at
+
+    def _workspace(self, n_buckets: int, max_distance: int, backward: int) -> int:
+        key = (n_buckets, max_distance, backward)
+        n = self._bytes.get(key)
+        if n is None:
+            n = self._bytes[key] = _check(_native.load_library().dptm_attention_workspace(self.words.ctypes.data, *key), "AttentionPlan")
+        return n
 
 
 def relative_buckets(n_buckets: int, max_distance: int, bidirectional: bool = True, device=0):
@@ -198,21 +243,18 @@ def rotary_table(n_positions: int, head_dim: int, base: float = 10000.0, device=
     return torch.from_numpy(cos).to(_device(device)), torch.from_numpy(sin).to(_device(device))
 
 
-def _bias(call: _Call, plan: AttentionPlan, table, buckets):
+def _bias(what: str, plan: AttentionPlan, table, buckets, dtype, device: int):
+    """Addresses of table and buckets, number of buckets and largest distance."""
     if table is None and buckets is None:
-        return None
+        return 0, 0, 0, 0
     if table is None or buckets is None:
-        raise ValueError(f"{call.what}: table and buckets go together")
+        raise ValueError(f"{what}: table and buckets go together")
     if table.dim() != 2 or table.shape[1] != plan.heads:
-        raise ValueError(f"{call.what}: table has shape {tuple(table.shape)}, expected [buckets, {plan.heads}]")
-    if buckets.dim() != 1 or buckets.numel() % 2 == 0:
-        raise ValueError(f"{call.what}: buckets must hold an odd number of entries, one per distance")
-    return _native.AttentionBias(call.flat(table, "table", table.shape, call.dtype), call.flat(buckets, "buckets", buckets.shape, torch.int32),
-                                 table.shape[0], buckets.numel() // 2)
-
-
-def _scale(plan: AttentionPlan, scale: Optional[float]) -> float:
-    return plan.head_dim ** -0.5 if scale is None else float(scale)
+        raise ValueError(f"{what}: table has shape {tuple(table.shape)}, expected [buckets, {plan.heads}]")
+    if buckets.dim() != 1 or buckets.shape[0] % 2 == 0:
+        raise ValueError(f"{what}: buckets must hold an odd number of entries, one per distance")
+    return (_flat(table, what, "table", table.shape, dtype, device), _flat(buckets, what, "buckets", buckets.shape, torch.int32, device),
+            table.shape[0], buckets.shape[0] // 2)
 
 
 def attention(q, k, v, plan: AttentionPlan, *, scale: Optional[float] = None, table=None, buckets=None, out=None, lse=None):
@@ -221,21 +263,27 @@ def attention(q, k, v, plan: AttentionPlan, *, scale: Optional[float] = None, ta
     Scores are ``scale * q.k`` (default ``head_dim ** -0.5``) plus ``table[buckets[j - p], head]`` where a relative position
     bias is given (``relative_buckets``; ``table [buckets, heads]`` of the tensors' type).  A row that sees no key gets zeros and
     ``-inf``.  ``out`` and ``lse`` may be given; rows of ``out`` behind the plan's are left as they are."""
-    lib = _native.load_library()
-    call = _Call("attention", q, plan.head_dim)
-    host, dev = plan._pair(call)
+    lib, what, dim = _native.load_library(), "attention", plan.head_dim
+    code, device = _first(q, what)
+    dtype, heads, nq, nk = q.dtype, plan.heads, plan.q_rows, plan.k_rows
+    host, dev = plan._words(what, device)
     if out is None:
-        out = call.empty(plan.q_rows, plan.heads, plan.head_dim)
+        out = _empty((nq, heads, dim), dtype, device)
     if lse is None:
-        lse = call.empty(plan.heads, plan.q_rows, dtype=torch.float32)
-    b = _bias(call, plan, table, buckets)
-    args = [call.rows(q, "q", plan.heads, plan.q_rows), call.rows(k, "k", plan.kv_heads, plan.k_rows),
-            call.rows(v, "v", plan.kv_heads, plan.k_rows), call.rows(out, "out", plan.heads, plan.q_rows)]
-    n = _check(lib.dptm_attention_workspace(host, 0, 0), "attention")
-    hold, ws = call.workspace(n)
-    _check(lib.dptm_attention_forward(host, dev, _TYPES[call.dtype], *[C.byref(x) for x in args],
-                                      call.flat(lse, "lse", (plan.heads, plan.q_rows), torch.float32), _scale(plan, scale),
-                                      None if b is None else C.byref(b), ws, n, call.device.index, call.stream()), "attention")
+        lse = _empty((heads, nq), torch.float32, device)
+    table_at, buckets_at, n_buckets, reach = _bias(what, plan, table, buckets, dtype, device)
+    n = plan._workspace(0, 0, 0)
+    hold = _empty(n, torch.uint8, device) if n else None
+    block = _block
+    _ATTENTION.pack_into(
+        block.attention, 0, host, dev, *_rows(q, what, "q", dtype, device, heads, dim, nq),
+        *_rows(k, what, "k", dtype, device, plan.kv_heads, dim, nk), *_rows(v, what, "v", dtype, device, plan.kv_heads, dim, nk),
+        *_rows(out, what, "out", dtype, device, heads, dim, nq), _flat(lse, what, "lse", (heads, nq), torch.float32, device),
+        table_at, buckets_at, hold.data_ptr() if n else 0, n, _stream(device), *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0,
+        code, device, n_buckets, reach, dim ** -0.5 if scale is None else scale)
+    rc = lib.dptm_attention_forward(block.attention_at)
+    if rc:
+        _check(rc, what)
     return out, lse
 
 
@@ -244,51 +292,49 @@ def attention_backward(dout, q, k, v, out, lse, plan: AttentionPlan, *, scale: O
     """Gradients of ``attention``: ``(dq, dk, dv, dtable)`` from the gradient of its ``out``; ``out`` and ``lse`` as it left
     them, ``dtable`` ``None`` without a bias.  ``dq`` / ``dk`` / ``dv`` may be given (views of one packed tensor, say).
     Nothing is added through atomics: equal calls give equal bits."""
-    lib = _native.load_library()
-    call = _Call("attention_backward", q, plan.head_dim)
-    host, dev = plan._pair(call)
+    lib, what, dim = _native.load_library(), "attention_backward", plan.head_dim
+    code, device = _first(q, what)
+    dtype, heads, kv_heads, nq, nk = q.dtype, plan.heads, plan.kv_heads, plan.q_rows, plan.k_rows
+    host, dev = plan._words(what, device)
     if dq is None:
-        dq = call.empty(plan.q_rows, plan.heads, plan.head_dim)
+        dq = _empty((nq, heads, dim), dtype, device)
     if dk is None:
-        dk = call.empty(plan.k_rows, plan.kv_heads, plan.head_dim)
+        dk = _empty((nk, kv_heads, dim), dtype, device)
     if dv is None:
-        dv = call.empty(plan.k_rows, plan.kv_heads, plan.head_dim)
-    b = _bias(call, plan, table, buckets)
-    dtable = None if b is None else call.empty(*table.shape)
-
-    def rq(t, name):
-        return call.rows(t, name, plan.heads, plan.q_rows)
-
-    def rk(t, name):
-        return call.rows(t, name, plan.kv_heads, plan.k_rows)
-
-    ins = [rq(dout, "dout"), rq(q, "q"), rk(k, "k"), rk(v, "v"), rq(out, "out")]
-    outs = [rq(dq, "dq"), rk(dk, "dk"), rk(dv, "dv")]
-    n = _check(lib.dptm_attention_workspace(host, 0 if b is None else b.n_buckets, 1), "attention_backward")
-    hold, ws = call.workspace(n)
-    _check(lib.dptm_attention_backward(host, dev, _TYPES[call.dtype], *[C.byref(x) for x in ins],
-                                       call.flat(lse, "lse", (plan.heads, plan.q_rows), torch.float32), _scale(plan, scale),
-                                       None if b is None else C.byref(b), *[C.byref(x) for x in outs],
-                                       None if dtable is None else dtable.data_ptr(), ws, n, call.device.index, call.stream()),
-           "attention_backward")
+        dv = _empty((nk, kv_heads, dim), dtype, device)
+    table_at, buckets_at, n_buckets, reach = _bias(what, plan, table, buckets, dtype, device)
+    dtable = _empty((n_buckets, heads), dtype, device) if n_buckets else None
+    n = plan._workspace(n_buckets, reach, 1)
+    hold = _empty(n, torch.uint8, device) if n else None
+    block = _block
+    _ATTENTION.pack_into(
+        block.attention, 0, host, dev, *_rows(q, what, "q", dtype, device, heads, dim, nq),
+        *_rows(k, what, "k", dtype, device, kv_heads, dim, nk), *_rows(v, what, "v", dtype, device, kv_heads, dim, nk),
+        *_rows(out, what, "out", dtype, device, heads, dim, nq), _flat(lse, what, "lse", (heads, nq), torch.float32, device),
+        table_at, buckets_at, hold.data_ptr() if n else 0, n, _stream(device),
+        *_rows(dout, what, "dout", dtype, device, heads, dim, nq), *_rows(dq, what, "dq", dtype, device, heads, dim, nq),
+        *_rows(dk, what, "dk", dtype, device, kv_heads, dim, nk), *_rows(dv, what, "dv", dtype, device, kv_heads, dim, nk),
+        dtable.data_ptr() if n_buckets else 0, code, device, n_buckets, reach, dim ** -0.5 if scale is None else scale)
+    rc = lib.dptm_attention_backward(block.attention_at)
+    if rc:
+        _check(rc, what)
     return dq, dk, dv, dtable
 
 
-def _norm_rope(what: str, q, k, cos, sin, q_gain, k_gain, positions, eps, interleaved):
-    if not isinstance(q, torch.Tensor) or not isinstance(k, torch.Tensor) or q.dim() != 3 or k.dim() != 3:
+def _norm_rope(what: str, q, k, cos, sin, q_gain, k_gain, positions, code, device: int):
+    """Sizes and the addresses that both directions share."""
+    if not isinstance(k, torch.Tensor) or q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"{what}: q and k must be tensors [rows, heads, head_dim]")
-    if q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+    n, heads, dim = q.shape
+    if k.shape[0] != n or k.shape[2] != dim:
         raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in rows or head_dim")
-    call = _Call(what, q, q.shape[2])
-    n = q.shape[0]
     if not isinstance(cos, torch.Tensor) or cos.dim() != 2:
         raise ValueError(f"{what}: cos must be a tensor [positions, head_dim / 2]")
-    table = (cos.shape[0], call.dim // 2)
-    d = _native.NormRopeDesc(_TYPES[call.dtype], call.dim, q.shape[1], k.shape[1], n, table[0], 1 if interleaved else 0, eps)
-    shared = [call.flat(q_gain, "q_gain", (call.dim,), torch.float32), call.flat(k_gain, "k_gain", (call.dim,), torch.float32),
-              call.flat(cos, "cos", table, torch.float32), call.flat(sin, "sin", table, torch.float32),
-              call.flat(positions, "positions", (n,), torch.int32)]
-    return call, d, shared
+    table, f32 = (cos.shape[0], dim // 2), torch.float32
+    return (n, heads, k.shape[1], dim, table[0],
+            (_flat(q_gain, what, "q_gain", (dim,), f32, device), _flat(k_gain, what, "k_gain", (dim,), f32, device),
+             _flat(cos, what, "cos", table, f32, device), _flat(sin, what, "sin", table, f32, device),
+             _flat(positions, what, "positions", (n,), torch.int32, device)))
 
 
 def qk_norm_rope(q, k, cos, sin, *, q_gain=None, k_gain=None, positions=None, eps: float = 1e-6, interleaved: bool = False,
@@ -299,14 +345,21 @@ def qk_norm_rope(q, k, cos, sin, *, q_gain=None, k_gain=None, positions=None, ep
     Row ``r`` stands at ``positions[r]`` (int32, default ``r``); ``cos`` / ``sin`` are ``rotary_table``'s.  The pairs ``(i, i +
     head_dim / 2)`` turn together, with ``interleaved`` the pairs ``(2 i, 2 i + 1)``.  A position outside the table makes its
     row NaN.  ``q_out`` / ``k_out`` may be given, also as the inputs themselves."""
-    lib = _native.load_library()
-    call, d, shared = _norm_rope("qk_norm_rope", q, k, cos, sin, q_gain, k_gain, positions, eps, interleaved)
-    q_out = call.empty(*q.shape) if q_out is None else q_out
-    k_out = call.empty(*k.shape) if k_out is None else k_out
-    ins = [call.rows(q, "q", d.heads, d.rows), call.rows(k, "k", d.kv_heads, d.rows)]
-    outs = [call.rows(q_out, "q_out", d.heads, d.rows), call.rows(k_out, "k_out", d.kv_heads, d.rows)]
-    _check(lib.dptm_qk_norm_rope_forward(C.byref(d), *[C.byref(x) for x in ins], *shared, *[C.byref(x) for x in outs],
-                                         call.device.index, call.stream()), "qk_norm_rope")
+    lib, what = _native.load_library(), "qk_norm_rope"
+    code, device = _first(q, what)
+    dtype = q.dtype
+    n, heads, kv_heads, dim, n_pos, shared = _norm_rope(what, q, k, cos, sin, q_gain, k_gain, positions, code, device)
+    q_out = _empty(q.shape, dtype, device) if q_out is None else q_out
+    k_out = _empty(k.shape, dtype, device) if k_out is None else k_out
+    block = _block
+    _NORM_ROPE.pack_into(
+        block.norm_rope, 0, *_rows(q, what, "q", dtype, device, heads, dim, n), *_rows(k, what, "k", dtype, device, kv_heads, dim, n),
+        *_rows(q_out, what, "q_out", dtype, device, heads, dim, n), *_rows(k_out, what, "k_out", dtype, device, kv_heads, dim, n),
+        *shared, _stream(device), *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0, 0, 0, n, code, device, dim, heads, kv_heads, n_pos,
+        1 if interleaved else 0, eps)
+    rc = lib.dptm_qk_norm_rope_forward(block.norm_rope_at)
+    if rc:
+        _check(rc, what)
     return q_out, k_out
 
 
@@ -314,18 +367,39 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, cos, sin, *, q_gain=None, k_gain
                           interleaved: bool = False, dq=None, dk=None):
     """Gradients of ``qk_norm_rope``: ``(dq, dk, dq_gain, dk_gain)``; ``q`` and ``k`` as it read them, a gain's gradient (float32)
     is ``None`` where there is no gain.  ``dq`` / ``dk`` may be given, also as ``dq_out`` / ``dk_out``."""
-    lib = _native.load_library()
-    call, d, shared = _norm_rope("qk_norm_rope_backward", q, k, cos, sin, q_gain, k_gain, positions, eps, interleaved)
-    dq = call.empty(*q.shape) if dq is None else dq
-    dk = call.empty(*k.shape) if dk is None else dk
-    ins = [call.rows(dq_out, "dq_out", d.heads, d.rows), call.rows(dk_out, "dk_out", d.kv_heads, d.rows),
-           call.rows(q, "q", d.heads, d.rows), call.rows(k, "k", d.kv_heads, d.rows)]
-    outs = [call.rows(dq, "dq", d.heads, d.rows), call.rows(dk, "dk", d.kv_heads, d.rows)]
-    dq_gain = None if q_gain is None else call.empty(call.dim, dtype=torch.float32)
-    dk_gain = None if k_gain is None else call.empty(call.dim, dtype=torch.float32)
-    n = _check(lib.dptm_qk_norm_rope_workspace(C.byref(d)), "qk_norm_rope_backward") if q_gain is not None or k_gain is not None else 0
-    hold, ws = call.workspace(n)
-    _check(lib.dptm_qk_norm_rope_backward(C.byref(d), *[C.byref(x) for x in ins], *shared, *[C.byref(x) for x in outs],
-                                          None if dq_gain is None else dq_gain.data_ptr(), None if dk_gain is None else dk_gain.data_ptr(),
-                                          ws, n, call.device.index, call.stream()), "qk_norm_rope_backward")
+    lib, what = _native.load_library(), "qk_norm_rope_backward"
+    code, device = _first(q, what)
+    dtype = q.dtype
+    n, heads, kv_heads, dim, n_pos, shared = _norm_rope(what, q, k, cos, sin, q_gain, k_gain, positions, code, device)
+    dq = _empty(q.shape, dtype, device) if dq is None else dq
+    dk = _empty(k.shape, dtype, device) if dk is None else dk
+    dq_gain = None if q_gain is None else _empty((dim,), torch.float32, device)
+    dk_gain = None if k_gain is None else _empty((dim,), torch.float32, device)
+
+    def pack(at, size):
+        _NORM_ROPE.pack_into(
+            _block.norm_rope, 0, *_rows(q, what, "q", dtype, device, heads, dim, n), *_rows(k, what, "k", dtype, device, kv_heads, dim, n),
+            *_NO_ROWS, *_NO_ROWS, *shared, _stream(device),
+            *_rows(dq_out, what, "dq_out", dtype, device, heads, dim, n), *_rows(dk_out, what, "dk_out", dtype, device, kv_heads, dim, n),
+            *_rows(dq, what, "dq", dtype, device, heads, dim, n), *_rows(dk, what, "dk", dtype, device, kv_heads, dim, n),
+            0 if dq_gain is None else dq_gain.data_ptr(), 0 if dk_gain is None else dk_gain.data_ptr(), at, size, n, code, device, dim,
+            heads, kv_heads, n_pos, 1 if interleaved else 0, eps)
+
+    size, hold = 0, None
+    if dq_gain is not None or dk_gain is not None:
+        key = (n, heads + kv_heads, dim)
+        size = _norm_rope_bytes.get(key)
+        if size is None:
+            pack(0, 0)
+            size = _check(lib.dptm_qk_norm_rope_workspace(_block.norm_rope_at), what)
+            if len(_norm_rope_bytes) < 4096:
+                _norm_rope_bytes[key] = size
+        hold = _empty(size, torch.uint8, device)
+    pack(hold.data_ptr() if size else 0, size)
+    rc = lib.dptm_qk_norm_rope_backward(_block.norm_rope_at)
+    if rc:
+        _check(rc, what)
     return dq, dk, dq_gain, dk_gain
+
+
+_norm_rope_bytes: dict = {}      # workspace sizes by row count, heads and head_dim

@@ -416,16 +416,6 @@ typedef struct dptm_attention_desc {
     int32_t training;   /* not 0: the plan also serves dptm_attention_backward */
 } dptm_attention_desc;
 
-/* Learned bias by relative position: buckets[max_distance + d] is the row of `table` ([n_buckets][heads], of the tensors'
- * type) that is added to the scaled score of a key d = j - p_i away, distances beyond max_distance counting as it.  1 to
- * 64 buckets, max_distance 0 to 1024; an entry outside 0..n_buckets-1 is clamped into it.  A table entry at or below -2^100 (-inf, or
- * the lowest value of float32 and bfloat16) hides the pairs of its bucket. */
-typedef struct dptm_attention_bias {
-    const void* table;
-    const int32_t* buckets;   /* [2 * max_distance + 1] */
-    int32_t n_buckets, max_distance;
-} dptm_attention_bias;
-
 /* Lays the work of one batch out: HOST arrays q_len / k_len [n_seqs] (k_len NULL: as q_len), q_positions [sum of q_len] or
  * NULL, in any order.  Writes the plan (32-bit words) if `capacity` holds it and returns its length, or a negative error code.
  * The caller keeps the plan and copies it to the device; a call takes both copies and reads the first 32 words of the host's.
@@ -433,48 +423,71 @@ typedef struct dptm_attention_bias {
 int64_t dptm_attention_plan(const dptm_attention_desc* d, const int32_t* q_len, const int32_t* k_len,
                             const int32_t* q_positions, int64_t n_seqs, int32_t* plan, int64_t capacity);
 
-/* Bytes of workspace (256-byte aligned, contents of no meaning before or after) of one forward or backward call. */
-int64_t dptm_attention_workspace(const int32_t* plan, int32_t n_buckets, int32_t backward);
+/* Everything one attention call takes.
+ *   plan, plan_dev   the plan on the host and on the device
+ *   q, k, v, out, lse  out [sum of q_len][heads][head_dim], lse float32 [heads][sum of q_len]
+ *   table, buckets   a learned bias by relative position, or NULL: buckets[max_distance + d] is the row of `table`
+ *                    ([n_buckets][heads], of the tensors' type) that is added to the scaled score of a key d = j - p_i away,
+ *                    distances beyond max_distance counting as it.  1 to 64 buckets, max_distance 0 to 1024; an entry outside
+ *                    0..n_buckets-1 is clamped into it.  A table entry at or below -2^100 (-inf, or the lowest value of
+ *                    float32 and bfloat16) hides the pairs of its bucket
+ *   workspace        dptm_attention_workspace bytes, 256-byte aligned, contents of no meaning before or after
+ *   dout .. dtable   the backward call only; dtable [n_buckets][heads] with a bias
+ *   scale            of the scores, positive */
+typedef struct dptm_attention_args {
+    const int32_t* plan;
+    const int32_t* plan_dev;
+    dptm_rows q, k, v, out;
+    float* lse;
+    const void* table;
+    const int32_t* buckets;
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+    dptm_rows dout, dq, dk, dv;
+    void* dtable;
+    int32_t dtype, device, n_buckets, max_distance;
+    float scale;
+} dptm_attention_args;
 
-/* out_i = sum_j exp(s_ij - lse_i) v_j over the keys that i sees, s_ij = scale q_i.k_j + bias, lse_i = log sum_j exp s_ij
- * (float32 [heads][sum of q_len]).  A row that sees no key gets zeros and -inf.  What hidden keys hold -- NaN and
- * infinities too -- does not reach a row.  scale must be positive; bias may be NULL. */
-int dptm_attention_forward(const int32_t* plan, const int32_t* plan_dev, int32_t dtype, const dptm_rows* q,
-                           const dptm_rows* k, const dptm_rows* v, const dptm_rows* out, float* lse, float scale,
-                           const dptm_attention_bias* bias, void* workspace, size_t workspace_bytes, int32_t device,
-                           void* stream);
+/* Bytes of workspace of one forward or backward call (n_buckets 0: no bias). */
+int64_t dptm_attention_workspace(const int32_t* plan, int32_t n_buckets, int32_t max_distance, int32_t backward);
+
+/* out_i = sum_j exp(s_ij - lse_i) v_j over the keys that i sees, s_ij = scale q_i.k_j + bias, lse_i = log sum_j exp s_ij.
+ * A row that sees no key gets zeros and -inf.  What hidden keys hold -- NaN and infinities too -- does not reach a row. */
+int dptm_attention_forward(const dptm_attention_args* args);
 
 /* Gradients of the above from dout, with out and lse as the forward call left them: dq, dk, dv (dk and dv summed over the
- * query heads that share a key head) and, with a bias, dtable [n_buckets][heads] of the tensors' type.  Keys that no row sees
- * get zeros.  No atomics: equal calls give equal bits. */
-int dptm_attention_backward(const int32_t* plan, const int32_t* plan_dev, int32_t dtype, const dptm_rows* dout,
-                            const dptm_rows* q, const dptm_rows* k, const dptm_rows* v, const dptm_rows* out,
-                            const float* lse, float scale, const dptm_attention_bias* bias, const dptm_rows* dq,
-                            const dptm_rows* dk, const dptm_rows* dv, void* dtable, void* workspace,
-                            size_t workspace_bytes, int32_t device, void* stream);
+ * query heads that share a key head) and, with a bias, dtable.  Keys that no row sees get zeros.  No sum depends on the
+ * order in which workgroups run: equal calls give equal bits. */
+int dptm_attention_backward(const dptm_attention_args* args);
 
 /* Norm of every query and key head and the rotation by position, one pass: y = x (mean x^2 + eps)^-1/2 gain over the
  * head, then the pairs (i, i + head_dim/2) -- interleaved not 0: (2i, 2i+1) -- turned by the angle whose cosine and sine stand in
  * cosv / sinv [n_positions][head_dim/2] (float32) at the row's position: positions[r], or r if NULL.  A position outside
- * the table makes its row NaN.  q_gain / k_gain float32 [head_dim] or NULL (no norm of that tensor).  The outputs may be the inputs. */
-typedef struct dptm_norm_rope_desc {
-    int32_t dtype, head_dim, heads, kv_heads;
+ * the table makes its row NaN.  q_gain / k_gain float32 [head_dim] or NULL (no norm of that tensor).  The outputs may be the
+ * inputs.  The backward call takes q and k as the forward call read them and dq_out / dk_out, the gradients of what it wrote; dq / dk
+ * may be dq_out / dk_out; dq_gain / dk_gain where there is a gain; workspace as for attention. */
+typedef struct dptm_norm_rope_args {
+    dptm_rows q, k, q_out, k_out;
+    const float* q_gain;
+    const float* k_gain;
+    const float* cosv;
+    const float* sinv;
+    const int32_t* positions;
+    void* stream;
+    dptm_rows dq_out, dk_out, dq, dk;
+    float* dq_gain;
+    float* dk_gain;
+    void* workspace;
+    size_t workspace_bytes;
     int64_t rows;
-    int32_t n_positions, interleaved;
+    int32_t dtype, device, head_dim, heads, kv_heads, n_positions, interleaved;
     float eps;
-} dptm_norm_rope_desc;
-int dptm_qk_norm_rope_forward(const dptm_norm_rope_desc* d, const dptm_rows* q, const dptm_rows* k, const float* q_gain,
-                              const float* k_gain, const float* cosv, const float* sinv, const int32_t* positions,
-                              const dptm_rows* q_out, const dptm_rows* k_out, int32_t device, void* stream);
-
-/* Gradients of the above: q and k as the forward call read them, dq_out / dk_out the gradients of what it wrote.  dq / dk may be
- * dq_out / dk_out.  dq_gain / dk_gain float32 [head_dim], where there is a gain.  Workspace as for attention. */
-int64_t dptm_qk_norm_rope_workspace(const dptm_norm_rope_desc* d);
-int dptm_qk_norm_rope_backward(const dptm_norm_rope_desc* d, const dptm_rows* dq_out, const dptm_rows* dk_out,
-                               const dptm_rows* q, const dptm_rows* k, const float* q_gain, const float* k_gain,
-                               const float* cosv, const float* sinv, const int32_t* positions, const dptm_rows* dq,
-                               const dptm_rows* dk, float* dq_gain, float* dk_gain, void* workspace,
-                               size_t workspace_bytes, int32_t device, void* stream);
+} dptm_norm_rope_args;
+int dptm_qk_norm_rope_forward(const dptm_norm_rope_args* args);
+int64_t dptm_qk_norm_rope_workspace(const dptm_norm_rope_args* args);   /* reads rows, head_dim, heads and kv_heads */
+int dptm_qk_norm_rope_backward(const dptm_norm_rope_args* args);
 const char* dptm_layer_last_error(void);
 
 

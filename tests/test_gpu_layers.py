@@ -110,6 +110,23 @@ def test_attention_few_queries(dtype, dim):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_heads_that_share_keys_share_a_tile(dtype):
+    attend(dtype, 32, [3, 1, 4], [400, 65, 4], heads=24, kv_heads=4, window=(300, 0), buckets=(32, 128, False), sinks=2, seed=30)
+    attend(dtype, 64, [1], [900], heads=16, kv_heads=2, buckets=(64, 1000, False), window=(-1, 0), train=False, seed=31)
+    attend(dtype, 64, [20, 13], [90, 40], heads=12, kv_heads=4, buckets=(16, 50, True), seed=32)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_given_positions_in_training(dtype):
+    """Rows at positions from a list, in any order, in the kernels of large batches too: bias gradient and masks."""
+    rng = np.random.default_rng(33)
+    lens = [140] * 6
+    pos = np.concatenate([rng.permutation(200)[:140] - 20 for _ in lens]).astype(np.int32)
+    attend(dtype, 32, lens, heads=48, kv_heads=24, positions=pos, window=(60, 50), sinks=3, buckets=(32, 40, True), seed=34)
+    attend(dtype, 64, [70], [90], heads=2, kv_heads=1, positions=rng.permutation(90)[:70].astype(np.int32), buckets=(8, 9, True), seed=35)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attention_rows_that_see_nothing(dtype):
     """More queries than keys under a window that only looks back: the first stand before the first key; positions far off;
     sequences without keys or without queries."""
@@ -153,20 +170,33 @@ def test_what_hidden_places_hold_does_not_matter(dtype, rows):
     sees[16:30] = True              # rows with 20 in [p - 9, p + 4]
     clear = ~sees
     clear[17:31] = False            # and those of 21
-    assert torch.equal(out2[clear], out[clear]) and torch.equal(lse2[:, clear], lse[:, clear])
+    want = R.attention(host(q), host(k), host(v), [rows], [rows], (9, 4), dout=host(dout), kernel_out=host(out), dtype=dtype)
+
+    def near(t, name, keep):
+        value, bound = want[name]
+        k = keep.cpu().numpy()
+        value, bound = (value[:, k], bound[:, k]) if name == "lse" else (value[k], bound[k])
+        within(t[:, keep] if name == "lse" else t[keep], (value, bound), name)
+
+    near(out2, "out", clear)
+    near(lse2, "lse", clear)
     assert torch.isnan(out2[sees]).all()
     assert torch.isposinf(out2[30, :, 3]).all() and torch.isfinite(out2[30, :, :3]).all()
     # a row whose query and gradient are not finite reaches the keys it sees alone
-    q2[100 % rows], dout2[100 % rows] = float("nan"), float("inf")
     r = 100 % rows
+    q2[r], dout2[r] = float("nan"), float("inf")
     out3, lse3 = layers.attention(q2, k, v, plan)
     grads3 = layers.attention_backward(dout2, q2, k, v, out3, lse3, plan)
     keys = torch.zeros(rows, dtype=torch.bool, device="cuda")
     keys[max(0, r - 9):r + 5] = True
-    others = torch.arange(rows, device="cuda") != r
-    assert torch.equal(grads3[0][others], grads[0][others])
-    for a, b in zip(grads3[1:3], grads[1:3]):
-        assert torch.equal(a[~keys], b[~keys]) and not torch.isfinite(a[keys]).any()
+    near(grads3[0], "dq", torch.arange(rows, device="cuda") != r)
+    for t, name in zip(grads3[1:3], ("dk", "dv")):
+        near(t, name, ~keys)
+        assert not torch.isfinite(t[keys]).any()
+    # and keys that are not finite leave the gradients of the rows that do not see them
+    grads4 = layers.attention_backward(dout, q, k2, v2, out2, lse2, plan)
+    near(grads4[0], "dq", clear)
+    assert torch.isnan(grads4[0][sees]).all()
 
 
 def test_strides_and_rows_behind_the_last():

@@ -34,13 +34,15 @@ BATCHES = [([], []), ([0], [0]), ([1], [1]), ([5, 0, 200], [5, 0, 200]), ([1, 1,
 
 @pytest.mark.parametrize("q_lens,k_lens", BATCHES)
 @pytest.mark.parametrize("window,sinks", [((-1, -1), 0), ((-1, 0), 0), ((20, 7), 3), ((0, 0), 40), ((5, -1), 2), ((300, 0), 130)])
-@pytest.mark.parametrize("heads", [1, 64])
+@pytest.mark.parametrize("heads", [1, 64, (24, 4)])
 @pytest.mark.parametrize("given", [False, True])
 def test_plan_covers_every_visible_pair_once(q_lens, k_lens, window, sinks, heads, given):
     rng = np.random.default_rng(sum(k_lens) + sinks)
     pos = np.concatenate([rng.integers(-3, b + 3, a) for a, b in zip(q_lens, k_lens)] or [np.zeros(0)]).astype(np.int32) if given else None
-    plan = layers.AttentionPlan(q_lens, k_lens, heads=heads, head_dim=32, window=window, sinks=sinks, q_positions=pos, device=None)
+    heads, kv_heads = heads if isinstance(heads, tuple) else (heads, heads)
+    plan = layers.AttentionPlan(q_lens, k_lens, heads=heads, kv_heads=kv_heads, head_dim=32, window=window, sinks=sinks, q_positions=pos, device=None)
     w = plan.words
+    assert heads // kv_heads % w[30] == 0 and w[30] * min(32, max(q_lens, default=0)) <= 32 * (w[30] > 1) + 32 * (w[30] == 1)
     p = pos if given else R.default_positions(q_lens, k_lens)
     m = see(q_lens, k_lens, window, sinks, p)
     starts = {}
@@ -50,7 +52,7 @@ def test_plan_covers_every_visible_pair_once(q_lens, k_lens, window, sinks, head
             starts[q0 + i] = (k0, b)
         q0, k0 = q0 + a, k0 + b
     # forward and dq: every row's visible keys lie in the ranges of its items, each once; parts are joined
-    for at, n, tile in ((w[13], w[12], (128, 64, 32)[w[11]]), (w[18], w[17], 32 * w[19])):
+    for at, n, tile in ((w[13], w[12], (128, 64, 32 // w[30])[w[11]]), (w[18], w[17], 32 * w[19])):
         count = np.zeros(m.shape, np.int64)
         slots = []
         for it in w[at:at + Q_ITEM * n].reshape(-1, Q_ITEM):
@@ -152,17 +154,18 @@ def test_c_calls_are_refused_before_anything_runs():
     """Bad sizes, strides, addresses and plans come back as DPTM_EINVAL: none of these addresses is ever touched."""
     lib = _native.load_library()
     plan = layers.AttentionPlan([10], heads=2, head_dim=64, device=None)
-    P, ref = plan.words.ctypes.data, C.byref
+    P = plan.words.ctypes.data
     good = rows_of(10, 2, 64)
 
-    def forward(plan_host=P, dtype=1, q=good, k=good, v=good, out=good, lse=1 << 20, scale=0.1, bias=None, ws=None, ws_bytes=0, dev=0):
-        return lib.dptm_attention_forward(plan_host, P, dtype, None if q is None else ref(q), ref(k), ref(v), ref(out), lse, scale,
-                                          None if bias is None else ref(bias), ws, ws_bytes, dev, None)
+    def forward(plan_host=P, dtype=1, q=good, k=good, v=good, out=good, lse=1 << 20, scale=0.1, bias=(0, 0, 0, 0), ws=None, ws_bytes=0):
+        x = _native.AttentionArgs(plan=plan_host, plan_dev=P, q=q, k=k, v=v, out=out, lse=lse, table=bias[0], buckets=bias[1],
+                                  workspace=ws, workspace_bytes=ws_bytes, dtype=dtype, n_buckets=bias[2], max_distance=bias[3], scale=scale)
+        return lib.dptm_attention_forward(C.addressof(x))
 
     def says(rc, text):
         assert rc == _native.DPTM_EINVAL and text in lib.dptm_layer_last_error().decode(), lib.dptm_layer_last_error()
 
-    need = lib.dptm_attention_workspace(P, 0, 0)
+    need = lib.dptm_attention_workspace(P, 0, 0, 0)
     ws = dict(ws=1 << 20, ws_bytes=need)
     says(forward(plan_host=None, **ws), "NULL plan")
     other = plan.words.copy()
@@ -172,7 +175,6 @@ def test_c_calls_are_refused_before_anything_runs():
     says(forward(scale=0.0, **ws), "scale")
     says(forward(scale=-1.0, **ws), "scale")
     says(forward(scale=float("nan"), **ws), "scale")
-    says(forward(q=None, **ws), "q is NULL")
     says(forward(q=_native.Rows(None, 10, 128, 64), **ws), "NULL buffer")
     says(forward(k=rows_of(9, 2, 64), **ws), "k has 9 rows")
     says(forward(v=rows_of(10, 2, 64, at=(1 << 20) + 8), **ws), "16 bytes")
@@ -184,48 +186,78 @@ def test_c_calls_are_refused_before_anything_runs():
     if need:
         says(forward(), "workspace")
         says(forward(ws=(1 << 20) + 16, ws_bytes=need), "256-byte")
+    at = 1 << 20
     for n, far in ((0, 5), (65, 5), (8, -1), (8, 1025)):
-        says(forward(bias=_native.AttentionBias(1 << 20, 1 << 20, n, far), **ws), "supported")
-    says(forward(bias=_native.AttentionBias(None, 1 << 20, 8, 9), **ws), "without")
+        says(forward(bias=(at, at, n, far), **ws), "supported")
+    says(forward(bias=(0, at, 8, 9), **ws), "together")
+    says(forward(bias=(at, 0, 8, 9), **ws), "together")
+    says(forward(bias=(at + 1, at, 8, 9), **ws), "aligned")
+    says(forward(bias=(at, at + 2, 8, 9), **ws), "aligned")
 
-    def backward(plan_host=P, dq=good, dk=good, bias=None, dtable=None, ws=1 << 20, ws_bytes=1 << 30, lse=1 << 20):
-        return lib.dptm_attention_backward(plan_host, P, 1, *[ref(good)] * 5, lse, 0.1, None if bias is None else ref(bias), ref(dq),
-                                           ref(dk), ref(good), dtable, ws, ws_bytes, 0, None)
+    def backward(plan_host=P, dq=good, dk=good, bias=(0, 0, 0, 0), dtable=None, ws=1 << 20, ws_bytes=1 << 30, lse=1 << 20):
+        x = _native.AttentionArgs(plan=plan_host, plan_dev=P, q=good, k=good, v=good, out=good, lse=lse, table=bias[0], buckets=bias[1],
+                                  workspace=ws, workspace_bytes=ws_bytes, dout=good, dq=dq, dk=dk, dv=good, dtable=dtable, dtype=1,
+                                  n_buckets=bias[2], max_distance=bias[3], scale=0.1)
+        return lib.dptm_attention_backward(C.addressof(x))
 
     says(backward(ws_bytes=16), "workspace")
     says(backward(dq=_native.Rows(1 << 20, 10, 128, 0)), "overlap")
     says(backward(dk=rows_of(3, 2, 64)), "dk has 3 rows")
-    says(backward(bias=_native.AttentionBias(1 << 20, 1 << 20, 8, 9)), "gradient")
+    says(backward(bias=(at, at, 8, 9)), "gradient")
     says(backward(lse=None), "lse")
     fwd_only = layers.AttentionPlan([10], heads=2, head_dim=64, training=False, device=None)
     says(backward(plan_host=fwd_only.words.ctypes.data), "without training")
-    assert lib.dptm_attention_workspace(None, 0, 0) == _native.DPTM_EINVAL
-    assert lib.dptm_attention_workspace(P, 65, 0) == _native.DPTM_EINVAL
+    says(lib.dptm_attention_forward(None), "NULL arguments")
+    says(lib.dptm_attention_backward(None), "NULL arguments")
+    says(lib.dptm_attention_workspace(None, 0, 0, 0), "NULL plan")
+    says(lib.dptm_attention_workspace(P, 65, 0, 0), "supported")
+    says(lib.dptm_attention_workspace(P, 8, 1025, 0), "supported")
     assert lib.dptm_attention_plan(None, None, None, None, 0, None, 0) == _native.DPTM_EINVAL
+
+
+def test_argument_blocks_match_the_header():
+    """The packed form of the argument blocks has the layout of the structures, which is the header's."""
+    assert layers._NORM_ROPE.size == C.sizeof(_native.NormRopeArgs)
+    a = _native.AttentionArgs
+    assert layers._ATTENTION.size == a.scale.offset + 4 and C.sizeof(a) == (layers._ATTENTION.size + 7) // 8 * 8
+    words = list(range(1, 1 + 2 + 16 + 6 + 16 + 1)) + [1, 2, 3, 4, 0.5]
+    x = a.from_buffer_copy(layers._ATTENTION.pack(*words) + b"\0" * 8)
+    assert (x.plan, x.plan_dev, x.q.data, x.out.head_stride, x.lse, x.stream, x.dout.data, x.dv.head_stride, x.dtable) == \
+        (1, 2, 3, 18, 19, 24, 25, 40, 41)
+    assert (x.dtype, x.device, x.n_buckets, x.max_distance, x.scale) == (1, 2, 3, 4, 0.5)
+    y = _native.NormRopeArgs.from_buffer_copy(layers._NORM_ROPE.pack(*range(1, 51), 0.25))
+    assert (y.q.data, y.k_out.head_stride, y.q_gain, y.stream, y.dq_out.data, y.dk.head_stride, y.dq_gain, y.rows, y.dtype, y.eps) == \
+        (1, 16, 17, 22, 23, 38, 39, 43, 44, 0.25) and y.interleaved == 50
 
 
 def test_c_norm_calls_are_refused_before_anything_runs():
     lib = _native.load_library()
-    ref, good = C.byref, rows_of(10, 2, 64)
+    good = rows_of(10, 2, 64)
     tab = 1 << 20
 
-    def call(q=good, out=good, cos=tab, gain=tab, positions=None, **d):
-        desc = _native.NormRopeDesc(**{**dict(dtype=1, head_dim=64, heads=2, kv_heads=2, rows=10, n_positions=10, interleaved=0, eps=1e-6), **d})
-        return lib.dptm_qk_norm_rope_forward(ref(desc), ref(q), ref(good), gain, gain, cos, tab, positions, ref(out), ref(good), 0, None)
+    def args(**more):
+        return _native.NormRopeArgs(**{**dict(q=good, k=good, q_out=good, k_out=good, q_gain=tab, k_gain=tab, cosv=tab, sinv=tab, dq_out=good,
+                                              dk_out=good, dq=good, dk=good, dtype=1, head_dim=64, heads=2, kv_heads=2, rows=10,
+                                              n_positions=10, eps=1e-6), **more})
+
+    def says(rc, text):
+        assert rc == _native.DPTM_EINVAL and text in lib.dptm_layer_last_error().decode(), (text, lib.dptm_layer_last_error())
 
     for bad, text in ((dict(dtype=7), "dtype"), (dict(head_dim=24), "head_dim"), (dict(heads=-1), "heads"),
                       (dict(heads=0, kv_heads=0), "heads"), (dict(rows=-1), "row"), (dict(eps=-1.0), "eps"),
-                      (dict(eps=float("nan")), "eps"), (dict(n_positions=-1), "positions"), (dict(cos=None), "cos"),
-                      (dict(cos=tab + 4), "16-byte"), (dict(gain=tab + 2), "aligned"), (dict(positions=tab + 2), "aligned"),
-                      (dict(q=rows_of(9, 2, 64)), "rows"), (dict(out=_native.Rows(tab, 10, 128, 0)), "overlap"),
-                      (dict(rows=2 ** 31), "row")):
-        rc = call(**bad)
-        assert rc == _native.DPTM_EINVAL and text in lib.dptm_layer_last_error().decode(), (text, lib.dptm_layer_last_error())
-    desc = _native.NormRopeDesc(1, 64, 2, 2, 10, 10, 0, 1e-6)
-    rc = lib.dptm_qk_norm_rope_backward(ref(desc), *[ref(good)] * 4, tab, tab, tab, tab, None, ref(good), ref(good), None, tab, tab, 1 << 20, 0, None)
-    assert rc == _native.DPTM_EINVAL and b"gradient" in lib.dptm_layer_last_error()
-    rc = lib.dptm_qk_norm_rope_backward(ref(desc), *[ref(good)] * 4, tab, tab, tab, tab, None, ref(good), ref(good), tab, tab, None, 0, 0, None)
-    assert rc == _native.DPTM_EINVAL and b"workspace" in lib.dptm_layer_last_error()
+                      (dict(eps=float("nan")), "eps"), (dict(n_positions=-1), "positions"), (dict(cosv=None), "cos"),
+                      (dict(cosv=tab + 4), "16-byte"), (dict(q_gain=tab + 4), "aligned"), (dict(positions=tab + 2), "aligned"),
+                      (dict(q=rows_of(9, 2, 64)), "rows"), (dict(q_out=_native.Rows(tab, 10, 128, 0)), "overlap"),
+                      (dict(k=_native.Rows(None, 10, 128, 64)), "NULL"), (dict(rows=2 ** 31), "row")):
+        x = args(**bad)
+        says(lib.dptm_qk_norm_rope_forward(C.addressof(x)), text)
+    for bad, text in ((dict(), "gradient"), (dict(dq_gain=tab, dk_gain=tab), "workspace"),
+                      (dict(dq=_native.Rows(tab, 10, 128, 0)), "overlap")):
+        x = args(**bad)
+        says(lib.dptm_qk_norm_rope_backward(C.addressof(x)), text)
+    says(lib.dptm_qk_norm_rope_forward(None), "NULL arguments")
+    says(lib.dptm_qk_norm_rope_backward(None), "NULL arguments")
+    says(lib.dptm_qk_norm_rope_workspace(None), "sizes")
 
 
 def test_python_refusals():
