@@ -34,6 +34,7 @@ template <> struct Elem<_Float16> {
     static constexpr unsigned kExp = 0x7c00;
 };
 template <> struct Elem<float> {
+    static constexpr unsigned kExp = 0x7f80;
     typedef float v8 __attribute__((ext_vector_type(8)));
     typedef float v4 __attribute__((ext_vector_type(4)));
 };
@@ -112,19 +113,29 @@ struct Tile {
     }
 };
 
-// ROWS rows of a strided tensor on the way to LDS through registers; rows from `valid` on become zeros
+// ROWS rows of a strided tensor on the way to LDS through registers; rows from `valid` on become zeros.  Offsets within
+// the rows are kept as 32 bits behind a uniform address (row strides are refused from 2^25 bytes on).
 template <typename T, int D, int ROWS, int NT>
 struct Stage {
     static constexpr int kChunks = Tile<T, D>::kChunks;
-    static constexpr int kAll = ROWS * kChunks, kMine = (kAll + NT - 1) / NT;
+    static constexpr int kAll = ROWS * kChunks, kMine = (kAll + NT - 1) / NT, kRowStep = NT / kChunks;
     u32x4_a r[kMine];
-    __device__ __forceinline__ void load(const char* base, int64_t row_bytes, int valid, int tid) {
+    unsigned at, step;     // this thread's first chunk, the next ones lie `step` bytes on
+    __device__ __forceinline__ Stage(int64_t row_bytes, int tid) {
+        at = (unsigned)(tid / kChunks) * (unsigned)row_bytes + (tid % kChunks) * 16;
+        step = kRowStep * (unsigned)row_bytes;
+    }
+    __device__ __forceinline__ void load(const char* base, int valid, int tid) {
+        if (valid >= ROWS && kAll % NT == 0) {
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-            const int c = tid + i * NT, row = c / kChunks;
-            r[i] = u32x4_a{0, 0, 0, 0};
-            if (row < valid && (kAll % NT == 0 || c < kAll))
-                r[i] = *reinterpret_cast<const u32x4_a*>(base + row * row_bytes + (c % kChunks) * 16);
+            for (int i = 0; i < kMine; ++i) r[i] = *reinterpret_cast<const u32x4_a*>(base + i * step + at);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int row = tid / kChunks + i * kRowStep;
+                r[i] = u32x4_a{0, 0, 0, 0};
+                if (row < min(valid, ROWS)) r[i] = *reinterpret_cast<const u32x4_a*>(base + i * step + at);
+            }
         }
     }
     __device__ __forceinline__ void store(char* t, int tid) const {
@@ -134,6 +145,17 @@ struct Stage {
             if (kAll % NT == 0 || c < kAll)
                 *reinterpret_cast<u32x4_a*>(t + row * (kChunks * 16) + (((c % kChunks) ^ Tile<T, D>::swz(row)) << 4)) = r[i];
         }
+    }
+    // not 0 if an element of this thread's part is an infinity or a NaN: adding 1 to an exponent of all ones reaches the sign
+    __device__ __forceinline__ unsigned not_finite() const {
+        constexpr unsigned kMask = sizeof(T) == 4 ? 0x7f800000u : Elem<T>::kExp * 0x10001u;
+        constexpr unsigned kOne = sizeof(T) == 4 ? 0x00800000u : (0x8000u - Elem<T>::kExp) * 0x10001u;
+        unsigned bits = 0;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bits |= (r[i][e] & kMask) + kOne;
+        return bits & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u);
     }
 };
 
@@ -186,8 +208,11 @@ __device__ __forceinline__ LaneMask lane_mask(const Window& w, int pos, int key0
     const int lo = pos - w.left - key0, hi = min(pos + w.right, key_end - 1) - key0;
     return LaneMask{lo, max(hi - lo + 1, 0), min(w.sinks - key0, hi + 1)};
 }
-__device__ __forceinline__ bool sees(const LaneMask& m, int c) {
-    return ((unsigned)(c - m.lo) < (unsigned)m.n) | (c < m.first);
+__device__ __forceinline__ bool in_window(const LaneMask& m, int c) { return (unsigned)(c - m.lo) < (unsigned)m.n; }
+// registers of hidden pairs become `value`
+__device__ __forceinline__ void hide(f32x16_a& s, const LaneMask& m, float value) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = (in_window(m, reg_row(r)) | (reg_row(r) < m.first)) ? s[r] : value;
 }
 // all pairs of positions [pmin, pmax] and keys [j0, j1): every one visible / none visible
 __device__ __forceinline__ bool all_visible(const Window& w, int pmin, int pmax, int j0, int j1) {
@@ -197,43 +222,40 @@ __device__ __forceinline__ bool none_visible(const Window& w, int pmin, int pmax
     return j0 - pmax > w.right || (j1 - 1 - pmin < -w.left && j0 >= w.sinks);
 }
 
-// A hidden pair's weight is 0, but 0 * inf and 0 * NaN are NaN.  Wavefronts that meet a tile with hidden pairs look whether its
-// rows hold such an element (tile_not_finite), and those that found one do their rows over at the end, pair by pair.
-template <typename T>
-__device__ __forceinline__ bool not_finite(T x) {
-    if constexpr (sizeof(T) == 2) return (__builtin_bit_cast(unsigned short, x) & Elem<T>::kExp) == Elem<T>::kExp;
-    else return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
-}
-template <typename T, int D, int ROWS>
-__device__ __forceinline__ bool tile_not_finite(const char* t, int row0, int lane) {
-    bool bad = false;
-    const char* p = t + row0 * (Tile<T, D>::kChunks * 16);
-#pragma unroll
-    for (int i = 0; i < (ROWS * Tile<T, D>::kChunks + 63) / 64; ++i) {
-        const int c = i * 64 + lane;
-        if (ROWS * Tile<T, D>::kChunks % 64 && c >= ROWS * Tile<T, D>::kChunks) break;
-        typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
-        const vec x = *reinterpret_cast<const vec*>(p + c * 16);
-#pragma unroll
-        for (int e = 0; e < 16 / (int)sizeof(T); ++e) bad |= not_finite(x[e]);
-    }
-    return __ballot(bad) != 0;
-}
-// ---- relative position bias in LDS: value per distance in units of log2, one head.  Entries at or below -2^100 hide their
-// ---- pairs, so that a table of the type's lowest value works as a mask does
+// A hidden pair's weight is 0, but 0 * inf and 0 * NaN are NaN.  Where a tile holds hidden pairs its threads look, on the way
+// to LDS, whether its rows hold such an element (Stage::not_finite), and workgroups that found one do their rows over at the
+// end, pair by pair.
+
+// ---- relative position bias in LDS: value per distance, divided by the scale of the scores, because the score products start
+// ---- from it (init_bias) instead of from zero: the bias costs no arithmetic per element, and no branch touches a score.
+// ---- Entries at or below -2^100 hide their pairs, so that a table of the type's lowest value works as a mask does
 // The table goes on for 31 distances on either side with the last value: a lane clamps the distance of its first key of a
 // tile alone (bias_at), and the others lie behind it.
 constexpr int kBiasPad = 31;
 __host__ __device__ inline int bias_room(int reach) { return (2 * reach + 1 + 2 * kBiasPad + 3) & ~3; }   // floats
 __device__ __forceinline__ int bias_at(int far, int reach) { return min(max(far, -reach - kBiasPad), reach) + reach + kBiasPad; }
-__device__ __forceinline__ float bias_value(float v) { return v <= -0x1p100f ? kMinusInf : v * kLog2e; }
+__device__ __forceinline__ float bias_value(float v, float inv_scale) { return v <= -0x1p100f ? kMinusInf : v * inv_scale; }
 template <typename T>
-__device__ __forceinline__ void load_bias(float* lds, const BiasArgs& b, int heads, int head, int tid, int nt) {
+__device__ __forceinline__ void load_bias(float* lds, const BiasArgs& b, float inv_scale, int heads, int head, int tid, int nt) {
     const T* table = static_cast<const T*>(b.table);
     for (int i = tid; i < 2 * b.reach + 1 + 2 * kBiasPad; i += nt) {
         const int k = min(max(b.buckets[min(max(i - kBiasPad, 0), 2 * b.reach)], 0), b.n_buckets - 1);
         const float v = (float)table[(int64_t)k * heads + head];
-        lds[i] = bias_value(v);
+        lds[i] = bias_value(v, inv_scale);
+    }
+}
+
+// accumulators of 32 keys from `key0` on, whose score registers start at key0 + 4h; `above` / `below`: the whole tile lies
+// beyond the largest distance
+__device__ __forceinline__ void init_bias(f32x16_a& s, const float* bias, int reach, int far, bool above, bool below) {
+    if (above | below) {
+        const float b = bias[above ? 2 * reach + kBiasPad : 0];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = b;
+    } else {
+        const float* b = bias + bias_at(far, reach);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = b[reg_row(r)];
     }
 }
 

@@ -16,7 +16,7 @@ namespace {
 // weight of an empty row (lse = -inf) is 0 everywhere: its reference is +inf
 __device__ __forceinline__ float lse_log2(float lse) { return lse == kMinusInf ? __builtin_inff() : lse * kLog2e; }
 
-// A wavefront's rows of dq once more, pair by pair (see tile_not_finite).
+// A wavefront's rows of dq once more, pair by pair (see Stage::not_finite).
 template <typename T, int D, int DT, bool BIAS>
 DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, int item, const T* q, const T* g, int hk, int pos, float ref, float delta, const float* bias, int h) {
     const QItem& it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[item];
@@ -26,9 +26,9 @@ DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, int item, const T* q, 
     for (int j = 0; j < it.ke; ++j) {
         if (j >= it.sink_end && j < it.kb) continue;
         const T* k = row_ptr<T>(a.k, (int64_t)it.k0 + j, hk);
-        float s = dot_rows<T, D>(q, k) * (a.scale * kLog2e);
+        float s = dot_rows<T, D>(q, k);
         if constexpr (BIAS) s += bias[bias_at(j - pos, a.bias.reach)];
-        const float ds = __builtin_amdgcn_exp2f(s - ref) * (dot_rows<T, D>(g, row_ptr<T>(a.v, (int64_t)it.k0 + j, hk)) - delta);
+        const float ds = __builtin_amdgcn_exp2f(fmaf(s, a.scale * kLog2e, -ref)) * (dot_rows<T, D>(g, row_ptr<T>(a.v, (int64_t)it.k0 + j, hk)) - delta);
         const bool see = visible(win, j - pos, j);
 #pragma unroll 1
         for (int i = 0; i < 16 * DT; ++i) acc[i] += see ? (float)(T)ds * (float)k[reg_col<D>(i >> 4, i & 15, h)] : 0.f;
@@ -37,11 +37,12 @@ DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, int item, const T* q, 
 
 // Bias gradient, in the kernel that owns queries.  Far tiles (one bucket) are summed in a register.  In a near one the
 // wavefront's rows stand at consecutive positions, so that equal distances are the diagonals of its 32 x 32 dS: it goes to LDS
-// with zeros between its rows, lane l adds diagonal l up (32 reads at a fixed stride, no bank twice) and keeps the
+// with zeros between its rows, lane l adds diagonal l up (32 reads at a fixed stride) and keeps the
 // sum by distance; what distances share a bucket is left to attn_dtable_kernel.  Adding every element into its bucket by LDS
 // atomics instead took 773 us of a 48-protein batch where this takes a fraction.  POS: rows at positions from a
 // list; each lane then adds into a column of its own per bucket, and no order but the program's enters either.
-constexpr int kShear = 32 * 64 + 32;   // floats: 32 zeros, then 32 rows of 32 values and 32 zeros
+constexpr int kShearRow = 68;                   // 32 values and 36 zeros: 17 chunks of 16 bytes, so that rows start on different banks
+constexpr int kShear = 32 * kShearRow + 32;   // floats, 32 zeros in front
 template <bool POS> __host__ __device__ inline int dq_lds_floats(int waves, int n_buckets, int reach) {
     return POS ? waves * n_buckets * 64 + (bias_room(reach) + 3) / 4 : waves * (kShear + ((2 * reach + 1 + 2 * kFarPad + 3) & ~3));
 }
@@ -94,32 +95,35 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
     const char* vbase = reinterpret_cast<const char*>(row_ptr<T>(a.v, it.k0, hk));
     const int64_t kstep = a.k.row * (int)sizeof(T), vstep = a.v.row * (int)sizeof(T);
     const int ns = (it.sink_end + kBK - 1) / kBK, n = ns + (it.ke - it.kb + kBK - 1) / kBK;
-    Stage<T, D, kBK, NW * 64> sk, sv;
+    Stage<T, D, kBK, NW * 64> sk(kstep, tid), sv(vstep, tid);
     auto fetch = [&](int t) {
         const int j0 = t < ns ? t * kBK : it.kb + (t - ns) * kBK, j1 = t < ns ? it.sink_end : it.ke;
-        sk.load(kbase + j0 * kstep, kstep, j1 - j0, tid);
-        sv.load(vbase + j0 * vstep, vstep, j1 - j0, tid);
+        sk.load(kbase + j0 * kstep, j1 - j0, tid);
+        sv.load(vbase + j0 * vstep, j1 - j0, tid);
+    };
+    unsigned odd = 0;
+    auto put = [&](int t) {
+        const int j0 = t < ns ? t * kBK : it.kb + (t - ns) * kBK, j1 = min(j0 + kBK, t < ns ? it.sink_end : it.ke);
+        sk.store(smem + (t & 1) * kBytes, tid);
+        sv.store(smem + (2 + (t & 1)) * kBytes, tid);
+        if (a.has_pos || !all_visible(win, it.pos0, it.pos0 + it.nq - 1, j0, j1)) odd |= sk.not_finite();
     };
     f32x16_a acc[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
-    bool over = false;
     float below = 0.f, above = 0.f;     // dS of distances up to -reach, from reach on
     if (n > 0) fetch(0);
     if constexpr (BIAS) {
-        load_bias<T>(bias, a.bias, a.heads, head, tid, NW * 64);
+        load_bias<T>(bias, a.bias, 1.f / a.scale, a.heads, head, tid, NW * 64);
         const int floats = POS ? NW * nb * 64 : NW * (kShear + room);
         for (int i = tid; i < floats; i += NW * 64) more[i] = 0.f;
         if constexpr (POS)
             for (int i = tid; i < bias_room(reach); i += NW * 64)
                 bucket[i] = (unsigned char)min(max(a.bias.buckets[min(max(i - kBiasPad, 0), 2 * reach)], 0), nb - 1);
     }
-    if (n > 0) {
-        sk.store(smem, tid);
-        sv.store(smem + 2 * kBytes, tid);
-    }
+    if (n > 0) put(0);
     __syncthreads();
     for (int t = 0; t < n; ++t) {
         if (t + 1 < n) fetch(t + 1);
@@ -131,37 +135,19 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
             const int a0 = j0 + 32 * k, a1 = min(a0 + 32, j1);
             if (active && a0 < j1 && !none_visible(win, rw.pmin, rw.pmax, a0, a1)) {
                 const bool full = a1 - a0 == 32 && all_visible(win, rw.pmin, rw.pmax, a0, a1);
+                const bool is_above = a0 - rw.pmax >= reach, is_below = a0 + 31 - rw.pmin <= -reach;   // one bucket for the tile
                 f32x16_a s, p;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = p[r] = 0.f;
+                if constexpr (BIAS) init_bias(s, bias, reach, a0 + 4 * h - rw.pos, is_above, is_below);
 #pragma unroll
                 for (int st = 0; st < ST; ++st) {
                     mma(s, Tile<T, D>::row_frag(kt, 32 * k + (lane & 31), st, h), q[st]);
                     mma(p, Tile<T, D>::row_frag(vt, 32 * k + (lane & 31), st, h), g[st]);
                 }
-                const bool is_above = a0 - rw.pmax >= reach, is_below = a0 + 31 - rw.pmin <= -reach;   // one bucket for the tile
-                const int at = BIAS ? bias_at(a0 + 4 * h - rw.pos, reach) : 0;
-                if constexpr (BIAS) {
-                    if (is_above | is_below) {
-                        const float b = bias[is_above ? 2 * reach + kBiasPad : 0];
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, b);
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, bias[at + reg_row(r)]);
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float x = BIAS ? s[r] - ref : fmaf(s[r], c, -ref);
-                    s[r] = __builtin_amdgcn_exp2f(x) * (p[r] - delta);
-                }
-                if (!full) {
-                    const LaneMask lm = lane_mask(win, rw.pos, a0 + 4 * h, j1);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = sees(lm, reg_row(r)) ? s[r] : 0.f;
-                    over |= tile_not_finite<T, D, 32>(kt, 32 * k, lane);
-                }
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ref)) * (p[r] - delta);
+                if (!full) hide(s, lane_mask(win, rw.pos, a0 + 4 * h, j1), 0.f);
                 if constexpr (BIAS) {
                     
                     if (is_above | is_below) {
@@ -172,13 +158,14 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
                         above += is_above ? sum : 0.f;
                         below += is_above ? 0.f : sum;
                     } else if constexpr (POS) {
+                        const int at = bias_at(a0 + 4 * h - rw.pos, reach);
                         if (row < it.nq) {
 #pragma unroll
                             for (int r = 0; r < 16; ++r)
                                 __hip_atomic_fetch_add(bins + bucket[at + reg_row(r)] * 64 + lane, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                         }
                     } else {
-                        float* mine = shear + 32 + (lane & 31) * 64 + 4 * h;
+                        float* mine = shear + 32 + (lane & 31) * kShearRow + 4 * h;
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
                             V4<float> y;
@@ -192,7 +179,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
                         const float* from = shear + 32 + lane - 31;
                         float sum = 0.f;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) sum += from[i * 65];
+                        for (int i = 0; i < 32; ++i) sum += from[i * (kShearRow + 1)];
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                         __builtin_amdgcn_wave_barrier();
                         const int dist = a0 + lane - 31 - (it.pos0 + 32 * w) + reach + kFarPad;
@@ -207,13 +194,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
                 }
             }
         }
-        if (t + 1 < n) {
-            sk.store(smem + ((t + 1) & 1) * kBytes, tid);
-            sv.store(smem + (2 + ((t + 1) & 1)) * kBytes, tid);
-        }
+        if (t + 1 < n) put(t + 1);
         __syncthreads();
     }
-    if (over) {
+    if (__syncthreads_or((int)odd)) {
         float t[16 * DT];
         dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, item, qrow, grow, hk, rw.pos, ref, delta, bias, h);
         take<DT>(acc, t);
@@ -267,35 +251,57 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
     }
 }
 
-// dtable[b][head] from the tiles' sums, in 64 bits and in a fixed order: sixteen wavefronts take tiles, their lanes distances
-template <typename T>
-__global__ __launch_bounds__(1024) void attn_dtable_kernel(AttnArgs a, int n_items) {
-    __shared__ double part[16];
-    const int nb = a.bias.n_buckets, reach = a.bias.reach, b = blockIdx.x % nb, head = blockIdx.x / nb;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    double x = 0.0;
-    if (a.has_pos) {
-        for (int i = threadIdx.x; i < n_items; i += 1024) x += (double)a.part_bias[((int64_t)head * n_items + i) * nb + b];
-    } else {
-        const int words = 2 * reach + 1 + 2 * kFarPad;
-        for (int i = lane; i < words; i += 64) {
-            const int of = min(max(a.bias.buckets[min(max(i - kFarPad, 0), 2 * reach)], 0), nb - 1);
-            if (of != b) continue;
-            const float* p = a.part_bias + (int64_t)head * n_items * words + i;
-#pragma unroll 4
-            for (int k = w; k < n_items; k += 16) x += (double)p[(int64_t)k * words];
-        }
-    }
-    for (int k = 32; k; k >>= 1) x += __shfl_xor(x, k);
-    if (lane == 0) part[w] = x;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < 16; ++k) x += part[k];
-        static_cast<T*>(a.dtable)[(int64_t)b * a.heads + head] = (T)(float)x;
+// The bias gradient from the tiles' sums, in 64 bits and in a fixed order.  First the tiles of a head in up to 64 groups, one
+// thread a word, then one block a head adds the groups up and takes the words of each bucket together.
+__global__ __launch_bounds__(256) void attn_dtable_groups_kernel(const float* part, double* groups, int n_items, int words, int per) {
+    const int head = blockIdx.y, first = blockIdx.x * per, last = min(first + per, n_items);
+    for (int i = threadIdx.x; i < words; i += 256) {
+        const float* p = part + ((int64_t)head * n_items + first) * words + i;
+        double x = 0.0;
+#pragma unroll 8
+        for (int k = 0; k < last - first; ++k) x += (double)p[(int64_t)k * words];
+        groups[((int64_t)head * gridDim.x + blockIdx.x) * words + i] = x;
     }
 }
+template <typename T>
+__global__ __launch_bounds__(1024) void attn_dtable_kernel(AttnArgs a, const double* groups, int n, int words) {
+    __shared__ double word[2 * 1024 + 1 + 2 * kFarPad];
+    __shared__ int of[2 * 1024 + 1 + 2 * kFarPad];
+    __shared__ double part[1024];
+    const int nb = a.bias.n_buckets, reach = a.bias.reach, head = blockIdx.x, tid = threadIdx.x;
+    for (int i = tid; i < words; i += 1024) {
+        const double* p = groups + (int64_t)head * n * words + i;
+        double x = 0.0;
+#pragma unroll 8
+        for (int k = 0; k < n; ++k) x += p[(int64_t)k * words];
+        word[i] = x;
+        of[i] = a.has_pos ? i : min(max(a.bias.buckets[min(max(i - kFarPad, 0), 2 * reach)], 0), nb - 1);
+    }
+    __syncthreads();
+    const int b = tid & 63, w = tid >> 6;     // the sixteen wavefronts take every sixteenth word
+    double x = 0.0;
+    for (int i = w; i < words; i += 16) x += of[i] == b ? word[i] : 0.0;
+    part[tid] = x;
+    __syncthreads();
+    if (tid < nb) {
+        for (int k = 1; k < 16; ++k) x += part[64 * k + tid];
+        static_cast<T*>(a.dtable)[(int64_t)tid * a.heads + head] = (T)(float)x;
+    }
+}
+template <typename T>
+hipError_t dtable_of(const AttnArgs& a, int n_items, hipStream_t s) {
+    const int words = dtable_words(a.has_pos, a.bias.n_buckets, a.bias.reach), n = dtable_groups(n_items);
+    if (n) {
+        const int per = (n_items + n - 1) / n;
+        hipLaunchKernelGGL(attn_dtable_groups_kernel, dim3(n, a.heads), dim3(256), 0, s, (const float*)a.part_bias, a.part_groups, n_items, words, per);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(attn_dtable_kernel<T>, dim3(a.heads), dim3(1024), 0, s, a, (const double*)a.part_groups, n, words);
+    return hipGetLastError();
+}
 
-// A wavefront's keys of dk and dv once more, pair by pair (see tile_not_finite).
+// A wavefront's keys of dk and dv once more, pair by pair (see Stage::not_finite).
 template <typename T, int D, int DT, bool BIAS>
 DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int item, const T* k, const T* v, int hk, int j, int h) {
     const KItem& it = reinterpret_cast<const KItem*>(a.plan + a.items_at)[item];
@@ -309,12 +315,12 @@ DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int item, c
             const int pos = row_position(a.plan, a.has_pos, a.pos_at, it.pos0, it.q0, i);
             const T* q = row_ptr<T>(a.q, row, head);
             const T* g = row_ptr<T>(a.dout, row, head);
-            float s = dot_rows<T, D>(q, k) * c;
+            float s = dot_rows<T, D>(q, k);
             if constexpr (BIAS) {
                 const int at = min(max(a.bias.buckets[min(max(j - pos, -a.bias.reach), a.bias.reach) + a.bias.reach], 0), a.bias.n_buckets - 1);
-                s += bias_value((float)static_cast<const T*>(a.bias.table)[(int64_t)at * a.heads + head]);
+                s += bias_value((float)static_cast<const T*>(a.bias.table)[(int64_t)at * a.heads + head], 1.f / a.scale);
             }
-            const float p = __builtin_amdgcn_exp2f(s - lse_log2(a.lse[(int64_t)head * a.q_rows + row]));
+            const float p = __builtin_amdgcn_exp2f(s * c - lse_log2(a.lse[(int64_t)head * a.q_rows + row]));
             const float ds = p * (dot_rows<T, D>(g, v) - a.delta[(int64_t)head * a.q_rows + row]);
             const bool see = visible(win, j - pos, j);
 #pragma unroll 1
@@ -364,19 +370,18 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
-    bool over = false;
-
     const int nt = (it.qe - it.qb + kBQ - 1) / kBQ;
     const int64_t qstep = a.q.row * (int)sizeof(T), gstep = a.dout.row * (int)sizeof(T);
-    Stage<T, D, kBQ, NW * 64> sq, sg;
+    Stage<T, D, kBQ, NW * 64> sq(qstep, tid), sg(gstep, tid);
+    unsigned odd = 0;
     float nref = 0.f, ndelta = 0.f;
     int npos = 0;
     auto fetch = [&](int head, int t) {
         const int i0 = it.qb + t * kBQ;
         const int64_t r0 = (int64_t)it.q0 + i0;
         const int valid = it.qe - i0;
-        sq.load(reinterpret_cast<const char*>(row_ptr<T>(a.q, r0, head)), qstep, valid, tid);
-        sg.load(reinterpret_cast<const char*>(row_ptr<T>(a.dout, r0, head)), gstep, valid, tid);
+        sq.load(reinterpret_cast<const char*>(row_ptr<T>(a.q, r0, head)), valid, tid);
+        sg.load(reinterpret_cast<const char*>(row_ptr<T>(a.dout, r0, head)), valid, tid);
         if (tid < kBQ) {
             const int64_t at = (int64_t)head * a.q_rows + r0 + min(tid, valid - 1);
             // rows behind the last weigh nothing: their reference is +inf
@@ -385,9 +390,11 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
             npos = a.has_pos ? a.plan[a.pos_at + it.q0 + i0 + min(tid, valid - 1)] : 0;
         }
     };
-    auto put = [&](int buf) {
+    auto put = [&](int t) {
+        const int buf = t & 1, i0 = it.qb + t * kBQ, i1 = min(i0 + kBQ, it.qe);
         sq.store(smem + buf * kBytes, tid);
         sg.store(smem + (2 + buf) * kBytes, tid);
+        if (a.has_pos || !all_visible(win, it.pos0 + i0, it.pos0 + i1 - 1, it.j0, it.j0 + it.nk)) odd |= sq.not_finite() | sg.not_finite();
         if (tid < kBQ) {
             rowref[buf * kBQ + tid] = nref;
             rowdelta[buf * kBQ + tid] = ndelta;
@@ -396,7 +403,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
     };
     for (int head = hk * a.group; head < (hk + 1) * a.group && nt > 0; ++head) {
         fetch(head, 0);
-        if constexpr (BIAS) load_bias<T>(bias, a.bias, a.heads, head, tid, NW * 64);
+        if constexpr (BIAS) load_bias<T>(bias, a.bias, 1.f / a.scale, a.heads, head, tid, NW * 64);
         put(0);
         __syncthreads();
         for (int t = 0; t < nt; ++t) {
@@ -419,37 +426,36 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
                 }
                 if (active && r0 < it.qe && !none_visible(win, pmin, pmax, j0, j1)) {
                     const bool full = all_visible(win, pmin, pmax, j0, j0 + 32);
-                    f32x16_a s, p;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = p[r] = 0.f;
-#pragma unroll
-                    for (int st = 0; st < ST; ++st) {
-                        mma(s, Tile<T, D>::row_frag(qt, 32 * u + (lane & 31), st, h), kf[st]);
-                        mma(p, Tile<T, D>::row_frag(gt, 32 * u + (lane & 31), st, h), vf[st]);
-                    }
                     const float* ref = rowref + buf * kBQ + 32 * u + 4 * h;
                     const float* del = rowdelta + buf * kBQ + 32 * u + 4 * h;
                     const int* pos = rowpos + buf * kBQ + 32 * u + 4 * h;
                     const int far = j - (it.pos0 + r0 + 4 * h);      // to the row of register 0, where the plan lists no positions
+                    f32x16_a s, p;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = p[r] = 0.f;
                     if constexpr (BIAS) {
                         const bool is_above = j0 - pmax >= reach, is_below = j0 + 31 - pmin <= -reach;
                         if (is_above | is_below) {
                             const float b = bias[is_above ? 2 * reach + kBiasPad : 0];
 #pragma unroll
-                            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, b);
+                            for (int r = 0; r < 16; ++r) s[r] = b;
                         } else if (a.has_pos) {
 #pragma unroll
-                            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, bias[bias_at(j - pos[reg_row(r)], reach)]);
+                            for (int r = 0; r < 16; ++r) s[r] = bias[bias_at(j - pos[reg_row(r)], reach)];
                         } else {
                             const float* b = bias + bias_at(far - kBiasPad, reach) + kBiasPad;
 #pragma unroll
-                            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, b[-reg_row(r)]);
+                            for (int r = 0; r < 16; ++r) s[r] = b[-reg_row(r)];
                         }
                     }
 #pragma unroll
+                    for (int st = 0; st < ST; ++st) {
+                        mma(s, Tile<T, D>::row_frag(qt, 32 * u + (lane & 31), st, h), kf[st]);
+                        mma(p, Tile<T, D>::row_frag(gt, 32 * u + (lane & 31), st, h), vf[st]);
+                    }
+#pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const float x = BIAS ? s[r] - ref[reg_row(r)] : fmaf(s[r], c, -ref[reg_row(r)]);
-                        s[r] = __builtin_amdgcn_exp2f(x);
+                        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ref[reg_row(r)]));
                         p[r] = s[r] * (p[r] - del[reg_row(r)]);
                     }
                     if (!full) {
@@ -470,7 +476,6 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
                                 p[r] = see ? p[r] : 0.f;
                             }
                         }
-                        over = over || tile_not_finite<T, D, 32>(qt, 32 * u, lane) || tile_not_finite<T, D, 32>(gt, 32 * u, lane);
                     }
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
@@ -483,11 +488,11 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
                     }
                 }
             }
-            if (t + 1 < nt) put((t + 1) & 1);
+            if (t + 1 < nt) put(t + 1);
             __syncthreads();
         }
     }
-    if (over) {
+    if (__syncthreads_or((int)odd)) {
         float x[16 * DT], y[16 * DT];
         dkv_by_pairs<T, D, DT, BIAS>(kernel_args(), x, y, id - hk * a.n_items, krow, vrow, hk, j, h);
         take<DT>(dk, x);
@@ -598,7 +603,5 @@ hipError_t dkv_join_dim(const AttnArgs& a, int n_join, int join_at, int tile_key
     hipError_t attn_dkv_join_##NAME(const AttnArgs& a, int dim, int n, int at, int keys, hipStream_t s) {                  \
         return DPTM_ATTN_BY_DIM(dkv_join_dim, a, n, at, keys, s);                                                          \
     }                                                                                                                      \
-    hipError_t attn_dtable_##NAME(const AttnArgs& a, int n_items, hipStream_t s) {                                         \
-        return start(attn_dtable_kernel<E>, (int64_t)a.bias.n_buckets * a.heads, 1024, 0, s, a, n_items);                  \
-    }                                                                                                                      \
+    hipError_t attn_dtable_##NAME(const AttnArgs& a, int n_items, hipStream_t s) { return dtable_of<E>(a, n_items, s); }   \
     }

@@ -19,47 +19,30 @@ template <> constexpr float kShift<float> = 0.f;
 constexpr float kLazy = 4.f;
 
 // keys of a tile in LDS: 64 where the registers that carry the next tile allow it
-template <typename T, int D> constexpr int kKeysPerTile = sizeof(T) == 2 && D <= 64 ? 64 : 32;
+template <typename T, int D> constexpr int kKeysPerTile = sizeof(T) == 2 ? 64 : 32;
 
 // what a wavefront knows of its 32 queries
 struct Rows {
     int pos, pmin, pmax;
 };
 
-// scores of 32 NK keys -> weights (in place), running maximum and sum, accumulators moved to the new maximum
-template <typename T, int NK, int DT, bool BIAS>
+// scores of 32 NK keys -> weights (in place), running maximum and sum, accumulators moved to the new maximum.  Per element
+// a multiply-add, an exp2, half a three-way maximum, an add and half a conversion: with head dimension 64 that is
+// half as long again as the element's matrix instructions, which is why nothing else is done per element.
+template <typename T, int NK, int DT>
 __device__ __forceinline__ void softmax_step(f32x16_a (&s)[NK], f32x16_a (&acc)[DT], float& m, float& l, float c, const Rows& w,
-                                             const Window& win, int j0, int j1, bool full, const float* bias, int reach, int h) {
-    if constexpr (BIAS) {
-#pragma unroll
-        for (int k = 0; k < NK; ++k) {
-            const int a = j0 + 32 * k, z = a + 31;
-            if (a - w.pmax >= reach || z - w.pmin <= -reach) {   // one value for the whole tile
-                const float b = bias[a - w.pmax >= reach ? 2 * reach + kBiasPad : 0];
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[k][r] = fmaf(s[k][r], c, b);
-            } else {
-                const float* b = bias + bias_at(a + 4 * h - w.pos, reach);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[k][r] = fmaf(s[k][r], c, b[reg_row(r)]);
-            }
-        }
-    }
+                                             const Window& win, int j0, int j1, bool full, int h) {
     if (!full) {
 #pragma unroll
-        for (int k = 0; k < NK; ++k) {
-            const LaneMask lm = lane_mask(win, w.pos, j0 + 32 * k + 4 * h, j1);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[k][r] = sees(lm, reg_row(r)) ? s[k][r] : kMinusInf;
-        }
+        for (int k = 0; k < NK; ++k) hide(s[k], lane_mask(win, w.pos, j0 + 32 * k + 4 * h, j1), kMinusInf);
     }
     float mx = s[0][0];
 #pragma unroll
     for (int k = 0; k < NK; ++k)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[k][r]);
+    mx *= c;
     mx = half_max(mx);
-    if constexpr (!BIAS) mx *= c;
     const bool grow = mx > m + kLazy || (m == kMinusInf && mx > m);
     if (__ballot(grow)) {
         const float alpha = grow ? __builtin_amdgcn_exp2f(m - mx) : 1.f;
@@ -76,7 +59,7 @@ __device__ __forceinline__ void softmax_step(f32x16_a (&s)[NK], f32x16_a (&acc)[
     for (int k = 0; k < NK; ++k)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float p = __builtin_amdgcn_exp2f(BIAS ? s[k][r] - ref : fmaf(s[k][r], c, -ref));
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[k][r], c, -ref));
             s[k][r] = p;
             sum += p;
         }
@@ -135,8 +118,9 @@ DPTM_COLD void forward_by_pairs(const AttnArgs& a, float* acc, float* ml, int it
     for (int t = first; t < n; t += every) {
         const int j0 = t < ns ? t * keys : it.kb + (t - ns) * keys, j1 = min(j0 + keys, t < ns ? it.sink_end : it.ke);
         for (int j = j0; j < j1; ++j) {
-            float s = dot_rows<T, D>(q, row_ptr<T>(a.k, (int64_t)it.k0 + j, hk)) * c;
+            float s = dot_rows<T, D>(q, row_ptr<T>(a.k, (int64_t)it.k0 + j, hk));
             if constexpr (BIAS) s += bias[bias_at(j - pos, a.bias.reach)];
+            s *= c;
             s = visible(win, j - pos, j) ? s : kMinusInf;
             const float top = fmaxf(m, s), f = m == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(m - top);
             const float p = s == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(s - top + kShift<T>);
@@ -176,7 +160,7 @@ __device__ __forceinline__ Rows rows_of(const AttnArgs& a, int q0, int pos0, int
 
 // ---- many queries: NW wavefronts of 32 queries share tiles of keys and values in LDS (two buffers, one barrier a tile)
 template <typename T, int D, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64, 2) void attn_fwd_wide_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, D <= 64 && sizeof(T) == 2 ? 3 : 2) void attn_fwd_wide_kernel(AttnArgs a) {
     constexpr int kBK = kKeysPerTile<T, D>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
     constexpr int kBytes = kBK * D * (int)sizeof(T);
     extern __shared__ char smem[];
@@ -204,11 +188,18 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_wide_kernel(AttnArgs a) {
     const int64_t kstep = a.k.row * (int)sizeof(T), vstep = a.v.row * (int)sizeof(T);
     const int ns = (it.sink_end + kBK - 1) / kBK, n = ns + (it.ke - it.kb + kBK - 1) / kBK;
 
-    Stage<T, D, kBK, NW * 64> sk, sv;
+    Stage<T, D, kBK, NW * 64> sk(kstep, tid), sv(vstep, tid);
     auto fetch = [&](int t) {
         const int j0 = t < ns ? t * kBK : it.kb + (t - ns) * kBK, j1 = t < ns ? it.sink_end : it.ke;
-        sk.load(kbase + j0 * kstep, kstep, j1 - j0, tid);
-        sv.load(vbase + j0 * vstep, vstep, j1 - j0, tid);
+        sk.load(kbase + j0 * kstep, j1 - j0, tid);
+        sv.load(vbase + j0 * vstep, j1 - j0, tid);
+    };
+    unsigned odd = 0;
+    auto put = [&](int t) {
+        const int j0 = t < ns ? t * kBK : it.kb + (t - ns) * kBK, j1 = min(j0 + kBK, t < ns ? it.sink_end : it.ke);
+        sk.store(smem + (t & 1) * kBytes, tid);
+        sv.store(smem + (2 + (t & 1)) * kBytes, tid);
+        if (a.has_pos || !all_visible(win, it.pos0, it.pos0 + it.nq - 1, j0, j1)) odd |= sv.not_finite();
     };
     f32x16_a acc[DT];
 #pragma unroll
@@ -216,14 +207,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_wide_kernel(AttnArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
     float m = kMinusInf, l = 0.f;
-    bool over = false;
 
     if (n > 0) fetch(0);
-    if constexpr (BIAS) load_bias<T>(bias, a.bias, a.heads, head, tid, NW * 64);
-    if (n > 0) {
-        sk.store(smem, tid);
-        sv.store(smem + 2 * kBytes, tid);
-    }
+    if constexpr (BIAS) load_bias<T>(bias, a.bias, 1.f / a.scale, a.heads, head, tid, NW * 64);
+    if (n > 0) put(0);
     __syncthreads();
     for (int t = 0; t < n; ++t) {
         if (t + 1 < n) fetch(t + 1);
@@ -235,22 +222,23 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_wide_kernel(AttnArgs a) {
             f32x16_a s[NK];
 #pragma unroll
             for (int k = 0; k < NK; ++k) {
+                if constexpr (BIAS) {
+                    const int k0 = j0 + 32 * k;
+                    init_bias(s[k], bias, a.bias.reach, k0 + 4 * h - rw.pos, k0 - rw.pmax >= a.bias.reach, k0 + 31 - rw.pmin <= -a.bias.reach);
+                } else {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[k][r] = 0.f;
+                    for (int r = 0; r < 16; ++r) s[k][r] = 0.f;
+                }
 #pragma unroll
                 for (int st = 0; st < ST; ++st) mma(s[k], Tile<T, D>::row_frag(kt, 32 * k + (lane & 31), st, h), q[st]);
             }
-            softmax_step<T, NK, DT, BIAS>(s, acc, m, l, c, rw, win, j0, j1, full, bias, a.bias.reach, h);
+            softmax_step<T, NK, DT>(s, acc, m, l, c, rw, win, j0, j1, full, h);
             weighted_values<T, D, NK, DT>(acc, s, vt, lane);
-            if (!full) over |= tile_not_finite<T, D, kBK>(vt, 0, lane);
         }
-        if (t + 1 < n) {
-            sk.store(smem + ((t + 1) & 1) * kBytes, tid);
-            sv.store(smem + (2 + ((t + 1) & 1)) * kBytes, tid);
-        }
+        if (t + 1 < n) put(t + 1);
         __syncthreads();
     }
-    if (over) {
+    if (__syncthreads_or((int)odd)) {
         float t[16 * DT], ml[2];
         forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, ml, id - head * a.n_items, row_ptr<T>(a.q, (int64_t)it.q0 + rowc, head), hk, rw.pos, 0, 1, kBK,
                                          bias, h);
@@ -305,18 +293,18 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_split_kernel(AttnArgs a) {
     const int64_t kstep = a.k.row * (int)sizeof(T), vstep = a.v.row * (int)sizeof(T);
     const int ns = (it.sink_end + 31) / 32, n = ns + (it.ke - it.kb + 31) / 32;
     V8<T> kf[ST];
-    Stage<T, D, 32, 64> sv;
+    Stage<T, D, 32, 64> sv(vstep, lane);
     char* vt = tiles + w * kBytes;
     auto fetch = [&](int t) {
         const int j0 = t < ns ? t * 32 : it.kb + (t - ns) * 32, j1 = t < ns ? it.sink_end : it.ke;
         const char* krow = kbase + min(j0 + (lane & 31), j1 - 1) * kstep;
 #pragma unroll
         for (int s = 0; s < ST; ++s) kf[s] = global_frag<T>(krow, s, h);
-        sv.load(vbase + j0 * vstep, vstep, j1 - j0, lane);
+        sv.load(vbase + j0 * vstep, j1 - j0, lane);
     };
     if (w < n) fetch(w);
     if constexpr (BIAS) {
-        for (int p = 0; p < pack; ++p) load_bias<T>(bias + p * room, a.bias, a.heads, head0 + p, tid, 256);
+        for (int p = 0; p < pack; ++p) load_bias<T>(bias + p * room, a.bias, 1.f / a.scale, a.heads, head0 + p, tid, 256);
         __syncthreads();
         bias += (head - head0) * room;
     }
@@ -326,25 +314,29 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_split_kernel(AttnArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
     float m = kMinusInf, l = 0.f;
-    bool over = false;
+    unsigned odd = 0;
     for (int t = w; t < n; t += NW) {
         const int j0 = t < ns ? t * 32 : it.kb + (t - ns) * 32, j1 = min(j0 + 32, t < ns ? it.sink_end : it.ke);
         f32x16_a s[1];
+        if constexpr (BIAS) {
+            init_bias(s[0], bias, a.bias.reach, j0 + 4 * h - rw.pos, j0 - rw.pmax >= a.bias.reach, j0 + 31 - rw.pmin <= -a.bias.reach);
+        } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+            for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+        }
 #pragma unroll
         for (int st = 0; st < ST; ++st) mma(s[0], kf[st], q[st]);
+        const bool full = j1 - j0 == 32 && all_visible(win, rw.pmin, rw.pmax, j0, j1);
         __builtin_amdgcn_wave_barrier();
         sv.store(vt, lane);
+        if (!full) odd |= sv.not_finite();
         if (t + NW < n) fetch(t + NW);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        const bool full = j1 - j0 == 32 && all_visible(win, rw.pmin, rw.pmax, j0, j1);
-        softmax_step<T, 1, DT, BIAS>(s, acc, m, l, c, rw, win, j0, j1, full, bias, a.bias.reach, h);
+        softmax_step<T, 1, DT>(s, acc, m, l, c, rw, win, j0, j1, full, h);
         weighted_values<T, D, 1, DT>(acc, s, vt, lane);
-        if (!full) over |= tile_not_finite<T, D, 32>(vt, 0, lane);
     }
-    if (over) {
+    if (__ballot(odd != 0)) {
         float t[16 * DT], x[2];
         forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, x, id - id / a.n_items * a.n_items, qrow, hk, rw.pos, w, NW, 32, bias, h);
         take<DT>(acc, t);

@@ -56,6 +56,7 @@ struct AttnArgs {
     float* part_o;         // forward partials [slot * heads + h][32][D]; backward: dk | dv partials
     float* part_ml;        // the same [32][2]
     float* part_bias;      // [heads][n_dq][dtable_words]
+    double* part_groups;   // [heads][dtable_groups][dtable_words]
     void* dtable;          // [n_buckets][heads]
     const int* plan;       // device copy
     BiasArgs bias;
@@ -81,6 +82,8 @@ DPTM_ATTN_LAUNCHERS(f32)
 // bucket where the plan lists positions
 constexpr int kFarPad = 62;
 inline int dtable_words(int has_pos, int n_buckets, int reach) { return has_pos ? n_buckets : 2 * reach + 1 + 2 * kFarPad; }
+
+inline int dtable_groups(int n_items) { return n_items < 64 ? n_items : 64; }
 
 struct NormRopeArgs {
     Strided x[2], y[2], dy[2], dx[2];   // q and k

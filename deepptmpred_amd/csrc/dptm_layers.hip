@@ -74,7 +74,9 @@ int check_rows(const char* who, const char* name, const dptm_rows& t, int64_t ro
     if ((reinterpret_cast<uintptr_t>(t.data) & 15) || (t.row_stride * size) % 16 || (t.head_stride * size) % 16)
         return fail(DPTM_EINVAL, at() + ": address and strides must be multiples of 16 bytes");
     if (t.row_stride < 0 || t.head_stride < 0) return fail(DPTM_EINVAL, at() + ": negative stride");
-    if (t.row_stride > (int64_t(1) << 40) || t.head_stride > (int64_t(1) << 40)) return fail(DPTM_EINVAL, at() + ": stride too large");
+    // a tile's rows are reached by 32-bit offsets from the first
+    if (t.row_stride * size >= (int64_t(1) << 25) || t.head_stride > (int64_t(1) << 40))
+        return fail(DPTM_EINVAL, at() + ": row stride of 32 MiB or more");
     if (written) {
         const bool rows_outside = (heads == 1 || t.head_stride >= dim) && (rows == 1 || t.row_stride >= (heads - 1) * t.head_stride + dim);
         const bool heads_outside = (rows == 1 || t.row_stride >= dim) && (heads == 1 || t.head_stride >= (rows - 1) * t.row_stride + dim);
@@ -206,8 +208,9 @@ int make_plan(const dptm_attention_desc& d, const int32_t* q_len, const int32_t*
     if (mode == kSplitKeys) {
         int64_t total = 0;
         for (const QItem& it : fwd) total += m.keys(it);
-        // keys of a workgroup: at least two tiles of each of its four wavefronts, and no more parts than fill the card
-        const int64_t chunk = std::max<int64_t>(256, up((total * (d.heads / pack) + kGroups - 1) / kGroups, 128));
+        // keys of a workgroup: at least four tiles of each of its four wavefronts (joining parts takes a launch of 4 us), and no
+        // more parts than fill the card
+        const int64_t chunk = std::max<int64_t>(512, up((total * (d.heads / pack) + kGroups - 1) / kGroups, 128));
         std::vector<QItem> cut;
         for (const QItem& it : fwd) {
             const int64_t n = it.ke - it.kb, parts = std::max<int64_t>(1, (n + chunk - 1) / chunk);
@@ -324,7 +327,7 @@ int check_plan(const char* who, const int32_t* plan, const int32_t* plan_dev) {
 }
 
 // byte sizes of the workspace's parts, each rounded up to 256
-struct Work { size_t fwd_o, fwd_ml, delta, dkv, bias; };
+struct Work { size_t fwd_o, fwd_ml, delta, dkv, bias, groups; };
 Work work_of(const int32_t* p, int n_buckets, int reach) {
     Work w;
     const size_t dim = p[kPlanHeadDim], heads = p[kPlanHeads], kv = p[kPlanKvHeads];
@@ -333,6 +336,7 @@ Work work_of(const int32_t* p, int n_buckets, int reach) {
     w.delta = up(heads * (size_t)p[kPlanQRows] * 4, 256);
     w.dkv = up((size_t)p[kPlanDkvSlots] * kv * 2 * 32 * (size_t)p[kPlanDkvWaves] * dim * 4, 256);
     w.bias = up(heads * (size_t)p[kPlanDq] * (size_t)(n_buckets ? dtable_words(p[kPlanHasPos], n_buckets, reach) : 0) * 4, 256);
+    w.groups = n_buckets ? up(heads * (size_t)dtable_groups(p[kPlanDq]) * (size_t)dtable_words(p[kPlanHasPos], n_buckets, reach) * 8, 256) : 0;
     return w;
 }
 
@@ -417,7 +421,7 @@ int64_t dptm_attention_workspace(const int32_t* plan, int32_t n_buckets, int32_t
     if (max_distance < 0 || max_distance > kMaxReach)
         return fail(DPTM_EINVAL, "dptm_attention_workspace: a largest distance of 0 to 1024 is supported");
     const Work w = work_of(plan, n_buckets, max_distance);
-    return (int64_t)(backward ? w.delta + w.dkv + w.bias : w.fwd_o + w.fwd_ml);
+    return (int64_t)(backward ? w.delta + w.dkv + w.bias + w.groups : w.fwd_o + w.fwd_ml);
 } catch (...) {
     return on_exception("dptm_attention_workspace");
 }
@@ -463,7 +467,7 @@ int dptm_attention_backward(const dptm_attention_args* args) try {
     AttnArgs a = common_args(plan, x.plan_dev, x.scale);
     OK_OR_RETURN(check_bias(who, x, &a.bias));
     const Work w = work_of(plan, a.bias.n_buckets, a.bias.reach);
-    OK_OR_RETURN(check_common(who, x, w.delta + w.dkv + w.bias));
+    OK_OR_RETURN(check_common(who, x, w.delta + w.dkv + w.bias + w.groups));
     const int heads = plan[kPlanHeads], kv = plan[kPlanKvHeads], dim = plan[kPlanHeadDim], dtype = x.dtype;
     const int64_t nq = plan[kPlanQRows], nk = plan[kPlanKRows];
     OK_OR_RETURN(check_rows(who, "dout", x.dout, nq, heads, dim, dtype, false, &a.dout));
@@ -481,6 +485,7 @@ int dptm_attention_backward(const dptm_attention_args* args) try {
     a.delta = static_cast<float*>(x.workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(x.workspace) + w.delta);
     a.part_bias = reinterpret_cast<float*>(static_cast<char*>(x.workspace) + w.delta + w.dkv);
+    a.part_groups = reinterpret_cast<double*>(static_cast<char*>(x.workspace) + w.delta + w.dkv + w.bias);
     a.dtable = x.dtable;
     const OnDevice on(x.device);
     if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");

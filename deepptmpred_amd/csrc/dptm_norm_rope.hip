@@ -30,30 +30,33 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 
 struct Angles { float c0[8], s0[8], c1[8], s1[8]; };   // of the first and the second eight elements, per element
 
-template <int D>
-__device__ __forceinline__ void load_angles(const NormRopeArgs& a, int64_t row, int chunk, bool neighbours, Angles& g) {
-    const int64_t pos = a.positions ? (int64_t)a.positions[row] : row;
-    if (pos < 0 || pos >= a.n_pos) {      // no such angle: the row says so
-#pragma unroll
-        for (int e = 0; e < 8; ++e) g.c0[e] = g.s0[e] = g.c1[e] = g.s1[e] = __builtin_nanf("");
-        return;
-    }
-    const float* c = a.cosv + pos * (D / 2);
-    const float* s = a.sinv + pos * (D / 2);
-    if (neighbours) {
+template <int D, bool NEIGHBOURS>
+__device__ __forceinline__ void load_angles(const float* cosv, const float* sinv, const int* positions, int n_pos, int64_t row, int chunk, Angles& g) {
+    const int64_t want = positions ? (int64_t)positions[row] : row;
+    const bool there = want >= 0 && want < n_pos;
+    const int64_t pos = there ? want : 0;
+    const float* c = cosv + pos * (D / 2);
+    const float* s = sinv + pos * (D / 2);
+    // no such angle: the row says so
+    const float none = __builtin_nanf("");
+    if constexpr (NEIGHBOURS) {
         typedef float f4 __attribute__((ext_vector_type(4)));
-        const f4 cl = *reinterpret_cast<const f4*>(c + 4 * chunk), ch = *reinterpret_cast<const f4*>(c + D / 4 + 4 * chunk);
-        const f4 sl = *reinterpret_cast<const f4*>(s + 4 * chunk), sh = *reinterpret_cast<const f4*>(s + D / 4 + 4 * chunk);
+        f4 cl{none, none, none, none}, ch = cl, sl = cl, sh = cl;
+        if (there) {
+            cl = *reinterpret_cast<const f4*>(c + 4 * chunk), ch = *reinterpret_cast<const f4*>(c + D / 4 + 4 * chunk);
+            sl = *reinterpret_cast<const f4*>(s + 4 * chunk), sh = *reinterpret_cast<const f4*>(s + D / 4 + 4 * chunk);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             g.c0[e] = cl[e / 2], g.s0[e] = sl[e / 2];
             g.c1[e] = ch[e / 2], g.s1[e] = sh[e / 2];
         }
     } else {
-        load8<float>(c + 8 * chunk, g.c0);
-        load8<float>(s + 8 * chunk, g.s0);
+        typedef float f8 __attribute__((ext_vector_type(8)));
+        f8 cl{none, none, none, none, none, none, none, none}, sl = cl;
+        if (there) cl = *reinterpret_cast<const f8*>(c + 8 * chunk), sl = *reinterpret_cast<const f8*>(s + 8 * chunk);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g.c1[e] = g.c0[e], g.s1[e] = g.s0[e];
+        for (int e = 0; e < 8; ++e) g.c0[e] = g.c1[e] = cl[e], g.s0[e] = g.s1[e] = sl[e];
     }
 }
 
@@ -88,79 +91,101 @@ __device__ __forceinline__ float sum_of(float v) {
 
 constexpr int kThreads = 256;
 
-// One block takes kThreads / (D / 16) units of (row, first head); a thread goes on with the heads head + hstep, ...
-// GRAD: the backward pass, with the sums for the gain gradients kept over all units of the block.
-template <typename T, int D, bool NEIGHBOURS, bool GRAD>
+// a head's place: the tensors of q and k lie apart; both addresses are formed and one chosen, because a choice between the
+// arguments themselves would move those to private memory
+template <typename T>
+__device__ __forceinline__ T* head_ptr(Strided q, Strided k, bool isk, int64_t row, int head, int chunk) {
+    T* pq = static_cast<T*>(q.p) + row * q.row + head * q.head + 8 * chunk;
+    T* pk = static_cast<T*>(k.p) + row * k.row + head * k.head + 8 * chunk;
+    return isk ? pk : pq;
+}
+
+// One block takes kThreads / (D / 16) units of (row, first head) at a time; a thread has the heads head, head + hstep, ...
+// (HEADS of them), all asked for before the first is used.  GRAD: the backward pass, with the sums for the gain
+// gradients kept over all units of the block.
+template <typename T, int D, bool NEIGHBOURS, bool GRAD, int HEADS>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs a, int hstep, int64_t units) {
     constexpr int L = D / 16;
     const int chunk = threadIdx.x % L, all = a.heads[0] + a.heads[1];
-    float g0[2][8], g1[2][8], d0[2][8], d1[2][8];
+    const bool norm_q = a.gain[0] != nullptr, norm_k = a.gain[1] != nullptr;
+    const int heads_q = a.heads[0];
+    float gq0[8], gq1[8], gk0[8], gk1[8], d0[2][8], d1[2][8];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            g0[t][e] = a.gain[t] ? a.gain[t][8 * chunk + e] : 1.f;
-            g1[t][e] = a.gain[t] ? a.gain[t][D / 2 + 8 * chunk + e] : 1.f;
-            d0[t][e] = d1[t][e] = 0.f;
-        }
+    for (int e = 0; e < 8; ++e) {
+        gq0[e] = gq1[e] = gk0[e] = gk1[e] = 1.f;
+        d0[0][e] = d0[1][e] = d1[0][e] = d1[1][e] = 0.f;
+    }
+    if (norm_q) load8<float>(a.gain[0] + 8 * chunk, gq0), load8<float>(a.gain[0] + D / 2 + 8 * chunk, gq1);
+    if (norm_k) load8<float>(a.gain[1] + 8 * chunk, gk0), load8<float>(a.gain[1] + D / 2 + 8 * chunk, gk1);
     // a whole group of lanes runs out of units together: units are counted per group
     for (int64_t u = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L; u < units; u += (int64_t)gridDim.x * (kThreads / L)) {
         const int64_t row = u / hstep;
+        const int first = (int)(u - row * hstep);
+        float x0[HEADS][8], x1[HEADS][8], y0[HEADS][8], y1[HEADS][8];
+#pragma unroll
+        for (int i = 0; i < HEADS; ++i) {
+            const int head = first + i * hstep;
+            if (head >= all) break;
+            const bool isk = head >= heads_q;
+            const int hh = isk ? head - heads_q : head;
+            const T* px = head_ptr<T>(a.x[0], a.x[1], isk, row, hh, chunk);
+            load8<T>(px, x0[i]);
+            load8<T>(px + D / 2, x1[i]);
+            if constexpr (GRAD) {
+                const T* pd = head_ptr<T>(a.dy[0], a.dy[1], isk, row, hh, chunk);
+                load8<T>(pd, y0[i]);
+                load8<T>(pd + D / 2, y1[i]);
+            }
+        }
         Angles ang;
-        load_angles<D>(a, row, chunk, NEIGHBOURS, ang);
-        for (int head = (int)(u - row * hstep); head < all; head += hstep) {
-            const bool isk = head >= a.heads[0];
-            const int t = isk ? 1 : 0, hh = isk ? head - a.heads[0] : head;
-            const bool norm = a.gain[t] != nullptr;
-            const T* px = static_cast<const T*>(a.x[t].p) + row * a.x[t].row + hh * a.x[t].head + 8 * chunk;
-            float x0[8], x1[8];
-            load8<T>(px, x0);
-            load8<T>(px + D / 2, x1);
+        load_angles<D, NEIGHBOURS>(a.cosv, a.sinv, a.positions, a.n_pos, row, chunk, ang);
+#pragma unroll
+        for (int i = 0; i < HEADS; ++i) {
+            const int head = first + i * hstep;
+            if (head >= all) break;
+            const bool isk = head >= heads_q, norm = isk ? norm_k : norm_q;
+            const int hh = isk ? head - heads_q : head;
             float r = 1.f;
             if (norm) {
                 float ss = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) ss = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], ss));
+                for (int e = 0; e < 8; ++e) ss = fmaf(x0[i][e], x0[i][e], fmaf(x1[i][e], x1[i][e], ss));
                 // sqrt and divide, not the approximate reciprocal root: the norm is part of every output
                 r = 1.f / sqrtf(sum_of<L>(ss) * (1.f / D) + a.eps);
             }
             if constexpr (!GRAD) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    x0[e] *= r * (isk ? g0[1][e] : g0[0][e]);
-                    x1[e] *= r * (isk ? g1[1][e] : g1[0][e]);
+                    x0[i][e] *= r * (isk ? gk0[e] : gq0[e]);
+                    x1[i][e] *= r * (isk ? gk1[e] : gq1[e]);
                 }
-                rotate<NEIGHBOURS>(x0, x1, ang, 1.f);
-                T* py = static_cast<T*>(a.y[t].p) + row * a.y[t].row + hh * a.y[t].head + 8 * chunk;
-                store8<T>(py, x0);
-                store8<T>(py + D / 2, x1);
+                rotate<NEIGHBOURS>(x0[i], x1[i], ang, 1.f);
+                T* py = head_ptr<T>(a.y[0], a.y[1], isk, row, hh, chunk);
+                store8<T>(py, x0[i]);
+                store8<T>(py + D / 2, x1[i]);
             } else {
-                const T* pd = static_cast<const T*>(a.dy[t].p) + row * a.dy[t].row + hh * a.dy[t].head + 8 * chunk;
-                float y0[8], y1[8];
-                load8<T>(pd, y0);
-                load8<T>(pd + D / 2, y1);
-                rotate<NEIGHBOURS>(y0, y1, ang, -1.f);
+                rotate<NEIGHBOURS>(y0[i], y1[i], ang, -1.f);
                 if (norm) {
                     float dot = 0.f;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float z0 = y0[e] * x0[e] * r, z1 = y1[e] * x1[e] * r;
+                        const float z0 = y0[i][e] * x0[i][e] * r, z1 = y1[i][e] * x1[i][e] * r;
                         d0[0][e] += isk ? 0.f : z0, d1[0][e] += isk ? 0.f : z1;
                         d0[1][e] += isk ? z0 : 0.f, d1[1][e] += isk ? z1 : 0.f;
-                        y0[e] *= isk ? g0[1][e] : g0[0][e];
-                        y1[e] *= isk ? g1[1][e] : g1[0][e];
-                        dot = fmaf(y0[e], x0[e], fmaf(y1[e], x1[e], dot));
+                        y0[i][e] *= isk ? gk0[e] : gq0[e];
+                        y1[i][e] *= isk ? gk1[e] : gq1[e];
+                        dot = fmaf(y0[i][e], x0[i][e], fmaf(y1[i][e], x1[i][e], dot));
                     }
                     const float f = sum_of<L>(dot) * (1.f / D) * r * r;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        y0[e] = r * fmaf(-f, x0[e], y0[e]);
-                        y1[e] = r * fmaf(-f, x1[e], y1[e]);
+                        y0[i][e] = r * fmaf(-f, x0[i][e], y0[i][e]);
+                        y1[i][e] = r * fmaf(-f, x1[i][e], y1[i][e]);
                     }
                 }
-                T* po = static_cast<T*>(a.dx[t].p) + row * a.dx[t].row + hh * a.dx[t].head + 8 * chunk;
-                store8<T>(po, y0);
-                store8<T>(po + D / 2, y1);
+                T* po = head_ptr<T>(a.dx[0], a.dx[1], isk, row, hh, chunk);
+                store8<T>(po, y0[i]);
+                store8<T>(po + D / 2, y1[i]);
             }
         }
     }
@@ -169,7 +194,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs a, int
         __shared__ float sums[kThreads * 17];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            if (!a.gain[t]) continue;
+            if (!(t ? norm_k : norm_q)) continue;
             __syncthreads();
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -180,53 +205,61 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs a, int
             if (threadIdx.x < D) {
                 const int e = threadIdx.x % (D / 2), c = e / 8, at = e % 8 + (threadIdx.x < D / 2 ? 0 : 8);
                 float x = 0.f;
+#pragma unroll 8
                 for (int i = c; i < kThreads; i += L) x += sums[i * 17 + at];
-                a.part[t][(int64_t)blockIdx.x * D + threadIdx.x] = x;
+                (t ? a.part[1] : a.part[0])[(int64_t)blockIdx.x * D + threadIdx.x] = x;
             }
         }
     }
 }
 
-// gain gradients from the blocks' sums, in 64 bits and in a fixed order: one wavefront a column
-__global__ __launch_bounds__(64) void gain_sum_kernel(const float* p0, const float* p1, float* o0, float* o1, int blocks, int dim) {
+// gain gradients from the blocks' sums, in 64 bits and in a fixed order: 64 columns a block where there are as many, the
+// threads in rows below each other
+__global__ __launch_bounds__(1024) void gain_sum_kernel(const float* p0, const float* p1, float* o0, float* o1, int blocks, int dim) {
+    __shared__ double sums[1024];
     const float* p = blockIdx.y ? p1 : p0;
     float* o = blockIdx.y ? o1 : o0;
     if (!o) return;
+    const int cols = dim < 16 ? dim : 16, rows = 1024 / cols;
+    const int col = blockIdx.x * cols + threadIdx.x % cols, row = threadIdx.x / cols;
     double x = 0.0;
-    for (int i = threadIdx.x; i < blocks; i += 64) x += (double)p[(int64_t)i * dim + blockIdx.x];
-    for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m);
-    if (threadIdx.x == 0) o[blockIdx.x] = (float)x;
+#pragma unroll 8
+    for (int i = row; i < blocks; i += rows) x += (double)p[(int64_t)i * dim + col];
+    sums[threadIdx.x] = x;
+    for (int k = rows / 2; k; k >>= 1) {
+        __syncthreads();
+        if (row < k) sums[threadIdx.x] += sums[threadIdx.x + k * cols];
+    }
+    if (row == 0) o[col] = (float)sums[threadIdx.x];
 }
 
-// heads a thread takes in a row: one while the call does not fill the card, four beyond
-int head_step(int64_t rows, int all, int dim) {
-    const int64_t threads = rows * all * (dim / 16);
-    return threads > 4 * 256 * 2048 ? (all + 3) / 4 : all;
-}
+// heads a thread takes in a row: one while the call does not fill the card, HEADS beyond
+constexpr int kForwardHeads = 4, kBackwardHeads = 2;
+bool large(int64_t rows, int all, int dim) { return rows * all * (dim / 16) > 4 * 256 * 2048; }
 
-template <typename T, int D>
-hipError_t forward(const NormRopeArgs& a, hipStream_t s) {
-    const int all = a.heads[0] + a.heads[1], step = head_step(a.rows, all, D);
-    const int64_t units = a.rows * step, blocks = (units + kThreads / (D / 16) - 1) / (kThreads / (D / 16));
+template <typename T, int D, bool GRAD, int HEADS>
+hipError_t run(const NormRopeArgs& a, int blocks, hipStream_t s) {
+    const int all = a.heads[0] + a.heads[1], step = (all + HEADS - 1) / HEADS;
+    const int64_t units = a.rows * step;
+    if (!GRAD) blocks = (int)((units + kThreads / (D / 16) - 1) / (kThreads / (D / 16)));
     if (a.interleaved)
-        hipLaunchKernelGGL((norm_rope_kernel<T, D, true, false>), dim3((unsigned)blocks), dim3(kThreads), 0, s, a, step, units);
+        hipLaunchKernelGGL((norm_rope_kernel<T, D, true, GRAD, HEADS>), dim3(blocks), dim3(kThreads), 0, s, a, step, units);
     else
-        hipLaunchKernelGGL((norm_rope_kernel<T, D, false, false>), dim3((unsigned)blocks), dim3(kThreads), 0, s, a, step, units);
+        hipLaunchKernelGGL((norm_rope_kernel<T, D, false, GRAD, HEADS>), dim3(blocks), dim3(kThreads), 0, s, a, step, units);
     return hipGetLastError();
 }
 
 template <typename T, int D>
+hipError_t forward(const NormRopeArgs& a, hipStream_t s) {
+    return large(a.rows, a.heads[0] + a.heads[1], D) ? run<T, D, false, kForwardHeads>(a, 0, s) : run<T, D, false, 1>(a, 0, s);
+}
+
+template <typename T, int D>
 hipError_t backward(const NormRopeArgs& a, hipStream_t s) {
-    const int all = a.heads[0] + a.heads[1], step = head_step(a.rows, all, D);
-    const int64_t units = a.rows * step;
-    const int blocks = norm_rope_blocks(a.rows, all, D);
-    if (a.interleaved)
-        hipLaunchKernelGGL((norm_rope_kernel<T, D, true, true>), dim3(blocks), dim3(kThreads), 0, s, a, step, units);
-    else
-        hipLaunchKernelGGL((norm_rope_kernel<T, D, false, true>), dim3(blocks), dim3(kThreads), 0, s, a, step, units);
-    hipError_t e = hipGetLastError();
+    const int all = a.heads[0] + a.heads[1], blocks = norm_rope_blocks(a.rows, all, D);
+    const hipError_t e = large(a.rows, all, D) ? run<T, D, true, kBackwardHeads>(a, blocks, s) : run<T, D, true, 1>(a, blocks, s);
     if (e != hipSuccess || (!a.gain[0] && !a.gain[1])) return e;
-    hipLaunchKernelGGL(gain_sum_kernel, dim3(D, 2), dim3(64), 0, s, a.part[0], a.part[1], a.gain[0] ? a.dgain[0] : nullptr,
+    hipLaunchKernelGGL(gain_sum_kernel, dim3(D / 16, 2), dim3(1024), 0, s, a.part[0], a.part[1], a.gain[0] ? a.dgain[0] : nullptr,
                        a.gain[1] ? a.dgain[1] : nullptr, blocks, D);
     return hipGetLastError();
 }
@@ -249,9 +282,9 @@ hipError_t by_type(const NormRopeArgs& a, int dtype, bool grad, hipStream_t s) {
 
 // blocks of the backward pass: they walk over the units, so that there are few partial sums
 int norm_rope_blocks(int64_t rows, int heads, int dim) {
-    const int64_t per = kThreads / (dim / 16), units = rows * head_step(rows, heads, dim);
-    const int64_t want = (units + per - 1) / per;
-    return (int)(want < 1024 ? (want < 1 ? 1 : want) : 1024);
+    const int64_t per = kThreads / (dim / 16), step = large(rows, heads, dim) ? (heads + kBackwardHeads - 1) / kBackwardHeads : heads;
+    const int64_t want = (rows * step + per - 1) / per;
+    return (int)(want < 1536 ? (want < 1 ? 1 : want) : 1536);
 }
 
 hipError_t norm_rope_forward(const NormRopeArgs& a, int dtype, hipStream_t s) { return by_type(a, dtype, false, s); }
