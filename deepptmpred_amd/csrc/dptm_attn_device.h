@@ -113,6 +113,58 @@ struct Tile {
     }
 };
 
+// Left to itself the compiler reads one LDS fragment, waits, and feeds it, to spare registers: a wavefront then stands for
+// the LDS latency of every fragment (56 % of its time in the dk, dv kernel).  For the 16-bit types a product's fragments are
+// therefore asked for as a group in front of a scheduling barrier in the backward kernels.  (The forward kernel has three
+// wavefronts a SIMD that cover for each other, and loses one or spills with more fragments in registers: 129 us as it is, 153
+// to 166 with groups.)  In fp32 a fragment feeds eight instructions and is
+// twice as large, and the order is left alone.
+template <typename T> __device__ __forceinline__ void after_reads() {
+    if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+}
+// c0 += A0 B0 and c1 += A1 B1 over the whole head dimension, A rows row0 .. row0 + 31 of two tiles; four steps at a time
+template <typename T, int D>
+__device__ __forceinline__ void row_products(f32x16_a& c0, f32x16_a& c1, const char* t0, const char* t1, int row0, const V8<T> (&b0)[D / 16],
+                                             const V8<T> (&b1)[D / 16], int lane) {
+    constexpr int G = D / 16 < 4 ? D / 16 : 4;
+#pragma unroll
+    for (int g = 0; g < D / 16; g += G) {
+        V8<T> f0[G], f1[G];
+#pragma unroll
+        for (int s = 0; s < G; ++s) {
+            f0[s] = Tile<T, D>::row_frag(t0, row0 + (lane & 31), g + s, lane >> 5);
+            f1[s] = Tile<T, D>::row_frag(t1, row0 + (lane & 31), g + s, lane >> 5);
+        }
+        after_reads<T>();
+#pragma unroll
+        for (int s = 0; s < G; ++s) {
+            mma(c0, f0[s], b0[g + s]);
+            mma(c1, f1[s], b1[g + s]);
+        }
+    }
+}
+// the transposed fragments of 32 rows of a tile
+template <typename T, int D>
+struct Cols {
+    static constexpr int DT = D >= 32 ? D / 32 : 1;
+    V8<T> f[2][DT];
+    __device__ __forceinline__ void read(const char* t, int row0, int lane) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) f[s][d] = Tile<T, D>::col_frag(t, row0 + 16 * s, d, lane);
+    }
+    // acc += rows^T w, w a 32 x 32 tile with the rows on its registers
+    __device__ __forceinline__ void product(f32x16_a (&acc)[DT], const f32x16_a& w) const {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const V8<T> b = pack8<T>(w, s);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) mma(acc[d], f[s][d], b);
+        }
+    }
+};
+
 // ROWS rows of a strided tensor on the way to LDS through registers; rows from `valid` on become zeros.  Offsets within
 // the rows are kept as 32 bits behind a uniform address (row strides are refused from 2^25 bytes on).
 template <typename T, int D, int ROWS, int NT>

@@ -87,7 +87,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
         for (int e = 0; e < 8; ++e) delta = fmaf((float)g[s][e], (float)o[e], delta);
     }
     delta = half_sum(delta);
-    const float ref = lse_log2(a.lse[(int64_t)head * a.q_rows + qr]);
+    // rows behind the last weigh nothing
+    const float ref = row < it.nq ? lse_log2(a.lse[(int64_t)head * a.q_rows + qr]) : __builtin_inff();
     if (h == 0 && row < it.nq) a.delta[(int64_t)head * a.q_rows + qr] = delta;
 
     const int hk = head / a.group;
@@ -113,6 +114,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+    f32x16_a less_delta;                // dP starts from -delta
+#pragma unroll
+    for (int r = 0; r < 16; ++r) less_delta[r] = -delta;
     float below = 0.f, above = 0.f;     // dS of distances up to -reach, from reach on
     if (n > 0) fetch(0);
     if constexpr (BIAS) {
@@ -136,25 +140,23 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
             if (active && a0 < j1 && !none_visible(win, rw.pmin, rw.pmax, a0, a1)) {
                 const bool full = a1 - a0 == 32 && all_visible(win, rw.pmin, rw.pmax, a0, a1);
                 const bool is_above = a0 - rw.pmax >= reach, is_below = a0 + 31 - rw.pmin <= -reach;   // one bucket for the tile
-                f32x16_a s, p;
+                f32x16_a s, p = less_delta;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = p[r] = 0.f;
+                for (int r = 0; r < 16; ++r) s[r] = 0.f;
                 if constexpr (BIAS) init_bias(s, bias, reach, a0 + 4 * h - rw.pos, is_above, is_below);
+                row_products<T, D>(s, p, kt, vt, 32 * k, q, g, lane);
+                Cols<T, D> cols;
+                cols.read(kt, 32 * k, lane);
+                after_reads<T>();
 #pragma unroll
-                for (int st = 0; st < ST; ++st) {
-                    mma(s, Tile<T, D>::row_frag(kt, 32 * k + (lane & 31), st, h), q[st]);
-                    mma(p, Tile<T, D>::row_frag(vt, 32 * k + (lane & 31), st, h), g[st]);
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ref)) * (p[r] - delta);
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ref)) * p[r];
                 if (!full) hide(s, lane_mask(win, rw.pos, a0 + 4 * h, j1), 0.f);
+                const bool near = BIAS && !(is_above || is_below);
                 if constexpr (BIAS) {
-                    
-                    if (is_above | is_below) {
+                    if (!near) {
                         float sum = 0.f;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) sum += s[r];
-                        sum = row < it.nq ? sum : 0.f;
                         above += is_above ? sum : 0.f;
                         below += is_above ? 0.f : sum;
                     } else if constexpr (POS) {
@@ -168,29 +170,26 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
                         float* mine = shear + 32 + (lane & 31) * kShearRow + 4 * h;
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            V4<float> y;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) y[e] = row < it.nq ? s[4 * x + e] : 0.f;
+                            const V4<float> y{s[4 * x], s[4 * x + 1], s[4 * x + 2], s[4 * x + 3]};
                             *reinterpret_cast<V4<float>*>(mine + 8 * x) = y;
                         }
+                    }
+                }
+                cols.product(acc, s);
+                if constexpr (BIAS && !POS) {
+                    if (near) {     // while the matrix instructions run
                         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
                         __builtin_amdgcn_wave_barrier();
                         // lane l: key - row = l - 31, which is the distance a0 + l - 31 - (position of row 0)
                         const float* from = shear + 32 + lane - 31;
-                        float sum = 0.f;
+                        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) sum += from[i * (kShearRow + 1)];
+                        for (int i = 0; i < 32; ++i) part[i & 3] += from[i * (kShearRow + 1)];
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                         __builtin_amdgcn_wave_barrier();
                         const int dist = a0 + lane - 31 - (it.pos0 + 32 * w) + reach + kFarPad;
-                        if (lane < 63) sums[dist] += sum;
+                        if (lane < 63) sums[dist] += (part[0] + part[1]) + (part[2] + part[3]);
                     }
-                }
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const V8<T> b = pack8<T>(s, x);
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) mma(acc[d], Tile<T, D>::col_frag(kt, 32 * k + 16 * x, d, lane), b);
                 }
             }
         }
@@ -384,9 +383,9 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
         sg.load(reinterpret_cast<const char*>(row_ptr<T>(a.dout, r0, head)), valid, tid);
         if (tid < kBQ) {
             const int64_t at = (int64_t)head * a.q_rows + r0 + min(tid, valid - 1);
-            // rows behind the last weigh nothing: their reference is +inf
-            nref = tid < valid ? lse_log2(a.lse[at]) : __builtin_inff();
-            ndelta = tid < valid ? a.delta[at] : 0.f;
+            // rows behind the last weigh nothing: their scores start from -inf
+            nref = tid < valid ? lse_log2(a.lse[at]) * (-1.f / c) : kMinusInf;
+            ndelta = tid < valid ? -a.delta[at] : 0.f;
             npos = a.has_pos ? a.plan[a.pos_at + it.q0 + i0 + min(tid, valid - 1)] : 0;
         }
     };
@@ -426,37 +425,44 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
                 }
                 if (active && r0 < it.qe && !none_visible(win, pmin, pmax, j0, j1)) {
                     const bool full = all_visible(win, pmin, pmax, j0, j0 + 32);
-                    const float* ref = rowref + buf * kBQ + 32 * u + 4 * h;
-                    const float* del = rowdelta + buf * kBQ + 32 * u + 4 * h;
                     const int* pos = rowpos + buf * kBQ + 32 * u + 4 * h;
                     const int far = j - (it.pos0 + r0 + 4 * h);      // to the row of register 0, where the plan lists no positions
+                    // The products start from what is taken off them: the scores from -lse (and the bias), dP from -delta
                     f32x16_a s, p;
+                    const V4<float>* less = reinterpret_cast<const V4<float>*>(rowref + buf * kBQ + 32 * u + 4 * h);
+                    const V4<float>* del = reinterpret_cast<const V4<float>*>(rowdelta + buf * kBQ + 32 * u + 4 * h);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = p[r] = 0.f;
+                    for (int x = 0; x < 4; ++x) {
+                        const V4<float> y = less[2 * x], z = del[2 * x];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[4 * x + e] = y[e], p[4 * x + e] = z[e];
+                    }
                     if constexpr (BIAS) {
                         const bool is_above = j0 - pmax >= reach, is_below = j0 + 31 - pmin <= -reach;
-                        if (is_above | is_below) {
+                        if (is_above || is_below) {
                             const float b = bias[is_above ? 2 * reach + kBiasPad : 0];
 #pragma unroll
-                            for (int r = 0; r < 16; ++r) s[r] = b;
+                            for (int r = 0; r < 16; ++r) s[r] += b;
                         } else if (a.has_pos) {
 #pragma unroll
-                            for (int r = 0; r < 16; ++r) s[r] = bias[bias_at(j - pos[reg_row(r)], reach)];
+                            for (int r = 0; r < 16; ++r) s[r] += bias[bias_at(j - pos[reg_row(r)], reach)];
                         } else {
                             const float* b = bias + bias_at(far - kBiasPad, reach) + kBiasPad;
 #pragma unroll
-                            for (int r = 0; r < 16; ++r) s[r] = b[-reg_row(r)];
+                            for (int r = 0; r < 16; ++r) s[r] += b[-reg_row(r)];
                         }
                     }
-#pragma unroll
-                    for (int st = 0; st < ST; ++st) {
-                        mma(s, Tile<T, D>::row_frag(qt, 32 * u + (lane & 31), st, h), kf[st]);
-                        mma(p, Tile<T, D>::row_frag(gt, 32 * u + (lane & 31), st, h), vf[st]);
+                    row_products<T, D>(s, p, qt, gt, 32 * u, kf, vf, lane);
+                    Cols<T, D> gc, qc;
+                    if constexpr (D <= 64) {
+                        gc.read(gt, 32 * u, lane);
+                        qc.read(qt, 32 * u, lane);
+                        after_reads<T>();
                     }
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ref[reg_row(r)]));
-                        p[r] = s[r] * (p[r] - del[reg_row(r)]);
+                        s[r] = __builtin_amdgcn_exp2f(s[r] * c);
+                        p[r] *= s[r];
                     }
                     if (!full) {
                         if (a.has_pos) {
@@ -477,15 +483,16 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
                             }
                         }
                     }
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const V8<T> pw = pack8<T>(s, x), ps = pack8<T>(p, x);
-#pragma unroll
-                        for (int d = 0; d < DT; ++d) {
-                            mma(dv[d], Tile<T, D>::col_frag(gt, 32 * u + 16 * x, d, lane), pw);
-                            mma(dk[d], Tile<T, D>::col_frag(qt, 32 * u + 16 * x, d, lane), ps);
-                        }
+                    if constexpr (D > 64) {
+                        gc.read(gt, 32 * u, lane);
+                        after_reads<T>();
+                        gc.product(dv, s);
+                        qc.read(qt, 32 * u, lane);
+                        after_reads<T>();
+                    } else {
+                        gc.product(dv, s);
                     }
+                    qc.product(dk, p);
                 }
             }
             if (t + 1 < nt) put(t + 1);

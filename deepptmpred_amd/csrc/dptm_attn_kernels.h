@@ -66,19 +66,6 @@ __device__ __forceinline__ void softmax_step(f32x16_a (&s)[NK], f32x16_a (&acc)[
     l += sum;
 }
 
-// acc += V^T P^T over 32 NK keys of a tile in LDS
-template <typename T, int D, int NK, int DT>
-__device__ __forceinline__ void weighted_values(f32x16_a (&acc)[DT], const f32x16_a (&p)[NK], const char* vt, int lane) {
-#pragma unroll
-    for (int k = 0; k < NK; ++k)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const V8<T> b = pack8<T>(p[k], s);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) mma(acc[d], Tile<T, D>::col_frag(vt, 32 * k + 16 * s, d, lane), b);
-        }
-}
-
 template <typename T>
 __device__ __forceinline__ const T* row_ptr(const Strided& t, int64_t row, int head) {
     return static_cast<const T*>(t.p) + row * t.row + (int64_t)head * t.head;
@@ -233,7 +220,12 @@ __global__ __launch_bounds__(NW * 64, D <= 64 && sizeof(T) == 2 ? 3 : 2) void at
                 for (int st = 0; st < ST; ++st) mma(s[k], Tile<T, D>::row_frag(kt, 32 * k + (lane & 31), st, h), q[st]);
             }
             softmax_step<T, NK, DT>(s, acc, m, l, c, rw, win, j0, j1, full, h);
-            weighted_values<T, D, NK, DT>(acc, s, vt, lane);
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                Cols<T, D> v;
+                v.read(vt, 32 * k, lane);
+                v.product(acc, s[k]);
+            }
         }
         if (t + 1 < n) put(t + 1);
         __syncthreads();
@@ -334,7 +326,9 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_split_kernel(AttnArgs a) {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         softmax_step<T, 1, DT>(s, acc, m, l, c, rw, win, j0, j1, full, h);
-        weighted_values<T, D, 1, DT>(acc, s, vt, lane);
+        Cols<T, D> v;
+        v.read(vt, 0, lane);
+        v.product(acc, s[0]);
     }
     if (__ballot(odd != 0)) {
         float t[16 * DT], x[2];
