@@ -266,13 +266,34 @@ __device__ __forceinline__ void hide(f32x16_a& s, const LaneMask& m, float value
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = (in_window(m, reg_row(r)) | (reg_row(r) < m.first)) ? s[r] : value;
 }
-// all pairs of positions [pmin, pmax] and keys [j0, j1): every one visible / none visible
-__device__ __forceinline__ bool all_visible(const Window& w, int pmin, int pmax, int j0, int j1) {
-    return j1 - 1 - pmin <= w.right && (j0 - pmax >= -w.left || j1 <= w.sinks);
-}
-__device__ __forceinline__ bool none_visible(const Window& w, int pmin, int pmax, int j0, int j1) {
-    return j0 - pmax > w.right || (j1 - 1 - pmin < -w.left && j0 >= w.sinks);
-}
+// What rows at positions [pmin, pmax] see of keys [j0, j0 + span), from limits that are formed once: a wavefront asks for
+// every tile, and scalar arithmetic with branches per tile costs as much as the tile's exponentials.
+struct Sight {
+    int none_from, none_to, full_to, full_from, sinks;
+    __device__ __forceinline__ Sight(const Window& w, int pmin, int pmax)
+        : none_from(pmax + w.right), none_to(pmin - w.left), full_to(pmin + w.right), full_from(pmax - w.left), sinks(w.sinks) {}
+    __device__ __forceinline__ bool none(int j0, int span) const {
+        return (j0 > none_from) | ((j0 + span <= none_to) & (j0 >= sinks));
+    }
+    __device__ __forceinline__ bool all(int j0, int span) const {
+        return (j0 + span - 1 <= full_to) & ((j0 >= full_from) | (j0 + span <= sinks));
+    }
+};
+// The keys of a tile of rows: first [0, sink_end), then [kb, ke), `step` keys at a time
+struct KeyWalk {
+    int j0, end;          // this tile's first key, end of its piece
+    int kb, ke;
+    bool first_keys;
+    __device__ __forceinline__ KeyWalk(const QItem& it)
+        : j0(it.sink_end > 0 ? 0 : it.kb), end(it.sink_end > 0 ? it.sink_end : it.ke), kb(it.kb), ke(it.ke), first_keys(it.sink_end > 0) {}
+    __device__ __forceinline__ bool more() const { return j0 < end; }
+    __device__ __forceinline__ KeyWalk next(int step) const {
+        KeyWalk n = *this;
+        n.j0 += step;
+        if (first_keys && n.j0 >= end) n.j0 = kb, n.end = ke, n.first_keys = false;
+        return n;
+    }
+};
 
 // A hidden pair's weight is 0, but 0 * inf and 0 * NaN are NaN.  Where a tile holds hidden pairs its threads look, on the way
 // to LDS, whether its rows hold such an element (Stage::not_finite), and workgroups that found one do their rows over at the

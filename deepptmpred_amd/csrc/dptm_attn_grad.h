@@ -48,7 +48,7 @@ template <bool POS> __host__ __device__ inline int dq_lds_floats(int waves, int 
 }
 
 template <typename T, int D, int NW, bool BIAS, bool POS>
-__global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 64 ? 3 : 2) void attn_dq_kernel(AttnArgs a) {
     constexpr int kBK = kKeysPerTile<T, D>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
     constexpr int kBytes = kBK * D * (int)sizeof(T);
     extern __shared__ char smem[];
@@ -95,19 +95,18 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
     const char* kbase = reinterpret_cast<const char*>(row_ptr<T>(a.k, it.k0, hk));
     const char* vbase = reinterpret_cast<const char*>(row_ptr<T>(a.v, it.k0, hk));
     const int64_t kstep = a.k.row * (int)sizeof(T), vstep = a.v.row * (int)sizeof(T);
-    const int ns = (it.sink_end + kBK - 1) / kBK, n = ns + (it.ke - it.kb + kBK - 1) / kBK;
     Stage<T, D, kBK, NW * 64> sk(kstep, tid), sv(vstep, tid);
-    auto fetch = [&](int t) {
-        const int j0 = t < ns ? t * kBK : it.kb + (t - ns) * kBK, j1 = t < ns ? it.sink_end : it.ke;
-        sk.load(kbase + j0 * kstep, j1 - j0, tid);
-        sv.load(vbase + j0 * vstep, j1 - j0, tid);
+    auto fetch = [&](const KeyWalk& at) {
+        sk.load(kbase + at.j0 * kstep, at.end - at.j0, tid);
+        sv.load(vbase + at.j0 * vstep, at.end - at.j0, tid);
     };
+    const Sight sight(win, rw.pmin, rw.pmax), whole(win, it.pos0, it.pos0 + it.nq - 1);
+    const int above_from = rw.pmax + reach, below_to = rw.pmin - reach - 31;     // tiles of one bucket
     unsigned odd = 0;
-    auto put = [&](int t) {
-        const int j0 = t < ns ? t * kBK : it.kb + (t - ns) * kBK, j1 = min(j0 + kBK, t < ns ? it.sink_end : it.ke);
-        sk.store(smem + (t & 1) * kBytes, tid);
-        sv.store(smem + (2 + (t & 1)) * kBytes, tid);
-        if (a.has_pos || !all_visible(win, it.pos0, it.pos0 + it.nq - 1, j0, j1)) odd |= sk.not_finite();
+    auto put = [&](const KeyWalk& at, int buf) {
+        sk.store(smem + buf * kBytes, tid);
+        sv.store(smem + (2 + buf) * kBytes, tid);
+        if (a.has_pos | !whole.all(at.j0, kBK)) odd |= sk.not_finite();
     };
     f32x16_a acc[DT];
 #pragma unroll
@@ -118,7 +117,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) less_delta[r] = -delta;
     float below = 0.f, above = 0.f;     // dS of distances up to -reach, from reach on
-    if (n > 0) fetch(0);
+    KeyWalk walk(it);
+    if (walk.more()) fetch(walk);
     if constexpr (BIAS) {
         load_bias<T>(bias, a.bias, 1.f / a.scale, a.heads, head, tid, NW * 64);
         const int floats = POS ? NW * nb * 64 : NW * (kShear + room);
@@ -127,19 +127,19 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
             for (int i = tid; i < bias_room(reach); i += NW * 64)
                 bucket[i] = (unsigned char)min(max(a.bias.buckets[min(max(i - kBiasPad, 0), 2 * reach)], 0), nb - 1);
     }
-    if (n > 0) put(0);
+    if (walk.more()) put(walk, 0);
     __syncthreads();
-    for (int t = 0; t < n; ++t) {
-        if (t + 1 < n) fetch(t + 1);
-        const char* kt = smem + (t & 1) * kBytes;
-        const char* vt = smem + (2 + (t & 1)) * kBytes;
-        const int j0 = t < ns ? t * kBK : it.kb + (t - ns) * kBK, j1 = min(j0 + kBK, t < ns ? it.sink_end : it.ke);
+    for (int buf = 0; walk.more(); buf ^= 1) {
+        const KeyWalk after = walk.next(kBK);
+        if (after.more()) fetch(after);
+        const char* kt = smem + buf * kBytes;
+        const char* vt = smem + (2 + buf) * kBytes;
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
-            const int a0 = j0 + 32 * k, a1 = min(a0 + 32, j1);
-            if (active && a0 < j1 && !none_visible(win, rw.pmin, rw.pmax, a0, a1)) {
-                const bool full = a1 - a0 == 32 && all_visible(win, rw.pmin, rw.pmax, a0, a1);
-                const bool is_above = a0 - rw.pmax >= reach, is_below = a0 + 31 - rw.pmin <= -reach;   // one bucket for the tile
+            const int a0 = walk.j0 + 32 * k;
+            if (active & (a0 < walk.end) & !sight.none(a0, 32)) {
+                const bool full = (a0 + 32 <= walk.end) & sight.all(a0, 32);
+                const bool is_above = a0 >= above_from, is_below = a0 <= below_to;   // one bucket for the tile
                 f32x16_a s, p = less_delta;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = 0.f;
@@ -150,8 +150,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
                 after_reads<T>();
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ref)) * p[r];
-                if (!full) hide(s, lane_mask(win, rw.pos, a0 + 4 * h, j1), 0.f);
-                const bool near = BIAS && !(is_above || is_below);
+                if (!full) hide(s, lane_mask(win, rw.pos, a0 + 4 * h, walk.end), 0.f);
+                const bool near = BIAS & !(is_above | is_below);
                 if constexpr (BIAS) {
                     if (!near) {
                         float sum = 0.f;
@@ -193,8 +193,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnArgs a) {
                 }
             }
         }
-        if (t + 1 < n) put(t + 1);
+        if (after.more()) put(after, buf ^ 1);
         __syncthreads();
+        walk = after;
     }
     if (__syncthreads_or((int)odd)) {
         float t[16 * DT];
@@ -355,7 +356,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
     const bool active = 32 * w < it.nk;
     const int key = 32 * w + (lane & 31), keyc = min(key, it.nk - 1);
     const int j = it.j0 + key;                                      // index in the sequence
-    const int j0 = it.j0 + 32 * w, j1 = it.j0 + min(32 * w + 32, it.nk);
+    const int j0 = it.j0 + 32 * w;
     const T* krow = row_ptr<T>(a.k, (int64_t)it.k0 + keyc, hk);
     const T* vrow = row_ptr<T>(a.v, (int64_t)it.k0 + keyc, hk);
     V8<T> kf[ST], vf[ST];
@@ -375,12 +376,20 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
     unsigned odd = 0;
     float nref = 0.f, ndelta = 0.f;
     int npos = 0;
+    // the next tile of rows: its addresses move on with it
+    const char *qat = nullptr, *gat = nullptr;
     auto fetch = [&](int head, int t) {
         const int i0 = it.qb + t * kBQ;
         const int64_t r0 = (int64_t)it.q0 + i0;
         const int valid = it.qe - i0;
-        sq.load(reinterpret_cast<const char*>(row_ptr<T>(a.q, r0, head)), valid, tid);
-        sg.load(reinterpret_cast<const char*>(row_ptr<T>(a.dout, r0, head)), valid, tid);
+        if (t == 0) {
+            qat = reinterpret_cast<const char*>(row_ptr<T>(a.q, r0, head));
+            gat = reinterpret_cast<const char*>(row_ptr<T>(a.dout, r0, head));
+        }
+        sq.load(qat, valid, tid);
+        sg.load(gat, valid, tid);
+        qat += kBQ * qstep;
+        gat += kBQ * gstep;
         if (tid < kBQ) {
             const int64_t at = (int64_t)head * a.q_rows + r0 + min(tid, valid - 1);
             // rows behind the last weigh nothing: their scores start from -inf
@@ -393,7 +402,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
         const int buf = t & 1, i0 = it.qb + t * kBQ, i1 = min(i0 + kBQ, it.qe);
         sq.store(smem + buf * kBytes, tid);
         sg.store(smem + (2 + buf) * kBytes, tid);
-        if (a.has_pos || !all_visible(win, it.pos0 + i0, it.pos0 + i1 - 1, it.j0, it.j0 + it.nk)) odd |= sq.not_finite() | sg.not_finite();
+        if (a.has_pos | !Sight(win, it.pos0 + i0, it.pos0 + i1 - 1).all(it.j0, it.nk)) odd |= sq.not_finite() | sg.not_finite();
         if (tid < kBQ) {
             rowref[buf * kBQ + tid] = nref;
             rowdelta[buf * kBQ + tid] = ndelta;
@@ -413,18 +422,15 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
 #pragma unroll
             for (int u = 0; u < NQ; ++u) {
                 const int r0 = i0 + 32 * u;
-                int pmin = 0, pmax = 0;
+                int pmin = it.pos0 + r0, pmax = it.pos0 + min(r0 + 31, it.nseq - 1);
                 if (a.has_pos) {
-                    if (r0 < it.qe) {
-                        pmin = a.plan[a.tiles_at + 2 * (it.tile0 + (r0 >> 5))];
-                        pmax = a.plan[a.tiles_at + 2 * (it.tile0 + (r0 >> 5)) + 1];
-                    }
-                } else {
-                    pmin = it.pos0 + r0;
-                    pmax = it.pos0 + min(r0 + 31, it.nseq - 1);
+                    const int tile = it.tile0 + (min(r0, it.nseq - 1) >> 5);
+                    pmin = a.plan[a.tiles_at + 2 * tile];
+                    pmax = a.plan[a.tiles_at + 2 * tile + 1];
                 }
-                if (active && r0 < it.qe && !none_visible(win, pmin, pmax, j0, j1)) {
-                    const bool full = all_visible(win, pmin, pmax, j0, j0 + 32);
+                const Sight sight(win, pmin, pmax);
+                if (active & (r0 < it.qe) & !sight.none(j0, 32)) {
+                    const bool full = sight.all(j0, 32);
                     const int* pos = rowpos + buf * kBQ + 32 * u + 4 * h;
                     const int far = j - (it.pos0 + r0 + 4 * h);      // to the row of register 0, where the plan lists no positions
                     // The products start from what is taken off them: the scores from -lse (and the bias), dP from -delta
@@ -439,7 +445,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
                     }
                     if constexpr (BIAS) {
                         const bool is_above = j0 - pmax >= reach, is_below = j0 + 31 - pmin <= -reach;
-                        if (is_above || is_below) {
+                        if (is_above | is_below) {
                             const float b = bias[is_above ? 2 * reach + kBiasPad : 0];
 #pragma unroll
                             for (int r = 0; r < 16; ++r) s[r] += b;

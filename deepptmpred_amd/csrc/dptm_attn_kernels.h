@@ -173,20 +173,17 @@ __global__ __launch_bounds__(NW * 64, D <= 64 && sizeof(T) == 2 ? 3 : 2) void at
     const char* kbase = static_cast<const char*>(a.k.p) + ((int64_t)it.k0 * a.k.row + (int64_t)hk * a.k.head) * (int)sizeof(T);
     const char* vbase = static_cast<const char*>(a.v.p) + ((int64_t)it.k0 * a.v.row + (int64_t)hk * a.v.head) * (int)sizeof(T);
     const int64_t kstep = a.k.row * (int)sizeof(T), vstep = a.v.row * (int)sizeof(T);
-    const int ns = (it.sink_end + kBK - 1) / kBK, n = ns + (it.ke - it.kb + kBK - 1) / kBK;
-
     Stage<T, D, kBK, NW * 64> sk(kstep, tid), sv(vstep, tid);
-    auto fetch = [&](int t) {
-        const int j0 = t < ns ? t * kBK : it.kb + (t - ns) * kBK, j1 = t < ns ? it.sink_end : it.ke;
-        sk.load(kbase + j0 * kstep, j1 - j0, tid);
-        sv.load(vbase + j0 * vstep, j1 - j0, tid);
+    auto fetch = [&](const KeyWalk& at) {
+        sk.load(kbase + at.j0 * kstep, at.end - at.j0, tid);
+        sv.load(vbase + at.j0 * vstep, at.end - at.j0, tid);
     };
+    const Sight sight(win, rw.pmin, rw.pmax), whole(win, it.pos0, it.pos0 + it.nq - 1);
     unsigned odd = 0;
-    auto put = [&](int t) {
-        const int j0 = t < ns ? t * kBK : it.kb + (t - ns) * kBK, j1 = min(j0 + kBK, t < ns ? it.sink_end : it.ke);
-        sk.store(smem + (t & 1) * kBytes, tid);
-        sv.store(smem + (2 + (t & 1)) * kBytes, tid);
-        if (a.has_pos || !all_visible(win, it.pos0, it.pos0 + it.nq - 1, j0, j1)) odd |= sv.not_finite();
+    auto put = [&](const KeyWalk& at, int buf) {
+        sk.store(smem + buf * kBytes, tid);
+        sv.store(smem + (2 + buf) * kBytes, tid);
+        if (a.has_pos | !whole.all(at.j0, kBK)) odd |= sv.not_finite();
     };
     f32x16_a acc[DT];
 #pragma unroll
@@ -195,23 +192,24 @@ __global__ __launch_bounds__(NW * 64, D <= 64 && sizeof(T) == 2 ? 3 : 2) void at
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
     float m = kMinusInf, l = 0.f;
 
-    if (n > 0) fetch(0);
+    KeyWalk at(it);
+    if (at.more()) fetch(at);
     if constexpr (BIAS) load_bias<T>(bias, a.bias, 1.f / a.scale, a.heads, head, tid, NW * 64);
-    if (n > 0) put(0);
+    if (at.more()) put(at, 0);
     __syncthreads();
-    for (int t = 0; t < n; ++t) {
-        if (t + 1 < n) fetch(t + 1);
-        const char* kt = smem + (t & 1) * kBytes;
-        const char* vt = smem + (2 + (t & 1)) * kBytes;
-        const int j0 = t < ns ? t * kBK : it.kb + (t - ns) * kBK, j1 = min(j0 + kBK, t < ns ? it.sink_end : it.ke);
-        if (active && !none_visible(win, rw.pmin, rw.pmax, j0, j1)) {
-            const bool full = j1 - j0 == kBK && all_visible(win, rw.pmin, rw.pmax, j0, j1);
+    for (int buf = 0; at.more(); buf ^= 1) {
+        const KeyWalk after = at.next(kBK);
+        if (after.more()) fetch(after);
+        const char* kt = smem + buf * kBytes;
+        const char* vt = smem + (2 + buf) * kBytes;
+        if (active & !sight.none(at.j0, kBK)) {
+            const bool full = (at.j0 + kBK <= at.end) & sight.all(at.j0, kBK);
             f32x16_a s[NK];
 #pragma unroll
             for (int k = 0; k < NK; ++k) {
                 if constexpr (BIAS) {
-                    const int k0 = j0 + 32 * k;
-                    init_bias(s[k], bias, a.bias.reach, k0 + 4 * h - rw.pos, k0 - rw.pmax >= a.bias.reach, k0 + 31 - rw.pmin <= -a.bias.reach);
+                    const int k0 = at.j0 + 32 * k;
+                    init_bias(s[k], bias, a.bias.reach, k0 + 4 * h - rw.pos, k0 >= rw.pmax + a.bias.reach, k0 + 31 <= rw.pmin - a.bias.reach);
                 } else {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[k][r] = 0.f;
@@ -219,7 +217,7 @@ __global__ __launch_bounds__(NW * 64, D <= 64 && sizeof(T) == 2 ? 3 : 2) void at
 #pragma unroll
                 for (int st = 0; st < ST; ++st) mma(s[k], Tile<T, D>::row_frag(kt, 32 * k + (lane & 31), st, h), q[st]);
             }
-            softmax_step<T, NK, DT>(s, acc, m, l, c, rw, win, j0, j1, full, h);
+            softmax_step<T, NK, DT>(s, acc, m, l, c, rw, win, at.j0, at.end, full, h);
 #pragma unroll
             for (int k = 0; k < NK; ++k) {
                 Cols<T, D> v;
@@ -227,8 +225,9 @@ __global__ __launch_bounds__(NW * 64, D <= 64 && sizeof(T) == 2 ? 3 : 2) void at
                 v.product(acc, s[k]);
             }
         }
-        if (t + 1 < n) put(t + 1);
+        if (after.more()) put(after, buf ^ 1);
         __syncthreads();
+        at = after;
     }
     if (__syncthreads_or((int)odd)) {
         float t[16 * DT], ml[2];
@@ -306,6 +305,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_split_kernel(AttnArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
     float m = kMinusInf, l = 0.f;
+    const Sight sight(win, rw.pmin, rw.pmax);
     unsigned odd = 0;
     for (int t = w; t < n; t += NW) {
         const int j0 = t < ns ? t * 32 : it.kb + (t - ns) * 32, j1 = min(j0 + 32, t < ns ? it.sink_end : it.ke);
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_split_kernel(AttnArgs a) {
         }
 #pragma unroll
         for (int st = 0; st < ST; ++st) mma(s[0], kf[st], q[st]);
-        const bool full = j1 - j0 == 32 && all_visible(win, rw.pmin, rw.pmax, j0, j1);
+        const bool full = (j1 - j0 == 32) & sight.all(j0, 32);
         __builtin_amdgcn_wave_barrier();
         sv.store(vt, lane);
         if (!full) odd |= sv.not_finite();

@@ -78,8 +78,8 @@ def attention(q, k, v, q_lens, k_lens, window=(-1, -1), sinks=0, positions=None,
                     delta = (G * out).sum(1, keepdims=True)
                     dS = P * (dP - delta)
                     eout = np.abs(np.asarray(kernel_out, np.float64)[q0:q0 + a, n] - out) if kernel_out is not None else eo
-                    # the weight from the stored lse: its error joins the score's
-                    epb = ep + 2 * e["lse"][n, q0:q0 + a][:, None]
+                    # the weight from the stored lse: its error joins the score's, and the score's sum starts from it
+                    epb = ep + 2 * e["lse"][n, q0:q0 + a][:, None] + 2 * (d + 8) * U * np.where(some, np.abs(lse[:, 0]), 0)[:, None]
                     eds = P * (epb * np.abs(dP - delta) + (d + 4) * U * (np.abs(G) @ np.abs(Vc).T) +
                                (np.abs(G) * eout).sum(1, keepdims=True) + (d + 4) * U * (np.abs(G) * np.abs(out)).sum(1, keepdims=True))
                     eds = np.where(ok, eds, 0)
