@@ -376,6 +376,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
     unsigned odd = 0;
     float nref = 0.f, ndelta = 0.f;
     int npos = 0;
+    const float minus_inv_c = -1.f / c;
     // the next tile of rows: its addresses move on with it
     const char *qat = nullptr, *gat = nullptr;
     auto fetch = [&](int head, int t) {
@@ -392,9 +393,8 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
         gat += kBQ * gstep;
         if (tid < kBQ) {
             const int64_t at = (int64_t)head * a.q_rows + r0 + min(tid, valid - 1);
-            // rows behind the last weigh nothing: their scores start from -inf
-            nref = tid < valid ? lse_log2(a.lse[at]) * (-1.f / c) : kMinusInf;
-            ndelta = tid < valid ? -a.delta[at] : 0.f;
+            nref = a.lse[at];       // as they are: a value worked on here would be waited for here
+            ndelta = a.delta[at];
             npos = a.has_pos ? a.plan[a.pos_at + it.q0 + i0 + min(tid, valid - 1)] : 0;
         }
     };
@@ -404,8 +404,9 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
         sg.store(smem + (2 + buf) * kBytes, tid);
         if (a.has_pos | !Sight(win, it.pos0 + i0, it.pos0 + i1 - 1).all(it.j0, it.nk)) odd |= sq.not_finite() | sg.not_finite();
         if (tid < kBQ) {
-            rowref[buf * kBQ + tid] = nref;
-            rowdelta[buf * kBQ + tid] = ndelta;
+            // rows behind the last weigh nothing: their scores start from -inf
+            rowref[buf * kBQ + tid] = tid < i1 - i0 ? lse_log2(nref) * minus_inv_c : kMinusInf;
+            rowdelta[buf * kBQ + tid] = tid < i1 - i0 ? -ndelta : 0.f;
             rowpos[buf * kBQ + tid] = npos;
         }
     };
