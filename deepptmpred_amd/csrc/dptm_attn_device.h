@@ -318,18 +318,11 @@ __device__ __forceinline__ void load_bias(float* lds, const BiasArgs& b, float i
     }
 }
 
-// accumulators of 32 keys from `key0` on, whose score registers start at key0 + 4h; `above` / `below`: the whole tile lies
-// beyond the largest distance
-__device__ __forceinline__ void init_bias(f32x16_a& s, const float* bias, int reach, int far, bool above, bool below) {
-    if (above | below) {
-        const float b = bias[above ? 2 * reach + kBiasPad : 0];
+// accumulators of 32 keys, the first of a lane `far` behind its query
+__device__ __forceinline__ void init_bias(f32x16_a& s, const float* bias, int reach, int far) {
+    const float* b = bias + bias_at(far, reach);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = b;
-    } else {
-        const float* b = bias + bias_at(far, reach);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = b[reg_row(r)];
-    }
+    for (int r = 0; r < 16; ++r) s[r] = b[reg_row(r)];
 }
 
 // blocks of one key head's tiles on one XCD, which has an L2 of its own: block b runs on XCD b % 8, and each XCD takes a

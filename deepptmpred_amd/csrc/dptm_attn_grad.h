@@ -140,18 +140,22 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 64 ? 3 : 2) void attn_dq_
             if (active & (a0 < walk.end) & !sight.none(a0, 32)) {
                 const bool full = (a0 + 32 <= walk.end) & sight.all(a0, 32);
                 const bool is_above = a0 >= above_from, is_below = a0 <= below_to;   // one bucket for the tile
+                const bool near = BIAS & !(is_above | is_below);
                 f32x16_a s, p = less_delta;
+                float less = -ref;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = 0.f;
-                if constexpr (BIAS) init_bias(s, bias, reach, a0 + 4 * h - rw.pos, is_above, is_below);
+                if constexpr (BIAS) {
+                    if (near) init_bias(s, bias, reach, a0 + 4 * h - rw.pos);
+                    else less += c * bias[is_above ? 2 * reach + kBiasPad : 0];
+                }
                 row_products<T, D>(s, p, kt, vt, 32 * k, q, g, lane);
                 Cols<T, D> cols;
                 cols.read(kt, 32 * k, lane);
                 after_reads<T>();
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ref)) * p[r];
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, less)) * p[r];
                 if (!full) hide(s, lane_mask(win, rw.pos, a0 + 4 * h, walk.end), 0.f);
-                const bool near = BIAS & !(is_above | is_below);
                 if constexpr (BIAS) {
                     if (!near) {
                         float sum = 0.f;

@@ -30,18 +30,20 @@ struct Rows {
 // a multiply-add, an exp2, half a three-way maximum, an add and half a conversion: with head dimension 64 that is
 // half as long again as the element's matrix instructions, which is why nothing else is done per element.
 template <typename T, int NK, int DT>
-__device__ __forceinline__ void softmax_step(f32x16_a (&s)[NK], f32x16_a (&acc)[DT], float& m, float& l, float c, const Rows& w,
+__device__ __forceinline__ void softmax_step(f32x16_a (&s)[NK], const float (&more)[NK], f32x16_a (&acc)[DT], float& m, float& l, float c, const Rows& w,
                                              const Window& win, int j0, int j1, bool full, int h) {
     if (!full) {
 #pragma unroll
         for (int k = 0; k < NK; ++k) hide(s[k], lane_mask(win, w.pos, j0 + 32 * k + 4 * h, j1), kMinusInf);
     }
-    float mx = s[0][0];
+    float mx = kMinusInf;
 #pragma unroll
-    for (int k = 0; k < NK; ++k)
+    for (int k = 0; k < NK; ++k) {
+        float x = s[k][0];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[k][r]);
-    mx *= c;
+        for (int r = 1; r < 16; ++r) x = fmaxf(x, s[k][r]);
+        mx = fmaxf(mx, fmaf(x, c, more[k]));
+    }
     mx = half_max(mx);
     const bool grow = mx > m + kLazy || (m == kMinusInf && mx > m);
     if (__ballot(grow)) {
@@ -56,13 +58,15 @@ __device__ __forceinline__ void softmax_step(f32x16_a (&s)[NK], f32x16_a (&acc)[
     const float ref = (m == kMinusInf ? 0.f : m) - kShift<T>;
     float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < NK; ++k)
+    for (int k = 0; k < NK; ++k) {
+        const float less = more[k] - ref;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[k][r], c, -ref));
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[k][r], c, less));
             s[k][r] = p;
             sum += p;
         }
+    }
     l += sum;
 }
 
@@ -179,6 +183,7 @@ __global__ __launch_bounds__(NW * 64, D <= 64 && sizeof(T) == 2 ? 3 : 2) void at
         sv.load(vbase + at.j0 * vstep, at.end - at.j0, tid);
     };
     const Sight sight(win, rw.pmin, rw.pmax), whole(win, it.pos0, it.pos0 + it.nq - 1);
+    const int above_from = rw.pmax + a.bias.reach, below_to = rw.pmin - a.bias.reach - 31;     // 32 keys of one bias
     unsigned odd = 0;
     auto put = [&](const KeyWalk& at, int buf) {
         sk.store(smem + buf * kBytes, tid);
@@ -205,19 +210,28 @@ __global__ __launch_bounds__(NW * 64, D <= 64 && sizeof(T) == 2 ? 3 : 2) void at
         if (active & !sight.none(at.j0, kBK)) {
             const bool full = (at.j0 + kBK <= at.end) & sight.all(at.j0, kBK);
             f32x16_a s[NK];
+            float more[NK];      // one bias for the 32 keys, where they are far
 #pragma unroll
             for (int k = 0; k < NK; ++k) {
-                if constexpr (BIAS) {
-                    const int k0 = at.j0 + 32 * k;
-                    init_bias(s[k], bias, a.bias.reach, k0 + 4 * h - rw.pos, k0 >= rw.pmax + a.bias.reach, k0 + 31 <= rw.pmin - a.bias.reach);
+                const V8<T> first_k = Tile<T, D>::row_frag(kt, 32 * k + (lane & 31), 0, h);
+                const int k0 = at.j0 + 32 * k;
+                const bool above = k0 >= above_from;
+                more[k] = 0.f;
+                if (BIAS && !(above | (k0 <= below_to))) {
+                    init_bias(s[k], bias, a.bias.reach, k0 + 4 * h - rw.pos);
+                    mma(s[k], first_k, q[0]);
                 } else {
+                    if constexpr (BIAS) more[k] = c * bias[above ? 2 * a.bias.reach + kBiasPad : 0];
+                    f32x16_a zero;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[k][r] = 0.f;
+                    for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+                    s[k] = zero;
+                    mma(s[k], first_k, q[0]);
                 }
 #pragma unroll
-                for (int st = 0; st < ST; ++st) mma(s[k], Tile<T, D>::row_frag(kt, 32 * k + (lane & 31), st, h), q[st]);
+                for (int st = 1; st < ST; ++st) mma(s[k], Tile<T, D>::row_frag(kt, 32 * k + (lane & 31), st, h), q[st]);
             }
-            softmax_step<T, NK, DT>(s, acc, m, l, c, rw, win, at.j0, at.end, full, h);
+            softmax_step<T, NK, DT>(s, more, acc, m, l, c, rw, win, at.j0, at.end, full, h);
 #pragma unroll
             for (int k = 0; k < NK; ++k) {
                 Cols<T, D> v;
@@ -310,11 +324,13 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_split_kernel(AttnArgs a) {
     for (int t = w; t < n; t += NW) {
         const int j0 = t < ns ? t * 32 : it.kb + (t - ns) * 32, j1 = min(j0 + 32, t < ns ? it.sink_end : it.ke);
         f32x16_a s[1];
-        if constexpr (BIAS) {
-            init_bias(s[0], bias, a.bias.reach, j0 + 4 * h - rw.pos, j0 - rw.pmax >= a.bias.reach, j0 + 31 - rw.pmin <= -a.bias.reach);
-        } else {
+        float more[1] = {0.f};
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+        for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+        if constexpr (BIAS) {
+            const bool above = j0 >= rw.pmax + a.bias.reach;
+            if (above | (j0 + 31 <= rw.pmin - a.bias.reach)) more[0] = c * bias[above ? 2 * a.bias.reach + kBiasPad : 0];
+            else init_bias(s[0], bias, a.bias.reach, j0 + 4 * h - rw.pos);
         }
 #pragma unroll
         for (int st = 0; st < ST; ++st) mma(s[0], kf[st], q[st]);
@@ -325,7 +341,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_split_kernel(AttnArgs a) {
         if (t + NW < n) fetch(t + NW);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        softmax_step<T, 1, DT>(s, acc, m, l, c, rw, win, j0, j1, full, h);
+        softmax_step<T, 1, DT>(s, more, acc, m, l, c, rw, win, j0, j1, full, h);
         Cols<T, D> v;
         v.read(vt, 0, lane);
         v.product(acc, s[0]);
