@@ -122,11 +122,11 @@ struct Tile {
 template <typename T> __device__ __forceinline__ void after_reads() {
     if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
 }
-// c0 += A0 B0 and c1 += A1 B1 over the whole head dimension, A rows row0 .. row0 + 31 of two tiles; four steps at a time
-template <typename T, int D>
+// c0 += A0 B0 and c1 += A1 B1 over the whole head dimension, A rows row0 .. row0 + 31 of two tiles; MOST steps at a time
+template <typename T, int D, int MOST>
 __device__ __forceinline__ void row_products(f32x16_a& c0, f32x16_a& c1, const char* t0, const char* t1, int row0, const V8<T> (&b0)[D / 16],
                                              const V8<T> (&b1)[D / 16], int lane) {
-    constexpr int G = D / 16 < 4 ? D / 16 : 4;
+    constexpr int G = D / 16 < MOST ? D / 16 : MOST;
 #pragma unroll
     for (int g = 0; g < D / 16; g += G) {
         V8<T> f0[G], f1[G];
@@ -141,6 +141,20 @@ __device__ __forceinline__ void row_products(f32x16_a& c0, f32x16_a& c1, const c
             mma(c0, f0[s], b0[g + s]);
             mma(c1, f1[s], b1[g + s]);
         }
+    }
+}
+// c0 += A0 B0 alone
+template <typename T, int D, int MOST>
+__device__ __forceinline__ void row_product(f32x16_a& c0, const char* t0, int row0, const V8<T> (&b0)[D / 16], int lane) {
+    constexpr int G = D / 16 < MOST ? D / 16 : MOST;
+#pragma unroll
+    for (int g = 0; g < D / 16; g += G) {
+        V8<T> f0[G];
+#pragma unroll
+        for (int s = 0; s < G; ++s) f0[s] = Tile<T, D>::row_frag(t0, row0 + (lane & 31), g + s, lane >> 5);
+        after_reads<T>();
+#pragma unroll
+        for (int s = 0; s < G; ++s) mma(c0, f0[s], b0[g + s]);
     }
 }
 // the transposed fragments of 32 rows of a tile

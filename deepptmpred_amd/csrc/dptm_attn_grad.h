@@ -35,6 +35,9 @@ DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, int item, const T* q, 
     }
 }
 
+// rows of a tile in LDS: fewer than in the forward pass where a wavefront's own operands and sums take the registers
+template <typename T, int D> constexpr int kRowsPerTile = sizeof(T) == 2 && D <= 64 ? 64 : 32;
+
 // Bias gradient, in the kernel that owns queries.  Far tiles (one bucket) are summed in a register.  In a near one the
 // wavefront's rows stand at consecutive positions, so that equal distances are the diagonals of its 32 x 32 dS: it goes to LDS
 // with zeros between its rows, lane l adds diagonal l up (32 reads at a fixed stride) and keeps the
@@ -48,8 +51,8 @@ template <bool POS> __host__ __device__ inline int dq_lds_floats(int waves, int 
 }
 
 template <typename T, int D, int NW, bool BIAS, bool POS>
-__global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 64 ? 3 : 2) void attn_dq_kernel(AttnArgs a) {
-    constexpr int kBK = kKeysPerTile<T, D>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
+__global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 64 ? 3 : D * sizeof(T) >= 512 ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
+    constexpr int kBK = kRowsPerTile<T, D>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
     constexpr int kBytes = kBK * D * (int)sizeof(T);
     extern __shared__ char smem[];
     float* bias = reinterpret_cast<float*>(smem + 4 * kBytes);
@@ -113,9 +116,11 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 64 ? 3 : 2) void attn_dq_
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
-    f32x16_a less_delta;                // dP starts from -delta
+    f32x16_a less_delta;                // dP starts from -delta, kept in registers of its own where there are some to spare
+    if constexpr (D <= 64) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) less_delta[r] = -delta;
+        for (int r = 0; r < 16; ++r) less_delta[r] = -delta;
+    }
     float below = 0.f, above = 0.f;     // dS of distances up to -reach, from reach on
     KeyWalk walk(it);
     if (walk.more()) fetch(walk);
@@ -141,7 +146,13 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 64 ? 3 : 2) void attn_dq_
                 const bool full = (a0 + 32 <= walk.end) & sight.all(a0, 32);
                 const bool is_above = a0 >= above_from, is_below = a0 <= below_to;   // one bucket for the tile
                 const bool near = BIAS & !(is_above | is_below);
-                f32x16_a s, p = less_delta;
+                f32x16_a s, p;
+                if constexpr (D <= 64) {
+                    p = less_delta;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) p[r] = -delta;
+                }
                 float less = -ref;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = 0.f;
@@ -149,10 +160,12 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 64 ? 3 : 2) void attn_dq_
                     if (near) init_bias(s, bias, reach, a0 + 4 * h - rw.pos);
                     else less += c * bias[is_above ? 2 * reach + kBiasPad : 0];
                 }
-                row_products<T, D>(s, p, kt, vt, 32 * k, q, g, lane);
+                row_products<T, D, D <= 64 ? 4 : 1>(s, p, kt, vt, 32 * k, q, g, lane);
                 Cols<T, D> cols;
-                cols.read(kt, 32 * k, lane);
-                after_reads<T>();
+                if constexpr (D <= 64) {
+                    cols.read(kt, 32 * k, lane);
+                    after_reads<T>();
+                }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, less)) * p[r];
                 if (!full) hide(s, lane_mask(win, rw.pos, a0 + 4 * h, walk.end), 0.f);
@@ -179,6 +192,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 64 ? 3 : 2) void attn_dq_
                         }
                     }
                 }
+                if constexpr (D > 64) cols.read(kt, 32 * k, lane);
                 cols.product(acc, s);
                 if constexpr (BIAS && !POS) {
                     if (near) {     // while the matrix instructions run
@@ -336,11 +350,15 @@ DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int item, c
         }
 }
 
-// rows of a tile of queries: fewer where a wavefront's own keys and sums take the registers
-template <typename T, int D> constexpr int kRowsPerTile = sizeof(T) == 2 && D <= 64 ? 64 : 32;
+// Heads of 128 of the 16-bit types take two launches, one for dk and one for dv (8 products then, the scores a third time):
+// together their operands and sums leave room for one wavefront a SIMD, and the two launches take 2392 us where the one took
+// 3018 (32,768 rows in sequences of 2,048, 20 heads).
+enum { kBoth, kOnlyDk, kOnlyDv };
+template <typename T, int D> constexpr bool kTwoLaunches = sizeof(T) == 2 && D == 128;
 
-template <typename T, int D, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
+template <typename T, int D, int NW, bool BIAS, int PART>
+__global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
+    constexpr bool DK = PART != kOnlyDv, DV = PART != kOnlyDk;
     constexpr int kBQ = kRowsPerTile<T, D>, NQ = kBQ / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
     constexpr int kBytes = kBQ * D * (int)sizeof(T);
     extern __shared__ char smem[];
@@ -367,7 +385,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
 #pragma unroll
     for (int s = 0; s < ST; ++s) {
         kf[s] = global_frag<T>(reinterpret_cast<const char*>(krow), s, h);
-        vf[s] = global_frag<T>(reinterpret_cast<const char*>(vrow), s, h);
+        if constexpr (DK) vf[s] = global_frag<T>(reinterpret_cast<const char*>(vrow), s, h);
     }
     f32x16_a dk[DT], dv[DT];
 #pragma unroll
@@ -444,9 +462,14 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
                     const V4<float>* del = reinterpret_cast<const V4<float>*>(rowdelta + buf * kBQ + 32 * u + 4 * h);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const V4<float> y = less[2 * x], z = del[2 * x];
+                        const V4<float> y = less[2 * x];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[4 * x + e] = y[e], p[4 * x + e] = z[e];
+                        for (int e = 0; e < 4; ++e) s[4 * x + e] = y[e];
+                        if constexpr (DK) {
+                            const V4<float> z = del[2 * x];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) p[4 * x + e] = z[e];
+                        }
                     }
                     if constexpr (BIAS) {
                         const bool is_above = j0 - pmax >= reach, is_below = j0 + 31 - pmin <= -reach;
@@ -463,7 +486,8 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
                             for (int r = 0; r < 16; ++r) s[r] += b[-reg_row(r)];
                         }
                     }
-                    row_products<T, D>(s, p, qt, gt, 32 * u, kf, vf, lane);
+                    if constexpr (DK) row_products<T, D, D <= 64 ? 4 : 2>(s, p, qt, gt, 32 * u, kf, vf, lane);
+                    else row_product<T, D, D <= 64 ? 4 : 2>(s, qt, 32 * u, kf, lane);
                     Cols<T, D> gc, qc;
                     if constexpr (D <= 64) {
                         gc.read(gt, 32 * u, lane);
@@ -473,15 +497,15 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         s[r] = __builtin_amdgcn_exp2f(s[r] * c);
-                        p[r] *= s[r];
+                        if constexpr (DK) p[r] *= s[r];
                     }
                     if (!full) {
                         if (a.has_pos) {
 #pragma unroll
                             for (int r = 0; r < 16; ++r) {
                                 const bool see = visible(win, j - pos[reg_row(r)], j);
-                                s[r] = see ? s[r] : 0.f;
-                                p[r] = see ? p[r] : 0.f;
+                                if constexpr (DV) s[r] = see ? s[r] : 0.f;
+                                if constexpr (DK) p[r] = see ? p[r] : 0.f;
                             }
                         } else {
                             // row c is seen if far - c <= right and far - c >= -left, or the key is one of the first
@@ -489,21 +513,25 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
 #pragma unroll
                             for (int r = 0; r < 16; ++r) {
                                 const bool see = (unsigned)(reg_row(r) - lo) < (unsigned)m;
-                                s[r] = see ? s[r] : 0.f;
-                                p[r] = see ? p[r] : 0.f;
+                                if constexpr (DV) s[r] = see ? s[r] : 0.f;
+                                if constexpr (DK) p[r] = see ? p[r] : 0.f;
                             }
                         }
                     }
-                    if constexpr (D > 64) {
-                        gc.read(gt, 32 * u, lane);
-                        after_reads<T>();
-                        gc.product(dv, s);
-                        qc.read(qt, 32 * u, lane);
-                        after_reads<T>();
-                    } else {
+                    if constexpr (DV) {
+                        if constexpr (D > 64) {
+                            gc.read(gt, 32 * u, lane);
+                            after_reads<T>();
+                        }
                         gc.product(dv, s);
                     }
-                    qc.product(dk, p);
+                    if constexpr (DK) {
+                        if constexpr (D > 64) {
+                            qc.read(qt, 32 * u, lane);
+                            after_reads<T>();
+                        }
+                        qc.product(dk, p);
+                    }
                 }
             }
             if (t + 1 < nt) put(t + 1);
@@ -513,8 +541,8 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
     if (__syncthreads_or((int)odd)) {
         float x[16 * DT], y[16 * DT];
         dkv_by_pairs<T, D, DT, BIAS>(kernel_args(), x, y, id - hk * a.n_items, krow, vrow, hk, j, h);
-        take<DT>(dk, x);
-        take<DT>(dv, y);
+        if constexpr (DK) take<DT>(dk, x);
+        if constexpr (DV) take<DT>(dv, y);
     }
     if (key < it.nk) {
         if (it.slot < 0) {
@@ -530,8 +558,8 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
                         y[e] = (T)(dk[d][4 * x + e] * a.scale);
                         z[e] = (T)dv[d][4 * x + e];
                     }
-                    *reinterpret_cast<V4<T>*>(ok + 32 * d + 8 * x + 4 * h) = y;
-                    *reinterpret_cast<V4<T>*>(ov + 32 * d + 8 * x + 4 * h) = z;
+                    if constexpr (DK) *reinterpret_cast<V4<T>*>(ok + 32 * d + 8 * x + 4 * h) = y;
+                    if constexpr (DV) *reinterpret_cast<V4<T>*>(ov + 32 * d + 8 * x + 4 * h) = z;
                 }
         } else {
             float* ok = a.part_o + (((int64_t)it.slot * kvh + hk) * 2 * (NW * 32) + key) * D;
@@ -546,8 +574,8 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 ? 2 : 1) void attn_dk
                         y[e] = dk[d][4 * x + e] * a.scale;
                         z[e] = dv[d][4 * x + e];
                     }
-                    *reinterpret_cast<V4<float>*>(ok + 32 * d + 8 * x + 4 * h) = y;
-                    *reinterpret_cast<V4<float>*>(ov + 32 * d + 8 * x + 4 * h) = z;
+                    if constexpr (DK) *reinterpret_cast<V4<float>*>(ok + 32 * d + 8 * x + 4 * h) = y;
+                    if constexpr (DV) *reinterpret_cast<V4<float>*>(ov + 32 * d + 8 * x + 4 * h) = z;
                 }
         }
     }
@@ -573,7 +601,7 @@ __global__ __launch_bounds__(kJoinRows * (D / 4)) void attn_dkv_join_kernel(Attn
 template <typename T, int D, int NW>
 hipError_t dq_waves(const AttnArgs& a, hipStream_t s) {
     const int64_t blocks = (int64_t)a.n_items * a.heads;
-    const size_t lds = 4 * kKeysPerTile<T, D> * D * sizeof(T) + bias_floats(a) * 4;
+    const size_t lds = 4 * kRowsPerTile<T, D> * D * sizeof(T) + bias_floats(a) * 4;
     if (!a.bias.table) return start(attn_dq_kernel<T, D, NW, false, false>, blocks, NW * 64, lds, s, a);
     if (a.has_pos)
         return start(attn_dq_kernel<T, D, NW, true, true>, blocks, NW * 64, lds + 4 * dq_lds_floats<true>(NW, a.bias.n_buckets, a.bias.reach), s, a);
@@ -584,13 +612,25 @@ hipError_t dq_dim(const AttnArgs& a, int waves, hipStream_t s) {
     return waves == 2 ? dq_waves<T, D, 2>(a, s) : dq_waves<T, D, 4>(a, s);
 }
 
-template <typename T, int D>
-hipError_t dkv_dim(const AttnArgs& a, int waves, hipStream_t s) {
+template <typename T, int D, int NW, int PART>
+hipError_t dkv_part(const AttnArgs& a, hipStream_t s) {
     const int64_t blocks = (int64_t)a.n_items * (a.heads / a.group);
     const size_t lds = 4 * kRowsPerTile<T, D> * D * sizeof(T) + 6 * kRowsPerTile<T, D> * 4 + bias_floats(a) * 4;
-    if (waves == 2)
-        return a.bias.table ? start(attn_dkv_kernel<T, D, 2, true>, blocks, 128, lds, s, a) : start(attn_dkv_kernel<T, D, 2, false>, blocks, 128, lds, s, a);
-    return a.bias.table ? start(attn_dkv_kernel<T, D, 4, true>, blocks, 256, lds, s, a) : start(attn_dkv_kernel<T, D, 4, false>, blocks, 256, lds, s, a);
+    return a.bias.table ? start(attn_dkv_kernel<T, D, NW, true, PART>, blocks, NW * 64, lds, s, a)
+                        : start(attn_dkv_kernel<T, D, NW, false, PART>, blocks, NW * 64, lds, s, a);
+}
+template <typename T, int D, int NW>
+hipError_t dkv_waves(const AttnArgs& a, hipStream_t s) {
+    if constexpr (kTwoLaunches<T, D>) {
+        const hipError_t e = dkv_part<T, D, NW, kOnlyDk>(a, s);
+        return e != hipSuccess ? e : dkv_part<T, D, NW, kOnlyDv>(a, s);
+    } else {
+        return dkv_part<T, D, NW, kBoth>(a, s);
+    }
+}
+template <typename T, int D>
+hipError_t dkv_dim(const AttnArgs& a, int waves, hipStream_t s) {
+    return waves == 2 ? dkv_waves<T, D, 2>(a, s) : dkv_waves<T, D, 4>(a, s);
 }
 
 template <typename T, int D>

@@ -21,6 +21,12 @@ constexpr float kLazy = 4.f;
 // keys of a tile in LDS: 64 where the registers that carry the next tile allow it
 template <typename T, int D> constexpr int kKeysPerTile = sizeof(T) == 2 ? 64 : 32;
 
+// Wavefronts a SIMD that the compiler is held to; more registers than that allows cost more than they give.  Three in the
+// forward kernel with 16-bit heads up to 64 (168 registers; two, with up to 198, took 171 us of a 48-protein batch where three take
+// 131); two otherwise; one for fp32 heads of 128, whose operands alone take 128 registers (two: 5.4 ms and a spill
+// of 64 registers, one: 3.6 ms without, 32,768 rows in sequences of 1,024).
+template <typename T, int D> constexpr int kForwardWaves = sizeof(T) * D >= 512 ? 1 : sizeof(T) == 2 && D <= 64 ? 3 : 2;
+
 // what a wavefront knows of its 32 queries
 struct Rows {
     int pos, pmin, pmax;
@@ -151,7 +157,7 @@ __device__ __forceinline__ Rows rows_of(const AttnArgs& a, int q0, int pos0, int
 
 // ---- many queries: NW wavefronts of 32 queries share tiles of keys and values in LDS (two buffers, one barrier a tile)
 template <typename T, int D, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64, D <= 64 && sizeof(T) == 2 ? 3 : 2) void attn_fwd_wide_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, (kForwardWaves<T, D>)) void attn_fwd_wide_kernel(AttnArgs a) {
     constexpr int kBK = kKeysPerTile<T, D>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
     constexpr int kBytes = kBK * D * (int)sizeof(T);
     extern __shared__ char smem[];
@@ -271,7 +277,7 @@ __global__ __launch_bounds__(NW * 64, D <= 64 && sizeof(T) == 2 ? 3 : 2) void at
 // ---- range of keys is cut over workgroups as well; the parts meet in LDS, those of several workgroups in attn_join_kernel.
 // ---- A row is a query of one of `pack` heads that share their keys, so that keys are read once for all of them
 template <typename T, int D, bool BIAS>
-__global__ __launch_bounds__(256, 2) void attn_fwd_split_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) * D >= 512 ? 1 : 2) void attn_fwd_split_kernel(AttnArgs a) {
     constexpr int NW = 4, DT = D >= 32 ? D / 32 : 1, ST = D / 16, kPad = D + 4;
     constexpr int kBytes = 32 * D * (int)sizeof(T);
     extern __shared__ char smem[];
