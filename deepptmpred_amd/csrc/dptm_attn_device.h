@@ -325,10 +325,18 @@ __device__ __forceinline__ float bias_value(float v, float inv_scale) { return v
 template <typename T>
 __device__ __forceinline__ void load_bias(float* lds, const BiasArgs& b, float inv_scale, int heads, int head, int tid, int nt) {
     const T* table = static_cast<const T*>(b.table);
-    for (int i = tid; i < 2 * b.reach + 1 + 2 * kBiasPad; i += nt) {
-        const int k = min(max(b.buckets[min(max(i - kBiasPad, 0), 2 * b.reach)], 0), b.n_buckets - 1);
-        const float v = (float)table[(int64_t)k * heads + head];
-        lds[i] = bias_value(v, inv_scale);
+    const int n = 2 * b.reach + 1 + 2 * kBiasPad;
+    // four entries at a time: the second load of an entry waits for its first
+    for (int i0 = tid; i0 < n; i0 += 4 * nt) {
+        int k[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) k[u] = b.buckets[min(max(i0 + u * nt - kBiasPad, 0), 2 * b.reach)];
+        float v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = (float)table[(int64_t)min(max(k[u], 0), b.n_buckets - 1) * heads + head];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i0 + u * nt < n) lds[i0 + u * nt] = bias_value(v[u], inv_scale);
     }
 }
 

@@ -273,7 +273,8 @@ __global__ __launch_bounds__(NW * 64, (kForwardWaves<T, D>)) void attn_fwd_wide_
     }
 }
 
-// ---- few queries: the four wavefronts of a workgroup hold the SAME 32 rows and take every fourth tile of 32 keys, and a long
+// ---- few queries: the four wavefronts of a workgroup (eight: 17 us instead of 12 for the 482 rows of one protein, 20 heads)
+// ---- hold the SAME 32 rows and take every fourth tile of 32 keys, and a long
 // ---- range of keys is cut over workgroups as well; the parts meet in LDS, those of several workgroups in attn_join_kernel.
 // ---- A row is a query of one of `pack` heads that share their keys, so that keys are read once for all of them
 template <typename T, int D, bool BIAS>
@@ -315,7 +316,7 @@ __global__ __launch_bounds__(256, sizeof(T) * D >= 512 ? 1 : 2) void attn_fwd_sp
     };
     if (w < n) fetch(w);
     if constexpr (BIAS) {
-        for (int p = 0; p < pack; ++p) load_bias<T>(bias + p * room, a.bias, 1.f / a.scale, a.heads, head0 + p, tid, 256);
+        for (int p = 0; p < pack; ++p) load_bias<T>(bias + p * room, a.bias, 1.f / a.scale, a.heads, head0 + p, tid, NW * 64);
         __syncthreads();
         bias += (head - head0) * room;
     }
@@ -379,7 +380,7 @@ __global__ __launch_bounds__(256, sizeof(T) * D >= 512 ? 1 : 2) void attn_fwd_sp
             *reinterpret_cast<V4<float>*>(o + (w * 32 + (lane & 31)) * kPad + 32 * d + 8 * g + 4 * h) = x;
         }
     __syncthreads();
-    for (int i = tid; i < rows * (D / 4); i += 256) {
+    for (int i = tid; i < rows * (D / 4); i += NW * 64) {
         const int r = i / (D / 4), d = (i % (D / 4)) * 4, qi = r / pack, hd = head0 + r - qi * pack;
         float t = kMinusInf, sum = 0.f;
 #pragma unroll
@@ -420,6 +421,7 @@ __global__ __launch_bounds__(kJoinRows * (D / 4)) void attn_join_kernel(AttnArgs
     if (r >= jn.n * pack) return;
     const int64_t first = ((int64_t)jn.slot0 * heads + hp) * 32 + r, next = (int64_t)heads * 32;
     float m = kMinusInf, l = 0.f;
+#pragma unroll 8
     for (int k = 0; k < jn.slots; ++k) m = fmaxf(m, a.part_ml[(first + k * next) * 2]);
     V4<float> x{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
@@ -458,13 +460,12 @@ inline size_t bias_floats(const AttnArgs& a) { return a.bias.table ? (size_t)bia
 
 template <typename T, int D>
 hipError_t forward_dim(const AttnArgs& a, int mode, hipStream_t s) {
-    int64_t blocks = (int64_t)a.n_items * a.heads;
+    const int64_t blocks = (int64_t)a.n_items * a.heads;
     if (mode == kSplitKeys) {
-        blocks /= a.pack;
         const size_t v = 4 * 32 * D * sizeof(T), o = 4 * 32 * (D + 4) * 4;
         const size_t lds = (4 * 64 + a.pack * bias_floats(a)) * 4 + (v > o ? v : o);
-        return a.bias.table ? start(attn_fwd_split_kernel<T, D, true>, blocks, 256, lds, s, a)
-                            : start(attn_fwd_split_kernel<T, D, false>, blocks, 256, lds, s, a);
+        return a.bias.table ? start(attn_fwd_split_kernel<T, D, true>, blocks / a.pack, 256, lds, s, a)
+                            : start(attn_fwd_split_kernel<T, D, false>, blocks / a.pack, 256, lds, s, a);
     }
     const size_t lds = 4 * kKeysPerTile<T, D> * D * sizeof(T) + bias_floats(a) * 4;
     if (mode == kWide64)

@@ -86,7 +86,7 @@ int check_rows(const char* who, const char* name, const dptm_rows& t, int64_t ro
     return DPTM_OK;
 }
 
-constexpr int kGroups = 1024;   // workgroups that fill the card four times over
+constexpr int kGroups = 768;   // workgroups that keys are cut for: three a processor
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
