@@ -18,9 +18,14 @@ __device__ __forceinline__ float lse_log2(float lse) { return lse == kMinusInf ?
 
 // A wavefront's rows of dq once more, pair by pair (see Stage::not_finite).
 template <typename T, int D, int DT, bool BIAS>
-DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, int item, const T* q, const T* g, int hk, int pos, float ref, float delta, const float* bias, int h) {
+DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, int item, int head, int row, int pos, const float* bias, int h) {
     const QItem& it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[item];
     const Window win{a.left, a.right, a.sinks};
+    const int hk = head / a.group;
+    const int64_t qr = (int64_t)it.q0 + row;
+    const T* q = row_ptr<T>(a.q, qr, head);
+    const T* g = row_ptr<T>(a.dout, qr, head);
+    const float ref = lse_log2(a.lse[(int64_t)head * a.q_rows + qr]), delta = a.delta[(int64_t)head * a.q_rows + qr];
 #pragma unroll 1
     for (int i = 0; i < 16 * DT; ++i) acc[i] = 0.f;
     for (int j = 0; j < it.ke; ++j) {
@@ -37,6 +42,13 @@ DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, int item, const T* q, 
 
 // rows of a tile in LDS: fewer than in the forward pass where a wavefront's own operands and sums take the registers
 template <typename T, int D> constexpr int kRowsPerTile = sizeof(T) == 2 && D <= 64 ? 64 : 32;
+// 16-bit heads of 64 in the kernel that owns queries.  Without a bias its registers fit three wavefronts a SIMD (tiles of
+// 32 keys, fragments asked for one product ahead, columns read after the scores); 32 proteins of 1,024 residues, 20
+// heads, bf16: 485 -> 414 us.  With a bias they do not (564 -> 573 us, 48 proteins of the training step 235 -> 246): two
+// wavefronts, tiles of 64 keys, and reads as early as they go.
+template <typename T, int D, bool BIAS> constexpr bool kDqThree = sizeof(T) == 2 && D == 64 && !BIAS;
+template <typename T, int D, bool BIAS> constexpr int kDqKeys = kDqThree<T, D, BIAS> ? 32 : kRowsPerTile<T, D>;
+template <typename T, int D, bool BIAS> constexpr int kDqWaves = D * sizeof(T) <= 64 || kDqThree<T, D, BIAS> ? 3 : D * sizeof(T) >= 512 ? 1 : 2;
 
 // Bias gradient, in the kernel that owns queries.  Far tiles (one bucket) are summed in a register.  In a near one the
 // wavefront's rows stand at consecutive positions, so that equal distances are the diagonals of its 32 x 32 dS: it goes to LDS
@@ -51,8 +63,9 @@ template <bool POS> __host__ __device__ inline int dq_lds_floats(int waves, int 
 }
 
 template <typename T, int D, int NW, bool BIAS, bool POS>
-__global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 64 ? 3 : D * sizeof(T) >= 512 ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
-    constexpr int kBK = kRowsPerTile<T, D>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
+__global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, BIAS>)) void attn_dq_kernel(AttnArgs a) {
+    constexpr int kBK = kDqKeys<T, D, BIAS>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
+    constexpr bool kEarly = D <= 64 && !kDqThree<T, D, BIAS>;
     constexpr int kBytes = kBK * D * (int)sizeof(T);
     extern __shared__ char smem[];
     float* bias = reinterpret_cast<float*>(smem + 4 * kBytes);
@@ -160,9 +173,9 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 64 ? 3 : D * sizeof(T) >=
                     if (near) init_bias(s, bias, reach, a0 + 4 * h - rw.pos);
                     else less += c * bias[is_above ? 2 * reach + kBiasPad : 0];
                 }
-                row_products<T, D, D <= 64 ? 4 : 1>(s, p, kt, vt, 32 * k, q, g, lane);
+                row_products<T, D, kEarly ? 4 : 1>(s, p, kt, vt, 32 * k, q, g, lane);
                 Cols<T, D> cols;
-                if constexpr (D <= 64) {
+                if constexpr (kEarly) {
                     cols.read(kt, 32 * k, lane);
                     after_reads<T>();
                 }
@@ -192,7 +205,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 64 ? 3 : D * sizeof(T) >=
                         }
                     }
                 }
-                if constexpr (D > 64) cols.read(kt, 32 * k, lane);
+                if constexpr (!kEarly) cols.read(kt, 32 * k, lane);
                 cols.product(acc, s);
                 if constexpr (BIAS && !POS) {
                     if (near) {     // while the matrix instructions run
@@ -217,7 +230,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 64 ? 3 : D * sizeof(T) >=
     }
     if (__syncthreads_or((int)odd)) {
         float t[16 * DT];
-        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, item, qrow, grow, hk, rw.pos, ref, delta, bias, h);
+        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, item, head, rowc, rw.pos, bias, h);
         take<DT>(acc, t);
     }
     if (row < it.nq) {
@@ -321,10 +334,13 @@ hipError_t dtable_of(const AttnArgs& a, int n_items, hipStream_t s) {
 
 // A wavefront's keys of dk and dv once more, pair by pair (see Stage::not_finite).
 template <typename T, int D, int DT, bool BIAS>
-DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int item, const T* k, const T* v, int hk, int j, int h) {
+DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int item, int hk, int key, int h) {
     const KItem& it = reinterpret_cast<const KItem*>(a.plan + a.items_at)[item];
     const Window win{a.left, a.right, a.sinks};
     const float c = a.scale * kLog2e;
+    const int j = it.j0 + key;
+    const T* k = row_ptr<T>(a.k, (int64_t)it.k0 + key, hk);
+    const T* v = row_ptr<T>(a.v, (int64_t)it.k0 + key, hk);
 #pragma unroll 1
     for (int i = 0; i < 16 * DT; ++i) dk[i] = dv[i] = 0.f;
     for (int head = hk * a.group; head < (hk + 1) * a.group; ++head)
@@ -540,7 +556,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
     }
     if (__syncthreads_or((int)odd)) {
         float x[16 * DT], y[16 * DT];
-        dkv_by_pairs<T, D, DT, BIAS>(kernel_args(), x, y, id - hk * a.n_items, krow, vrow, hk, j, h);
+        dkv_by_pairs<T, D, DT, BIAS>(kernel_args(), x, y, id - hk * a.n_items, hk, keyc, h);
         if constexpr (DK) take<DT>(dk, x);
         if constexpr (DV) take<DT>(dv, y);
     }
@@ -601,8 +617,8 @@ __global__ __launch_bounds__(kJoinRows * (D / 4)) void attn_dkv_join_kernel(Attn
 template <typename T, int D, int NW>
 hipError_t dq_waves(const AttnArgs& a, hipStream_t s) {
     const int64_t blocks = (int64_t)a.n_items * a.heads;
-    const size_t lds = 4 * kRowsPerTile<T, D> * D * sizeof(T) + bias_floats(a) * 4;
-    if (!a.bias.table) return start(attn_dq_kernel<T, D, NW, false, false>, blocks, NW * 64, lds, s, a);
+    if (!a.bias.table) return start(attn_dq_kernel<T, D, NW, false, false>, blocks, NW * 64, 4 * kDqKeys<T, D, false> * D * sizeof(T), s, a);
+    const size_t lds = 4 * kDqKeys<T, D, true> * D * sizeof(T) + bias_floats(a) * 4;
     if (a.has_pos)
         return start(attn_dq_kernel<T, D, NW, true, true>, blocks, NW * 64, lds + 4 * dq_lds_floats<true>(NW, a.bias.n_buckets, a.bias.reach), s, a);
     return start(attn_dq_kernel<T, D, NW, true, false>, blocks, NW * 64, lds + 4 * dq_lds_floats<false>(NW, a.bias.n_buckets, a.bias.reach), s, a);

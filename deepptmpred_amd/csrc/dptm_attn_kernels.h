@@ -103,11 +103,13 @@ __device__ __forceinline__ const AttnArgs& kernel_args() {
 
 // The rows of a wavefront once more, pair by pair: hidden pairs do not enter.  For tiles `first`, `first + every`, ... of `keys` keys.
 template <typename T, int D, int DT, bool BIAS>
-DPTM_COLD void forward_by_pairs(const AttnArgs& a, float* acc, float* ml, int item, const T* q, int hk, int pos, int first, int every, int keys,
+DPTM_COLD void forward_by_pairs(const AttnArgs& a, float* acc, float* ml, int item, int head, int row, int pos, int first, int every, int keys,
                                 const float* bias, int h) {
     const QItem& it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[item];
     const Window win{a.left, a.right, a.sinks};
     const float c = a.scale * kLog2e;
+    const int hk = head / a.group;
+    const T* q = row_ptr<T>(a.q, (int64_t)it.q0 + row, head);
     const int ns = (it.sink_end + keys - 1) / keys, n = ns + (it.ke - it.kb + keys - 1) / keys;
 #pragma unroll 1
     for (int i = 0; i < 16 * DT; ++i) acc[i] = 0.f;
@@ -251,8 +253,7 @@ __global__ __launch_bounds__(NW * 64, (kForwardWaves<T, D>)) void attn_fwd_wide_
     }
     if (__syncthreads_or((int)odd)) {
         float t[16 * DT], ml[2];
-        forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, ml, id - head * a.n_items, row_ptr<T>(a.q, (int64_t)it.q0 + rowc, head), hk, rw.pos, 0, 1, kBK,
-                                         bias, h);
+        forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, ml, id - head * a.n_items, head, rowc, rw.pos, 0, 1, kBK, bias, h);
         take<DT>(acc, t);
         m = ml[0], l = ml[1];
     }
@@ -355,7 +356,7 @@ __global__ __launch_bounds__(256, sizeof(T) * D >= 512 ? 1 : 2) void attn_fwd_sp
     }
     if (__ballot(odd != 0)) {
         float t[16 * DT], x[2];
-        forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, x, id - id / a.n_items * a.n_items, qrow, hk, rw.pos, w, NW, 32, bias, h);
+        forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, x, id - id / a.n_items * a.n_items, head, query, rw.pos, w, NW, 32, bias, h);
         take<DT>(acc, t);
         m = x[0], l = x[1];
     }
