@@ -52,7 +52,7 @@ __device__ __forceinline__ void attend(const float* kp, const float* vp, const f
                     kb[(t + 1) & 1][i] = *reinterpret_cast<const f32x4*>(kp + (t + 1) * kLdsStride + 4 * i);
             }
             const f32x4 (&k)[4] = kb[t & 1];
-            // two partial sums per row so that the 16 products go through 8 packed FMAs; the rows'
+            // two partial sums per row so that the 16 products form two chains of 8 FMAs; the rows'
             // chains are written interleaved so that consecutive instructions are independent
             f32x2 a2[NR];
 #pragma unroll
