@@ -5,6 +5,7 @@
 #include <cmath>
 #include <cstring>
 #include <exception>
+#include <initializer_list>
 #include <new>
 #include <string>
 #include <vector>
@@ -48,7 +49,7 @@ struct OnDevice {
     bool ok = false;
     explicit OnDevice(int device) {
         if (hipGetDevice(&before) != hipSuccess) before = -1;
-        ok = before == device || hipSetDevice(device) == hipSuccess;
+        ok = (before >= 0 && before == device) || hipSetDevice(device) == hipSuccess;
     }
     ~OnDevice() {
         int now = -1;
@@ -71,18 +72,62 @@ int check_rows(const char* who, const char* name, const dptm_rows& t, int64_t ro
     const int size = size_of(dtype);
     if (!t.data) return fail(DPTM_EINVAL, at() + ": NULL buffer");
     if (t.rows < rows) return fail(DPTM_EINVAL, at() + " has " + std::to_string(t.rows) + " rows, the call needs " + std::to_string(rows));
-    if ((reinterpret_cast<uintptr_t>(t.data) & 15) || (t.row_stride * size) % 16 || (t.head_stride * size) % 16)
-        return fail(DPTM_EINVAL, at() + ": address and strides must be multiples of 16 bytes");
     if (t.row_stride < 0 || t.head_stride < 0) return fail(DPTM_EINVAL, at() + ": negative stride");
     // a tile's rows are reached by 32-bit offsets from the first
-    if (t.row_stride * size >= (int64_t(1) << 25) || t.head_stride > (int64_t(1) << 40))
+    if (t.row_stride >= (int64_t(1) << 25) / size || t.head_stride > (int64_t(1) << 40))
         return fail(DPTM_EINVAL, at() + ": row stride of 32 MiB or more");
+    if ((reinterpret_cast<uintptr_t>(t.data) & 15) || (t.row_stride * size) % 16 || (t.head_stride * size) % 16)
+        return fail(DPTM_EINVAL, at() + ": address and strides must be multiples of 16 bytes");
     if (written) {
         const bool rows_outside = (heads == 1 || t.head_stride >= dim) && (rows == 1 || t.row_stride >= (heads - 1) * t.head_stride + dim);
         const bool heads_outside = (rows == 1 || t.row_stride >= dim) && (heads == 1 || t.head_stride >= (rows - 1) * t.row_stride + dim);
         if (!rows_outside && !heads_outside) return fail(DPTM_EINVAL, at() + ": rows or heads of a written tensor overlap");
     }
     *out = Strided{t.data, t.row_stride, t.head_stride};
+    return DPTM_OK;
+}
+
+// A tensor of a call, for check_apart.
+struct Place {
+    const char* name;
+    const Strided& t;
+    int64_t rows;
+    int heads, dim, size;
+    int64_t row() const { return t.row * size; }
+    int64_t head() const { return heads > 1 ? t.head * size : (int64_t)dim * size; }
+    int64_t row_bytes() const { return (heads - 1) * head() + (int64_t)dim * size; }
+    int64_t bytes() const { return (rows - 1) * row() + row_bytes(); }
+    bool empty() const { return rows == 0 || heads == 0 || !t.p; }
+    uintptr_t at() const { return reinterpret_cast<uintptr_t>(t.p); }
+};
+
+// Whether two tensors share memory.  Columns of one packed tensor ([rows][q k v heads][dim], or [rows][heads][q k v][dim])
+// do not; for strides that fit neither the answer is no unless they start at the same address.
+bool overlap(const Place& a, const Place& b) {
+    if (a.empty() || b.empty() || a.at() + a.bytes() <= b.at() || b.at() + b.bytes() <= a.at()) return false;
+    if (a.at() == b.at()) return true;
+    const Place &lo = a.at() < b.at() ? a : b, &hi = a.at() < b.at() ? b : a;
+    auto beside = [](int64_t off, int64_t w_lo, int64_t w_hi, int64_t step) { return off >= w_lo && off + w_hi <= step; };
+    auto rows_packed = [](const Place& x) { return x.rows == 1 || x.row() >= x.row_bytes(); };
+    if (!rows_packed(lo) || !rows_packed(hi)) return false;
+    const int64_t step = lo.rows > 1 ? lo.row() : hi.row();
+    if (lo.rows > 1 && hi.rows > 1 && lo.row() != hi.row()) {
+        // one without gaps between its rows: does it reach a row of the other?
+        const Place &whole = lo.row() == lo.row_bytes() ? lo : hi, &other = &whole == &lo ? hi : lo;
+        if (whole.row() != whole.row_bytes()) return false;
+        const int64_t from = (int64_t)(whole.at() - other.at()), first = from < other.row_bytes() ? 0 : (from - other.row_bytes()) / other.row() + 1;
+        return first < other.rows && first * other.row() < from + whole.bytes();
+    }
+    const int64_t off = lo.rows > 1 || hi.rows > 1 ? (int64_t)(hi.at() - lo.at()) % step : (int64_t)(hi.at() - lo.at());
+    if (lo.rows > 1 || hi.rows > 1 ? beside(off, lo.row_bytes(), hi.row_bytes(), step) : off >= lo.row_bytes()) return false;
+    const int64_t dim = (int64_t)lo.dim * lo.size;
+    return !(lo.heads > 1 && lo.head() == hi.head() && beside(off % lo.head(), dim, dim, lo.head()));
+}
+
+// What a call writes lies apart from what it reads and from what else it writes.
+int check_apart(const char* who, const Place& written, std::initializer_list<const Place*> others) {
+    for (const Place* o : others)
+        if (overlap(written, *o)) return fail(DPTM_EINVAL, std::string(who) + ": " + written.name + " shares memory with " + o->name);
     return DPTM_OK;
 }
 
@@ -283,7 +328,8 @@ int make_plan(const dptm_attention_desc& d, const int32_t* q_len, const int32_t*
             std::stable_sort(dkv.begin(), dkv.end(), [](const KItem& a, const KItem& b) { return a.qe - a.qb > b.qe - b.qb; });
         }
     }
-    const int64_t most = (int64_t(1) << 31) - 1;
+    // threads of a launch are counted in 32 bits
+    const int64_t most = (int64_t(1) << 32) / 256 - 1;
     if ((int64_t)fwd.size() * d.heads > most || (int64_t)dq.size() * d.heads > most || (int64_t)dkv.size() * d.kv_heads > most)
         return fail(DPTM_EINVAL, std::string(who) + "too many tiles for one launch");
 
@@ -360,7 +406,8 @@ int check_common(const char* who, const dptm_attention_args& x, size_t need) {
     const void* ws = x.workspace;
     const size_t have = x.workspace_bytes;
     if (!good_type(x.dtype)) return fail(DPTM_EINVAL, std::string(who) + ": dtype must be DPTM_PREC_F32, _BF16 or _F16");
-    if (!(scale > 0.f) || !std::isfinite(scale)) return fail(DPTM_EINVAL, std::string(who) + ": scale must be positive and finite");
+    // the kernels start the score products from lse and bias over the scale
+    if (!(scale >= 0x1p-64f && scale <= 0x1p64f)) return fail(DPTM_EINVAL, std::string(who) + ": scale must be in 2^-64..2^64");
     if (need && (!ws || have < need))
         return fail(DPTM_EINVAL, std::string(who) + ": workspace of " + std::to_string(need) + " bytes needed, " + std::to_string(ws ? have : 0) + " given");
     if (need && (reinterpret_cast<uintptr_t>(ws) & 255)) return fail(DPTM_EINVAL, std::string(who) + ": workspace must be 256-byte aligned");
@@ -444,6 +491,9 @@ int dptm_attention_forward(const dptm_attention_args* args) try {
     OK_OR_RETURN(check_bias(who, x, &a.bias));
     if (nq == 0) return DPTM_OK;
     if (!x.lse || (reinterpret_cast<uintptr_t>(x.lse) & 3)) return fail(DPTM_EINVAL, std::string(who) + ": lse is NULL or misaligned");
+    const int size = size_of(dtype);
+    const Place pq{"q", a.q, nq, heads, dim, size}, pk{"k", a.k, nk, kv, dim, size}, pv{"v", a.v, nk, kv, dim, size};
+    OK_OR_RETURN(check_apart(who, Place{"out", a.out, nq, heads, dim, size}, {&pq, &pk, &pv}));
     a.lse = x.lse;
     a.part_o = static_cast<float*>(x.workspace);
     a.part_ml = reinterpret_cast<float*>(static_cast<char*>(x.workspace) + w.fwd_o);
@@ -481,6 +531,13 @@ int dptm_attention_backward(const dptm_attention_args* args) try {
     if (nq && (!x.lse || (reinterpret_cast<uintptr_t>(x.lse) & 3))) return fail(DPTM_EINVAL, std::string(who) + ": lse is NULL or misaligned");
     if (a.bias.table && (!x.dtable || (reinterpret_cast<uintptr_t>(x.dtable) & 3 & (size_of(dtype) - 1))))
         return fail(DPTM_EINVAL, std::string(who) + ": bias without an aligned buffer for its gradient");
+    const int size = size_of(dtype);
+    const Place pq{"q", a.q, nq, heads, dim, size}, pk{"k", a.k, nk, kv, dim, size}, pv{"v", a.v, nk, kv, dim, size};
+    const Place po{"out", a.out, nq, heads, dim, size}, pg{"dout", a.dout, nq, heads, dim, size};
+    const Place pdq{"dq", a.dq, nq, heads, dim, size}, pdk{"dk", a.dk, nk, kv, dim, size}, pdv{"dv", a.dv, nk, kv, dim, size};
+    OK_OR_RETURN(check_apart(who, pdq, {&pq, &pk, &pv, &po, &pg, &pdk, &pdv}));
+    OK_OR_RETURN(check_apart(who, pdk, {&pq, &pk, &pv, &po, &pg, &pdv}));
+    OK_OR_RETURN(check_apart(who, pdv, {&pq, &pk, &pv, &po, &pg}));
     a.lse = x.lse;
     a.delta = static_cast<float*>(x.workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(x.workspace) + w.delta);
@@ -509,8 +566,8 @@ static int norm_rope_args(const char* who, const dptm_norm_rope_args* x, NormRop
     if (x->rows < 0 || x->rows > (int64_t(1) << 31) - 1) return fail(DPTM_EINVAL, std::string(who) + ": bad row count");
     if (!(x->eps >= 0.f) || !std::isfinite(x->eps)) return fail(DPTM_EINVAL, std::string(who) + ": eps must be finite and not negative");
     if (x->n_positions < 0) return fail(DPTM_EINVAL, std::string(who) + ": negative number of positions");
-    // every row's heads, D / 16 lanes each, in blocks of 256 threads: the grid stays below 2^31
-    if (x->rows * (x->heads + x->kv_heads) * (x->head_dim / 16) / 256 >= (int64_t(1) << 31) - 1)
+    // every row's heads, D / 16 lanes each: threads of a launch are counted in 32 bits
+    if (x->rows * (x->heads + x->kv_heads) * (x->head_dim / 16) >= (int64_t(1) << 32) - 256)
         return fail(DPTM_EINVAL, std::string(who) + ": too many rows for one launch");
     if (x->rows && (!x->cosv || !x->sinv || (reinterpret_cast<uintptr_t>(x->cosv) & 15) || (reinterpret_cast<uintptr_t>(x->sinv) & 15)))
         return fail(DPTM_EINVAL, std::string(who) + ": cos / sin are NULL or not 16-byte aligned");
@@ -526,12 +583,28 @@ static int norm_rope_args(const char* who, const dptm_norm_rope_args* x, NormRop
     return DPTM_OK;
 }
 
+// A head's result may take the place of what it is made from, element for element, and lies apart from the rest.
+static int norm_rope_apart(const char* who, const dptm_norm_rope_args& x, const Strided (&from)[2], const Strided (&to)[2], const char* const (&name)[4]) {
+    const int size = size_of(x.dtype), n[2] = {x.heads, x.kv_heads};
+    const Place f0{name[0], from[0], x.rows, n[0], x.head_dim, size}, f1{name[1], from[1], x.rows, n[1], x.head_dim, size};
+    const Place t0{name[2], to[0], x.rows, n[0], x.head_dim, size}, t1{name[3], to[1], x.rows, n[1], x.head_dim, size};
+    auto same = [](const Place& a, const Place& b) {
+        return a.at() == b.at() && (a.rows == 1 || a.t.row == b.t.row) && (a.heads == 1 || a.t.head == b.t.head);
+    };
+    OK_OR_RETURN(check_apart(who, t0, {&f1, &t1}));
+    OK_OR_RETURN(check_apart(who, t1, {&f0}));
+    if (!same(t0, f0)) OK_OR_RETURN(check_apart(who, t0, {&f0}));
+    if (!same(t1, f1)) OK_OR_RETURN(check_apart(who, t1, {&f1}));
+    return DPTM_OK;
+}
+
 int dptm_qk_norm_rope_forward(const dptm_norm_rope_args* x) try {
     const char* who = "dptm_qk_norm_rope_forward";
     NormRopeArgs a;
     OK_OR_RETURN(norm_rope_args(who, x, &a));
     OK_OR_RETURN(check_rows(who, "q_out", x->q_out, x->heads ? x->rows : 0, x->heads, x->head_dim, x->dtype, true, &a.y[0]));
     OK_OR_RETURN(check_rows(who, "k_out", x->k_out, x->kv_heads ? x->rows : 0, x->kv_heads, x->head_dim, x->dtype, true, &a.y[1]));
+    OK_OR_RETURN(norm_rope_apart(who, *x, a.x, a.y, {"q", "k", "q_out", "k_out"}));
     if (x->rows == 0) return DPTM_OK;
     const OnDevice on(x->device);
     if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
@@ -560,6 +633,8 @@ int dptm_qk_norm_rope_backward(const dptm_norm_rope_args* x) try {
     const int64_t half = dptm_qk_norm_rope_workspace(x) / 2;
     if ((x->q_gain || x->k_gain) && (!x->workspace || x->workspace_bytes < (size_t)half * 2 || (reinterpret_cast<uintptr_t>(x->workspace) & 255)))
         return fail(DPTM_EINVAL, std::string(who) + ": workspace of " + std::to_string(half * 2) + " bytes, 256-byte aligned, needed");
+    OK_OR_RETURN(norm_rope_apart(who, *x, a.dy, a.dx, {"dq_out", "dk_out", "dq", "dk"}));
+    OK_OR_RETURN(norm_rope_apart(who, *x, a.x, a.dx, {"q", "k", "dq", "dk"}));
     a.part[0] = static_cast<float*>(x->workspace);
     a.part[1] = x->workspace ? reinterpret_cast<float*>(static_cast<char*>(x->workspace) + half) : nullptr;
     a.dgain[0] = x->dq_gain, a.dgain[1] = x->dk_gain;

@@ -433,7 +433,9 @@ int64_t dptm_attention_plan(const dptm_attention_desc* d, const int32_t* q_len, 
  *                    float32 and bfloat16) hides the pairs of its bucket
  *   workspace        dptm_attention_workspace bytes, 256-byte aligned, contents of no meaning before or after
  *   dout .. dtable   the backward call only; dtable [n_buckets][heads] with a bias
- *   scale            of the scores, positive */
+ *   scale            of the scores, 2^-64..2^64
+ * What a call writes (out; dq, dk, dv) lies apart from what it reads and from what else it writes; columns of one packed
+ * tensor do.  Row strides are below 32 MiB */
 typedef struct dptm_attention_args {
     const int32_t* plan;
     const int32_t* plan_dev;
@@ -465,9 +467,9 @@ int dptm_attention_backward(const dptm_attention_args* args);
 /* Norm of every query and key head and the rotation by position, one pass: y = x (mean x^2 + eps)^-1/2 gain over the
  * head, then the pairs (i, i + head_dim/2) -- interleaved not 0: (2i, 2i+1) -- turned by the angle whose cosine and sine stand in
  * cosv / sinv [n_positions][head_dim/2] (float32) at the row's position: positions[r], or r if NULL.  A position outside
- * the table makes its row NaN.  q_gain / k_gain float32 [head_dim] or NULL (no norm of that tensor).  The outputs may be the
- * inputs.  The backward call takes q and k as the forward call read them and dq_out / dk_out, the gradients of what it wrote; dq / dk
- * may be dq_out / dk_out; dq_gain / dk_gain where there is a gain; workspace as for attention. */
+ * the table makes its row NaN.  q_gain / k_gain float32 [head_dim] or NULL (no norm of that tensor).  q_out / k_out may be
+ * q / k themselves and lie apart otherwise.  The backward call takes q and k as the forward call read them and dq_out / dk_out, the gradients of what it wrote; dq / dk
+ * may be dq_out / dk_out or q / k themselves; dq_gain / dk_gain where there is a gain; workspace as for attention. */
 typedef struct dptm_norm_rope_args {
     dptm_rows q, k, q_out, k_out;
     const float* q_gain;

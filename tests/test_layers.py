@@ -302,3 +302,89 @@ def test_the_restated_gradients_are_the_differences_of_the_forward_pass(window, 
                 d = rng.normal(size=6)
                 slope = ((f(x["q"], None, gn + 1e-6 * d)["y"][0] - f(x["q"], None, gn - 1e-6 * d)["y"][0]) * w).sum() / 2e-6
                 assert abs(slope - (r["dgain"][0] * d).sum()) < 1e-6
+
+
+def test_results_that_share_memory_with_others_are_refused():
+    """What a call writes lies apart from what it reads and from what else it writes; columns of one packed tensor do."""
+    lib = _native.load_library()
+    plan = layers.AttentionPlan([10], heads=2, head_dim=64, device=None)
+    P, n = plan.words.ctypes.data, 1 << 22
+
+    def packed(part, row=6 * 64, head=64):     # two heads of a tensor [10][q k v][64], bfloat16
+        return _native.Rows((1 << 24) + part * 2 * 64 * 2, 10, row, head)
+
+    def forward(out, q=packed(0), k=packed(1), v=packed(2)):
+        x = _native.AttentionArgs(plan=P, plan_dev=P, q=q, k=k, v=v, out=out, lse=n, dtype=1, scale=0.1, device=4096, workspace=n, workspace_bytes=n)
+        return lib.dptm_attention_forward(C.addressof(x))
+
+    def says(rc, text):
+        assert rc == _native.DPTM_EINVAL and text in lib.dptm_layer_last_error().decode(), (text, lib.dptm_layer_last_error())
+
+    apart = "no such device"                   # the last check before anything runs
+    says(forward(rows_of(10, 2, 64, at=1 << 20)), apart)
+    for part, name in enumerate("qkv"):
+        says(forward(packed(part)), f"out shares memory with {name}")
+    says(forward(packed(1), k=packed(2)), apart)
+    says(forward(rows_of(10, 2, 64, at=(1 << 24) + 9 * 6 * 128)), "shares memory")                     # inside the last row
+    says(forward(rows_of(10, 2, 64, at=(1 << 24) + (9 * 6 + 6) * 128)), apart)                         # right behind it
+    says(forward(_native.Rows((1 << 24) + 128, 10, 128, 64), *(rows_of(10, 2, 64, at=(1 << 24)),) * 3), "out shares memory with q")
+    # [row][head][q k v][64]
+    by_head = [_native.Rows((1 << 24) + part * 128, 10, 6 * 64, 3 * 64) for part in range(3)]
+    says(forward(by_head[1], by_head[0], by_head[2], by_head[2]), apart)
+    says(forward(by_head[1], by_head[0], by_head[1], by_head[2]), "out shares memory with k")
+    says(forward(_native.Rows((1 << 24) + 64, 10, 6 * 64, 3 * 64), *by_head), "shares memory")
+
+    def backward(dq=packed(0), dk=packed(1), dv=packed(2)):
+        some = rows_of(10, 2, 64, at=1 << 20)
+        x = _native.AttentionArgs(plan=P, plan_dev=P, q=some, k=some, v=some, out=some, lse=n, workspace=1 << 30, workspace_bytes=1 << 30, dout=some,
+                                  dq=dq, dk=dk, dv=dv, dtype=1, scale=0.1, device=4096)
+        return lib.dptm_attention_backward(C.addressof(x))
+
+    says(backward(), apart)
+    says(backward(dk=packed(0)), "dq shares memory with dk")
+    says(backward(dv=packed(1)), "dk shares memory with dv")
+    says(backward(dv=rows_of(10, 2, 64, at=1 << 20)), "dv shares memory with q")
+
+    def norm(back=False, **more):
+        x = _native.NormRopeArgs(**{**dict(q=packed(0), k=packed(1), q_out=packed(0), k_out=packed(1), cosv=n, sinv=n, dq_out=packed(2, 8 * 64),
+                                           dk_out=packed(3, 8 * 64), dq=packed(2, 8 * 64), dk=packed(3, 8 * 64), dtype=1, head_dim=64, heads=2,
+                                           kv_heads=2, rows=10, n_positions=10, eps=1e-6, device=4096), **more})
+        if back:
+            x.q, x.k = rows_of(10, 2, 64, at=1 << 20), rows_of(10, 2, 64, at=1 << 21)
+        return (lib.dptm_qk_norm_rope_backward if back else lib.dptm_qk_norm_rope_forward)(C.addressof(x))
+
+    says(norm(), apart)                        # in place
+    says(norm(q_out=packed(2)), apart)
+    says(norm(q_out=packed(1), k_out=packed(0)), "shares memory")
+    says(norm(k_out=packed(0)), "shares memory")
+    says(norm(q_out=packed(0, 7 * 64)), "q_out shares memory with")
+    says(norm(back=True), apart)
+    says(norm(back=True, dq=packed(3, 8 * 64)), "shares memory")
+
+
+def test_sizes_that_no_launch_or_offset_holds_are_refused():
+    lib = _native.load_library()
+    plan = layers.AttentionPlan([10], heads=2, head_dim=64, device=None)
+    P, n = plan.words.ctypes.data, 1 << 22
+
+    def forward(scale=0.1, **more):
+        x = _native.AttentionArgs(**{**dict(plan=P, plan_dev=P, q=rows_of(10, 2, 64), k=rows_of(10, 2, 64), v=rows_of(10, 2, 64), lse=n, dtype=0,
+                                            out=rows_of(10, 2, 64, at=1 << 24), device=4096, workspace=n, workspace_bytes=n), **more}, scale=scale)
+        return lib.dptm_attention_forward(C.addressof(x))
+
+    def says(rc, text):
+        assert rc == _native.DPTM_EINVAL and text in lib.dptm_layer_last_error().decode(), (text, lib.dptm_layer_last_error())
+
+    for row in (1 << 23, 1 << 40, 1 << 62, (1 << 62) + 128):                # 32 MiB and more, also where the bytes wrap
+        says(forward(q=_native.Rows(1 << 20, 10, row, 64)), "32 MiB")
+    says(forward(q=_native.Rows(1 << 20, 10, (1 << 23) - 4, 64)), "no such device")
+    says(forward(v=_native.Rows(1 << 20, 10, 128, 1 << 62)), "32 MiB")
+    for scale in (1e-20, 1e-39, 1e20, float("inf")):
+        says(forward(scale=scale), "scale")
+    # threads of a launch are counted in 32 bits: 4,096 heads, tiles of 128 rows
+    with pytest.raises(ValueError, match="one launch"):
+        layers.AttentionPlan([128] * 4096, heads=4096, head_dim=16, training=False, device=None)
+    layers.AttentionPlan([128] * 4095, heads=4096, head_dim=16, training=False, device=None)
+    x = _native.NormRopeArgs(q=rows_of(2 ** 24, 256, 16), k=rows_of(2 ** 24, 1, 16), dtype=1, head_dim=16, heads=256, kv_heads=1, rows=2 ** 24,
+                             cosv=n, sinv=n, eps=1e-6, device=4096)
+    says(lib.dptm_qk_norm_rope_forward(C.addressof(x)), "one launch")
