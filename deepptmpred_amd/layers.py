@@ -8,10 +8,11 @@ site is scored from (pred/train_PTM/predict.py:487-501) can be computed and trai
 ``Scorer.score_protein_device`` without leaving it.
 
 Tensors are torch tensors on one GPU, ``[rows, heads, head_dim]`` with the rows of all sequences one behind the other; any
-strides of rows and heads do, if addresses and strides are multiples of 16 bytes and a head's elements are adjacent.  Types are
-float32, bfloat16 and float16.  Calls go out on the current stream of the tensors' GPU and wait for nothing; what they need
+strides of rows and heads do, if addresses and strides are multiples of 16 bytes, rows are less than 32 MiB apart and a head's
+elements are adjacent.  What a call writes shares no memory with what it reads, except where it says so.  Types are float32,
+bfloat16 and float16.  Calls go out on the current stream of the tensors' GPU and wait for nothing; what they need
 besides their results they take from torch's allocator, so calls on several streams and captured graphs do not share
-memory.  Gradients are explicit calls, as everywhere in this package: a tensor that requires grad is refused while autograd
+memory.  A plan may be dropped while calls on any stream still run; a captured graph needs its plans kept as it needs its inputs.  Gradients are explicit calls, as everywhere in this package: a tensor that requires grad is refused while autograd
 records.
 """
 from __future__ import annotations
@@ -129,6 +130,14 @@ def _empty(shape, dtype, device: int):
     return torch.empty(shape, dtype=dtype, device=_gpu(device))
 
 
+def _result(t, like, what: str, name: str, device: int, heads: int, dim: int, rows: int):
+    """A result tensor [rows, heads, dim], the caller's or a new one of ``like``'s type, and its address, rows and strides."""
+    if t is not None:
+        return t, _rows(t, what, name, like.dtype, device, heads, dim, rows)
+    t = like.new_empty((rows, heads, dim))
+    return t, (t.data_ptr(), rows, heads * dim, dim)
+
+
 _gpus: dict = {}
 
 
@@ -191,14 +200,19 @@ class AttentionPlan:
         self.device = None if device is None else _device(device)
         self.device_words = None if device is None else torch.from_numpy(self.words).to(self.device)
         self._at = None if device is None else (self.words.ctypes.data, self.device_words.data_ptr())
+        self._streams = set() if device is None else {_stream(self.device.index)}
         self._bytes: dict = {}
 
-    def _words(self, what: str, device: int):
-        """Addresses of the plan's two copies."""
+    def _words(self, what: str, device: int, stream: int):
+        """Addresses of the plan's two copies, for a call on ``stream``."""
         if self._at is None:
             raise ValueError(f"{what}: the plan was made for the host only")
         if self.device.index != device:
             raise ValueError(f"{what}: the plan is on {self.device}, the tensors are on cuda:{device}")
+        if stream not in self._streams:
+            # the plan may be dropped while that stream still reads it
+            self.device_words.record_stream(torch.cuda.current_stream(device))
+            self._streams.add(stream)
         return self._at
 
     def _workspace(self, n_buckets: int, max_distance: int, backward: int) -> int:
@@ -262,13 +276,13 @@ def attention(q, k, v, plan: AttentionPlan, *, scale: Optional[float] = None, ta
 
     Scores are ``scale * q.k`` (default ``head_dim ** -0.5``) plus ``table[buckets[j - p], head]`` where a relative position
     bias is given (``relative_buckets``; ``table [buckets, heads]`` of the tensors' type).  A row that sees no key gets zeros and
-    ``-inf``.  ``out`` and ``lse`` may be given; rows of ``out`` behind the plan's are left as they are."""
+    ``-inf``; a table entry at or below ``-2^100`` hides the pairs of its bucket.  ``out`` and ``lse`` may be given; rows of ``out`` behind the plan's are left as they are."""
     lib, what, dim = _native.load_library(), "attention", plan.head_dim
     code, device = _first(q, what)
     dtype, heads, nq, nk = q.dtype, plan.heads, plan.q_rows, plan.k_rows
-    host, dev = plan._words(what, device)
-    if out is None:
-        out = _empty((nq, heads, dim), dtype, device)
+    stream = _stream(device)
+    host, dev = plan._words(what, device, stream)
+    out, out_rows = _result(out, q, what, "out", device, heads, dim, nq)
     if lse is None:
         lse = _empty((heads, nq), torch.float32, device)
     table_at, buckets_at, n_buckets, reach = _bias(what, plan, table, buckets, dtype, device)
@@ -278,8 +292,8 @@ def attention(q, k, v, plan: AttentionPlan, *, scale: Optional[float] = None, ta
     _ATTENTION.pack_into(
         block.attention, 0, host, dev, *_rows(q, what, "q", dtype, device, heads, dim, nq),
         *_rows(k, what, "k", dtype, device, plan.kv_heads, dim, nk), *_rows(v, what, "v", dtype, device, plan.kv_heads, dim, nk),
-        *_rows(out, what, "out", dtype, device, heads, dim, nq), _flat(lse, what, "lse", (heads, nq), torch.float32, device),
-        table_at, buckets_at, hold.data_ptr() if n else 0, n, _stream(device), *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0,
+        *out_rows, _flat(lse, what, "lse", (heads, nq), torch.float32, device),
+        table_at, buckets_at, hold.data_ptr() if n else 0, n, stream, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0,
         code, device, n_buckets, reach, dim ** -0.5 if scale is None else scale)
     rc = lib.dptm_attention_forward(block.attention_at)
     if rc:
@@ -295,13 +309,11 @@ def attention_backward(dout, q, k, v, out, lse, plan: AttentionPlan, *, scale: O
     lib, what, dim = _native.load_library(), "attention_backward", plan.head_dim
     code, device = _first(q, what)
     dtype, heads, kv_heads, nq, nk = q.dtype, plan.heads, plan.kv_heads, plan.q_rows, plan.k_rows
-    host, dev = plan._words(what, device)
-    if dq is None:
-        dq = _empty((nq, heads, dim), dtype, device)
-    if dk is None:
-        dk = _empty((nk, kv_heads, dim), dtype, device)
-    if dv is None:
-        dv = _empty((nk, kv_heads, dim), dtype, device)
+    stream = _stream(device)
+    host, dev = plan._words(what, device, stream)
+    dq, dq_rows = _result(dq, q, what, "dq", device, heads, dim, nq)
+    dk, dk_rows = _result(dk, q, what, "dk", device, kv_heads, dim, nk)
+    dv, dv_rows = _result(dv, q, what, "dv", device, kv_heads, dim, nk)
     table_at, buckets_at, n_buckets, reach = _bias(what, plan, table, buckets, dtype, device)
     dtable = _empty((n_buckets, heads), dtype, device) if n_buckets else None
     n = plan._workspace(n_buckets, reach, 1)
@@ -311,9 +323,8 @@ def attention_backward(dout, q, k, v, out, lse, plan: AttentionPlan, *, scale: O
         block.attention, 0, host, dev, *_rows(q, what, "q", dtype, device, heads, dim, nq),
         *_rows(k, what, "k", dtype, device, kv_heads, dim, nk), *_rows(v, what, "v", dtype, device, kv_heads, dim, nk),
         *_rows(out, what, "out", dtype, device, heads, dim, nq), _flat(lse, what, "lse", (heads, nq), torch.float32, device),
-        table_at, buckets_at, hold.data_ptr() if n else 0, n, _stream(device),
-        *_rows(dout, what, "dout", dtype, device, heads, dim, nq), *_rows(dq, what, "dq", dtype, device, heads, dim, nq),
-        *_rows(dk, what, "dk", dtype, device, kv_heads, dim, nk), *_rows(dv, what, "dv", dtype, device, kv_heads, dim, nk),
+        table_at, buckets_at, hold.data_ptr() if n else 0, n, stream,
+        *_rows(dout, what, "dout", dtype, device, heads, dim, nq), *dq_rows, *dk_rows, *dv_rows,
         dtable.data_ptr() if n_buckets else 0, code, device, n_buckets, reach, dim ** -0.5 if scale is None else scale)
     rc = lib.dptm_attention_backward(block.attention_at)
     if rc:
@@ -349,13 +360,12 @@ def qk_norm_rope(q, k, cos, sin, *, q_gain=None, k_gain=None, positions=None, ep
     code, device = _first(q, what)
     dtype = q.dtype
     n, heads, kv_heads, dim, n_pos, shared = _norm_rope(what, q, k, cos, sin, q_gain, k_gain, positions, code, device)
-    q_out = _empty(q.shape, dtype, device) if q_out is None else q_out
-    k_out = _empty(k.shape, dtype, device) if k_out is None else k_out
+    q_out, q_out_rows = _result(q_out, q, what, "q_out", device, heads, dim, n)
+    k_out, k_out_rows = _result(k_out, q, what, "k_out", device, kv_heads, dim, n)
     block = _block
     _NORM_ROPE.pack_into(
         block.norm_rope, 0, *_rows(q, what, "q", dtype, device, heads, dim, n), *_rows(k, what, "k", dtype, device, kv_heads, dim, n),
-        *_rows(q_out, what, "q_out", dtype, device, heads, dim, n), *_rows(k_out, what, "k_out", dtype, device, kv_heads, dim, n),
-        *shared, _stream(device), *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0, 0, 0, n, code, device, dim, heads, kv_heads, n_pos,
+        *q_out_rows, *k_out_rows, *shared, _stream(device), *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0, 0, 0, n, code, device, dim, heads, kv_heads, n_pos,
         1 if interleaved else 0, eps)
     rc = lib.dptm_qk_norm_rope_forward(block.norm_rope_at)
     if rc:
@@ -371,8 +381,8 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, cos, sin, *, q_gain=None, k_gain
     code, device = _first(q, what)
     dtype = q.dtype
     n, heads, kv_heads, dim, n_pos, shared = _norm_rope(what, q, k, cos, sin, q_gain, k_gain, positions, code, device)
-    dq = _empty(q.shape, dtype, device) if dq is None else dq
-    dk = _empty(k.shape, dtype, device) if dk is None else dk
+    dq, dq_rows = _result(dq, q, what, "dq", device, heads, dim, n)
+    dk, dk_rows = _result(dk, q, what, "dk", device, kv_heads, dim, n)
     dq_gain = None if q_gain is None else _empty((dim,), torch.float32, device)
     dk_gain = None if k_gain is None else _empty((dim,), torch.float32, device)
 
@@ -381,8 +391,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, cos, sin, *, q_gain=None, k_gain
             _block.norm_rope, 0, *_rows(q, what, "q", dtype, device, heads, dim, n), *_rows(k, what, "k", dtype, device, kv_heads, dim, n),
             *_NO_ROWS, *_NO_ROWS, *shared, _stream(device),
             *_rows(dq_out, what, "dq_out", dtype, device, heads, dim, n), *_rows(dk_out, what, "dk_out", dtype, device, kv_heads, dim, n),
-            *_rows(dq, what, "dq", dtype, device, heads, dim, n), *_rows(dk, what, "dk", dtype, device, kv_heads, dim, n),
-            0 if dq_gain is None else dq_gain.data_ptr(), 0 if dk_gain is None else dk_gain.data_ptr(), at, size, n, code, device, dim,
+            *dq_rows, *dk_rows, 0 if dq_gain is None else dq_gain.data_ptr(), 0 if dk_gain is None else dk_gain.data_ptr(), at, size, n, code, device, dim,
             heads, kv_heads, n_pos, 1 if interleaved else 0, eps)
 
     size, hold = 0, None

@@ -422,3 +422,32 @@ def test_a_layer_in_front_of_the_classifier():
     want = scorer.score_protein(codes, out.reshape(L, 1280).cpu().numpy(), sites + 1, strct)
     assert np.abs(proba.cpu().numpy() - want).max() <= 1e-6
     scorer.close()
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_most_shared_memory(given):
+    """fp32 heads of 128 with the largest bias: four wavefronts of the backward pass, and eight heads in a tile."""
+    rng = np.random.default_rng(40)
+    pos = rng.permutation(1024).astype(np.int32) if given else None
+    attend("f32", 128, [1024] if given else [256] * 2, [1500] if given else None, heads=64, kv_heads=64, positions=pos, window=(200, 100),
+           buckets=(64, 1024, True), seed=41)
+    attend("f32", 128, [3, 4], [1300, 40], heads=16, kv_heads=2, buckets=(64, 1024, False), train=False, seed=42)
+
+
+def test_a_plan_dropped_while_another_stream_reads_it():
+    """The plan's memory is not handed out again before the calls that read it have run."""
+    rng = np.random.default_rng(43)
+    q, k, v = (tensor(rng, "bf16", 900, 2, 64) for _ in range(3))
+    want, _ = layers.attention(q, k, v, layers.AttentionPlan([900], heads=2, head_dim=64))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    plan = layers.AttentionPlan([900], heads=2, head_dim=64)
+    at, size = plan.device_words.data_ptr(), plan.device_words.numel()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(int(2e8))                 # some 0.1 s
+        out, _ = layers.attention(q, k, v, plan)
+    del plan
+    new = [torch.zeros(size, dtype=torch.int32, device="cuda") for _ in range(4)]
+    assert not side.query() and all(t.data_ptr() != at for t in new)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
