@@ -1,4 +1,4 @@
 // Attention kernels for f16 tensors.
-#include "dptm_attn_grad.h"
+#include "dptm_attn_short.h"
 
 DPTM_ATTN_DEFINE(f16, _Float16)

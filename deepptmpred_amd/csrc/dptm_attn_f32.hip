@@ -1,4 +1,4 @@
 // Attention kernels for f32 tensors.
-#include "dptm_attn_grad.h"
+#include "dptm_attn_short.h"
 
 DPTM_ATTN_DEFINE(f32, float)

@@ -334,8 +334,8 @@ hipError_t dtable_of(const AttnArgs& a, int n_items, hipStream_t s) {
 
 // A wavefront's keys of dk and dv once more, pair by pair (see Stage::not_finite).
 template <typename T, int D, int DT, bool BIAS>
-DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int item, int hk, int key, int h) {
-    const KItem& it = reinterpret_cast<const KItem*>(a.plan + a.items_at)[item];
+DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int items_at, int item, int hk, int key, int h) {
+    const KItem& it = reinterpret_cast<const KItem*>(a.plan + items_at)[item];
     const Window win{a.left, a.right, a.sinks};
     const float c = a.scale * kLog2e;
     const int j = it.j0 + key;
@@ -556,7 +556,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
     }
     if (__syncthreads_or((int)odd)) {
         float x[16 * DT], y[16 * DT];
-        dkv_by_pairs<T, D, DT, BIAS>(kernel_args(), x, y, id - hk * a.n_items, hk, keyc, h);
+        dkv_by_pairs<T, D, DT, BIAS>(kernel_args(), x, y, a.items_at, id - hk * a.n_items, hk, keyc, h);
         if constexpr (DK) take<DT>(dk, x);
         if constexpr (DV) take<DT>(dv, y);
     }
@@ -677,5 +677,6 @@ hipError_t dkv_join_dim(const AttnArgs& a, int n_join, int join_at, int tile_key
     hipError_t attn_dkv_join_##NAME(const AttnArgs& a, int dim, int n, int at, int keys, hipStream_t s) {                  \
         return DPTM_ATTN_BY_DIM(dkv_join_dim, a, n, at, keys, s);                                                          \
     }                                                                                                                      \
+    hipError_t attn_short_grad_##NAME(const AttnArgs& a, int dim, int k_items_at, hipStream_t s) { return DPTM_ATTN_BY_DIM(short_grad_dim, a, k_items_at, s); } \
     hipError_t attn_dtable_##NAME(const AttnArgs& a, int n_items, hipStream_t s) { return dtable_of<E>(a, n_items, s); }   \
     }

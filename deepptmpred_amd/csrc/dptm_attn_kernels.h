@@ -167,8 +167,8 @@ __global__ __launch_bounds__(NW * 64, (kForwardWaves<T, D>)) void attn_fwd_wide_
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int id = xcd_order(blockIdx.x, gridDim.x);
-    const int head = id / a.n_items;
-    const QItem it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[id - head * a.n_items];
+    const int head = a.by_sequence ? id % a.heads : id / a.n_items, item = a.by_sequence ? id / a.heads : id - head * a.n_items;
+    const QItem it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[item];
     const Window win{a.left, a.right, a.sinks};
     const float c = a.scale * kLog2e;
 
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(NW * 64, (kForwardWaves<T, D>)) void attn_fwd_wide_
     }
     if (__syncthreads_or((int)odd)) {
         float t[16 * DT], ml[2];
-        forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, ml, id - head * a.n_items, head, rowc, rw.pos, 0, 1, kBK, bias, h);
+        forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, ml, item, head, rowc, rw.pos, 0, 1, kBK, bias, h);
         take<DT>(acc, t);
         m = ml[0], l = ml[1];
     }

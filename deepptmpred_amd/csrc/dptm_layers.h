@@ -20,6 +20,10 @@ constexpr int kFar = 1 << 29;            // a window side without limit; lengths
 // forward modes: rows of a workgroup's tile, and whether its wavefronts share the keys or split them
 enum { kWide128 = 0, kWide64 = 1, kSplitKeys = 2 };
 
+// kPlanDqWaves of a plan whose dq and dk, dv are formed together (dptm_attn_short.h): no sequence has more than 64 rows or keys,
+// heads are not larger than this, and entry i of both lists is sequence i of those that are not empty
+constexpr int kTogether = 1, kShortDim = 64;
+
 struct QItem {       // a tile of query rows: forward and dq
     int q0, nq;      // first row of the packed q, rows
     int k0;          // first row of the sequence in the packed k
@@ -63,6 +67,7 @@ struct AttnArgs {
     float scale;           // of the scores
     int heads, group;      // query heads, query heads per key head
     int left, right, sinks, q_rows, n_items, items_at, has_pos, pos_at, tiles_at;
+    int by_sequence;       // the wide forward kernel takes the heads of a tile one behind the other, not the tiles of a head
     int pack;              // heads of a group that share a tile of rows where the keys are split
 };
 
@@ -73,6 +78,7 @@ struct AttnArgs {
     hipError_t attn_dkv_##T(const AttnArgs& a, int dim, int waves, hipStream_t s);                      \
     hipError_t attn_join_##T(const AttnArgs& a, int dim, int n_join, int join_at, hipStream_t s);       \
     hipError_t attn_dkv_join_##T(const AttnArgs& a, int dim, int n_join, int join_at, int tile_keys, hipStream_t s); \
+    hipError_t attn_short_grad_##T(const AttnArgs& a, int dim, int k_items_at, hipStream_t s);         \
     hipError_t attn_dtable_##T(const AttnArgs& a, int n_items, hipStream_t s);
 DPTM_ATTN_LAUNCHERS(bf16)
 DPTM_ATTN_LAUNCHERS(f16)

@@ -451,3 +451,53 @@ def test_a_plan_dropped_while_another_stream_reads_it():
     assert not side.query() and all(t.data_ptr() != at for t in new)
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim", [16, 32, 64])
+@pytest.mark.parametrize("buckets", [None, (32, 40, True), (8, 9, False), (8, 200, True)])
+def test_short_sequences(dtype, dim, buckets):
+    """Windows: dq, dk, dv and the bias gradient from one kernel.  Sequences without rows or keys, of one, of a wavefront's 32, of
+    all 64; rows in front of the first key and keys that no row sees."""
+    attend(dtype, dim, [51, 64, 33, 1, 21, 32], heads=3, kv_heads=3, buckets=buckets, seed=50, packed=True)
+    attend(dtype, dim, [0, 3, 64, 0, 10, 1, 40], [5, 64, 3, 0, 0, 1, 33], buckets=buckets, window=(20, 13), sinks=3, seed=51)
+    attend(dtype, dim, [64, 64], [64, 2], heads=1, kv_heads=1, buckets=buckets, window=(-1, 0), seed=52)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_short_sequences_with_hidden_nan(dtype):
+    """What a hidden key or row of a window holds does not reach the gradients of the others, and rows behind stay as they are."""
+    rng = np.random.default_rng(53)
+    lens, n = [51, 40], 91
+    q, k, v, dout = (tensor(rng, dtype, n, 2, 32) for _ in range(4))
+    plan = layers.AttentionPlan(lens, heads=2, head_dim=32, window=(-1, 0))
+    b = layers.relative_buckets(8, 20)
+    table = tensor(rng, dtype, 8, 2)
+
+    def run(q, k, v, dout):
+        out, lse = layers.attention(q, k, v, plan, table=table, buckets=b)
+        into = {x: torch.full((n + 2, 2, 32), 7.0, dtype=q.dtype, device="cuda") for x in ("dq", "dk", "dv")}
+        layers.attention_backward(dout, q, k, v, out, lse, plan, table=table, buckets=b, **into)
+        assert all((x[n:] == 7.0).all() for x in into.values())
+        return out, [x[:n] for x in into.values()]
+
+    out, plain = run(q, k, v, dout)
+    want = R.attention(host(q), host(k), host(v), lens, lens, (-1, 0), 0, None, None, host(table), b.cpu().numpy(), host(dout), host(out), dtype)
+
+    def near(t, name, rows):
+        within(t[rows], (want[name][0][rows], want[name][1][rows]), name)
+
+    for t, name in zip(plain, ("dq", "dk", "dv")):
+        near(t, name, slice(0, n))
+    k2, v2 = k.clone(), v.clone()
+    k2[50], v2[50] = float("nan"), float("inf")       # seen by row 50 alone
+    out2, (dq, _, _) = run(q, k2, v2, dout)
+    near(dq, "dq", slice(0, 50))
+    near(dq, "dq", slice(51, n))
+    assert torch.isfinite(out2[:50]).all() and not torch.isfinite(out2[50]).any()
+    q2, dout2 = q.clone(), dout.clone()
+    q2[0], dout2[0] = float("nan"), float("inf")      # sees key 0 alone
+    _, (_, dk, dv) = run(q2, k, v, dout2)
+    for t, name in ((dk, "dk"), (dv, "dv")):
+        near(t, name, slice(1, n))
+        assert not torch.isfinite(t[0]).all()
