@@ -677,6 +677,8 @@ hipError_t dkv_join_dim(const AttnArgs& a, int n_join, int join_at, int tile_key
     hipError_t attn_dkv_join_##NAME(const AttnArgs& a, int dim, int n, int at, int keys, hipStream_t s) {                  \
         return DPTM_ATTN_BY_DIM(dkv_join_dim, a, n, at, keys, s);                                                          \
     }                                                                                                                      \
-    hipError_t attn_short_grad_##NAME(const AttnArgs& a, int dim, int k_items_at, hipStream_t s) { return DPTM_ATTN_BY_DIM(short_grad_dim, a, k_items_at, s); } \
+    hipError_t attn_short_grad_##NAME(const AttnArgs& a, int dim, int waves, int k_items_at, hipStream_t s) {                \
+        return DPTM_ATTN_BY_DIM(short_grad_dim, a, waves, k_items_at, s);                                                 \
+    }                                                                                                                      \
     hipError_t attn_dtable_##NAME(const AttnArgs& a, int n_items, hipStream_t s) { return dtable_of<E>(a, n_items, s); }   \
     }

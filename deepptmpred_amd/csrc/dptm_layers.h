@@ -78,7 +78,7 @@ struct AttnArgs {
     hipError_t attn_dkv_##T(const AttnArgs& a, int dim, int waves, hipStream_t s);                      \
     hipError_t attn_join_##T(const AttnArgs& a, int dim, int n_join, int join_at, hipStream_t s);       \
     hipError_t attn_dkv_join_##T(const AttnArgs& a, int dim, int n_join, int join_at, int tile_keys, hipStream_t s); \
-    hipError_t attn_short_grad_##T(const AttnArgs& a, int dim, int k_items_at, hipStream_t s);         \
+    hipError_t attn_short_grad_##T(const AttnArgs& a, int dim, int waves, int k_items_at, hipStream_t s); \
     hipError_t attn_dtable_##T(const AttnArgs& a, int n_items, hipStream_t s);
 DPTM_ATTN_LAUNCHERS(bf16)
 DPTM_ATTN_LAUNCHERS(f16)

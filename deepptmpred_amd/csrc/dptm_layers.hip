@@ -286,10 +286,10 @@ int make_plan(const dptm_attention_desc& d, const int32_t* q_len, const int32_t*
     std::vector<KItem> dkv;
     std::vector<Join> dkv_joins;
     int dq_waves = 4, dkv_waves = 4, dkv_slots = 0;
-    bool together = d.training && !q_pos && d.heads == d.kv_heads && d.head_dim <= kShortDim;
-    for (const Seq& s : m.seqs) together = together && s.nq <= 64 && s.nk <= 64;
-    if (together) {
-        dq_waves = kTogether, dkv_waves = 2;
+    int longest = 0;
+    for (const Seq& s : m.seqs) longest = std::max(longest, std::max(s.nq, s.nk));
+    if (d.training && !q_pos && d.heads == d.kv_heads && d.head_dim <= kShortDim && longest <= 64) {
+        dq_waves = kTogether, dkv_waves = longest <= 32 ? 1 : 2;
         for (const Seq& s : m.seqs) {
             if (s.nq + s.nk == 0) continue;
             dq.push_back(m.q_item(s, 0, s.nq));
@@ -562,7 +562,7 @@ int dptm_attention_backward(const dptm_attention_args* args) try {
     const hipStream_t s = static_cast<hipStream_t>(x.stream);
     a.n_items = plan[kPlanDq], a.items_at = plan[kPlanDqAt];
     if (plan[kPlanDqWaves] == kTogether) {
-        OK_OR_RETURN(hip_result(who, BY_TYPE(attn_short_grad, a, dim, plan[kPlanDkvAt], s)));
+        OK_OR_RETURN(hip_result(who, BY_TYPE(attn_short_grad, a, dim, plan[kPlanDkvWaves], plan[kPlanDkvAt], s)));
         return a.bias.table ? hip_result(who, BY_TYPE(attn_dtable, a, plan[kPlanDq], s)) : DPTM_OK;
     }
     OK_OR_RETURN(hip_result(who, BY_TYPE(attn_dq, a, dim, plan[kPlanDqWaves], s)));

@@ -462,13 +462,16 @@ def test_short_sequences(dtype, dim, buckets):
     attend(dtype, dim, [51, 64, 33, 1, 21, 32], heads=3, kv_heads=3, buckets=buckets, seed=50, packed=True)
     attend(dtype, dim, [0, 3, 64, 0, 10, 1, 40], [5, 64, 3, 0, 0, 1, 33], buckets=buckets, window=(20, 13), sinks=3, seed=51)
     attend(dtype, dim, [64, 64], [64, 2], heads=1, kv_heads=1, buckets=buckets, window=(-1, 0), seed=52)
+    attend(dtype, dim, [21, 32, 0, 7, 1], [21, 32, 3, 0, 30], heads=3, kv_heads=3, buckets=buckets, window=(12, 9), sinks=1, seed=54)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-def test_short_sequences_with_hidden_nan(dtype):
+@pytest.mark.parametrize("rows", [51, 32])
+def test_short_sequences_with_hidden_nan(dtype, rows):
     """What a hidden key or row of a window holds does not reach the gradients of the others, and rows behind stay as they are."""
     rng = np.random.default_rng(53)
-    lens, n = [51, 40], 91
+    lens, n = [rows, rows - 8], 2 * rows - 8
+    last = rows - 1
     q, k, v, dout = (tensor(rng, dtype, n, 2, 32) for _ in range(4))
     plan = layers.AttentionPlan(lens, heads=2, head_dim=32, window=(-1, 0))
     b = layers.relative_buckets(8, 20)
@@ -490,11 +493,11 @@ def test_short_sequences_with_hidden_nan(dtype):
     for t, name in zip(plain, ("dq", "dk", "dv")):
         near(t, name, slice(0, n))
     k2, v2 = k.clone(), v.clone()
-    k2[50], v2[50] = float("nan"), float("inf")       # seen by row 50 alone
+    k2[last], v2[last] = float("nan"), float("inf")       # seen by the last row alone
     out2, (dq, _, _) = run(q, k2, v2, dout)
-    near(dq, "dq", slice(0, 50))
-    near(dq, "dq", slice(51, n))
-    assert torch.isfinite(out2[:50]).all() and not torch.isfinite(out2[50]).any()
+    near(dq, "dq", slice(0, last))
+    near(dq, "dq", slice(rows, n))
+    assert torch.isfinite(out2[:last]).all() and not torch.isfinite(out2[last]).any()
     q2, dout2 = q.clone(), dout.clone()
     q2[0], dout2[0] = float("nan"), float("inf")      # sees key 0 alone
     _, (_, dk, dv) = run(q2, k, v, dout2)
