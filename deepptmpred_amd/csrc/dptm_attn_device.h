@@ -177,6 +177,17 @@ struct Cols {
             for (int d = 0; d < DT; ++d) mma(acc[d], f[s][d], b);
         }
     }
+    // the same, 16-bit weights of every other 16 rows in twice as many bits: what their rounding leaves goes through again
+    __device__ __forceinline__ void product_more_bits(f32x16_a (&acc)[DT], const f32x16_a& w) const {
+        product(acc, w);
+        if constexpr (sizeof(T) == 2) {
+            V8<T> left;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) left[e] = (T)(w[e] - (float)(T)w[e]);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) mma(acc[d], f[0][d], left);
+        }
+    }
 };
 
 // ROWS rows of a strided tensor on the way to LDS through registers; rows from `valid` on become zeros.  Offsets within
@@ -237,7 +248,6 @@ __device__ __forceinline__ V8<T> global_frag(const char* row, int step, int h) {
     }
 }
 
-__device__ __forceinline__ float half_other(float v) { return __shfl_xor(v, 32); }
 __device__ __forceinline__ float half_max(float v) {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));

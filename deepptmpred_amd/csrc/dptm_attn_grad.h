@@ -62,6 +62,12 @@ template <bool POS> __host__ __device__ inline int dq_lds_floats(int waves, int 
     return POS ? waves * n_buckets * 64 + (bias_room(reach) + 3) / 4 : waves * (kShear + ((2 * reach + 1 + 2 * kFarPad + 3) & ~3));
 }
 
+// Rounding in the 16-bit types.  delta is taken from `out`, which was rounded, and dS is rounded for the product with K: with rounding the
+// result, three errors of the same size, and dq and dk of rows that see few keys were off by 1.5 to 1.7 times what rounding
+// the results alone gives.  The first is mended for dk: a row's dS has to add up to nothing, so what they do add up to is what delta
+// lacks, and the kernel leaves the sum of both behind.  For dq it comes too late; there half of what rounding dS takes away
+// goes through the product a second time (Cols::product_more_bits), and both gradients stay within 1.43 times.  Together they cost
+// 8 % of this kernel (48 proteins 232 -> 250 us); the whole of what the rounding takes away would cost another 6 %.
 template <typename T, int D, int NW, bool BIAS, bool POS>
 __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, BIAS>)) void attn_dq_kernel(AttnArgs a) {
     constexpr int kBK = kDqKeys<T, D, BIAS>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
@@ -134,6 +140,7 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, BIAS>)) void attn_dq_kerne
 #pragma unroll
         for (int r = 0; r < 16; ++r) less_delta[r] = -delta;
     }
+    float over = 0.f;                   // sum of the row's dS, which is what delta lacks
     float below = 0.f, above = 0.f;     // dS of distances up to -reach, from reach on
     KeyWalk walk(it);
     if (walk.more()) fetch(walk);
@@ -182,11 +189,14 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, BIAS>)) void attn_dq_kerne
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, less)) * p[r];
                 if (!full) hide(s, lane_mask(win, rw.pos, a0 + 4 * h, walk.end), 0.f);
+                float sum = 0.f;
+                if (sizeof(T) == 2 || (BIAS && !near)) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sum += s[r];
+                }
+                over += sum;
                 if constexpr (BIAS) {
                     if (!near) {
-                        float sum = 0.f;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) sum += s[r];
                         above += is_above ? sum : 0.f;
                         below += is_above ? 0.f : sum;
                     } else if constexpr (POS) {
@@ -206,7 +216,7 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, BIAS>)) void attn_dq_kerne
                     }
                 }
                 if constexpr (!kEarly) cols.read(kt, 32 * k, lane);
-                cols.product(acc, s);
+                cols.product_more_bits(acc, s);
                 if constexpr (BIAS && !POS) {
                     if (near) {     // while the matrix instructions run
                         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -227,6 +237,10 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, BIAS>)) void attn_dq_kerne
         if (after.more()) put(after, buf ^ 1);
         __syncthreads();
         walk = after;
+    }
+    if constexpr (sizeof(T) == 2) {
+        over = half_sum(over);
+        if (h == 0 && row < it.nq) a.delta[(int64_t)head * a.q_rows + qr] = delta + over;
     }
     if (__syncthreads_or((int)odd)) {
         float t[16 * DT];

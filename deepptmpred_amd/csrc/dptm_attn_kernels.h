@@ -16,6 +16,7 @@ namespace {
 // weight is 2^(kShift + kLazy): 2^14 in float16, whose largest number is 65504.
 template <typename T> constexpr float kShift = sizeof(T) == 2 && Elem<T>::kExp == 0x7c00 ? 10.f : 0.f;
 template <> constexpr float kShift<float> = 0.f;
+template <typename T> constexpr float kUnshift = kShift<T> > 0.f ? 0x1p-10f : 1.f;    // before the logarithm: lse keeps its last bits
 constexpr float kLazy = 4.f;
 
 // keys of a tile in LDS: 64 where the registers that carry the next tile allow it
@@ -270,7 +271,7 @@ __global__ __launch_bounds__(NW * 64, (kForwardWaves<T, D>)) void attn_fwd_wide_
                 for (int e = 0; e < 4; ++e) x[e] = (T)(acc[d][4 * g + e] * inv);
                 *reinterpret_cast<V4<T>*>(o + 32 * d + 8 * g + 4 * h) = x;
             }
-        if (h == 0) a.lse[(int64_t)head * a.q_rows + it.q0 + row] = m == kMinusInf ? kMinusInf : (m - kShift<T> + __log2f(l)) * kLn2;
+        if (h == 0) a.lse[(int64_t)head * a.q_rows + it.q0 + row] = m == kMinusInf ? kMinusInf : (m + __log2f(l * kUnshift<T>)) * kLn2;
     }
 }
 
@@ -400,7 +401,7 @@ __global__ __launch_bounds__(256, sizeof(T) * D >= 512 ? 1 : 2) void attn_fwd_sp
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * inv);
             *reinterpret_cast<V4<T>*>(const_cast<T*>(row_ptr<T>(a.out, (int64_t)it.q0 + qi, hd)) + d) = y;
-            if (d == 0) a.lse[(int64_t)hd * a.q_rows + it.q0 + qi] = t == kMinusInf ? kMinusInf : (t - kShift<T> + __log2f(sum)) * kLn2;
+            if (d == 0) a.lse[(int64_t)hd * a.q_rows + it.q0 + qi] = t == kMinusInf ? kMinusInf : (t + __log2f(sum * kUnshift<T>)) * kLn2;
         } else {
             const int64_t at = ((int64_t)it.slot * (a.heads / pack) + head0 / pack) * 32 + r;
             *reinterpret_cast<V4<float>*>(a.part_o + at * D + d) = x;
@@ -441,7 +442,7 @@ __global__ __launch_bounds__(kJoinRows * (D / 4)) void attn_join_kernel(AttnArgs
     for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * inv);
     const int qi = r / pack, head = hp * pack + r - qi * pack;
     *reinterpret_cast<V4<T>*>(const_cast<T*>(row_ptr<T>(a.out, (int64_t)jn.row0 + qi, head)) + d) = y;
-    if (d == 0) a.lse[(int64_t)head * a.q_rows + jn.row0 + qi] = m == kMinusInf ? kMinusInf : (m - kShift<T> + __log2f(l)) * kLn2;
+    if (d == 0) a.lse[(int64_t)head * a.q_rows + jn.row0 + qi] = m == kMinusInf ? kMinusInf : (m + __log2f(l * kUnshift<T>)) * kLn2;
 }
 
 template <typename K>
