@@ -1,5 +1,5 @@
 // Device helpers of the attention kernels: operand fragments of the 32x32 matrix instructions for the three element
-// types, tiles in LDS, visibility of a pair, and the product that keeps non-finite operands out of hidden pairs.
+// types, tiles in LDS on the way there, visibility of a pair, the relative position bias.
 //
 // Layout.  v_mfma_f32_32x32x16 leaves D[row][col] with col = lane % 32 and row = 8 (r / 4) + 4 (lane / 32) + r % 4 for
 // register r.  Taken as S^T = K Q^T a lane holds one query's scores of 16 keys, so row sums and maxima are in-lane but for
@@ -116,8 +116,8 @@ struct Tile {
 // Left to itself the compiler reads one LDS fragment, waits, and feeds it, to spare registers: a wavefront then stands for
 // the LDS latency of every fragment (56 % of its time in the dk, dv kernel).  For the 16-bit types a product's fragments are
 // therefore asked for as a group in front of a scheduling barrier in the backward kernels.  (The forward kernel has three
-// wavefronts a SIMD that cover for each other, and loses one or spills with more fragments in registers: 129 us as it is, 153
-// to 166 with groups.)  In fp32 a fragment feeds eight instructions and is
+// wavefronts a SIMD that cover for each other, and loses one or spills with more fragments in registers: 127 us for 48
+// proteins as it is, 153 to 166 with groups.)  In fp32 a fragment feeds eight instructions and is
 // twice as large, and the order is left alone.
 template <typename T> __device__ __forceinline__ void after_reads() {
     if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);

@@ -7,6 +7,10 @@
 // the key head).  Scores are computed twice, 7 products for the 5 a single kernel would need, and in turn nothing is added
 // through atomics: results do not depend on the order in which workgroups run.  P and dS are rounded to the tensors' type for
 // the products that sum them; everything else stays in 32 bits.
+//
+// Bound by instructions, vector and matrix together (they do not run side by side on this hardware): 48 proteins of up to 1,024
+// residues, 20 heads of 64, with a bias 240 us for dq and 238 for dk, dv; 32,768 rows in sequences of 4,096 without one 610
+// TFLOP/s by the five products that count, heads of 128 512.
 #pragma once
 #include "dptm_attn_kernels.h"
 
@@ -44,8 +48,8 @@ DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, int item, int head, in
 template <typename T, int D> constexpr int kRowsPerTile = sizeof(T) == 2 && D <= 64 ? 64 : 32;
 // 16-bit heads of 64 in the kernel that owns queries.  Without a bias its registers fit three wavefronts a SIMD (tiles of
 // 32 keys, fragments asked for one product ahead, columns read after the scores); 32 proteins of 1,024 residues, 20
-// heads, bf16: 485 -> 414 us.  With a bias they do not (564 -> 573 us, 48 proteins of the training step 235 -> 246): two
-// wavefronts, tiles of 64 keys, and reads as early as they go.
+// heads, bf16: 485 -> 406 us, and 443 with the bits more that dS has had since.  With a bias they do not fit (564 -> 573 us, 48 proteins of the
+// training step 235 -> 246): two wavefronts, tiles of 64 keys, and reads as early as they go.
 template <typename T, int D, bool BIAS> constexpr bool kDqThree = sizeof(T) == 2 && D == 64 && !BIAS;
 template <typename T, int D, bool BIAS> constexpr int kDqKeys = kDqThree<T, D, BIAS> ? 32 : kRowsPerTile<T, D>;
 template <typename T, int D, bool BIAS> constexpr int kDqWaves = D * sizeof(T) <= 64 || kDqThree<T, D, BIAS> ? 3 : D * sizeof(T) >= 512 ? 1 : 2;
@@ -53,8 +57,8 @@ template <typename T, int D, bool BIAS> constexpr int kDqWaves = D * sizeof(T) <
 // Bias gradient, in the kernel that owns queries.  Far tiles (one bucket) are summed in a register.  In a near one the
 // wavefront's rows stand at consecutive positions, so that equal distances are the diagonals of its 32 x 32 dS: it goes to LDS
 // with zeros between its rows, lane l adds diagonal l up (32 reads at a fixed stride) and keeps the
-// sum by distance; what distances share a bucket is left to attn_dtable_kernel.  Adding every element into its bucket by LDS
-// atomics instead took 773 us of a 48-protein batch where this takes a fraction.  POS: rows at positions from a
+// sum by distance; what distances share a bucket is left to attn_dtable_kernel.  With every element added into its bucket by LDS
+// atomics instead this kernel took 773 us for a 48-protein batch.  POS: rows at positions from a
 // list; each lane then adds into a column of its own per bucket, and no order but the program's enters either.
 constexpr int kShearRow = 68;                   // 32 values and 36 zeros: 17 chunks of 16 bytes, so that rows start on different banks
 constexpr int kShear = 32 * kShearRow + 32;   // floats, 32 zeros in front
@@ -67,7 +71,8 @@ template <bool POS> __host__ __device__ inline int dq_lds_floats(int waves, int 
 // the results alone gives.  The first is mended for dk: a row's dS has to add up to nothing, so what they do add up to is what delta
 // lacks, and the kernel leaves the sum of both behind.  For dq it comes too late; there half of what rounding dS takes away
 // goes through the product a second time (Cols::product_more_bits), and both gradients stay within 1.43 times.  Together they cost
-// 8 % of this kernel (48 proteins 232 -> 250 us); the whole of what the rounding takes away would cost another 6 %.
+// 4 to 10 % of this kernel (48 proteins 232 -> 240 us, without a bias 406 -> 443); the whole of what the rounding takes away would
+// cost another 6 to 10 %.  The bias gradient is left with delta as it was.
 template <typename T, int D, int NW, bool BIAS, bool POS>
 __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, BIAS>)) void attn_dq_kernel(AttnArgs a) {
     constexpr int kBK = kDqKeys<T, D, BIAS>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
@@ -381,8 +386,8 @@ DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int items_a
 }
 
 // Heads of 128 of the 16-bit types take two launches, one for dk and one for dv (8 products then, the scores a third time):
-// together their operands and sums leave room for one wavefront a SIMD, and the two launches take 2392 us where the one took
-// 3018 (32,768 rows in sequences of 2,048, 20 heads).
+// together their operands and sums leave room for one wavefront a SIMD, and the two launches took 2,392 us where the one took
+// 3,018 (32,768 rows in sequences of 2,048, 20 heads).
 enum { kBoth, kOnlyDk, kOnlyDv };
 template <typename T, int D> constexpr bool kTwoLaunches = sizeof(T) == 2 && D == 128;
 

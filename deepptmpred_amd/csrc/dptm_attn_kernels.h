@@ -5,6 +5,12 @@
 //
 // One pass over the keys with a running maximum m and sum l per query, in units of log2 and in 32 bits.  The weights are
 // rounded to the tensors' type for the second product (fp32: not at all), l sums them unrounded.
+//
+// What bounds them.  Long sequences in 16 bits: the vector unit, which works on a tile's softmax for half as long again as its
+// matrix instructions take at heads of 64 (32,768 rows, 20 heads, bf16: 620 TFLOP/s in sequences of 1,024, 708 of 4,096; heads
+// of 128 704 and 812; a large plain product reaches 1,228).  Few queries over long keys: memory (64 new tokens over caches of up to
+// 4,099 keys, 8 key heads of 128: 839 MB in 164 us, 5.1 TB/s; a large copy reaches 5.05).  One short protein: the way of a tile
+// from memory through two products and a join in LDS (482 rows, 20 heads: 12.8 us for 5 MB).
 #pragma once
 #include "dptm_attn_device.h"
 
@@ -23,8 +29,8 @@ constexpr float kLazy = 4.f;
 template <typename T, int D> constexpr int kKeysPerTile = sizeof(T) == 2 ? 64 : 32;
 
 // Wavefronts a SIMD that the compiler is held to; more registers than that allows cost more than they give.  Three in the
-// forward kernel with 16-bit heads up to 64 (168 registers; two, with up to 198, took 171 us of a 48-protein batch where three take
-// 131); two otherwise; one for fp32 heads of 128, whose operands alone take 128 registers (two: 5.4 ms and a spill
+// forward kernel with 16-bit heads up to 64 (168 registers; two, with up to 198, took 171 us of a 48-protein batch where three took
+// 131, now 127); two otherwise; one for fp32 heads of 128, whose operands alone take 128 registers (two: 5.4 ms and a spill
 // of 64 registers, one: 3.6 ms without, 32,768 rows in sequences of 1,024).
 template <typename T, int D> constexpr int kForwardWaves = sizeof(T) * D >= 512 ? 1 : sizeof(T) == 2 && D <= 64 ? 3 : 2;
 
@@ -275,9 +281,9 @@ __global__ __launch_bounds__(NW * 64, (kForwardWaves<T, D>)) void attn_fwd_wide_
     }
 }
 
-// ---- few queries: the four wavefronts of a workgroup (eight: 17 us instead of 12 for the 482 rows of one protein, 20 heads)
-// ---- hold the SAME 32 rows and take every fourth tile of 32 keys, and a long
-// ---- range of keys is cut over workgroups as well; the parts meet in LDS, those of several workgroups in attn_join_kernel.
+// ---- few queries: the four wavefronts of a workgroup (eight: 17.1 us instead of 12.6 for the 482 rows of one protein, 20 heads)
+// ---- hold the SAME 32 rows and take every fourth tile of 32 keys, and a long range of keys is cut over workgroups as well (53
+// ---- rows over 34,003 keys, 20 heads: 42 us, and 6 to join); the parts meet in LDS, those of several workgroups in attn_join_kernel.
 // ---- A row is a query of one of `pack` heads that share their keys, so that keys are read once for all of them
 template <typename T, int D, bool BIAS>
 __global__ __launch_bounds__(256, sizeof(T) * D >= 512 ? 1 : 2) void attn_fwd_split_kernel(AttnArgs a) {

@@ -6,7 +6,8 @@
 // Bound by memory: 2 (forward) or 3 (backward) times the data.  D / 16 lanes share a head; a lane holds eight elements of either
 // half, so both kinds of pairs are its own, the loads are 16 bytes wide, and the sum over the head is at most three
 // exchanges.  A thread keeps the angles and gains of its elements in registers over the heads of a row that it takes.
-// All arithmetic is fp32; results are rounded once to the tensors' type.
+// All arithmetic is fp32; results are rounded once to the tensors' type.  65,539 rows of 40 heads of 64, bf16: forward 125 us for
+// 671 MB (5.4 TB/s), backward 232 + 6 us for 1,007 MB (4.2 TB/s; a large copy reaches 5.05); 482 rows 4.3 us, the launch.
 #include "dptm_layers.h"
 
 namespace dptm {
@@ -233,7 +234,8 @@ __global__ __launch_bounds__(1024) void gain_sum_kernel(const float* p0, const f
     if (row == 0) o[col] = (float)sums[threadIdx.x];
 }
 
-// heads a thread takes in a row: one while the call does not fill the card, HEADS beyond
+// heads a thread takes in a row: one while the call does not fill the card (8,000 rows of 40 heads of 64, bf16: forward 17.3 us and
+// backward 31.6, with more heads 18.2 and 34.7), HEADS beyond (65,539 rows: 145 and 218 with one, 122 and 212)
 constexpr int kForwardHeads = 4, kBackwardHeads = 2;
 bool large(int64_t rows, int all, int dim) { return rows * all * (dim / 16) > 4 * 256 * 2048; }
 
