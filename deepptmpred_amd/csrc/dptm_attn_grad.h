@@ -3,14 +3,14 @@
 //   P_ij = exp(s_ij - lse_i);  delta_i = dout_i . out_i;  dP_ij = dout_i . v_j;  dS = P (dP - delta)
 //   dq_i = scale sum_j dS_ij k_j;  dk_j = scale sum_i dS_ij q_i;  dv_j = sum_i P_ij dout_i;  dtable[b] = sum dS over bucket b
 //
-// Two kernels, one that owns queries (dq, delta, bias) and one that owns keys (dk, dv, over the query heads that share
-// the key head).  Scores are computed twice, 7 products for the 5 a single kernel would need, and in turn nothing is added
-// through atomics: results do not depend on the order in which workgroups run.  P and dS are rounded to the tensors' type for
-// the products that sum them; everything else stays in 32 bits.
+// Two kernels, one that owns queries (dq, delta) and one that owns keys (dk, dv over the query heads that share the key head,
+// and the bias gradient).  Scores are computed twice, 7 products for the 5 a single kernel would need, and in turn nothing is
+// added through atomics: results do not depend on the order in which workgroups run.  P and dS are rounded to the tensors'
+// type for the products that sum them; everything else stays in 32 bits.
 //
 // Bound by instructions, vector and matrix together (they do not run side by side on this hardware): 48 proteins of up to 1,024
-// residues, 20 heads of 64, with a bias 240 us for dq and 238 for dk, dv; 32,768 rows in sequences of 4,096 without one 610
-// TFLOP/s by the five products that count, heads of 128 512.
+// residues, 20 heads of 64, with a bias 175 us for dq and 303 for dk, dv and the bias; 32,768 rows in sequences of 4,096 without one
+// 610 TFLOP/s by the five products that count, heads of 128 512.
 #pragma once
 #include "dptm_attn_kernels.h"
 
@@ -46,49 +46,47 @@ DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, int item, int head, in
 
 // rows of a tile in LDS: fewer than in the forward pass where a wavefront's own operands and sums take the registers
 template <typename T, int D> constexpr int kRowsPerTile = sizeof(T) == 2 && D <= 64 ? 64 : 32;
-// 16-bit heads of 64 in the kernel that owns queries.  Without a bias its registers fit three wavefronts a SIMD (tiles of
-// 32 keys, fragments asked for one product ahead, columns read after the scores); 32 proteins of 1,024 residues, 20
-// heads, bf16: 485 -> 406 us, and 443 with the bits more that dS has had since.  With a bias they do not fit (564 -> 573 us, 48 proteins of the
-// training step 235 -> 246): two wavefronts, tiles of 64 keys, and reads as early as they go.
-template <typename T, int D, bool BIAS> constexpr bool kDqThree = sizeof(T) == 2 && D == 64 && !BIAS;
-template <typename T, int D, bool BIAS> constexpr int kDqKeys = kDqThree<T, D, BIAS> ? 32 : kRowsPerTile<T, D>;
-template <typename T, int D, bool BIAS> constexpr int kDqWaves = D * sizeof(T) <= 64 || kDqThree<T, D, BIAS> ? 3 : D * sizeof(T) >= 512 ? 1 : 2;
+// 16-bit heads of 64 in the kernel that owns queries: its registers fit three wavefronts a SIMD (tiles of 32 keys, fragments asked
+// for one product ahead, columns read after the scores), 32 proteins of 1,024 residues, 20 heads, bf16: 485 -> 406 us, with a bias
+// 524 -> 450.  With the bins of a list of positions (POS) they do not: two wavefronts, tiles of 64 keys, reads as early as they go.
+template <typename T, int D, bool POS> constexpr bool kDqThree = sizeof(T) == 2 && D == 64 && !POS;
+template <typename T, int D, bool POS> constexpr int kDqKeys = kDqThree<T, D, POS> ? 32 : kRowsPerTile<T, D>;
+template <typename T, int D, bool POS> constexpr int kDqWaves = D * sizeof(T) <= 64 || kDqThree<T, D, POS> ? 3 : D * sizeof(T) >= 512 ? 1 : 2;
 
-// Bias gradient, in the kernel that owns queries.  Far tiles (one bucket) are summed in a register.  In a near one the
-// wavefront's rows stand at consecutive positions, so that equal distances are the diagonals of its 32 x 32 dS: it goes to LDS
-// with zeros between its rows, lane l adds diagonal l up (32 reads at a fixed stride) and keeps the
-// sum by distance; what distances share a bucket is left to attn_dtable_kernel.  With every element added into its bucket by LDS
-// atomics instead this kernel took 773 us for a 48-protein batch.  POS: rows at positions from a
-// list; each lane then adds into a column of its own per bucket, and no order but the program's enters either.
+// Bias gradient, in the kernel that owns keys.  Far tiles (one bucket) are summed in a register.  In a near one the rows
+// stand at consecutive positions, so that equal distances are the diagonals of its 32 x 32 dS: it goes to LDS with zeros between its
+// rows, lane l adds diagonal l up (32 reads at a fixed stride) and keeps the sum by distance; what distances share a bucket is
+// left to attn_dtable_kernel.  With every element added into its bucket by LDS atomics instead 48 proteins took 540 us more.  The kernel
+// that owns queries would do it some 30 us faster, but before delta is known to its last bits (see below): the gradient
+// of a bucket was off by up to 1.65 times what rounding it gives, and here is not by more.
+// Rows at positions from a list (POS) have no diagonals.  There it is the kernel that owns queries; each lane adds into a column
+// of its own per bucket, and no order but the program's enters either.
 constexpr int kShearRow = 68;                   // 32 values and 36 zeros: 17 chunks of 16 bytes, so that rows start on different banks
 constexpr int kShear = 32 * kShearRow + 32;   // floats, 32 zeros in front
-template <bool POS> __host__ __device__ inline int dq_lds_floats(int waves, int n_buckets, int reach) {
-    return POS ? waves * n_buckets * 64 + (bias_room(reach) + 3) / 4 : waves * (kShear + ((2 * reach + 1 + 2 * kFarPad + 3) & ~3));
-}
+__host__ __device__ inline int bin_floats(int waves, int n_buckets, int reach) { return waves * n_buckets * 64 + (bias_room(reach) + 3) / 4; }
+__host__ __device__ inline int diagonal_room(int reach) { return (2 * reach + 1 + 2 * kFarPad + 3) & ~3; }
+__host__ __device__ inline int diagonal_floats(int waves, int reach) { return waves * (kShear + diagonal_room(reach)); }
 
-// Rounding in the 16-bit types.  delta is taken from `out`, which was rounded, and dS is rounded for the product with K: with rounding the
-// result, three errors of the same size, and dq and dk of rows that see few keys were off by 1.5 to 1.7 times what rounding
-// the results alone gives.  The first is mended for dk: a row's dS has to add up to nothing, so what they do add up to is what delta
-// lacks, and the kernel leaves the sum of both behind.  For dq it comes too late; there half of what rounding dS takes away
-// goes through the product a second time (Cols::product_more_bits), and both gradients stay within 1.43 times.  Together they cost
-// 4 to 10 % of this kernel (48 proteins 232 -> 240 us, without a bias 406 -> 443); the whole of what the rounding takes away would
-// cost another 6 to 10 %.  The bias gradient is left with delta as it was.
+// Rounding in the 16-bit types.  delta is taken from `out`, which was rounded, and dS is rounded for the product with K: with rounding
+// the result, three errors of the same size, and dq and dk of rows that see few keys were off by 1.5 to 1.7 times what
+// rounding the results alone gives.  The first is mended for dk and the bias: a row's dS has to add up to nothing, so what they do
+// add up to is what delta lacks, and the kernel leaves the sum of both behind.  For dq it comes too late; there half of what
+// rounding dS takes away goes through the product a second time (Cols::product_more_bits), and both gradients stay within 1.43
+// times.  Together they cost 4 to 10 % of this kernel (without a bias 406 -> 443 us); the whole of what the rounding takes
+// away would cost another 6 to 10 %.
 template <typename T, int D, int NW, bool BIAS, bool POS>
-__global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, BIAS>)) void attn_dq_kernel(AttnArgs a) {
-    constexpr int kBK = kDqKeys<T, D, BIAS>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
-    constexpr bool kEarly = D <= 64 && !kDqThree<T, D, BIAS>;
+__global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, POS>)) void attn_dq_kernel(AttnArgs a) {
+    constexpr int kBK = kDqKeys<T, D, POS>, NK = kBK / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
+    constexpr bool kEarly = D <= 64 && !kDqThree<T, D, POS>;
     constexpr int kBytes = kBK * D * (int)sizeof(T);
     extern __shared__ char smem[];
     float* bias = reinterpret_cast<float*>(smem + 4 * kBytes);
     const int reach = a.bias.reach, nb = a.bias.n_buckets;
-    const int words = 2 * reach + 1 + 2 * kFarPad, room = (words + 3) & ~3;
-    float* more = bias + (BIAS ? bias_room(reach) : 0);
-    unsigned char* bucket = reinterpret_cast<unsigned char*>(more + NW * nb * 64);   // POS
+    float* more = bias + (BIAS ? bias_room(reach) : 0);                              // POS: bins of the wavefronts, [nb][64] each
+    unsigned char* bucket = reinterpret_cast<unsigned char*>(more + NW * nb * 64);
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    float* shear = more + w * kShear;                     // not POS
-    float* sums = more + NW * kShear + w * room;          // by distance, from -reach - kFarPad
-    float* bins = more + w * nb * 64;                     // POS: [nb][64]
+    float* bins = more + w * nb * 64;
     const int id = xcd_order(blockIdx.x, gridDim.x);
     const int head = id / a.n_items, item = id - head * a.n_items;
     const QItem it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[item];
@@ -151,11 +149,11 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, BIAS>)) void attn_dq_kerne
     if (walk.more()) fetch(walk);
     if constexpr (BIAS) {
         load_bias<T>(bias, a.bias, 1.f / a.scale, a.heads, head, tid, NW * 64);
-        const int floats = POS ? NW * nb * 64 : NW * (kShear + room);
-        for (int i = tid; i < floats; i += NW * 64) more[i] = 0.f;
-        if constexpr (POS)
+        if constexpr (POS) {
+            for (int i = tid; i < NW * nb * 64; i += NW * 64) more[i] = 0.f;
             for (int i = tid; i < bias_room(reach); i += NW * 64)
                 bucket[i] = (unsigned char)min(max(a.bias.buckets[min(max(i - kBiasPad, 0), 2 * reach)], 0), nb - 1);
+        }
     }
     if (walk.more()) put(walk, 0);
     __syncthreads();
@@ -195,48 +193,24 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, BIAS>)) void attn_dq_kerne
                 for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, less)) * p[r];
                 if (!full) hide(s, lane_mask(win, rw.pos, a0 + 4 * h, walk.end), 0.f);
                 float sum = 0.f;
-                if (sizeof(T) == 2 || (BIAS && !near)) {
+                if (sizeof(T) == 2 || (POS && !near)) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) sum += s[r];
                 }
                 over += sum;
-                if constexpr (BIAS) {
+                if constexpr (POS) {
                     if (!near) {
                         above += is_above ? sum : 0.f;
                         below += is_above ? 0.f : sum;
-                    } else if constexpr (POS) {
+                    } else if (row < it.nq) {
                         const int at = bias_at(a0 + 4 * h - rw.pos, reach);
-                        if (row < it.nq) {
 #pragma unroll
-                            for (int r = 0; r < 16; ++r)
-                                __hip_atomic_fetch_add(bins + bucket[at + reg_row(r)] * 64 + lane, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                        }
-                    } else {
-                        float* mine = shear + 32 + (lane & 31) * kShearRow + 4 * h;
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const V4<float> y{s[4 * x], s[4 * x + 1], s[4 * x + 2], s[4 * x + 3]};
-                            *reinterpret_cast<V4<float>*>(mine + 8 * x) = y;
-                        }
+                        for (int r = 0; r < 16; ++r)
+                            __hip_atomic_fetch_add(bins + bucket[at + reg_row(r)] * 64 + lane, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                     }
                 }
                 if constexpr (!kEarly) cols.read(kt, 32 * k, lane);
                 cols.product_more_bits(acc, s);
-                if constexpr (BIAS && !POS) {
-                    if (near) {     // while the matrix instructions run
-                        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                        __builtin_amdgcn_wave_barrier();
-                        // lane l: key - row = l - 31, which is the distance a0 + l - 31 - (position of row 0)
-                        const float* from = shear + 32 + lane - 31;
-                        float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) part[i & 3] += from[i * (kShearRow + 1)];
-                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                        __builtin_amdgcn_wave_barrier();
-                        const int dist = a0 + lane - 31 - (it.pos0 + 32 * w) + reach + kFarPad;
-                        if (lane < 63) sums[dist] += (part[0] + part[1]) + (part[2] + part[3]);
-                    }
-                }
             }
         }
         if (after.more()) put(after, buf ^ 1);
@@ -264,39 +238,24 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, BIAS>)) void attn_dq_kerne
                 *reinterpret_cast<V4<T>*>(o + 32 * d + 8 * x + 4 * h) = y;
             }
     }
-    if constexpr (BIAS) {
+    if constexpr (POS) {
 #pragma unroll
         for (int k = 32; k; k >>= 1) {
             above += __shfl_xor(above, k);
             below += __shfl_xor(below, k);
         }
-        if constexpr (POS) {
-            if (lane == 0) {
-                bins[bucket[2 * reach + kBiasPad] * 64] += above;
-                bins[bucket[0] * 64] += below;
-            }
-            __syncthreads();
-            for (int b = w; b < nb; b += NW) {
-                float sum = 0.f;
+        if (lane == 0) {
+            bins[bucket[2 * reach + kBiasPad] * 64] += above;
+            bins[bucket[0] * 64] += below;
+        }
+        __syncthreads();
+        for (int b = w; b < nb; b += NW) {
+            float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < NW; ++i) sum += more[(i * nb + b) * 64 + lane];
+            for (int i = 0; i < NW; ++i) sum += more[(i * nb + b) * 64 + lane];
 #pragma unroll
-                for (int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
-                if (lane == 0) a.part_bias[((int64_t)head * a.n_items + item) * nb + b] = sum;
-            }
-        } else {
-            if (lane == 0) {
-                sums[words - 1] += above;
-                sums[0] += below;
-            }
-            __syncthreads();
-            const float* all = more + NW * kShear;
-            for (int i = tid; i < words; i += NW * 64) {
-                float sum = 0.f;
-#pragma unroll
-                for (int k = 0; k < NW; ++k) sum += all[k * room + i];
-                a.part_bias[((int64_t)head * a.n_items + item) * words + i] = sum;
-            }
+            for (int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
+            if (lane == 0) a.part_bias[((int64_t)head * a.n_items + item) * nb + b] = sum;
         }
     }
 }
@@ -388,26 +347,35 @@ DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int items_a
 // Heads of 128 of the 16-bit types take two launches, one for dk and one for dv (8 products then, the scores a third time):
 // together their operands and sums leave room for one wavefront a SIMD, and the two launches took 2,392 us where the one took
 // 3,018 (32,768 rows in sequences of 2,048, 20 heads).
+// SUMS: with the bias gradient.  With heads of 64 it takes the registers of half a tile of rows (64 rows: spills, 48 proteins 330 us
+// for 303) and of columns read early; smaller heads have them (heads of 32: 552 us with 32 rows, 514 with 64).
+template <typename T, int D, bool SUMS> constexpr int kDkvRows = SUMS && D == 64 ? 32 : kRowsPerTile<T, D>;
 enum { kBoth, kOnlyDk, kOnlyDv };
 template <typename T, int D> constexpr bool kTwoLaunches = sizeof(T) == 2 && D == 128;
 
-template <typename T, int D, int NW, bool BIAS, int PART>
+template <typename T, int D, int NW, bool BIAS, bool SUMS, int PART>
 __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
     constexpr bool DK = PART != kOnlyDv, DV = PART != kOnlyDk;
-    constexpr int kBQ = kRowsPerTile<T, D>, NQ = kBQ / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
+    constexpr int kBQ = kDkvRows<T, D, SUMS>, NQ = kBQ / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
+    constexpr bool kEarly = D <= 64 && !(SUMS && D == 64);
+    constexpr int kGroup = kEarly ? 4 : 2;
     constexpr int kBytes = kBQ * D * (int)sizeof(T);
     extern __shared__ char smem[];
     float* rowref = reinterpret_cast<float*>(smem + 4 * kBytes);   // [2][kBQ] each
     float* rowdelta = rowref + 2 * kBQ;
     int* rowpos = reinterpret_cast<int*>(rowdelta + 2 * kBQ);
     float* bias = reinterpret_cast<float*>(rowpos + 2 * kBQ);
-    const int reach = a.bias.reach;
+    const int reach = a.bias.reach, words = 2 * reach + 1 + 2 * kFarPad, room = diagonal_room(reach);
+    float* more = bias + (BIAS ? bias_room(reach) : 0);             // SUMS
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = a.heads / a.group;
     const int id = xcd_order(blockIdx.x, gridDim.x);
-    const int hk = id / a.n_items;
-    const KItem it = reinterpret_cast<const KItem*>(a.plan + a.items_at)[id - hk * a.n_items];
+    const int hk = id / a.n_items, item = id - hk * a.n_items;
+    const KItem it = reinterpret_cast<const KItem*>(a.plan + a.items_at)[item];
+    float* shear = more + w * kShear;
+    float* sums = more + NW * kShear + w * room;                    // by distance, from -reach - kFarPad
+    float below = 0.f, above = 0.f;                                 // dS of distances up to -reach, from reach on
     const Window win{a.left, a.right, a.sinks};
     const float c = a.scale * kLog2e;
     const bool active = 32 * w < it.nk;
@@ -467,6 +435,12 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
             rowpos[buf * kBQ + tid] = npos;
         }
     };
+    if constexpr (SUMS) {
+        for (int i = tid; i < NW * (kShear + room); i += NW * 64) more[i] = 0.f;
+        if (nt == 0)
+            for (int i = tid; i < a.group * words; i += NW * 64)
+                a.part_bias[((int64_t)(hk * a.group + i / words) * a.n_items + item) * words + i % words] = 0.f;
+    }
     for (int head = hk * a.group; head < (hk + 1) * a.group && nt > 0; ++head) {
         fetch(head, 0);
         if constexpr (BIAS) load_bias<T>(bias, a.bias, 1.f / a.scale, a.heads, head, tid, NW * 64);
@@ -488,7 +462,9 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                 }
                 const Sight sight(win, pmin, pmax);
                 if (active & (r0 < it.qe) & !sight.none(j0, 32)) {
-                    const bool full = sight.all(j0, 32);
+                    // with SUMS lanes behind the last key and rows behind the last count as hidden
+                    const bool full = sight.all(j0, 32) & (!SUMS || ((32 * w + 32 <= it.nk) & (r0 + 32 <= it.qe)));
+                    bool near = false;
                     const int* pos = rowpos + buf * kBQ + 32 * u + 4 * h;
                     const int far = j - (it.pos0 + r0 + 4 * h);      // to the row of register 0, where the plan lists no positions
                     // The products start from what is taken off them: the scores from -lse (and the bias), dP from -delta
@@ -506,9 +482,10 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                             for (int e = 0; e < 4; ++e) p[4 * x + e] = z[e];
                         }
                     }
+                    const bool is_above = j0 - pmax >= reach, is_below = j0 + 31 - pmin <= -reach;
                     if constexpr (BIAS) {
-                        const bool is_above = j0 - pmax >= reach, is_below = j0 + 31 - pmin <= -reach;
-                        if (is_above | is_below) {
+                        near = !(is_above | is_below);
+                        if (!near) {
                             const float b = bias[is_above ? 2 * reach + kBiasPad : 0];
 #pragma unroll
                             for (int r = 0; r < 16; ++r) s[r] += b;
@@ -521,10 +498,10 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                             for (int r = 0; r < 16; ++r) s[r] += b[-reg_row(r)];
                         }
                     }
-                    if constexpr (DK) row_products<T, D, D <= 64 ? 4 : 2>(s, p, qt, gt, 32 * u, kf, vf, lane);
+                    if constexpr (DK) row_products<T, D, kGroup>(s, p, qt, gt, 32 * u, kf, vf, lane);
                     else row_product<T, D, D <= 64 ? 4 : 2>(s, qt, 32 * u, kf, lane);
                     Cols<T, D> gc, qc;
-                    if constexpr (D <= 64) {
+                    if constexpr (kEarly) {
                         gc.read(gt, 32 * u, lane);
                         qc.read(qt, 32 * u, lane);
                         after_reads<T>();
@@ -544,7 +521,10 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                             }
                         } else {
                             // row c is seen if far - c <= right and far - c >= -left, or the key is one of the first
-                            const int lo = far - win.right, hi = j < win.sinks ? kFar : far + win.left, m = max(hi - lo + 1, 0);
+                            const int lo = far - win.right;
+                            int hi = j < win.sinks ? kFar : far + win.left;
+                            if constexpr (SUMS) hi = min(hi, it.qe - 1 - r0 - 4 * h);
+                            const int m = !SUMS || key < it.nk ? max(hi - lo + 1, 0) : 0;
 #pragma unroll
                             for (int r = 0; r < 16; ++r) {
                                 const bool see = (unsigned)(reg_row(r) - lo) < (unsigned)m;
@@ -553,29 +533,84 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                             }
                         }
                     }
+                    if constexpr (SUMS) {
+                        if (near) {
+                            float* mine = shear + 32 + (lane & 31) * kShearRow + 4 * h;
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const V4<float> y{p[4 * x], p[4 * x + 1], p[4 * x + 2], p[4 * x + 3]};
+                                *reinterpret_cast<V4<float>*>(mine + 8 * x) = y;
+                            }
+                        } else {
+                            float sum = 0.f;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) sum += p[r];
+                            above += is_above ? sum : 0.f;
+                            below += is_above ? 0.f : sum;
+                        }
+                    }
                     if constexpr (DV) {
-                        if constexpr (D > 64) {
+                        if constexpr (!kEarly) {
                             gc.read(gt, 32 * u, lane);
                             after_reads<T>();
                         }
                         gc.product(dv, s);
                     }
                     if constexpr (DK) {
-                        if constexpr (D > 64) {
+                        if constexpr (!kEarly) {
                             qc.read(qt, 32 * u, lane);
                             after_reads<T>();
                         }
                         qc.product(dk, p);
+                    }
+                    if constexpr (SUMS) {
+                        if (near) {     // while the matrix instructions run
+                            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                            __builtin_amdgcn_wave_barrier();
+                            // lane l: row - key = l - 31, which is the distance 31 - l + (j0 - position of row r0)
+                            const float* from = shear + 32 + lane - 31;
+                            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) part[i & 3] += from[i * (kShearRow + 1)];
+                            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                            __builtin_amdgcn_wave_barrier();
+                            const int dist = j0 + 31 - lane - (it.pos0 + r0) + reach + kFarPad;
+                            if (lane < 63) sums[dist] += (part[0] + part[1]) + (part[2] + part[3]);
+                        }
                     }
                 }
             }
             if (t + 1 < nt) put(t + 1);
             __syncthreads();
         }
+        if constexpr (SUMS) {
+#pragma unroll
+            for (int k = 32; k; k >>= 1) {
+                above += __shfl_xor(above, k);
+                below += __shfl_xor(below, k);
+            }
+            if (lane == 0) {
+                sums[words - 1] += above;
+                sums[0] += below;
+            }
+            above = below = 0.f;
+            __syncthreads();
+            float* all = more + NW * kShear;
+            float* out = a.part_bias + ((int64_t)head * a.n_items + item) * words;
+            for (int i = tid; i < words; i += NW * 64) {
+                float sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < NW; ++k) {
+                    sum += all[k * room + i];
+                    all[k * room + i] = 0.f;
+                }
+                out[i] = sum;
+            }
+        }
     }
     if (__syncthreads_or((int)odd)) {
         float x[16 * DT], y[16 * DT];
-        dkv_by_pairs<T, D, DT, BIAS>(kernel_args(), x, y, a.items_at, id - hk * a.n_items, hk, keyc, h);
+        dkv_by_pairs<T, D, DT, BIAS>(kernel_args(), x, y, a.items_at, item, hk, keyc, h);
         if constexpr (DK) take<DT>(dk, x);
         if constexpr (DV) take<DT>(dv, y);
     }
@@ -636,23 +671,29 @@ __global__ __launch_bounds__(kJoinRows * (D / 4)) void attn_dkv_join_kernel(Attn
 template <typename T, int D, int NW>
 hipError_t dq_waves(const AttnArgs& a, hipStream_t s) {
     const int64_t blocks = (int64_t)a.n_items * a.heads;
-    if (!a.bias.table) return start(attn_dq_kernel<T, D, NW, false, false>, blocks, NW * 64, 4 * kDqKeys<T, D, false> * D * sizeof(T), s, a);
-    const size_t lds = 4 * kDqKeys<T, D, true> * D * sizeof(T) + bias_floats(a) * 4;
-    if (a.has_pos)
-        return start(attn_dq_kernel<T, D, NW, true, true>, blocks, NW * 64, lds + 4 * dq_lds_floats<true>(NW, a.bias.n_buckets, a.bias.reach), s, a);
-    return start(attn_dq_kernel<T, D, NW, true, false>, blocks, NW * 64, lds + 4 * dq_lds_floats<false>(NW, a.bias.n_buckets, a.bias.reach), s, a);
+    const size_t tiles = 4 * kDqKeys<T, D, false> * D * sizeof(T), tiles_pos = 4 * kDqKeys<T, D, true> * D * sizeof(T), bias = bias_floats(a) * 4;
+    if (!a.bias.table) return start(attn_dq_kernel<T, D, NW, false, false>, blocks, NW * 64, tiles, s, a);
+    if (!a.has_pos) return start(attn_dq_kernel<T, D, NW, true, false>, blocks, NW * 64, tiles + bias, s, a);
+    return start(attn_dq_kernel<T, D, NW, true, true>, blocks, NW * 64, tiles_pos + bias + 4 * bin_floats(NW, a.bias.n_buckets, a.bias.reach), s, a);
 }
 template <typename T, int D>
 hipError_t dq_dim(const AttnArgs& a, int waves, hipStream_t s) {
     return waves == 2 ? dq_waves<T, D, 2>(a, s) : dq_waves<T, D, 4>(a, s);
 }
 
+template <typename T, int D, int NW, bool BIAS, bool SUMS, int PART>
+hipError_t dkv_start(const AttnArgs& a, hipStream_t s) {
+    const int64_t blocks = (int64_t)a.n_items * (a.heads / a.group);
+    constexpr int kRows = kDkvRows<T, D, SUMS>;
+    const size_t lds = 4 * kRows * D * sizeof(T) + 6 * kRows * 4 + (bias_floats(a) + (SUMS ? diagonal_floats(NW, a.bias.reach) : 0)) * 4;
+    return start(attn_dkv_kernel<T, D, NW, BIAS, SUMS, PART>, blocks, NW * 64, lds, s, a);
+}
 template <typename T, int D, int NW, int PART>
 hipError_t dkv_part(const AttnArgs& a, hipStream_t s) {
-    const int64_t blocks = (int64_t)a.n_items * (a.heads / a.group);
-    const size_t lds = 4 * kRowsPerTile<T, D> * D * sizeof(T) + 6 * kRowsPerTile<T, D> * 4 + bias_floats(a) * 4;
-    return a.bias.table ? start(attn_dkv_kernel<T, D, NW, true, PART>, blocks, NW * 64, lds, s, a)
-                        : start(attn_dkv_kernel<T, D, NW, false, PART>, blocks, NW * 64, lds, s, a);
+    if (!a.bias.table) return dkv_start<T, D, NW, false, false, PART>(a, s);
+    if constexpr (PART != kOnlyDv)
+        if (!a.has_pos) return dkv_start<T, D, NW, true, true, PART>(a, s);
+    return dkv_start<T, D, NW, true, false, PART>(a, s);
 }
 template <typename T, int D, int NW>
 hipError_t dkv_waves(const AttnArgs& a, hipStream_t s) {

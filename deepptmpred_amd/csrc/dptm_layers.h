@@ -59,7 +59,7 @@ struct AttnArgs {
     float* delta;          // [heads][q_rows]
     float* part_o;         // forward partials [slot * heads + h][32][D]; backward: dk | dv partials
     float* part_ml;        // the same [32][2]
-    float* part_bias;      // [heads][n_dq][dtable_words]
+    float* part_bias;      // [heads][tiles][dtable_words]
     double* part_groups;   // [heads][dtable_groups][dtable_words]
     void* dtable;          // [n_buckets][heads]
     const int* plan;       // device copy

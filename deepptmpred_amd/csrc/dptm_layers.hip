@@ -385,6 +385,8 @@ int check_plan(const char* who, const int32_t* plan, const int32_t* plan_dev) {
 
 // byte sizes of the workspace's parts, each rounded up to 256
 struct Work { size_t fwd_o, fwd_ml, delta, dkv, bias, groups; };
+// the tiles whose sums make the bias gradient: of keys, or of rows where the plan lists positions
+int bias_items(const int32_t* p) { return p[p[kPlanHasPos] ? kPlanDq : kPlanDkv]; }
 Work work_of(const int32_t* p, int n_buckets, int reach) {
     Work w;
     const size_t dim = p[kPlanHeadDim], heads = p[kPlanHeads], kv = p[kPlanKvHeads];
@@ -392,8 +394,8 @@ Work work_of(const int32_t* p, int n_buckets, int reach) {
     w.fwd_ml = up((size_t)p[kPlanSlots] * (heads / p[kPlanPack]) * 32 * 2 * 4, 256);
     w.delta = up(heads * (size_t)p[kPlanQRows] * 4, 256);
     w.dkv = up((size_t)p[kPlanDkvSlots] * kv * 2 * 32 * (size_t)p[kPlanDkvWaves] * dim * 4, 256);
-    w.bias = up(heads * (size_t)p[kPlanDq] * (size_t)(n_buckets ? dtable_words(p[kPlanHasPos], n_buckets, reach) : 0) * 4, 256);
-    w.groups = n_buckets ? up(heads * (size_t)dtable_groups(p[kPlanDq]) * (size_t)dtable_words(p[kPlanHasPos], n_buckets, reach) * 8, 256) : 0;
+    w.bias = up(heads * (size_t)bias_items(p) * (size_t)(n_buckets ? dtable_words(p[kPlanHasPos], n_buckets, reach) : 0) * 4, 256);
+    w.groups = n_buckets ? up(heads * (size_t)dtable_groups(bias_items(p)) * (size_t)dtable_words(p[kPlanHasPos], n_buckets, reach) * 8, 256) : 0;
     return w;
 }
 
@@ -566,9 +568,9 @@ int dptm_attention_backward(const dptm_attention_args* args) try {
         return a.bias.table ? hip_result(who, BY_TYPE(attn_dtable, a, plan[kPlanDq], s)) : DPTM_OK;
     }
     OK_OR_RETURN(hip_result(who, BY_TYPE(attn_dq, a, dim, plan[kPlanDqWaves], s)));
-    if (a.bias.table) OK_OR_RETURN(hip_result(who, BY_TYPE(attn_dtable, a, plan[kPlanDq], s)));
     a.n_items = plan[kPlanDkv], a.items_at = plan[kPlanDkvAt];
     OK_OR_RETURN(hip_result(who, BY_TYPE(attn_dkv, a, dim, plan[kPlanDkvWaves], s)));
+    if (a.bias.table) OK_OR_RETURN(hip_result(who, BY_TYPE(attn_dtable, a, bias_items(plan), s)));
     return hip_result(who, BY_TYPE(attn_dkv_join, a, dim, plan[kPlanDkvJoin], plan[kPlanDkvJoinAt], 32 * plan[kPlanDkvWaves], s));
 } catch (...) {
     return on_exception("dptm_attention_backward");
