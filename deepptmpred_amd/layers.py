@@ -263,6 +263,8 @@ def _bias(what: str, plan: AttentionPlan, table, buckets, dtype, device: int):
         return 0, 0, 0, 0
     if table is None or buckets is None:
         raise ValueError(f"{what}: table and buckets go together")
+    if not isinstance(table, torch.Tensor) or not isinstance(buckets, torch.Tensor):
+        raise ValueError(f"{what}: table and buckets must be torch tensors")
     if table.dim() != 2 or table.shape[1] != plan.heads:
         raise ValueError(f"{what}: table has shape {tuple(table.shape)}, expected [buckets, {plan.heads}]")
     if buckets.dim() != 1 or buckets.shape[0] % 2 == 0:

@@ -504,3 +504,64 @@ def test_short_sequences_with_hidden_nan(dtype, rows):
     for t, name in ((dk, "dk"), (dv, "dv")):
         near(t, name, slice(1, n))
         assert not torch.isfinite(t[0]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("buckets", [None, (16, 50, True)])
+def test_keys_that_no_row_sees(dtype, buckets):
+    """Sequences without rows, and keys ahead of every row: zeros in dk and dv, nothing in the bias gradient."""
+    attend(dtype, 64, [0, 200, 30], [130, 200, 400], heads=4, kv_heads=2, buckets=buckets, window=(60, 0), seed=60)
+    pos = np.arange(90, dtype=np.int32)
+    attend(dtype, 64, [90], [500], heads=4, kv_heads=4, positions=pos, buckets=buckets, window=(40, 5), seed=61)
+
+
+def test_offsets_past_32_bits():
+    """Rows 16 MiB apart: 300 of them span 4.7 GB, forward and backward, rows and keys."""
+    rng = np.random.default_rng(62)
+    n, heads, dim, row = 300, 2, 64, 1 << 23                  # elements of two bytes between rows
+    buf = torch.empty(n * row, dtype=torch.bfloat16, device="cuda")
+    at = iter(range(0, 1 << 20, 4096))
+
+    def far(x=None):
+        t = buf.as_strided((n, heads, dim), (row, dim, 1), next(at))
+        return t if x is None else t.copy_(x)
+
+    q, k, v, dout = (tensor(rng, "bf16", n, heads, dim) for _ in range(4))
+    plan = layers.AttentionPlan([n], heads=heads, head_dim=dim, window=(150, 100))
+    cos, sin = layers.rotary_table(n, dim)
+    gain = torch.ones(dim, device="cuda")
+
+    def run(f):
+        a, b, c, g = f(q), f(k), f(v), f(dout)
+        a, b = layers.qk_norm_rope(a, b, cos, sin, q_gain=gain, k_gain=gain, q_out=f(), k_out=f())
+        out, lse = layers.attention(a, b, c, plan, out=f())
+        dq, dk, dv, _ = layers.attention_backward(g, a, b, c, out, lse, plan, dq=f(), dk=f(), dv=f())
+        return [t.clone() for t in (a, b, out, lse, dq, dk, dv)]
+
+    near = run(lambda x=None: torch.empty(n, heads, dim, dtype=torch.bfloat16, device="cuda") if x is None else x.clone())
+    for x, y in zip(run(far), near):
+        assert torch.equal(x, y)
+
+
+def test_captured_with_the_most_shared_memory():
+    """Kernels that need more than 64 KB of it are set up outside the stream: a first call may be a captured one."""
+    rng = np.random.default_rng(63)
+    q, k, v, dout = (tensor(rng, "f32", 256, 48, 128) for _ in range(4))
+    b = layers.relative_buckets(64, 900)
+    table = tensor(rng, "f32", 64, 48)
+    plan = layers.AttentionPlan([256], heads=48, head_dim=128, window=(90, 90))
+
+    def run():
+        out, lse = layers.attention(q, k, v, plan, table=table, buckets=b)
+        return (out, lse) + layers.attention_backward(dout, q, k, v, out, lse, plan, table=table, buckets=b)
+
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        r = run()
+    for step in range(3):
+        q.copy_(tensor(np.random.default_rng(70 + step), "f32", *q.shape))
+        for t in r:
+            t.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(r, run()))

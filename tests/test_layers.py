@@ -388,3 +388,9 @@ def test_sizes_that_no_launch_or_offset_holds_are_refused():
     x = _native.NormRopeArgs(q=rows_of(2 ** 24, 256, 16), k=rows_of(2 ** 24, 1, 16), dtype=1, head_dim=16, heads=256, kv_heads=1, rows=2 ** 24,
                              cosv=n, sinv=n, eps=1e-6, device=4096)
     says(lib.dptm_qk_norm_rope_forward(C.addressof(x)), "one launch")
+
+
+def test_a_bias_that_is_no_tensor_is_refused():
+    plan = layers.AttentionPlan([5], heads=2, head_dim=16, device=None)
+    with pytest.raises(ValueError, match="torch tensors"):
+        layers._bias("attention", plan, np.zeros((8, 2), np.float32), layers.relative_buckets(8, 20, device=None), torch.float32, 0)
