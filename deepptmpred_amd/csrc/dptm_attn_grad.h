@@ -9,8 +9,8 @@
 // type for the products that sum them; everything else stays in 32 bits.
 //
 // Bound by instructions, vector and matrix together (they do not run side by side on this hardware): 48 proteins of up to 1,024
-// residues, 20 heads of 64, with a bias 175 us for dq and 303 for dk, dv and the bias; 32,768 rows in sequences of 4,096 without one
-// 610 TFLOP/s by the five products that count, heads of 128 512.
+// residues, 20 heads of 64, with a bias 175 us for dq and 291 for dk, dv and the bias; 32,768 rows in sequences of 4,096 without one
+// 621 TFLOP/s by the five products that count, heads of 128 520.
 #pragma once
 #include "dptm_attn_kernels.h"
 
@@ -347,18 +347,19 @@ DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int items_a
 // Heads of 128 of the 16-bit types take two launches, one for dk and one for dv (8 products then, the scores a third time):
 // together their operands and sums leave room for one wavefront a SIMD, and the two launches took 2,392 us where the one took
 // 3,018 (32,768 rows in sequences of 2,048, 20 heads).
-// SUMS: with the bias gradient.  With heads of 64 it takes the registers of half a tile of rows (64 rows: spills, 48 proteins 330 us
-// for 303) and of columns read early; smaller heads have them (heads of 32: 552 us with 32 rows, 514 with 64).
-template <typename T, int D, bool SUMS> constexpr int kDkvRows = SUMS && D == 64 ? 32 : kRowsPerTile<T, D>;
+//
+// Tiles of 64 rows with heads of 64: the 32 that one barrier's second half works on are a loop of its own and columns are read
+// when they are needed, which keeps the sums of the bias gradient (SUMS) out of scratch: 48 proteins 291 us; unrolled with early
+// reads 401, tiles of 32 rows 303.  Without a bias all of these are the same (558 to 563 us, 32 x 1,024 residues).
 enum { kBoth, kOnlyDk, kOnlyDv };
 template <typename T, int D> constexpr bool kTwoLaunches = sizeof(T) == 2 && D == 128;
 
 template <typename T, int D, int NW, bool BIAS, bool SUMS, int PART>
 __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
     constexpr bool DK = PART != kOnlyDv, DV = PART != kOnlyDk;
-    constexpr int kBQ = kDkvRows<T, D, SUMS>, NQ = kBQ / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
-    constexpr bool kEarly = D <= 64 && !(SUMS && D == 64);
-    constexpr int kGroup = kEarly ? 4 : 2;
+    constexpr int kBQ = kRowsPerTile<T, D>, NQ = kBQ / 32, DT = D >= 32 ? D / 32 : 1, ST = D / 16;
+    constexpr bool kEarly = D < 64;
+    constexpr int kGroup = D <= 64 ? 4 : 2;
     constexpr int kBytes = kBQ * D * (int)sizeof(T);
     extern __shared__ char smem[];
     float* rowref = reinterpret_cast<float*>(smem + 4 * kBytes);   // [2][kBQ] each
@@ -451,7 +452,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
             const int buf = t & 1, i0 = it.qb + t * kBQ;
             const char* qt = smem + buf * kBytes;
             const char* gt = smem + (2 + buf) * kBytes;
-#pragma unroll
+#pragma unroll D == 64 ? 1 : NQ
             for (int u = 0; u < NQ; ++u) {
                 const int r0 = i0 + 32 * u;
                 int pmin = it.pos0 + r0, pmax = it.pos0 + min(r0 + 31, it.nseq - 1);
@@ -684,7 +685,7 @@ hipError_t dq_dim(const AttnArgs& a, int waves, hipStream_t s) {
 template <typename T, int D, int NW, bool BIAS, bool SUMS, int PART>
 hipError_t dkv_start(const AttnArgs& a, hipStream_t s) {
     const int64_t blocks = (int64_t)a.n_items * (a.heads / a.group);
-    constexpr int kRows = kDkvRows<T, D, SUMS>;
+    constexpr int kRows = kRowsPerTile<T, D>;
     const size_t lds = 4 * kRows * D * sizeof(T) + 6 * kRows * 4 + (bias_floats(a) + (SUMS ? diagonal_floats(NW, a.bias.reach) : 0)) * 4;
     return start(attn_dkv_kernel<T, D, NW, BIAS, SUMS, PART>, blocks, NW * 64, lds, s, a);
 }
