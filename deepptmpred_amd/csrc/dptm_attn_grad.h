@@ -351,6 +351,10 @@ DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int items_a
 // Tiles of 64 rows with heads of 64: the 32 that one barrier's second half works on are a loop of its own and columns are read
 // when they are needed, which keeps the sums of the bias gradient (SUMS) out of scratch: 48 proteins 291 us; unrolled with early
 // reads 401, tiles of 32 rows 303.  Without a bias all of these are the same (558 to 563 us, 32 x 1,024 residues).
+// fp32 scores start from zero (or the bias) and lse is taken off by the multiply-add in front of the exponential: sums that start
+// from -lse / scale round where that is, which made dk of 2,000 keys 1.7 times as far off as it has to be.  The weights of
+// the 16-bit types are rounded far above that, and there the start is free.
+template <typename T> constexpr bool kLseLast = sizeof(T) == 4;
 enum { kBoth, kOnlyDk, kOnlyDv };
 template <typename T, int D> constexpr bool kTwoLaunches = sizeof(T) == 2 && D == 128;
 
@@ -402,7 +406,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
     unsigned odd = 0;
     float nref = 0.f, ndelta = 0.f;
     int npos = 0;
-    const float minus_inv_c = -1.f / c;
+    const float from_lse = kLseLast<T> ? -1.f : -1.f / c;
     // the next tile of rows: its addresses move on with it
     const char *qat = nullptr, *gat = nullptr;
     auto fetch = [&](int head, int t) {
@@ -431,7 +435,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
         if (a.has_pos | !Sight(win, it.pos0 + i0, it.pos0 + i1 - 1).all(it.j0, it.nk)) odd |= sq.not_finite() | sg.not_finite();
         if (tid < kBQ) {
             // rows behind the last weigh nothing: their scores start from -inf
-            rowref[buf * kBQ + tid] = tid < i1 - i0 ? lse_log2(nref) * minus_inv_c : kMinusInf;
+            rowref[buf * kBQ + tid] = tid < i1 - i0 ? lse_log2(nref) * from_lse : kMinusInf;
             rowdelta[buf * kBQ + tid] = tid < i1 - i0 ? -ndelta : 0.f;
             rowpos[buf * kBQ + tid] = npos;
         }
@@ -468,13 +472,13 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                     bool near = false;
                     const int* pos = rowpos + buf * kBQ + 32 * u + 4 * h;
                     const int far = j - (it.pos0 + r0 + 4 * h);      // to the row of register 0, where the plan lists no positions
-                    // The products start from what is taken off them: the scores from -lse (and the bias), dP from -delta
+                    // The products start from what is taken off them: the scores from -lse (fp32: see kLseLast) and the bias, dP from -delta
                     f32x16_a s, p;
                     const V4<float>* less = reinterpret_cast<const V4<float>*>(rowref + buf * kBQ + 32 * u + 4 * h);
                     const V4<float>* del = reinterpret_cast<const V4<float>*>(rowdelta + buf * kBQ + 32 * u + 4 * h);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const V4<float> y = less[2 * x];
+                        const V4<float> y = kLseLast<T> ? V4<float>{0.f, 0.f, 0.f, 0.f} : less[2 * x];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[4 * x + e] = y[e];
                         if constexpr (DK) {
@@ -508,9 +512,15 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                         after_reads<T>();
                     }
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        s[r] = __builtin_amdgcn_exp2f(s[r] * c);
-                        if constexpr (DK) p[r] *= s[r];
+                    for (int x = 0; x < 4; ++x) {
+                        V4<float> y{0.f, 0.f, 0.f, 0.f};
+                        if constexpr (kLseLast<T>) y = less[2 * x];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = 4 * x + e;
+                            s[r] = __builtin_amdgcn_exp2f(kLseLast<T> ? fmaf(s[r], c, y[e]) : s[r] * c);
+                            if constexpr (DK) p[r] *= s[r];
+                        }
                     }
                     if (!full) {
                         if (a.has_pos) {

@@ -108,7 +108,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
     sk.store(kt, tid);
     unsigned odd = 0;
     if (!Sight(win, pos0, pos0 + nq - 1).all(0, nk)) odd = sq.not_finite() | sg.not_finite() | sk.not_finite();
-    if (h == 0) rowref[mine] = mine < nq ? lse_log2(lse) * (-1.f / c) : kMinusInf;      // rows behind the last weigh nothing
+    if (h == 0) rowref[mine] = mine < nq ? lse_log2(lse) * (kLseLast<T> ? -1.f : -1.f / c) : kMinusInf;      // rows behind the last weigh nothing
     const bool redo = __syncthreads_or((int)odd);
     if (redo) {
         if (h == 0 && mine < nq) a.delta[(int64_t)head * a.q_rows + qr] = dot_rows<T, D>(row_ptr<T>(a.dout, qr, head), row_ptr<T>(a.out, qr, head));
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
             const V4<float>* less = reinterpret_cast<const V4<float>*>(rowref + r0 + 4 * h);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const V4<float> y = less[2 * x];
+                const V4<float> y = kLseLast<T> ? V4<float>{0.f, 0.f, 0.f, 0.f} : less[2 * x];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[4 * x + e] = y[e];
             }
@@ -146,9 +146,15 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
             }
             row_products<T, D, 4>(s, p, qt, gt, r0, kf, vf, lane);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[r] = __builtin_amdgcn_exp2f(s[r] * c);
-                p[r] *= s[r];
+            for (int x = 0; x < 4; ++x) {
+                V4<float> y{0.f, 0.f, 0.f, 0.f};
+                if constexpr (kLseLast<T>) y = less[2 * x];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * x + e;
+                    s[r] = __builtin_amdgcn_exp2f(kLseLast<T> ? fmaf(s[r], c, y[e]) : s[r] * c);
+                    p[r] *= s[r];
+                }
             }
             if (!full) {
                 // row c is seen if far - c <= right and far - c >= -left, or the key is one of the first
