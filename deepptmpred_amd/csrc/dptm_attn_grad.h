@@ -302,12 +302,10 @@ hipError_t dtable_of(const AttnArgs& a, int n_items, hipStream_t s) {
     const int words = dtable_words(a.has_pos, a.bias.n_buckets, a.bias.reach), n = dtable_groups(n_items);
     if (n) {
         const int per = (n_items + n - 1) / n;
-        hipLaunchKernelGGL(attn_dtable_groups_kernel, dim3(n, a.heads), dim3(256), 0, s, (const float*)a.part_bias, a.part_groups, n_items, words, per);
-        const hipError_t e = hipGetLastError();
+        const hipError_t e = launch(attn_dtable_groups_kernel, dim3(n, a.heads), dim3(256), 0, s, a.part_bias, a.part_groups, n_items, words, per);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(attn_dtable_kernel<T>, dim3(a.heads), dim3(1024), 0, s, a, (const double*)a.part_groups, n, words);
-    return hipGetLastError();
+    return launch(attn_dtable_kernel<T>, dim3(a.heads), dim3(1024), 0, s, a, a.part_groups, n, words);
 }
 
 // A wavefront's keys of dk and dv once more, pair by pair (see Stage::not_finite).
@@ -723,9 +721,8 @@ hipError_t dkv_dim(const AttnArgs& a, int waves, hipStream_t s) {
 template <typename T, int D>
 hipError_t dkv_join_dim(const AttnArgs& a, int n_join, int join_at, int tile_keys, hipStream_t s) {
     if (n_join == 0) return hipSuccess;
-    hipLaunchKernelGGL((attn_dkv_join_kernel<T, D>), dim3((unsigned)n_join * (a.heads / a.group), 2 * (tile_keys / kJoinRows)),
-                       dim3(kJoinRows * (D / 4)), 0, s, a, n_join, join_at, tile_keys);
-    return hipGetLastError();
+    return launch(attn_dkv_join_kernel<T, D>, dim3((unsigned)n_join * (a.heads / a.group), 2 * (tile_keys / kJoinRows)), dim3(kJoinRows * (D / 4)), 0, s, a,
+                  n_join, join_at, tile_keys);
 }
 
 }  // namespace

@@ -461,8 +461,7 @@ hipError_t start(K kernel, int64_t blocks, int threads, size_t lds, hipStream_t 
     if (blocks == 0) return hipSuccess;
     const hipError_t e = lds_room(kernel, lds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, s, args...);
-    return hipGetLastError();
+    return launch(kernel, dim3((unsigned)blocks), dim3(threads), lds, s, args...);
 }
 inline size_t bias_floats(const AttnArgs& a) { return a.bias.table ? (size_t)bias_room(a.bias.reach) : 0; }
 
@@ -486,9 +485,8 @@ hipError_t forward_dim(const AttnArgs& a, int mode, hipStream_t s) {
 template <typename T, int D>
 hipError_t join_dim(const AttnArgs& a, int n_join, int join_at, hipStream_t s) {
     if (n_join == 0) return hipSuccess;
-    hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3((unsigned)(n_join * (a.heads / a.pack)), 32 / kJoinRows), dim3(kJoinRows * (D / 4)), 0, s, a,
-                       n_join, join_at);
-    return hipGetLastError();
+    return launch(attn_join_kernel<T, D>, dim3((unsigned)(n_join * (a.heads / a.pack)), 32 / kJoinRows), dim3(kJoinRows * (D / 4)), 0, s, a, n_join,
+                  join_at);
 }
 
 }  // namespace

@@ -4,7 +4,21 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <tuple>
+
 namespace dptm {
+
+// A kernel's launch with its own result: the last error of the thread may be another call's.
+template <typename... P, typename... A>
+inline hipError_t launch(void (*kernel)(P...), dim3 blocks, dim3 threads, size_t lds, hipStream_t s, const A&... args) {
+    std::tuple<P...> kept(args...);
+    return std::apply(
+        [&](P&... p) {
+            void* at[] = {static_cast<void*>(&p)...};
+            return hipLaunchKernel(reinterpret_cast<const void*>(kernel), blocks, threads, at, lds, s);
+        },
+        kept);
+}
 
 // The attention plan is one array of 32-bit words that dptm_attention_plan fills on the host; the caller keeps one copy
 // there (the launchers read the header) and one on the device (the kernels read the lists behind it).

@@ -50,6 +50,7 @@ struct OnDevice {
     explicit OnDevice(int device) {
         if (hipGetDevice(&before) != hipSuccess) before = -1;
         ok = (before >= 0 && before == device) || hipSetDevice(device) == hipSuccess;
+        if (!ok) (void)hipGetLastError();      // the refusal is the call's result and nobody else's
     }
     ~OnDevice() {
         int now = -1;

@@ -244,11 +244,8 @@ hipError_t run(const NormRopeArgs& a, int blocks, hipStream_t s) {
     const int all = a.heads[0] + a.heads[1], step = (all + HEADS - 1) / HEADS;
     const int64_t units = a.rows * step;
     if (!GRAD) blocks = (int)((units + kThreads / (D / 16) - 1) / (kThreads / (D / 16)));
-    if (a.interleaved)
-        hipLaunchKernelGGL((norm_rope_kernel<T, D, true, GRAD, HEADS>), dim3(blocks), dim3(kThreads), 0, s, a, step, units);
-    else
-        hipLaunchKernelGGL((norm_rope_kernel<T, D, false, GRAD, HEADS>), dim3(blocks), dim3(kThreads), 0, s, a, step, units);
-    return hipGetLastError();
+    return launch(a.interleaved ? norm_rope_kernel<T, D, true, GRAD, HEADS> : norm_rope_kernel<T, D, false, GRAD, HEADS>, dim3(blocks), dim3(kThreads), 0, s,
+                  a, step, units);
 }
 
 template <typename T, int D>
@@ -261,9 +258,8 @@ hipError_t backward(const NormRopeArgs& a, hipStream_t s) {
     const int all = a.heads[0] + a.heads[1], blocks = norm_rope_blocks(a.rows, all, D);
     const hipError_t e = large(a.rows, all, D) ? run<T, D, true, kBackwardHeads>(a, blocks, s) : run<T, D, true, 1>(a, blocks, s);
     if (e != hipSuccess || (!a.gain[0] && !a.gain[1])) return e;
-    hipLaunchKernelGGL(gain_sum_kernel, dim3(D / 16, 2), dim3(1024), 0, s, a.part[0], a.part[1], a.gain[0] ? a.dgain[0] : nullptr,
-                       a.gain[1] ? a.dgain[1] : nullptr, blocks, D);
-    return hipGetLastError();
+    return launch(gain_sum_kernel, dim3(D / 16, 2), dim3(1024), 0, s, a.part[0], a.part[1], a.gain[0] ? a.dgain[0] : nullptr,
+                  a.gain[1] ? a.dgain[1] : nullptr, blocks, D);
 }
 
 template <typename T>

@@ -378,7 +378,8 @@ def qk_norm_rope(q, k, cos, sin, *, q_gain=None, k_gain=None, positions=None, ep
 def qk_norm_rope_backward(dq_out, dk_out, q, k, cos, sin, *, q_gain=None, k_gain=None, positions=None, eps: float = 1e-6,
                           interleaved: bool = False, dq=None, dk=None):
     """Gradients of ``qk_norm_rope``: ``(dq, dk, dq_gain, dk_gain)``; ``q`` and ``k`` as it read them, a gain's gradient (float32)
-    is ``None`` where there is no gain.  ``dq`` / ``dk`` may be given, also as ``dq_out`` / ``dk_out``."""
+    is ``None`` where there is no gain.  ``dq`` / ``dk`` may be given, also as ``dq_out`` / ``dk_out`` or ``q`` / ``k``.  Padding
+    rows need a position inside the table too: one outside makes the gains' gradients NaN with its row."""
     lib, what = _native.load_library(), "qk_norm_rope_backward"
     code, device = _first(q, what)
     dtype = q.dtype

@@ -1,5 +1,7 @@
 """Layer operators (deepptmpred_amd/layers.py) on the GPU against their restatement in float64 (oracle/layers_ref.py), whose
 bounds follow the kernels' roundings: every element of every output has to be within its own bound."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -565,3 +567,18 @@ def test_captured_with_the_most_shared_memory():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(r, run()))
+
+
+def test_an_error_of_an_earlier_call_is_not_reported_again():
+    """A call refused for its device leaves the next one alone."""
+    lib = _native.load_library()
+    rng = np.random.default_rng(80)
+    q, k, v = (tensor(rng, "bf16", 70, 2, 64) for _ in range(3))
+    plan = layers.AttentionPlan([70], heads=2, head_dim=64)
+    want, _ = layers.attention(q, k, v, plan)
+    rows = [_native.Rows(t.data_ptr(), 70, 128, 64) for t in (q, k, v, torch.empty_like(q))]
+    x = _native.AttentionArgs(plan=plan.words.ctypes.data, plan_dev=plan.device_words.data_ptr(), q=rows[0], k=rows[1], v=rows[2], out=rows[3],
+                              lse=torch.empty(140, device="cuda").data_ptr(), dtype=_native.PRECISIONS["bf16"], device=4096, scale=0.125)
+    assert lib.dptm_attention_forward(C.addressof(x)) == _native.DPTM_EINVAL and b"no such device" in lib.dptm_layer_last_error()
+    got, _ = layers.attention(q, k, v, plan)
+    assert torch.equal(got, want)
