@@ -582,3 +582,56 @@ def test_an_error_of_an_earlier_call_is_not_reported_again():
     assert lib.dptm_attention_forward(C.addressof(x)) == _native.DPTM_EINVAL and b"no such device" in lib.dptm_layer_last_error()
     got, _ = layers.attention(q, k, v, plan)
     assert torch.equal(got, want)
+
+
+def test_norm_and_rotation_backward_in_place():
+    """Gradients in the place of the ones they are made from, or of the rows; a gain for one of the two tensors only."""
+    rng = np.random.default_rng(81)
+    cos, sin = layers.rotary_table(200, 64)
+    gain = torch.full((64,), 0.9, device="cuda")
+    x, g = tensor(rng, "bf16", 200, 6, 64), tensor(rng, "bf16", 200, 6, 64)
+    for gains in ({"q_gain": gain, "k_gain": gain}, {"q_gain": gain}, {"k_gain": gain}, {}):
+        want = layers.qk_norm_rope_backward(g[:, :4], g[:, 4:], x[:, :4], x[:, 4:], cos, sin, **gains)
+        g2, x2 = g.clone(), x.clone()
+        got = layers.qk_norm_rope_backward(g2[:, :4], g2[:, 4:], x[:, :4], x[:, 4:], cos, sin, dq=g2[:, :4], dk=g2[:, 4:], **gains)
+        into = layers.qk_norm_rope_backward(g[:, :4], g[:, 4:], x2[:, :4], x2[:, 4:], cos, sin, dq=x2[:, :4], dk=x2[:, 4:], **gains)
+        for a, b, c, name in zip(want, got, into, ("q_gain", "k_gain", "q_gain", "k_gain")):
+            assert (a is None and b is None and c is None) or (torch.equal(a, b) and torch.equal(a, c)), name
+        assert (want[2] is None) == ("q_gain" not in gains) and (want[3] is None) == ("k_gain" not in gains)
+
+
+def test_two_threads_at_once():
+    """Calls of two host threads, each on a stream of its own."""
+    import threading
+
+    rng = np.random.default_rng(82)
+    b = layers.relative_buckets(16, 50)
+    jobs = []
+    for n, heads, dim in ((300, 4, 64), (70, 2, 32)):
+        t = [tensor(rng, "bf16", n, heads, dim) for _ in range(4)]
+        jobs.append((t, layers.AttentionPlan([n], heads=heads, head_dim=dim), tensor(rng, "bf16", 16, heads)))
+
+    def run(job):
+        (q, k, v, dout), plan, table = job
+        out, lse = layers.attention(q, k, v, plan, table=table, buckets=b)
+        return (out, lse) + layers.attention_backward(dout, q, k, v, out, lse, plan, table=table, buckets=b)
+
+    want = [run(j) for j in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(30):
+                r = run(jobs[i])
+            s.synchronize()
+            if not all(torch.equal(a, c) for a, c in zip(r, want[i])):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
