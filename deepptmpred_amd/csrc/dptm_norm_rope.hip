@@ -7,7 +7,7 @@
 // half, so both kinds of pairs are its own, the loads are 16 bytes wide, and the sum over the head is at most three
 // exchanges.  A thread keeps the angles and gains of its elements in registers over the heads of a row that it takes.
 // All arithmetic is fp32; results are rounded once to the tensors' type.  65,539 rows of 40 heads of 64, bf16: forward 125 us for
-// 671 MB (5.4 TB/s), backward 232 + 6 us for 1,007 MB (4.2 TB/s; a large copy reaches 5.05); 482 rows 4.3 us, the launch.
+// 671 MB (5.4 TB/s), backward 219 + 6 us for 1,007 MB (4.5 TB/s; a large copy reaches 5.05); 482 rows 4.3 us, the launch.
 #include "dptm_layers.h"
 
 namespace dptm {
@@ -191,8 +191,11 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs a, int
         }
     }
     if constexpr (GRAD) {
-        // the block's threads with one chunk, in order of their index
-        __shared__ float sums[kThreads * 17];
+        // the block's threads with one chunk: kThreads / D threads a column for every so many of them, in order of their index
+        // (one thread a column walks over 4096 / D of them: at heads of 32 two thirds of a short call's last 3 us)
+        __shared__ float sums[kThreads * 17], some[kThreads];
+        constexpr int kSplit = kThreads / D;
+        const int col = threadIdx.x % D, c = col % (D / 2) / 8, at = col % 8 + (col < D / 2 ? 0 : 8);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             if (!(t ? norm_k : norm_q)) continue;
@@ -203,12 +206,15 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs a, int
                 sums[threadIdx.x * 17 + 8 + e] = d1[t][e];
             }
             __syncthreads();
-            if (threadIdx.x < D) {
-                const int e = threadIdx.x % (D / 2), c = e / 8, at = e % 8 + (threadIdx.x < D / 2 ? 0 : 8);
-                float x = 0.f;
+            float x = 0.f;
 #pragma unroll 8
-                for (int i = c; i < kThreads; i += L) x += sums[i * 17 + at];
-                (t ? a.part[1] : a.part[0])[(int64_t)blockIdx.x * D + threadIdx.x] = x;
+            for (int i = c + L * (threadIdx.x / D); i < kThreads; i += L * kSplit) x += sums[i * 17 + at];
+            some[threadIdx.x] = x;
+            __syncthreads();
+            if (threadIdx.x < D) {
+#pragma unroll
+                for (int k = 1; k < kSplit; ++k) x += some[k * D + col];
+                (t ? a.part[1] : a.part[0])[(int64_t)blockIdx.x * D + col] = x;
             }
         }
     }

@@ -30,6 +30,8 @@ from . import _native
 _TYPES = {torch.float32: _native.PRECISIONS["f32"], torch.bfloat16: _native.PRECISIONS["bf16"],
           torch.float16: _native.PRECISIONS["f16"]}
 
+_SIZES = {_native.PRECISIONS["f32"]: 4, _native.PRECISIONS["bf16"]: 2, _native.PRECISIONS["f16"]: 2}
+
 # The argument blocks of the C calls, packed in one go: a call's cost on the host counts where a protein is short.
 _ROWS = "Qqqq"
 _NO_ROWS = (0, 0, 0, 0)
@@ -126,26 +128,12 @@ def _flat(t, what: str, name: str, shape, dtype, device: int) -> int:
     return t.data_ptr()
 
 
-def _empty(shape, dtype, device: int):
-    return torch.empty(shape, dtype=dtype, device=_gpu(device))
-
-
 def _result(t, like, what: str, name: str, device: int, heads: int, dim: int, rows: int):
     """A result tensor [rows, heads, dim], the caller's or a new one of ``like``'s type, and its address, rows and strides."""
     if t is not None:
         return t, _rows(t, what, name, like.dtype, device, heads, dim, rows)
     t = like.new_empty((rows, heads, dim))
     return t, (t.data_ptr(), rows, heads * dim, dim)
-
-
-_gpus: dict = {}
-
-
-def _gpu(index: int) -> torch.device:
-    d = _gpus.get(index)
-    if d is None:
-        d = _gpus[index] = torch.device("cuda", index)
-    return d
 
 
 def _lengths(a, name: str) -> np.ndarray:
@@ -286,10 +274,10 @@ def attention(q, k, v, plan: AttentionPlan, *, scale: Optional[float] = None, ta
     host, dev = plan._words(what, device, stream)
     out, out_rows = _result(out, q, what, "out", device, heads, dim, nq)
     if lse is None:
-        lse = _empty((heads, nq), torch.float32, device)
+        lse = q.new_empty((heads, nq), dtype=torch.float32)
     table_at, buckets_at, n_buckets, reach = _bias(what, plan, table, buckets, dtype, device)
     n = plan._workspace(0, 0, 0)
-    hold = _empty(n, torch.uint8, device) if n else None
+    hold = q.new_empty((n // _SIZES[code],)) if n else None
     block = _block
     _ATTENTION.pack_into(
         block.attention, 0, host, dev, *_rows(q, what, "q", dtype, device, heads, dim, nq),
@@ -317,9 +305,9 @@ def attention_backward(dout, q, k, v, out, lse, plan: AttentionPlan, *, scale: O
     dk, dk_rows = _result(dk, q, what, "dk", device, kv_heads, dim, nk)
     dv, dv_rows = _result(dv, q, what, "dv", device, kv_heads, dim, nk)
     table_at, buckets_at, n_buckets, reach = _bias(what, plan, table, buckets, dtype, device)
-    dtable = _empty((n_buckets, heads), dtype, device) if n_buckets else None
+    dtable = q.new_empty((n_buckets, heads)) if n_buckets else None
     n = plan._workspace(n_buckets, reach, 1)
-    hold = _empty(n, torch.uint8, device) if n else None
+    hold = q.new_empty((n // _SIZES[code],)) if n else None
     block = _block
     _ATTENTION.pack_into(
         block.attention, 0, host, dev, *_rows(q, what, "q", dtype, device, heads, dim, nq),
@@ -386,8 +374,8 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, cos, sin, *, q_gain=None, k_gain
     n, heads, kv_heads, dim, n_pos, shared = _norm_rope(what, q, k, cos, sin, q_gain, k_gain, positions, code, device)
     dq, dq_rows = _result(dq, q, what, "dq", device, heads, dim, n)
     dk, dk_rows = _result(dk, q, what, "dk", device, kv_heads, dim, n)
-    dq_gain = None if q_gain is None else _empty((dim,), torch.float32, device)
-    dk_gain = None if k_gain is None else _empty((dim,), torch.float32, device)
+    dq_gain = None if q_gain is None else cos.new_empty((dim,))
+    dk_gain = None if k_gain is None else cos.new_empty((dim,))
 
     def pack(at, size):
         _NORM_ROPE.pack_into(
@@ -406,7 +394,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, cos, sin, *, q_gain=None, k_gain
             size = _check(lib.dptm_qk_norm_rope_workspace(_block.norm_rope_at), what)
             if len(_norm_rope_bytes) < 4096:
                 _norm_rope_bytes[key] = size
-        hold = _empty(size, torch.uint8, device)
+        hold = cos.new_empty((size // 4,))
     pack(hold.data_ptr() if size else 0, size)
     rc = lib.dptm_qk_norm_rope_backward(_block.norm_rope_at)
     if rc:
