@@ -635,3 +635,28 @@ def test_two_threads_at_once():
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[51, 17, 64], [21, 32]])
+def test_short_sequences_in_packed_tensors(dtype, lens):
+    """Inputs and gradients as columns of packed tensors, [rows][heads][q k v][dim] too; the columns between are left alone."""
+    rng = np.random.default_rng(83)
+    n = sum(lens)
+    plan = layers.AttentionPlan(lens, heads=3, head_dim=32, window=(30, 10), sinks=1)
+    b = layers.relative_buckets(16, 20)
+    table = tensor(rng, dtype, 16, 3)
+    q, k, v, dout = (tensor(rng, dtype, n, 3, 32) for _ in range(4))
+    out, lse = layers.attention(q, k, v, plan, table=table, buckets=b)
+    want = layers.attention_backward(dout, q, k, v, out, lse, plan, table=table, buckets=b)
+    for split in ((lambda t: [t[:, 3 * i:3 * i + 3] for i in range(4)]), (lambda t: [t.view(n + 2, 3, 4, 32)[:, :, i] for i in range(4)])):
+        x, g = (torch.full((n + 2, 12, 32), 5.0, dtype=q.dtype, device="cuda") for _ in range(2))
+        for to, t in zip(split(x), (q, k, v, dout)):
+            to[:n].copy_(t)
+        qs, ks, vs, ds = split(x)
+        dq, dk, dv, spare = split(g)
+        o, l = layers.attention(qs, ks, vs, plan, table=table, buckets=b)
+        dt = layers.attention_backward(ds, qs, ks, vs, o, l, plan, table=table, buckets=b, dq=dq, dk=dk, dv=dv)[3]
+        for a, c in zip((o, l, dq[:n], dk[:n], dv[:n], dt), (out, lse) + want):
+            assert torch.equal(a, c)
+        assert (spare == 5.0).all() and (g[n:] == 5.0).all()
