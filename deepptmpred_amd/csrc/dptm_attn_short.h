@@ -7,7 +7,7 @@
 //
 // dS_ij = P_ij (dP_ij - delta_i): delta_i = sum_j P_ij dP_ij is summed from the pairs themselves, in fp32, and `out` is not read.  From
 // out as it was rounded (dout_i . out_i, as the other kernels have it) the error of dq and dk of a bf16 window of some 50 keys
-// is 1.7 times that of rounding the results, so 1.4 times.
+// is 1.7 times that of rounding the results, so 1.4 times.  Where a delta is not finite, dS of hidden pairs is set to zero once more.
 //
 // Backward pass of 1,000 windows, 8 heads, with a bias, this kernel against those two, in us: 51 rows, bf16 heads of 64 144 : 280,
 // of 32 75 : 154, f16 heads of 16 61 : 137, fp32 heads of 64 323 : 695; 33 rows, fp32 heads of 32 149 : 251; 21 rows, bf16 heads of 64
@@ -117,6 +117,16 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
 #pragma unroll
     for (int s = 0; s < ST; ++s) kf[s] = Tile<T, D>::row_frag(kt, mine, s, h);
 
+    // pairs of this lane's key and the 32 rows from 32 u on that do not count become zero: row c is seen if far - c <= right and
+    // far - c >= -left, or the key is one of the first
+    auto hide_rows = [&](f32x16_a& x, int u) {
+        const int r0 = 32 * u + 4 * h, far = mine - (pos0 + r0);      // to the row of register 0
+        const int lo = far - win.right, hi = min(mine < win.sinks ? kFar : far + win.left, nq - 1 - r0);
+        const int m = mine < nk ? max(hi - lo + 1, 0) : 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = (unsigned)(reg_row(r) - lo) < (unsigned)m ? x[r] : 0.f;
+    };
+    bool lost = false;                                      // a row's delta is not finite
     f32x16_a dk[DT], dv[DT], weight[N], d_s[N];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -157,24 +167,19 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
                 }
             }
             if (!full) {
-                // row c is seen if far - c <= right and far - c >= -left, or the key is one of the first
-                const int lo = far - win.right, hi = min(mine < win.sinks ? kFar : far + win.left, nq - 1 - r0 - 4 * h);
-                const int m = mine < nk ? max(hi - lo + 1, 0) : 0;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const bool see = (unsigned)(reg_row(r) - lo) < (unsigned)m;
-                    s[r] = see ? s[r] : 0.f;
-                    p[r] = see ? p[r] : 0.f;
-                }
+                hide_rows(s, u);
+                hide_rows(p, u);
             }
             Cols<T, D> cols;
             cols.read(gt, r0, lane);
             cols.product(dv, s);
         }
         const float sum = lane_sums(p, lane);
+        lost |= !(fabsf(sum) < __builtin_inff());
         if ((lane & 16) == 0) rowdelta[kRows * w + r0 + reg_row(lane & 15) + 4 * h] = sum;
     }
-    __syncthreads();
+    // (a value row of NaN, say): what it is multiplied with is zero where pairs are hidden, but the product is not
+    lost = __syncthreads_or((int)lost);
 #pragma unroll
     for (int u = 0; u < N; ++u)
         if ((32 * w < nk) & (32 * u < nq)) {
@@ -186,6 +191,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) d_s[u][4 * x + e] = fmaf(-y[e], weight[u][4 * x + e], d_s[u][4 * x + e]);
             }
+            if (lost) hide_rows(d_s[u], u);
             Cols<T, D> cols;
             cols.read(qt, 32 * u, lane);
             cols.product(dk, d_s[u]);
