@@ -321,7 +321,8 @@ struct KeyWalk {
 
 // A hidden pair's weight is 0, but 0 * inf and 0 * NaN are NaN.  Where a tile holds hidden pairs its threads look, on the way
 // to LDS, whether its rows hold such an element (Stage::not_finite), and workgroups that found one do their rows over at the
-// end, pair by pair.
+// end, pair by pair.  Pairs that the bias table hides are not looked for tile by tile: a score of -inf takes up any NaN, so that a
+// result that came out finite met none.  Where one did not and the table hides something, the rows are done over as well.
 
 // ---- relative position bias in LDS: value per distance, divided by the scale of the scores, because the score products start
 // ---- from it (init_bias) instead of from zero: the bias costs no arithmetic per element, and no branch touches a score.
@@ -332,6 +333,25 @@ constexpr int kBiasPad = 31;
 __host__ __device__ inline int bias_room(int reach) { return (2 * reach + 1 + 2 * kBiasPad + 3) & ~3; }   // floats
 __device__ __forceinline__ int bias_at(int far, int reach) { return min(max(far, -reach - kBiasPad), reach) + reach + kBiasPad; }
 __device__ __forceinline__ float bias_value(float v, float inv_scale) { return v <= -0x1p100f ? kMinusInf : v * inv_scale; }
+// whether the table hides a bucket of the heads [head, head + n); the same answer in every lane.  64 buckets at most, one a lane
+template <typename T>
+__device__ __forceinline__ bool table_hides(const BiasArgs& b, int heads, int head, int n) {
+    const int lane = threadIdx.x & 63;
+    bool any = false;
+    for (int i = 0; i < n; ++i)
+        any |= lane < b.n_buckets && bias_value((float)static_cast<const T*>(b.table)[(int64_t)lane * heads + head + i], 1.f) == kMinusInf;
+    return __ballot(any) != 0;
+}
+// 0, or NaN if one of the accumulators is not finite
+template <int DT>
+__device__ __forceinline__ float zero_if_finite(const f32x16_a (&acc)[DT]) {
+    float z = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z = fmaf(acc[d][r], 0.f, z);
+    return z;
+}
 template <typename T>
 __device__ __forceinline__ void load_bias(float* lds, const BiasArgs& b, float inv_scale, int heads, int head, int tid, int nt) {
     const T* table = static_cast<const T*>(b.table);

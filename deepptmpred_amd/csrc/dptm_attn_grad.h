@@ -20,28 +20,32 @@ namespace {
 // weight of an empty row (lse = -inf) is 0 everywhere: its reference is +inf
 __device__ __forceinline__ float lse_log2(float lse) { return lse == kMinusInf ? __builtin_inff() : lse * kLog2e; }
 
-// A wavefront's rows of dq once more, pair by pair (see Stage::not_finite).
+// A wavefront's rows of dq once more, pair by pair (see Stage::not_finite); *over: the sum of a row's dS.
 template <typename T, int D, int DT, bool BIAS>
-DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, int item, int head, int row, int pos, const float* bias, int h) {
+DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, float* over, int item, int head, int row, int pos, float delta, const float* bias, int h) {
     const QItem& it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[item];
     const Window win{a.left, a.right, a.sinks};
     const int hk = head / a.group;
     const int64_t qr = (int64_t)it.q0 + row;
     const T* q = row_ptr<T>(a.q, qr, head);
     const T* g = row_ptr<T>(a.dout, qr, head);
-    const float ref = lse_log2(a.lse[(int64_t)head * a.q_rows + qr]), delta = a.delta[(int64_t)head * a.q_rows + qr];
+    const float ref = lse_log2(a.lse[(int64_t)head * a.q_rows + qr]);
 #pragma unroll 1
     for (int i = 0; i < 16 * DT; ++i) acc[i] = 0.f;
+    float sum = 0.f;
     for (int j = 0; j < it.ke; ++j) {
         if (j >= it.sink_end && j < it.kb) continue;
         const T* k = row_ptr<T>(a.k, (int64_t)it.k0 + j, hk);
         float s = dot_rows<T, D>(q, k);
-        if constexpr (BIAS) s += bias[bias_at(j - pos, a.bias.reach)];
+        const float b = BIAS ? bias[bias_at(j - pos, a.bias.reach)] : 0.f;
+        s += b;
         const float ds = __builtin_amdgcn_exp2f(fmaf(s, a.scale * kLog2e, -ref)) * (dot_rows<T, D>(g, row_ptr<T>(a.v, (int64_t)it.k0 + j, hk)) - delta);
-        const bool see = visible(win, j - pos, j);
+        const bool see = visible(win, j - pos, j) & (b != kMinusInf);
+        sum += see ? ds : 0.f;
 #pragma unroll 1
         for (int i = 0; i < 16 * DT; ++i) acc[i] += see ? (float)(T)ds * (float)k[reg_col<D>(i >> 4, i & 15, h)] : 0.f;
     }
+    *over = sum;
 }
 
 // rows of a tile in LDS: fewer than in the forward pass where a wavefront's own operands and sums take the registers
@@ -217,14 +221,15 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, POS>)) void attn_dq_kernel
         __syncthreads();
         walk = after;
     }
-    if constexpr (sizeof(T) == 2) {
-        over = half_sum(over);
-        if (h == 0 && row < it.nq) a.delta[(int64_t)head * a.q_rows + qr] = delta + over;
-    }
-    if (__syncthreads_or((int)odd)) {
+    over = half_sum(over);
+    const bool lost = BIAS && fmaf(over, 0.f, zero_if_finite<DT>(acc)) != 0.f;
+    if (__syncthreads_or((int)odd | (int)lost) && (!BIAS || __syncthreads_or((int)odd) || table_hides<T>(a.bias, a.heads, head, 1))) {
         float t[16 * DT];
-        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, item, head, rowc, rw.pos, bias, h);
+        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, &over, item, head, rowc, rw.pos, delta, bias, h);
         take<DT>(acc, t);
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (h == 0 && row < it.nq) a.delta[(int64_t)head * a.q_rows + qr] = delta + over;
     }
     if (row < it.nq) {
         T* o = const_cast<T*>(row_ptr<T>(a.dq, (int64_t)it.q0 + row, head));
@@ -294,7 +299,10 @@ __global__ __launch_bounds__(1024) void attn_dtable_kernel(AttnArgs a, const dou
     __syncthreads();
     if (tid < nb) {
         for (int k = 1; k < 16; ++k) x += part[64 * k + tid];
-        static_cast<T*>(a.dtable)[(int64_t)tid * a.heads + head] = (T)(float)x;
+        const int64_t at = (int64_t)tid * a.heads + head;
+        // the pairs of a bucket that is hidden have no gradient, whatever their operands hold; no other bucket's sum holds theirs
+        const bool hidden = bias_value((float)static_cast<const T*>(a.bias.table)[at], 1.f) == kMinusInf;
+        static_cast<T*>(a.dtable)[at] = (T)(hidden ? 0.f : (float)x);
     }
 }
 template <typename T>
@@ -326,13 +334,15 @@ DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int items_a
             const T* q = row_ptr<T>(a.q, row, head);
             const T* g = row_ptr<T>(a.dout, row, head);
             float s = dot_rows<T, D>(q, k);
+            bool see = visible(win, j - pos, j);
             if constexpr (BIAS) {
                 const int at = min(max(a.bias.buckets[min(max(j - pos, -a.bias.reach), a.bias.reach) + a.bias.reach], 0), a.bias.n_buckets - 1);
-                s += bias_value((float)static_cast<const T*>(a.bias.table)[(int64_t)at * a.heads + head], 1.f / a.scale);
+                const float b = bias_value((float)static_cast<const T*>(a.bias.table)[(int64_t)at * a.heads + head], 1.f / a.scale);
+                s += b;
+                see &= b != kMinusInf;
             }
             const float p = __builtin_amdgcn_exp2f(s * c - lse_log2(a.lse[(int64_t)head * a.q_rows + row]));
             const float ds = p * (dot_rows<T, D>(g, v) - a.delta[(int64_t)head * a.q_rows + row]);
-            const bool see = visible(win, j - pos, j);
 #pragma unroll 1
             for (int x = 0; x < 16 * DT; ++x) {
                 const int col = reg_col<D>(x >> 4, x & 15, h);
@@ -617,7 +627,10 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
             }
         }
     }
-    if (__syncthreads_or((int)odd)) {
+    bool lost = false;
+    if constexpr (BIAS && DK) lost |= zero_if_finite<DT>(dk) != 0.f;
+    if constexpr (BIAS && DV) lost |= zero_if_finite<DT>(dv) != 0.f;
+    if (__syncthreads_or((int)odd | (int)lost) && (!BIAS || __syncthreads_or((int)odd) || table_hides<T>(a.bias, a.heads, hk * a.group, a.group))) {
         float x[16 * DT], y[16 * DT];
         dkv_by_pairs<T, D, DT, BIAS>(kernel_args(), x, y, a.items_at, item, hk, keyc, h);
         if constexpr (DK) take<DT>(dk, x);

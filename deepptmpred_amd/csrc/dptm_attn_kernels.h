@@ -125,9 +125,9 @@ DPTM_COLD void forward_by_pairs(const AttnArgs& a, float* acc, float* ml, int it
         const int j0 = t < ns ? t * keys : it.kb + (t - ns) * keys, j1 = min(j0 + keys, t < ns ? it.sink_end : it.ke);
         for (int j = j0; j < j1; ++j) {
             float s = dot_rows<T, D>(q, row_ptr<T>(a.k, (int64_t)it.k0 + j, hk));
-            if constexpr (BIAS) s += bias[bias_at(j - pos, a.bias.reach)];
-            s *= c;
-            s = visible(win, j - pos, j) ? s : kMinusInf;
+            const float b = BIAS ? bias[bias_at(j - pos, a.bias.reach)] : 0.f;
+            s = (s + b) * c;
+            s = visible(win, j - pos, j) & (b != kMinusInf) ? s : kMinusInf;
             const float top = fmaxf(m, s), f = m == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(m - top);
             const float p = s == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(s - top + kShift<T>);
             m = top;
@@ -258,7 +258,8 @@ __global__ __launch_bounds__(NW * 64, (kForwardWaves<T, D>)) void attn_fwd_wide_
         __syncthreads();
         at = after;
     }
-    if (__syncthreads_or((int)odd)) {
+    const bool lost = BIAS && fmaf(l, 0.f, zero_if_finite<DT>(acc)) != 0.f;
+    if (__syncthreads_or((int)odd | (int)lost) && (!BIAS || __syncthreads_or((int)odd) || table_hides<T>(a.bias, a.heads, head, 1))) {
         float t[16 * DT], ml[2];
         forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, ml, item, head, rowc, rw.pos, 0, 1, kBK, bias, h);
         take<DT>(acc, t);
@@ -361,7 +362,8 @@ __global__ __launch_bounds__(256, sizeof(T) * D >= 512 ? 1 : 2) void attn_fwd_sp
         v.read(vt, 0, lane);
         v.product(acc, s[0]);
     }
-    if (__ballot(odd != 0)) {
+    const bool lost = BIAS && fmaf(l, 0.f, zero_if_finite<DT>(acc)) != 0.f;
+    if (__ballot((odd != 0) | lost) && (!BIAS || __ballot(odd != 0) || table_hides<T>(a.bias, a.heads, head0, pack))) {
         float t[16 * DT], x[2];
         forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, x, id - id / a.n_items * a.n_items, head, query, rw.pos, w, NW, 32, bias, h);
         take<DT>(acc, t);

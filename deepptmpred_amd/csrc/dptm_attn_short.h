@@ -107,11 +107,13 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
     sg.store(gt, tid);
     sk.store(kt, tid);
     unsigned odd = 0;
-    if (!Sight(win, pos0, pos0 + nq - 1).all(0, nk)) odd = sq.not_finite() | sg.not_finite() | sk.not_finite();
+    const bool whole = Sight(win, pos0, pos0 + nq - 1).all(0, nk);
+    if (BIAS | !whole) odd = sq.not_finite() | sg.not_finite() | sk.not_finite();
     if (h == 0) rowref[mine] = mine < nq ? lse_log2(lse) * (kLseLast<T> ? -1.f : -1.f / c) : kMinusInf;      // rows behind the last weigh nothing
-    const bool redo = __syncthreads_or((int)odd);
+    bool redo = __syncthreads_or((int)odd) && (!BIAS || !whole || table_hides<T>(a.bias, a.heads, head, 1));
+    auto delta_of_out = [&] { return dot_rows<T, D>(row_ptr<T>(a.dout, qr, head), row_ptr<T>(a.out, qr, head)); };
     if (redo) {
-        if (h == 0 && mine < nq) a.delta[(int64_t)head * a.q_rows + qr] = dot_rows<T, D>(row_ptr<T>(a.dout, qr, head), row_ptr<T>(a.out, qr, head));
+        if (h == 0 && mine < nq) a.delta[(int64_t)head * a.q_rows + qr] = delta_of_out();
         __syncthreads();
     }
 #pragma unroll
@@ -125,6 +127,19 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
         const int m = mine < nk ? max(hi - lo + 1, 0) : 0;
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[r] = (unsigned)(reg_row(r) - lo) < (unsigned)m ? x[r] : 0.f;
+    };
+    auto bias_of = [&](int u) { return bias + bias_at(mine - (pos0 + 32 * u + 4 * h) - kBiasPad, reach) + kBiasPad; };     // minus the row
+    // the same for the pairs that the table hides
+    auto hide_buckets = [&](f32x16_a& x, int u) {
+        const float* b = bias_of(u);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = b[-reg_row(r)] == kMinusInf ? 0.f : x[r];
+    };
+    // sums of a row's pairs over this wavefront's keys, by row
+    auto row_sums = [&](const f32x16_a& x, int u) {
+        const float sum = lane_sums(x, lane);
+        if ((lane & 16) == 0) rowdelta[kRows * w + 32 * u + reg_row(lane & 15) + 4 * h] = sum;
+        return sum;
     };
     bool lost = false;                                      // a row's delta is not finite
     f32x16_a dk[DT], dv[DT], weight[N], d_s[N];
@@ -141,7 +156,6 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
         const Sight sight(win, pos0 + r0, pos0 + min(r0 + 31, nq - 1));
         {
             const bool full = (32 * w + 32 <= nk) & (r0 + 32 <= nq) & sight.all(32 * w, 32);
-            const int far = mine - (pos0 + r0 + 4 * h);     // to the row of register 0
             const V4<float>* less = reinterpret_cast<const V4<float>*>(rowref + r0 + 4 * h);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
@@ -150,7 +164,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
                 for (int e = 0; e < 4; ++e) s[4 * x + e] = y[e];
             }
             if constexpr (BIAS) {
-                const float* b = bias + bias_at(far - kBiasPad, reach) + kBiasPad;
+                const float* b = bias_of(u);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] += b[-reg_row(r)];
             }
@@ -174,12 +188,25 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
             cols.read(gt, r0, lane);
             cols.product(dv, s);
         }
-        const float sum = lane_sums(p, lane);
-        lost |= !(fabsf(sum) < __builtin_inff());
-        if ((lane & 16) == 0) rowdelta[kRows * w + r0 + reg_row(lane & 15) + 4 * h] = sum;
+        lost |= !(fabsf(row_sums(p, u)) < __builtin_inff());
     }
     // (a value row of NaN, say): what it is multiplied with is zero where pairs are hidden, but the product is not
     lost = __syncthreads_or((int)lost);
+    bool hides = false;
+    if constexpr (BIAS) {
+        if (lost && table_hides<T>(a.bias, a.heads, head, 1)) {
+            hides = true;
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                hide_buckets(weight[u], u);
+                hide_buckets(d_s[u], u);
+                row_sums(d_s[u], u);
+            }
+            if (!redo && h == 0 && mine < nq) a.delta[(int64_t)head * a.q_rows + qr] = delta_of_out();
+            redo = true;
+            __syncthreads();
+        }
+    }
 #pragma unroll
     for (int u = 0; u < N; ++u)
         if ((32 * w < nk) & (32 * u < nq)) {
@@ -192,6 +219,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
                 for (int e = 0; e < 4; ++e) d_s[u][4 * x + e] = fmaf(-y[e], weight[u][4 * x + e], d_s[u][4 * x + e]);
             }
             if (lost) hide_rows(d_s[u], u);
+            if (hides) hide_buckets(d_s[u], u);
             Cols<T, D> cols;
             cols.read(qt, 32 * u, lane);
             cols.product(dk, d_s[u]);
@@ -258,8 +286,8 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
         sums[2 * kRows * half + kRows + l] = up[0] + up[1];
     }
     if (redo) {
-        float t[16 * DT];
-        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, item, head, rowc, pos0 + rowc, bias, h);
+        float t[16 * DT], over;
+        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, &over, item, head, rowc, pos0 + rowc, a.delta[(int64_t)head * a.q_rows + qr], bias, h);
         take<DT>(dq, t);
     }
     if (mine < nq) {

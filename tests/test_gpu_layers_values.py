@@ -47,3 +47,63 @@ def test_short_sequences_with_a_hidden_value_row_that_is_not_finite(dtype, rows)
     # distances -5 .. 4 take buckets 0, 1, 2 and 5, 6
     d = host(dtable)
     assert (d[[3, 7]] == 0).all() and np.isnan(d[[0, 1, 2, 5, 6]]).all()
+
+
+# sequences, heads, dim, listed positions: the short backward kernel, the split forward kernel, the two wide ones
+HIDING = [([51, 20], 2, 32, False), ([64], 2, 64, False), ([90, 33], 2, 32, False), ([90], 3, 64, True), ([70], 2, 128, False),
+          ([200], 64, 32, False), ([256] * 4, 64, 16, False), ([256] * 4, 64, 64, True)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lens,heads,dim,given", HIDING)
+def test_pairs_hidden_by_the_table_and_operands_that_are_not_finite(dtype, lens, heads, dim, given):
+    """A table entry that hides its bucket hides it from NaN and infinities too, in both directions."""
+    rng = np.random.default_rng(91)
+    n = sum(lens)
+    q, k, v, dout = (tensor(rng, dtype, n, heads, dim) for _ in range(4))
+    b = layers.relative_buckets(8, 9)
+    table = tensor(rng, dtype, 8, heads)
+    table[[3, 7]] = -INF                             # distances of 5 and more (bucket 2: 2 to 4)
+    table[:, heads - 1] = -INF                       # the last head sees nothing
+    hidden = [3, 7]
+    pos = R.default_positions(lens, lens).astype(np.int32)
+    plan = layers.AttentionPlan(lens, heads=heads, head_dim=dim, q_positions=pos if given else None)
+
+    def run(q, k, v, dout):
+        out, lse = layers.attention(q, k, v, plan, table=table, buckets=b)
+        return (out, lse) + layers.attention_backward(dout, q, k, v, out, lse, plan, table=table, buckets=b)
+
+    plain = run(q, k, v, dout)
+    names = ("out", "lse", "dq", "dk", "dv", "dtable")
+    want = R.attention(host(q), host(k), host(v), lens, lens, (-1, -1), 0, None, None, host(table), b.cpu().numpy(), host(dout), host(plain[0]), dtype)
+    for t, name in zip(plain, names):
+        within(t, want[name], name)
+    of = b.cpu().numpy()
+    start = np.repeat(np.cumsum([0] + lens[:-1]), lens)
+    see = (start[:, None] == start[None]) & ~np.isin(of[np.clip(np.arange(n)[None] - np.arange(n)[:, None], -9, 9) + 9], hidden)
+
+    def rest(got, met_rows, met_keys, dv_keys):
+        for t, name, keep in zip(got, names, (~met_rows, None, ~met_rows, ~met_keys, ~dv_keys)):
+            if name == "lse":
+                value, bound = want[name]
+                within(t[:, torch.from_numpy(~met_rows).cuda()], (value[:, ~met_rows], bound[:, ~met_rows]), name)
+            else:
+                rows_within(t, want, name, keep)
+        d = host(got[5])
+        assert (d[hidden] == 0).all() and (d[:, heads - 1] == 0).all() and np.isnan(d[:, 0][[0, 1, 2, 5, 6]]).all()
+        # the last head is empty whatever its operands hold
+        assert not got[0][:, -1].any() and torch.isneginf(got[1][-1]).all() and not any(t[:, -1].any() for t in got[2:5])
+
+    # keys of NaN and infinity, values of infinity
+    k2, v2 = k.clone(), v.clone()
+    k2[12], k2[13, :, 1], v2[13], v2[14] = NAN, INF, INF, -INF
+    met = see[:, [12, 13, 14]].any(1)
+    rest(run(q, k2, v2, dout), met, see[met].any(0), see[met].any(0))
+    # a row of NaN, and a gradient of infinity
+    q2, dout2 = q.clone(), dout.clone()
+    q2[15], dout2[16] = NAN, INF
+    met = np.isin(np.arange(n), (15, 16))
+    got = run(q2, k, v, dout2)
+    rest((plain[0], plain[1]) + got[2:], met, see[met].any(0), see[met].any(0))
+    rows_within(got[0], want, "out", np.arange(n) != 15)
+    rows_within(got[1].T, {"lse": (want["lse"][0].T, want["lse"][1].T)}, "lse", np.arange(n) != 15)
