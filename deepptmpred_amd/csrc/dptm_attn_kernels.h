@@ -24,6 +24,11 @@ template <typename T> constexpr float kShift = sizeof(T) == 2 && Elem<T>::kExp =
 template <> constexpr float kShift<float> = 0.f;
 template <typename T> constexpr float kUnshift = kShift<T> > 0.f ? 0x1p-10f : 1.f;    // before the logarithm: lse keeps its last bits
 constexpr float kLazy = 4.f;
+// A maximum leaves NaN out, the sum does not: a row that meets NaN has lse NaN, and -inf stays with rows that see nothing.
+template <typename T>
+__device__ __forceinline__ float lse_of(float m, float l) {
+    return l == 0.f ? kMinusInf : (m + __log2f(l * kUnshift<T>)) * kLn2;
+}
 
 // keys of a tile in LDS: 64 where the registers that carry the next tile allow it
 template <typename T, int D> constexpr int kKeysPerTile = sizeof(T) == 2 ? 64 : 32;
@@ -278,7 +283,7 @@ __global__ __launch_bounds__(NW * 64, (kForwardWaves<T, D>)) void attn_fwd_wide_
                 for (int e = 0; e < 4; ++e) x[e] = (T)(acc[d][4 * g + e] * inv);
                 *reinterpret_cast<V4<T>*>(o + 32 * d + 8 * g + 4 * h) = x;
             }
-        if (h == 0) a.lse[(int64_t)head * a.q_rows + it.q0 + row] = m == kMinusInf ? kMinusInf : (m + __log2f(l * kUnshift<T>)) * kLn2;
+        if (h == 0) a.lse[(int64_t)head * a.q_rows + it.q0 + row] = lse_of<T>(m, l);
     }
 }
 
@@ -398,7 +403,7 @@ __global__ __launch_bounds__(256, sizeof(T) * D >= 512 ? 1 : 2) void attn_fwd_sp
 #pragma unroll
         for (int k = 0; k < NW; ++k) {
             const float mk = ml[(k * 32 + r) * 2];
-            sum += mk == kMinusInf ? 0.f : ml[(k * 32 + r) * 2 + 1] * __builtin_amdgcn_exp2f(mk - t);
+            sum += ml[(k * 32 + r) * 2 + 1] * (mk == kMinusInf ? 1.f : __builtin_amdgcn_exp2f(mk - t));     // without a score 0, or NaN
         }
         V4<float> x = *reinterpret_cast<V4<float>*>(o + r * kPad + d);
 #pragma unroll
@@ -409,7 +414,7 @@ __global__ __launch_bounds__(256, sizeof(T) * D >= 512 ? 1 : 2) void attn_fwd_sp
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * inv);
             *reinterpret_cast<V4<T>*>(const_cast<T*>(row_ptr<T>(a.out, (int64_t)it.q0 + qi, hd)) + d) = y;
-            if (d == 0) a.lse[(int64_t)hd * a.q_rows + it.q0 + qi] = t == kMinusInf ? kMinusInf : (t + __log2f(sum * kUnshift<T>)) * kLn2;
+            if (d == 0) a.lse[(int64_t)hd * a.q_rows + it.q0 + qi] = lse_of<T>(t, sum);
         } else {
             const int64_t at = ((int64_t)it.slot * (a.heads / pack) + head0 / pack) * 32 + r;
             *reinterpret_cast<V4<float>*>(a.part_o + at * D + d) = x;
@@ -440,7 +445,7 @@ __global__ __launch_bounds__(kJoinRows * (D / 4)) void attn_join_kernel(AttnArgs
         const float mk = a.part_ml[at * 2], lk = a.part_ml[at * 2 + 1];
         const V4<float> xk = *reinterpret_cast<const V4<float>*>(a.part_o + at * D + d);
         const float f = mk == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(mk - m);
-        l += lk * f;
+        l += mk == kMinusInf ? lk : lk * f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] += xk[e] * f;
     }
@@ -450,7 +455,7 @@ __global__ __launch_bounds__(kJoinRows * (D / 4)) void attn_join_kernel(AttnArgs
     for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * inv);
     const int qi = r / pack, head = hp * pack + r - qi * pack;
     *reinterpret_cast<V4<T>*>(const_cast<T*>(row_ptr<T>(a.out, (int64_t)jn.row0 + qi, head)) + d) = y;
-    if (d == 0) a.lse[(int64_t)head * a.q_rows + jn.row0 + qi] = m == kMinusInf ? kMinusInf : (m + __log2f(l * kUnshift<T>)) * kLn2;
+    if (d == 0) a.lse[(int64_t)head * a.q_rows + jn.row0 + qi] = lse_of<T>(m, l);
 }
 
 template <typename K>

@@ -107,3 +107,27 @@ def test_pairs_hidden_by_the_table_and_operands_that_are_not_finite(dtype, lens,
     rest((plain[0], plain[1]) + got[2:], met, see[met].any(0), see[met].any(0))
     rows_within(got[0], want, "out", np.arange(n) != 15)
     rows_within(got[1].T, {"lse": (want["lse"][0].T, want["lse"][1].T)}, "lse", np.arange(n) != 15)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lens,k_lens,heads,kv_heads", [([70], [70], 2, 2), ([200], [200], 64, 64), ([256] * 4, [256] * 4, 64, 64), ([53], [2100], 4, 4),
+                                                        ([2], [3000], 8, 2)])
+def test_lse_of_rows_whose_scores_are_nan(dtype, lens, k_lens, heads, kv_heads):
+    """lse is NaN where out is: a row of NaN, and a row that meets NaN in a range of its keys; -inf is left to rows that see nothing."""
+    rng = np.random.default_rng(92)
+    n, nk = sum(lens), sum(k_lens)
+    q, k, v = tensor(rng, dtype, n, heads, 64), tensor(rng, dtype, nk, kv_heads, 64), tensor(rng, dtype, nk, kv_heads, 64)
+    plan = layers.AttentionPlan(lens, k_lens, heads=heads, kv_heads=kv_heads, head_dim=64, training=False)
+    want = R.attention(host(q), host(k), host(v), lens, k_lens, dtype=dtype)["lse"]
+    q2 = q.clone()
+    q2[1] = NAN
+    out, lse = layers.attention(q2, k, v, plan)
+    others = np.arange(n) != 1
+    assert torch.isnan(out[1]).all() and torch.isnan(lse[:, 1]).all()
+    within(lse.T[torch.from_numpy(others).cuda()], (want[0].T[others], want[1].T[others]), "lse")
+    k2 = k.clone()
+    k2[32:k_lens[0]] = NAN                           # whole tiles, and whole parts where keys are split
+    out, lse = layers.attention(q, k2, v, plan)
+    assert torch.isnan(out[:lens[0]]).all() and torch.isnan(lse[:, :lens[0]]).all()
+    if n > lens[0]:
+        within(lse.T[lens[0]:], (want[0].T[lens[0]:], want[1].T[lens[0]:]), "lse")
