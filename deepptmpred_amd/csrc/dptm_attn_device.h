@@ -342,16 +342,17 @@ __device__ __forceinline__ bool table_hides(const BiasArgs& b, int heads, int he
         any |= lane < b.n_buckets && bias_value((float)static_cast<const T*>(b.table)[(int64_t)lane * heads + head + i], 1.f) == kMinusInf;
     return __ballot(any) != 0;
 }
-// 0, or NaN if one of the accumulators is not finite
+// not finite if one of the accumulators is not
 template <int DT>
-__device__ __forceinline__ float zero_if_finite(const f32x16_a (&acc)[DT]) {
-    float z = 0.f;
+__device__ __forceinline__ float sum_of_all(const f32x16_a (&acc)[DT]) {
+    float z[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) z = fmaf(acc[d][r], 0.f, z);
-    return z;
+        for (int r = 0; r < 16; ++r) z[r & 3] += acc[d][r];
+    return (z[0] + z[1]) + (z[2] + z[3]);
 }
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
 template <typename T>
 __device__ __forceinline__ void load_bias(float* lds, const BiasArgs& b, float inv_scale, int heads, int head, int tid, int nt) {
     const T* table = static_cast<const T*>(b.table);

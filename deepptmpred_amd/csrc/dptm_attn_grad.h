@@ -20,6 +20,52 @@ namespace {
 // weight of an empty row (lse = -inf) is 0 everywhere: its reference is +inf
 __device__ __forceinline__ float lse_log2(float lse) { return lse == kMinusInf ? __builtin_inff() : lse * kLog2e; }
 
+// float16 holds 2^-24 to 65504, and the pairs' P and dS of a long row or a small gradient lie below that (8,192 keys, dout of size
+// 1e-3: dq and dk 7 times as far off as rounding them makes them, of size 1e-4 10 % of their size; gradients of some 1e5 were infinite).
+// For float16 alone both are therefore formed larger by a power of two, which is part of the exponent that exp2 takes.
+//   dk, dv and short sequences: 2^13.  What rounding a pair then takes away is 2^-38 at least, and the results' own rounding 2^-25.  A
+// lane -- a key -- that meets a |dS| above 2^14 so lifted goes on with a smaller power of two, and its sums move along: eight three-way
+// maxima a tile (16,001 rows, window of 512, with the bias: 161 -> 172 us).
+//   dq: a lane is a query, and its dout says how large dS is, so that no tile has to be looked at: the power takes the largest |dout| to
+// 2^4.  P of 2^-20 still keeps all bits then; rows whose sums come out infinite (|dP - delta| of thousands of times |dout|, values in the
+// hundreds or thousands) are done over pair by pair.
+template <typename T> struct Lift {
+    static constexpr bool kOn = sizeof(T) == 2 && Elem<T>::kExp == 0x7c00;
+    static constexpr int kFirst = kOn ? 13 : 0;
+    int e = kFirst;
+    bool moved = false;       // some lane of the wavefront has another power than 2^kFirst
+    __device__ __forceinline__ float log2() const { return kOn ? (float)e : 0.f; }
+    __device__ __forceinline__ float off(float x) const { return kOn ? __builtin_amdgcn_ldexpf(x, -e) : x; }
+    // of what was lifted by 2^kFirst
+    __device__ __forceinline__ static float off_first(float x) { return kOn ? x * 0x1p-13f : x; }
+    __device__ __forceinline__ static void down(f32x16_a& x, int by) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_ldexpf(x[r], -by);
+    }
+    // w is lifted by 2^e and about to be summed, sums are what earlier ones have been summed in
+    template <int DT, typename... Sums>
+    __device__ __forceinline__ void settle(f32x16_a& w, f32x16_a (&acc)[DT], Sums&... sums) {
+        if constexpr (kOn) {
+            float top = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(fabsf(w[r]), fabsf(w[r + 1])), top);
+            top = half_max(top);
+            if (__ballot(top > 0x1p14f)) {
+                const int by = top > 0x1p14f ? min((int)(__float_as_uint(top) >> 23) - 127 - 12, e + 100) : 0;
+                e -= by;
+                moved = true;
+                down(w, by);
+                auto all = [&](f32x16_a (&x)[DT]) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) down(x[d], by);
+                };
+                all(acc);
+                (all(sums), ...);
+            }
+        }
+    }
+};
+
 // A wavefront's rows of dq once more, pair by pair (see Stage::not_finite); *over: the sum of a row's dS.
 template <typename T, int D, int DT, bool BIAS>
 DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, float* over, int item, int head, int row, int pos, float delta, const float* bias, int h) {
@@ -43,7 +89,7 @@ DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, float* over, int item,
         const bool see = visible(win, j - pos, j) & (b != kMinusInf);
         sum += see ? ds : 0.f;
 #pragma unroll 1
-        for (int i = 0; i < 16 * DT; ++i) acc[i] += see ? (float)(T)ds * (float)k[reg_col<D>(i >> 4, i & 15, h)] : 0.f;
+        for (int i = 0; i < 16 * DT; ++i) acc[i] += see ? ds * (float)k[reg_col<D>(i >> 4, i & 15, h)] : 0.f;
     }
     *over = sum;
 }
@@ -147,6 +193,16 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, POS>)) void attn_dq_kernel
 #pragma unroll
         for (int r = 0; r < 16; ++r) less_delta[r] = -delta;
     }
+    int lift = 0;
+    if constexpr (Lift<T>::kOn) {
+        float top = 0.f;
+#pragma unroll
+        for (int s = 0; s < ST; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf((float)g[s][e]));
+        lift = min(4 + 127 - (int)(__float_as_uint(half_max(top)) >> 23), 40);
+    }
+    auto off = [&](float x) { return Lift<T>::kOn ? __builtin_amdgcn_ldexpf(x, -lift) : x; };
     float over = 0.f;                   // sum of the row's dS, which is what delta lacks
     float below = 0.f, above = 0.f;     // dS of distances up to -reach, from reach on
     KeyWalk walk(it);
@@ -180,7 +236,7 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, POS>)) void attn_dq_kernel
 #pragma unroll
                     for (int r = 0; r < 16; ++r) p[r] = -delta;
                 }
-                float less = -ref;
+                float less = (float)lift - ref;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = 0.f;
                 if constexpr (BIAS) {
@@ -210,7 +266,7 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, POS>)) void attn_dq_kernel
                         const int at = bias_at(a0 + 4 * h - rw.pos, reach);
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
-                            __hip_atomic_fetch_add(bins + bucket[at + reg_row(r)] * 64 + lane, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                            __hip_atomic_fetch_add(bins + bucket[at + reg_row(r)] * 64 + lane, off(s[r]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                     }
                 }
                 if constexpr (!kEarly) cols.read(kt, 32 * k, lane);
@@ -222,16 +278,26 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, POS>)) void attn_dq_kernel
         walk = after;
     }
     over = half_sum(over);
-    const bool lost = BIAS && fmaf(over, 0.f, zero_if_finite<DT>(acc)) != 0.f;
-    if (__syncthreads_or((int)odd | (int)lost) && (!BIAS || __syncthreads_or((int)odd) || table_hides<T>(a.bias, a.heads, head, 1))) {
+    over = off(over), below = off(below), above = off(above);
+    bool redo = __syncthreads_or((int)odd);
+    if constexpr (BIAS || Lift<T>::kOn) {
+        const bool lost = !finite(over + sum_of_all(acc));
+        if (!redo && __ballot(lost)) {
+            if constexpr (Lift<T>::kOn) redo = __ballot(lost & finite(delta));
+            if constexpr (BIAS) redo |= table_hides<T>(a.bias, a.heads, head, 1);
+        }
+    }
+    if (redo) {
         float t[16 * DT];
         dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, &over, item, head, rowc, rw.pos, delta, bias, h);
         take<DT>(acc, t);
+        lift = 0;
     }
     if constexpr (sizeof(T) == 2) {
         if (h == 0 && row < it.nq) a.delta[(int64_t)head * a.q_rows + qr] = delta + over;
     }
     if (row < it.nq) {
+        const float by = off(a.scale);
         T* o = const_cast<T*>(row_ptr<T>(a.dq, (int64_t)it.q0 + row, head));
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -239,7 +305,7 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, POS>)) void attn_dq_kernel
             for (int x = 0; x < (D >= 32 ? 4 : 2); ++x) {
                 V4<T> y;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = (T)(acc[d][4 * x + e] * a.scale);
+                for (int e = 0; e < 4; ++e) y[e] = (T)(acc[d][4 * x + e] * by);
                 *reinterpret_cast<V4<T>*>(o + 32 * d + 8 * x + 4 * h) = y;
             }
     }
@@ -346,8 +412,8 @@ DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int items_a
 #pragma unroll 1
             for (int x = 0; x < 16 * DT; ++x) {
                 const int col = reg_col<D>(x >> 4, x & 15, h);
-                dk[x] += see ? (float)(T)ds * (float)q[col] : 0.f;
-                dv[x] += see ? (float)(T)p * (float)g[col] : 0.f;
+                dk[x] += see ? ds * (float)q[col] : 0.f;
+                dv[x] += see ? p * (float)g[col] : 0.f;
             }
         }
 }
@@ -415,6 +481,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
     float nref = 0.f, ndelta = 0.f;
     int npos = 0;
     const float from_lse = kLseLast<T> ? -1.f : -1.f / c;
+    Lift<T> lift;
     // the next tile of rows: its addresses move on with it
     const char *qat = nullptr, *gat = nullptr;
     auto fetch = [&](int head, int t) {
@@ -480,6 +547,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                     bool near = false;
                     const int* pos = rowpos + buf * kBQ + 32 * u + 4 * h;
                     const int far = j - (it.pos0 + r0 + 4 * h);      // to the row of register 0, where the plan lists no positions
+                    const float up = lift.log2();
                     // The products start from what is taken off them: the scores from -lse (fp32: see kLseLast) and the bias, dP from -delta
                     f32x16_a s, p;
                     const V4<float>* less = reinterpret_cast<const V4<float>*>(rowref + buf * kBQ + 32 * u + 4 * h);
@@ -526,7 +594,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int r = 4 * x + e;
-                            s[r] = __builtin_amdgcn_exp2f(kLseLast<T> ? fmaf(s[r], c, y[e]) : s[r] * c);
+                            s[r] = __builtin_amdgcn_exp2f(kLseLast<T> ? fmaf(s[r], c, y[e]) : Lift<T>::kOn ? fmaf(s[r], c, up) : s[r] * c);
                             if constexpr (DK) p[r] *= s[r];
                         }
                     }
@@ -554,19 +622,32 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                     }
                     if constexpr (SUMS) {
                         if (near) {
+                            f32x16_a d = p;
+                            if (Lift<T>::kOn && lift.moved) Lift<T>::down(d, lift.e - Lift<T>::kFirst);     // keys meet in a sum
                             float* mine = shear + 32 + (lane & 31) * kShearRow + 4 * h;
 #pragma unroll
                             for (int x = 0; x < 4; ++x) {
-                                const V4<float> y{p[4 * x], p[4 * x + 1], p[4 * x + 2], p[4 * x + 3]};
+                                const V4<float> y{d[4 * x], d[4 * x + 1], d[4 * x + 2], d[4 * x + 3]};
                                 *reinterpret_cast<V4<float>*>(mine + 8 * x) = y;
                             }
                         } else {
                             float sum = 0.f;
 #pragma unroll
                             for (int r = 0; r < 16; ++r) sum += p[r];
+                            sum = lift.off(sum);
                             above += is_above ? sum : 0.f;
                             below += is_above ? 0.f : sum;
                         }
+                    }
+                    if constexpr (DK && DV) {
+                        // P and dS of a key by one power of two
+                        if constexpr (Lift<T>::kOn) {
+                            const int before = lift.e;
+                            lift.settle(p, dk, dv);
+                            if (lift.moved) Lift<T>::down(s, before - lift.e);
+                        }
+                    } else if constexpr (DK) {
+                        lift.settle(p, dk);
                     }
                     if constexpr (DV) {
                         if constexpr (!kEarly) {
@@ -594,7 +675,7 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                             __builtin_amdgcn_wave_barrier();
                             const int dist = j0 + 31 - lane - (it.pos0 + r0) + reach + kFarPad;
-                            if (lane < 63) sums[dist] += (part[0] + part[1]) + (part[2] + part[3]);
+                            if (lane < 63) sums[dist] += Lift<T>::off_first((part[0] + part[1]) + (part[2] + part[3]));
                         }
                     }
                 }
@@ -627,14 +708,16 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
             }
         }
     }
-    bool lost = false;
-    if constexpr (BIAS && DK) lost |= zero_if_finite<DT>(dk) != 0.f;
-    if constexpr (BIAS && DV) lost |= zero_if_finite<DT>(dv) != 0.f;
-    if (__syncthreads_or((int)odd | (int)lost) && (!BIAS || __syncthreads_or((int)odd) || table_hides<T>(a.bias, a.heads, hk * a.group, a.group))) {
+    float dk_by = lift.off(a.scale), dv_by = lift.off(1.f);
+    bool redo = __syncthreads_or((int)odd);
+    if constexpr (BIAS)
+        if (!redo && __ballot(!finite((DK ? sum_of_all(dk) : 0.f) + (DV ? sum_of_all(dv) : 0.f)))) redo = table_hides<T>(a.bias, a.heads, hk * a.group, a.group);
+    if (redo) {
         float x[16 * DT], y[16 * DT];
         dkv_by_pairs<T, D, DT, BIAS>(kernel_args(), x, y, a.items_at, item, hk, keyc, h);
         if constexpr (DK) take<DT>(dk, x);
         if constexpr (DV) take<DT>(dv, y);
+        dk_by = a.scale, dv_by = 1.f;
     }
     if (key < it.nk) {
         if (it.slot < 0) {
@@ -647,8 +730,8 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                     V4<T> y, z;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        y[e] = (T)(dk[d][4 * x + e] * a.scale);
-                        z[e] = (T)dv[d][4 * x + e];
+                        y[e] = (T)(dk[d][4 * x + e] * dk_by);
+                        z[e] = (T)(dv[d][4 * x + e] * dv_by);
                     }
                     if constexpr (DK) *reinterpret_cast<V4<T>*>(ok + 32 * d + 8 * x + 4 * h) = y;
                     if constexpr (DV) *reinterpret_cast<V4<T>*>(ov + 32 * d + 8 * x + 4 * h) = z;
@@ -663,8 +746,8 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                     V4<float> y, z;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        y[e] = dk[d][4 * x + e] * a.scale;
-                        z[e] = dv[d][4 * x + e];
+                        y[e] = dk[d][4 * x + e] * dk_by;
+                        z[e] = dv[d][4 * x + e] * dv_by;
                     }
                     if constexpr (DK) *reinterpret_cast<V4<float>*>(ok + 32 * d + 8 * x + 4 * h) = y;
                     if constexpr (DV) *reinterpret_cast<V4<float>*>(ov + 32 * d + 8 * x + 4 * h) = z;

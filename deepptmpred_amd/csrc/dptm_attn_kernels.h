@@ -263,8 +263,10 @@ __global__ __launch_bounds__(NW * 64, (kForwardWaves<T, D>)) void attn_fwd_wide_
         __syncthreads();
         at = after;
     }
-    const bool lost = BIAS && fmaf(l, 0.f, zero_if_finite<DT>(acc)) != 0.f;
-    if (__syncthreads_or((int)odd | (int)lost) && (!BIAS || __syncthreads_or((int)odd) || table_hides<T>(a.bias, a.heads, head, 1))) {
+    bool redo = __syncthreads_or((int)odd);
+    if constexpr (BIAS)
+        if (!redo && __ballot(!finite(l + sum_of_all(acc)))) redo = table_hides<T>(a.bias, a.heads, head, 1);
+    if (redo) {
         float t[16 * DT], ml[2];
         forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, ml, item, head, rowc, rw.pos, 0, 1, kBK, bias, h);
         take<DT>(acc, t);
@@ -367,8 +369,10 @@ __global__ __launch_bounds__(256, sizeof(T) * D >= 512 ? 1 : 2) void attn_fwd_sp
         v.read(vt, 0, lane);
         v.product(acc, s[0]);
     }
-    const bool lost = BIAS && fmaf(l, 0.f, zero_if_finite<DT>(acc)) != 0.f;
-    if (__ballot((odd != 0) | lost) && (!BIAS || __ballot(odd != 0) || table_hides<T>(a.bias, a.heads, head0, pack))) {
+    bool redo = __ballot(odd != 0);
+    if constexpr (BIAS)
+        if (!redo && __ballot(!finite(l + sum_of_all(acc)))) redo = table_hides<T>(a.bias, a.heads, head0, pack);
+    if (redo) {
         float t[16 * DT], x[2];
         forward_by_pairs<T, D, DT, BIAS>(kernel_args(), t, x, id - id / a.n_items * a.n_items, head, query, rw.pos, w, NW, 32, bias, h);
         take<DT>(acc, t);

@@ -137,7 +137,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
     };
     // sums of a row's pairs over this wavefront's keys, by row
     auto row_sums = [&](const f32x16_a& x, int u) {
-        const float sum = lane_sums(x, lane);
+        const float sum = Lift<T>::off_first(lane_sums(x, lane));
         if ((lane & 16) == 0) rowdelta[kRows * w + 32 * u + reg_row(lane & 15) + 4 * h] = sum;
         return sum;
     };
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 4 * x + e;
-                    s[r] = __builtin_amdgcn_exp2f(kLseLast<T> ? fmaf(s[r], c, y[e]) : s[r] * c);
+                    s[r] = __builtin_amdgcn_exp2f(kLseLast<T> ? fmaf(s[r], c, y[e]) : Lift<T>::kOn ? fmaf(s[r], c, Lift<T>().log2()) : s[r] * c);
                     p[r] *= s[r];
                 }
             }
@@ -188,10 +188,11 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
             cols.read(gt, r0, lane);
             cols.product(dv, s);
         }
-        lost |= !(fabsf(row_sums(p, u)) < __builtin_inff());
+        lost |= !finite(row_sums(p, u));
     }
     // (a value row of NaN, say): what it is multiplied with is zero where pairs are hidden, but the product is not
     lost = __syncthreads_or((int)lost);
+    Lift<T> lift_k, lift_q;      // of dk and dq; weight and d_s hold what is lifted by the first power, and so do dv's sums
     bool hides = false;
     if constexpr (BIAS) {
         if (lost && table_hides<T>(a.bias, a.heads, head, 1)) {
@@ -222,13 +223,18 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
             if (hides) hide_buckets(d_s[u], u);
             Cols<T, D> cols;
             cols.read(qt, 32 * u, lane);
-            cols.product(dk, d_s[u]);
+            f32x16_a x = d_s[u];
+            if (Lift<T>::kOn && lift_k.moved) Lift<T>::down(x, Lift<T>::kFirst - lift_k.e);
+            lift_k.settle(x, dk);
+            cols.product(dk, x);
         }
+    float dk_by = lift_k.off(a.scale), dv_by = Lift<T>::off_first(1.f);
     if (redo) {
         float x[16 * DT], y[16 * DT];
         dkv_by_pairs<T, D, DT, BIAS>(kernel_args(), x, y, k_items_at, item, head, keyc, h);
         take<DT>(dk, x);
         take<DT>(dv, y);
+        dk_by = a.scale, dv_by = 1.f;
     }
     __syncthreads();
 #pragma unroll
@@ -245,7 +251,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
             for (int x = 0; x < (D >= 32 ? 4 : 2); ++x) {
                 V4<T> y, z;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = (T)(dk[d][4 * x + e] * a.scale), z[e] = (T)dv[d][4 * x + e];
+                for (int e = 0; e < 4; ++e) y[e] = (T)(dk[d][4 * x + e] * dk_by), z[e] = (T)(dv[d][4 * x + e] * dv_by);
                 *reinterpret_cast<V4<T>*>(ok + 32 * d + 8 * x + 4 * h) = y;
                 *reinterpret_cast<V4<T>*>(ov + 32 * d + 8 * x + 4 * h) = z;
             }
@@ -267,6 +273,8 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[4 * x + e] = y[e];
             }
+            if (Lift<T>::kOn && lift_q.moved) Lift<T>::down(s, Lift<T>::kFirst - lift_q.e);
+            lift_q.settle(s, dq);
             cols.product(dq, s);
         }
     if constexpr (BIAS) {
@@ -285,10 +293,12 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
         sums[2 * kRows * half + l] = down[0] + down[1];
         sums[2 * kRows * half + kRows + l] = up[0] + up[1];
     }
+    float dq_by = lift_q.off(a.scale);
     if (redo) {
         float t[16 * DT], over;
         dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, &over, item, head, rowc, pos0 + rowc, a.delta[(int64_t)head * a.q_rows + qr], bias, h);
         take<DT>(dq, t);
+        dq_by = a.scale;
     }
     if (mine < nq) {
         T* o = const_cast<T*>(row_ptr<T>(a.dq, (int64_t)qi.q0 + mine, head));
@@ -298,7 +308,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
             for (int x = 0; x < (D >= 32 ? 4 : 2); ++x) {
                 V4<T> y;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = (T)(dq[d][4 * x + e] * a.scale);
+                for (int e = 0; e < 4; ++e) y[e] = (T)(dq[d][4 * x + e] * dq_by);
                 *reinterpret_cast<V4<T>*>(o + 32 * d + 8 * x + 4 * h) = y;
             }
     }
@@ -310,7 +320,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
             const int from = i == 0 ? 0 : max(t, 0), to = i == words - 1 ? last : min(t, last);
             float x = 0.f;
             for (int k = from; k <= to; ++k) x += sums[k] + sums[2 * kRows + k];
-            part[i] = x;
+            part[i] = Lift<T>::off_first(x);
         }
     }
 }

@@ -460,9 +460,8 @@ int64_t dptm_attention_workspace(const int32_t* plan, int32_t n_buckets, int32_t
 int dptm_attention_forward(const dptm_attention_args* args);
 
 /* Gradients of the above from dout, with out and lse as the forward call left them: dq, dk, dv (dk and dv summed over the
- * query heads that share a key head) and, with a bias, dtable.  Keys that no row sees get zeros.  In float16 a pair's gradient
- * before the scale, P_ij (dP_ij - delta_i), has to stay below 65504.  No sum depends on the
- * order in which workgroups run: equal calls give equal bits. */
+ * query heads that share a key head) and, with a bias, dtable.  Keys that no row sees get zeros.  Results, not the gradients of
+ * single pairs, have to lie in the type's range.  No sum depends on the order in which workgroups run: equal calls give equal bits. */
 int dptm_attention_backward(const dptm_attention_args* args);
 
 /* Norm of every query and key head and the rotation by position, one pass: y = x (mean x^2 + eps)^-1/2 gain over the

@@ -131,3 +131,70 @@ def test_lse_of_rows_whose_scores_are_nan(dtype, lens, k_lens, heads, kv_heads):
     assert torch.isnan(out[:lens[0]]).all() and torch.isnan(lse[:, :lens[0]]).all()
     if n > lens[0]:
         within(lse.T[lens[0]:], (want[0].T[lens[0]:], want[1].T[lens[0]:]), "lse")
+
+
+# sequences of rows and keys, dim, listed positions, size of q and k, of v, of dout
+FAR_GRADIENTS = [([2048], [2048], 64, False, 1.0, 1.0, 1e-3), ([2048], [2048], 128, False, 1.0, 1.0, 1e-4), ([1500], [1500], 32, True, 1.0, 1.0, 1e-4),
+                 ([64], [20000], 64, False, 1.0, 1.0, 100.0), ([51] * 8, [51] * 8, 32, False, 1.0, 1.0, 1e-5),
+                 ([51] * 8, [51] * 8, 64, False, 0.01, 100.0, 3000.0), ([700], [700], 64, False, 0.01, 100.0, 10000.0),
+                 ([300], [300], 64, False, 2.0, 3000.0, 0.01), ([300], [300], 64, True, 2.0, 3000.0, 0.01)]
+
+
+def rounding_of_pairs(q, k, v, dout, out, lens, k_lens, positions, table, buckets):
+    """What rounding single pairs to float16 and delta from a rounded out leave in dq, dk and dv, per element, as variances.  A rounding is
+    off by at most half a step, 2^-11 of the value, and evenly spread: its variance is at most (2^-11 value)^2 / 3.  delta is off by
+    dout . (out - its exact value), known here, and takes that times scale sum_j P_ij k_j from dq."""
+    var = {"dq": np.zeros(q.shape), "dk": np.zeros(k.shape), "dv": np.zeros(v.shape)}
+    scale, a0, b0 = q.shape[2] ** -0.5, 0, 0
+    pos = R.default_positions(lens, k_lens) if positions is None else np.asarray(positions)
+    for a, b in zip(lens, k_lens):
+        rows, keys = slice(a0, a0 + a), slice(b0, b0 + b)
+        for h in range(q.shape[1]):
+            Q, K, V, G = q[rows, h], k[keys, h], v[keys, h], dout[rows, h]
+            s = scale * Q @ K.T
+            if table is not None:
+                reach = len(buckets) // 2
+                s += table[buckets[np.clip(np.arange(b)[None] - pos[rows][:, None], -reach, reach) + reach], h]
+            P = np.exp(s - s.max(1, keepdims=True))
+            P /= P.sum(1, keepdims=True)
+            y = P @ V
+            dS = P * (G @ V.T - (G * y).sum(1, keepdims=True))
+            third = 2.0 ** -22 / 3
+            off = (G * (out[rows, h] - y)).sum(1, keepdims=True)
+            var["dq"][rows, h] = third * scale ** 2 * dS ** 2 @ K ** 2 + (scale * off * (P @ K)) ** 2
+            var["dk"][keys, h] = third * scale ** 2 * (dS ** 2).T @ Q ** 2
+            var["dv"][keys, h] = third * (P ** 2).T @ G ** 2
+        a0, b0 = a0 + a, b0 + b
+    return var
+
+
+@pytest.mark.parametrize("lens,k_lens,dim,given,size,size_v,size_dout", FAR_GRADIENTS)
+@pytest.mark.parametrize("biased", [False, True])
+def test_float16_gradients_far_from_one(lens, k_lens, dim, given, size, size_v, size_dout, biased):
+    """float16 gradients keep their bits where the pairs' own lie below or above what float16 holds: their error's root mean square is that
+    of three independent roundings -- the result's, the pairs' and out's (rounding_of_pairs) -- and 4 % for fp32 sums and the sample.
+    The bias gradient is summed from dS that is not rounded: the result's alone."""
+    rng = np.random.default_rng(93)
+    n, nk, heads = sum(lens), sum(k_lens), 2
+    q, k, v = tensor(rng, "f16", n, heads, dim, by=size), tensor(rng, "f16", nk, heads, dim, by=size), tensor(rng, "f16", nk, heads, dim, by=size_v)
+    dout = tensor(rng, "f16", n, heads, dim, by=size_dout)
+    b = table = None
+    if biased:
+        b, table = layers.relative_buckets(16, 50), tensor(rng, "f16", 16, heads)
+    pos = rng.permutation(nk)[:n].astype(np.int32) if given else None
+    plan = layers.AttentionPlan(lens, k_lens, heads=heads, head_dim=dim, q_positions=pos)
+    out, lse = layers.attention(q, k, v, plan, table=table, buckets=b)
+    got = layers.attention_backward(dout, q, k, v, out, lse, plan, table=table, buckets=b)
+    bias = (None, None) if b is None else (host(table), b.cpu().numpy())
+    want = R.attention(host(q), host(k), host(v), lens, k_lens, positions=pos, table=bias[0], buckets=bias[1], dout=host(dout), kernel_out=host(out),
+                       dtype="f16")
+    var = rounding_of_pairs(host(q), host(k), host(v), host(dout), host(out), lens, k_lens, pos, *bias)
+    # where pairs' gradients pass 65504, so do their sums by bucket; rows at listed positions have a test of their own
+    for t, name in zip(got, ("dq", "dk", "dv") + (("dtable",) if biased and size_dout < 1000 and not given else ())):
+        value = want[name][0]
+        assert np.abs(value).max() < 65504, name
+        alone = (value.astype(np.float16).astype(np.float64) - value) ** 2
+        off = np.sqrt(np.mean((host(t) - value) ** 2))
+        most = np.sqrt(np.mean(alone + var.get(name, 0)))
+        print(f"{name}: {off / np.sqrt(np.mean(alone)):.3f} times the error of rounding it, {off / most:.3f} of what is left to it")
+        assert off <= 1.04 * most, f"{name}: {off / most:.3g} of what is left to it"
