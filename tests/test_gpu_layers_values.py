@@ -198,3 +198,26 @@ def test_float16_gradients_far_from_one(lens, k_lens, dim, given, size, size_v, 
         most = np.sqrt(np.mean(alone + var.get(name, 0)))
         print(f"{name}: {off / np.sqrt(np.mean(alone)):.3f} times the error of rounding it, {off / most:.3f} of what is left to it")
         assert off <= 1.04 * most, f"{name}: {off / most:.3g} of what is left to it"
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,keys,heads,dim", [(1500, 1500, 2, 32), (130, 400, 2, 64), (53, 2100, 4, 64), (300, 300, 48, 128)])
+def test_bias_gradient_of_listed_positions(dtype, rows, keys, heads, dim):
+    """The bias gradient is summed in 32 bits and more from dS that is not rounded, with a delta that owes nothing to the rounding of
+    out: what is left is the rounding of the result, and 5 % of it for the fp32 sums and the sample."""
+    rng = np.random.default_rng(95)
+    q, k, v, dout = tensor(rng, dtype, rows, heads, dim), tensor(rng, dtype, keys, heads, dim), tensor(rng, dtype, keys, heads, dim), tensor(rng, dtype, rows, heads, dim)
+    b, table = layers.relative_buckets(16, 50), tensor(rng, dtype, 16, heads)
+    pos = rng.permutation(keys)[:rows].astype(np.int32)
+    plan = layers.AttentionPlan([rows], [keys], heads=heads, head_dim=dim, q_positions=pos)
+    out, lse = layers.attention(q, k, v, plan, table=table, buckets=b)
+    got = layers.attention_backward(dout, q, k, v, out, lse, plan, table=table, buckets=b)
+    want = R.attention(host(q), host(k), host(v), [rows], [keys], positions=pos, table=host(table), buckets=b.cpu().numpy(), dout=host(dout),
+                       kernel_out=host(out), dtype=dtype)
+    for t, name in zip(got, ("dq", "dk", "dv", "dtable")):
+        within(t, want[name], name)
+    value = want["dtable"][0]
+    rounded = torch.from_numpy(value).to(q.dtype).double().numpy()
+    alone, off = (np.sqrt(np.mean((x - value) ** 2)) for x in (rounded, host(got[3])))
+    print(f"dtable: {off / alone:.3f} times the error of rounding it")
+    assert off <= 1.05 * alone
