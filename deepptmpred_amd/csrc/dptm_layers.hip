@@ -217,6 +217,7 @@ int make_plan(const dptm_attention_desc& d, const int32_t* q_len, const int32_t*
         if (nq < 0 || nk < 0 || nq >= kFar || nk >= kFar)
             return fail(DPTM_EINVAL, std::string(who) + "length of sequence " + std::to_string(b) + " is outside 0..2^29-1");
         m.seqs.push_back(Seq{(int)q0, nq, (int)k0, nk, nk - nq, (int)(m.bounds.size() / 2)});
+        int nearest = q_pos ? kFar : nk - nq;
         if (q_pos)
             for (int i = 0; i < nq; i += 32) {
                 int lo = kFar, hi = -kFar;
@@ -227,7 +228,11 @@ int make_plan(const dptm_attention_desc& d, const int32_t* q_len, const int32_t*
                 }
                 m.bounds.push_back(lo);
                 m.bounds.push_back(hi);
+                nearest = std::min(nearest, lo);
             }
+        // a side without limit is one of 2^29
+        if (m.right == kFar && nq && nk && (int64_t)nk - 1 - nearest > kFar)
+            return fail(DPTM_EINVAL, std::string(who) + "a key lies more than 2^29 positions ahead of a row of a window without a right limit");
         q0 += nq, k0 += nk;
         if (q0 > INT32_MAX || k0 > INT32_MAX) return fail(DPTM_EINVAL, std::string(who) + "more than 2^31-1 rows");
     }

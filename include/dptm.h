@@ -408,7 +408,8 @@ typedef struct dptm_rows {
  * Query row i stands at position p_i -- q_positions[i], or (NULL) i + k_len - q_len within its sequence, so that the last
  * query stands at the last key -- and sees key j of its sequence if
  *     j <= p_i + window_right  and  (j >= p_i - window_left  or  j < sinks);
- * a negative window side has no limit.  heads must be a multiple of kv_heads: query head h reads key head
+ * a negative window side has no limit.  Lengths are below 2^29, positions between -2^29 and 2^29; without a right limit no key may
+ * lie more than 2^29 ahead of a row of its sequence.  heads must be a multiple of kv_heads: query head h reads key head
  * h / (heads / kv_heads).  head_dim 16, 32, 64 or 128. */
 typedef struct dptm_attention_desc {
     int32_t heads, kv_heads, head_dim;

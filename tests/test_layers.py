@@ -394,3 +394,19 @@ def test_a_bias_that_is_no_tensor_is_refused():
     plan = layers.AttentionPlan([5], heads=2, head_dim=16, device=None)
     with pytest.raises(ValueError, match="torch tensors"):
         layers._bias("attention", plan, np.zeros((8, 2), np.float32), layers.relative_buckets(8, 20, device=None), torch.float32, 0)
+
+
+def test_keys_out_of_reach_of_a_window_without_limit_are_refused():
+    """A side without limit reaches 2^29 positions: a batch whose keys lie further ahead would lose them without a word."""
+    ok = dict(heads=1, head_dim=64, device=None)
+    far = 2 ** 29
+    for window in ((-1, -1), (7, -1), (-1, 2 ** 31 - 1)):
+        with pytest.raises(ValueError, match="2\\^29"):
+            layers.AttentionPlan([1], [100], q_positions=[-far + 1], window=window, **ok)
+        with pytest.raises(ValueError, match="2\\^29"):
+            layers.AttentionPlan([3, 2], [7, 100], q_positions=[0, 1, 2, 50, -far + 98], window=window, **ok)
+    # the last that is in reach sees all of its keys, and so do rows that are limited or far behind
+    for position, window, keys in ((-far + 99, (-1, -1), 100), (far - 1, (-1, -1), 100), (-far + 1, (-1, 5), 0), (far - 1, (-1, 0), 100)):
+        w = layers.AttentionPlan([1], [100], q_positions=[position], window=window, **ok).words
+        assert [int(x) for x in w[w[13] + 4:w[13] + 6]] == [0, keys] and w[12] == 1
+    assert layers.AttentionPlan([0, 1], [far - 1, 4], window=(-1, -1), **ok).k_rows == far + 3
