@@ -88,41 +88,72 @@ int check_rows(const char* who, const char* name, const dptm_rows& t, int64_t ro
     return DPTM_OK;
 }
 
-// A tensor of a call, for check_apart.
+// The memory of a tensor of a call, for check_apart: runs of `run` bytes at at + i * step[0] + j * step[1], i < n[0], j < n[1].
 struct Place {
     const char* name;
-    const Strided& t;
-    int64_t rows;
-    int heads, dim, size;
-    int64_t row() const { return t.row * size; }
-    int64_t head() const { return heads > 1 ? t.head * size : (int64_t)dim * size; }
-    int64_t row_bytes() const { return (heads - 1) * head() + (int64_t)dim * size; }
-    int64_t bytes() const { return (rows - 1) * row() + row_bytes(); }
-    bool empty() const { return rows == 0 || heads == 0 || !t.p; }
-    uintptr_t at() const { return reinterpret_cast<uintptr_t>(t.p); }
+    uintptr_t at;
+    int64_t n[2], step[2], run;
+
+    Place(const char* name, const Strided& t, int64_t rows, int heads, int dim, int size)
+        : name(name), at(reinterpret_cast<uintptr_t>(t.p)), n{rows, heads}, step{t.row * size, t.head * size}, run((int64_t)dim * size) {
+        tidy();
+    }
+    Place(const char* name, const void* p, int64_t bytes) : name(name), at(reinterpret_cast<uintptr_t>(p)), n{1, 1}, step{0, 0}, run(p ? bytes : 0) {}
+
+    bool empty() const { return !at || n[0] <= 0 || n[1] <= 0 || run <= 0; }
+    int64_t bytes() const { return (n[0] - 1) * step[0] + (n[1] - 1) * step[1] + run; }
+    // the larger step first, repeated memory once, steps that leave no gap as one run
+    void tidy() {
+        if (empty()) return;
+        for (int d = 0; d < 2; ++d)
+            if (n[d] == 1 || step[d] == 0) n[d] = 1, step[d] = 0;
+        if (step[0] < step[1]) std::swap(step[0], step[1]), std::swap(n[0], n[1]);
+        for (int d = 1; d >= 0; --d)
+            if (n[d] > 1 && step[d] <= run && (d || n[1] == 1)) run += (n[d] - 1) * step[d], n[d] = 1, step[d] = 0;
+    }
+    // whether [from, from + len), counted from `at`, meets a run.  For what is written: there the inner runs of an outer
+    // step end before the next one begins (check_rows)
+    bool meets(int64_t from, int64_t len) const {
+        // the outer steps whose span [i step0, i step0 + span) the bytes touch
+        const int64_t span = (n[1] - 1) * step[1] + run;
+        auto first_not_before = [](int64_t x, int64_t step, int64_t width) {      // smallest i >= 0 with i step + width > x
+            return x < width || step == 0 ? 0 : (x - width) / step + 1;
+        };
+        for (int64_t i = first_not_before(from, step[0], span); i < n[0] && i * step[0] < from + len; ++i) {
+            const int64_t x = from - i * step[0], j = first_not_before(x, step[1], run);
+            if (j < n[1] && j * step[1] < x + len && j * step[1] + run > x) return true;
+        }
+        return false;
+    }
 };
 
-// Whether two tensors share memory.  Columns of one packed tensor ([rows][q k v heads][dim], or [rows][heads][q k v][dim])
-// do not; for strides that fit neither the answer is no unless they start at the same address.
+// Whether two tensors share memory; `a` is written.  Exact: where both go by the same steps -- views of one packed tensor -- from the
+// difference of their addresses, otherwise by the runs of `b`, one by one.  Tensors beside each other are told by their bounds.
 bool overlap(const Place& a, const Place& b) {
-    if (a.empty() || b.empty() || a.at() + a.bytes() <= b.at() || b.at() + b.bytes() <= a.at()) return false;
-    if (a.at() == b.at()) return true;
-    const Place &lo = a.at() < b.at() ? a : b, &hi = a.at() < b.at() ? b : a;
-    auto beside = [](int64_t off, int64_t w_lo, int64_t w_hi, int64_t step) { return off >= w_lo && off + w_hi <= step; };
-    auto rows_packed = [](const Place& x) { return x.rows == 1 || x.row() >= x.row_bytes(); };
-    if (!rows_packed(lo) || !rows_packed(hi)) return false;
-    const int64_t step = lo.rows > 1 ? lo.row() : hi.row();
-    if (lo.rows > 1 && hi.rows > 1 && lo.row() != hi.row()) {
-        // one without gaps between its rows: does it reach a row of the other?
-        const Place &whole = lo.row() == lo.row_bytes() ? lo : hi, &other = &whole == &lo ? hi : lo;
-        if (whole.row() != whole.row_bytes()) return false;
-        const int64_t from = (int64_t)(whole.at() - other.at()), first = from < other.row_bytes() ? 0 : (from - other.row_bytes()) / other.row() + 1;
-        return first < other.rows && first * other.row() < from + whole.bytes();
+    if (a.empty() || b.empty() || a.at + a.bytes() <= b.at || b.at + b.bytes() <= a.at) return false;
+    const int64_t off = (int64_t)(b.at - a.at);
+    int64_t step[2];
+    bool alike = true;
+    for (int d = 0; d < 2; ++d) {
+        step[d] = b.n[d] == 1 ? a.step[d] : b.step[d];
+        alike &= a.n[d] == 1 || a.step[d] == step[d];
     }
-    const int64_t off = lo.rows > 1 || hi.rows > 1 ? (int64_t)(hi.at() - lo.at()) % step : (int64_t)(hi.at() - lo.at());
-    if (lo.rows > 1 || hi.rows > 1 ? beside(off, lo.row_bytes(), hi.row_bytes(), step) : off >= lo.row_bytes()) return false;
-    const int64_t dim = (int64_t)lo.dim * lo.size;
-    return !(lo.heads > 1 && lo.head() == hi.head() && beside(off % lo.head(), dim, dim, lo.head()));
+    if (!alike) {
+        for (int64_t i = 0; i < b.n[0]; ++i)
+            for (int64_t j = 0; j < b.n[1]; ++j)
+                if (a.meets(off + i * b.step[0] + j * b.step[1], b.run)) return true;
+        return false;
+    }
+    // runs that are di and dj steps apart meet if -b.run < off + di step + dj step' < a.run: every dj of the shorter direction, and the
+    // largest di that satisfies the right side
+    const int s = a.n[0] + b.n[0] < a.n[1] + b.n[1] ? 0 : 1, l = 1 - s;
+    for (int64_t dj = 1 - a.n[s]; dj < b.n[s]; ++dj) {
+        const int64_t x = off + dj * step[s], room = a.run - 1 - x;
+        int64_t di = 0;
+        if (step[l]) di = std::min(room >= 0 ? room / step[l] : -((-room + step[l] - 1) / step[l]), b.n[l] - 1);
+        if (di > -a.n[l] && x + di * step[l] < a.run && x + di * step[l] > -b.run) return true;
+    }
+    return false;
 }
 
 // What a call writes lies apart from what it reads and from what else it writes.
@@ -131,6 +162,22 @@ int check_apart(const char* who, const Place& written, std::initializer_list<con
         if (overlap(written, *o)) return fail(DPTM_EINVAL, std::string(who) + ": " + written.name + " shares memory with " + o->name);
     return DPTM_OK;
 }
+
+// The same for the small buffers of a call: the first pair that shares memory.  Reported with the device, which is the last check: a call
+// refused for its device says so first.
+struct Shared {
+    const char *written = nullptr, *with = nullptr;
+    void look(const Place& w, std::initializer_list<const Place*> others) {
+        for (const Place* o : others)
+            if (!written && overlap(w, *o)) written = w.name, with = o->name;
+    }
+    int check(const char* who, bool device) const {
+        if (device && !written) return DPTM_OK;
+        std::string msg = std::string(who) + (device ? "" : ": no such device");
+        if (written) msg += std::string(device ? ": " : "; ") + written + " shares memory with " + with;
+        return fail(DPTM_EINVAL, msg);
+    }
+};
 
 constexpr int kGroups = 768;   // workgroups that keys are cut for: three a processor
 
@@ -515,7 +562,14 @@ int dptm_attention_forward(const dptm_attention_args* args) try {
     if (!x.lse || (reinterpret_cast<uintptr_t>(x.lse) & 3)) return fail(DPTM_EINVAL, std::string(who) + ": lse is NULL or misaligned");
     const int size = size_of(dtype);
     const Place pq{"q", a.q, nq, heads, dim, size}, pk{"k", a.k, nk, kv, dim, size}, pv{"v", a.v, nk, kv, dim, size};
-    OK_OR_RETURN(check_apart(who, Place{"out", a.out, nq, heads, dim, size}, {&pq, &pk, &pv}));
+    const Place po{"out", a.out, nq, heads, dim, size}, pl{"lse", x.lse, 4 * heads * nq}, pw{"workspace", x.workspace, (int64_t)(w.fwd_o + w.fwd_ml)};
+    const Place pt{"table", a.bias.table, (int64_t)a.bias.n_buckets * heads * size}, pb{"buckets", a.bias.buckets, 4 * (2 * (int64_t)a.bias.reach + 1)};
+    const Place pp{"plan", x.plan_dev, 4 * (int64_t)plan[kPlanWords]};
+    OK_OR_RETURN(check_apart(who, po, {&pq, &pk, &pv}));
+    Shared shared;
+    shared.look(po, {&pl, &pw, &pt, &pb, &pp});
+    shared.look(pl, {&pq, &pk, &pv, &pw, &pt, &pb, &pp});
+    shared.look(pw, {&pq, &pk, &pv, &pt, &pb, &pp});
     a.lse = x.lse;
     a.part_o = static_cast<float*>(x.workspace);
     a.part_ml = reinterpret_cast<float*>(static_cast<char*>(x.workspace) + w.fwd_o);
@@ -523,7 +577,7 @@ int dptm_attention_forward(const dptm_attention_args* args) try {
     // tiles that share no keys: better the heads' parts of the same cache lines together (heads of 64 bytes: 58 -> 54 us)
     a.by_sequence = plan[kPlanFwd] <= plan[kPlanSeqs];
     const OnDevice on(x.device);
-    if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
+    OK_OR_RETURN(shared.check(who, on.ok));
     const hipStream_t s = static_cast<hipStream_t>(x.stream);
     OK_OR_RETURN(hip_result(who, BY_TYPE(attn_forward, a, dim, plan[kPlanMode], s)));
     return hip_result(who, BY_TYPE(attn_join, a, dim, plan[kPlanJoin], plan[kPlanJoinAt], s));
@@ -559,9 +613,17 @@ int dptm_attention_backward(const dptm_attention_args* args) try {
     const Place pq{"q", a.q, nq, heads, dim, size}, pk{"k", a.k, nk, kv, dim, size}, pv{"v", a.v, nk, kv, dim, size};
     const Place po{"out", a.out, nq, heads, dim, size}, pg{"dout", a.dout, nq, heads, dim, size};
     const Place pdq{"dq", a.dq, nq, heads, dim, size}, pdk{"dk", a.dk, nk, kv, dim, size}, pdv{"dv", a.dv, nk, kv, dim, size};
+    const Place pl{"lse", x.lse, 4 * heads * nq}, pw{"workspace", x.workspace, (int64_t)(w.delta + w.dkv + w.bias + w.groups)};
+    const int64_t entries = (int64_t)a.bias.n_buckets * heads * size;
+    const Place pt{"table", a.bias.table, entries}, pb{"buckets", a.bias.buckets, 4 * (2 * (int64_t)a.bias.reach + 1)}, pdt{"dtable", x.dtable, entries};
+    const Place pp{"plan", x.plan_dev, 4 * (int64_t)plan[kPlanWords]};
     OK_OR_RETURN(check_apart(who, pdq, {&pq, &pk, &pv, &po, &pg, &pdk, &pdv}));
     OK_OR_RETURN(check_apart(who, pdk, {&pq, &pk, &pv, &po, &pg, &pdv}));
     OK_OR_RETURN(check_apart(who, pdv, {&pq, &pk, &pv, &po, &pg}));
+    Shared shared;
+    for (const Place* p : {&pdq, &pdk, &pdv}) shared.look(*p, {&pl, &pt, &pb, &pp, &pdt, &pw});
+    shared.look(pdt, {&pq, &pk, &pv, &po, &pg, &pl, &pt, &pb, &pp, &pw});
+    shared.look(pw, {&pq, &pk, &pv, &po, &pg, &pl, &pt, &pb, &pp});
     a.lse = x.lse;
     a.delta = static_cast<float*>(x.workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(x.workspace) + w.delta);
@@ -569,7 +631,7 @@ int dptm_attention_backward(const dptm_attention_args* args) try {
     a.part_groups = reinterpret_cast<double*>(static_cast<char*>(x.workspace) + w.delta + w.dkv + w.bias);
     a.dtable = x.dtable;
     const OnDevice on(x.device);
-    if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
+    OK_OR_RETURN(shared.check(who, on.ok));
     const hipStream_t s = static_cast<hipStream_t>(x.stream);
     a.n_items = plan[kPlanDq], a.items_at = plan[kPlanDqAt];
     if (plan[kPlanDqWaves] == kTogether) {
@@ -612,17 +674,22 @@ static int norm_rope_args(const char* who, const dptm_norm_rope_args* x, NormRop
 }
 
 // A head's result may take the place of what it is made from, element for element, and lies apart from the rest.
-static int norm_rope_apart(const char* who, const dptm_norm_rope_args& x, const Strided (&from)[2], const Strided (&to)[2], const char* const (&name)[4]) {
+static int norm_rope_apart(const char* who, const dptm_norm_rope_args& x, const Strided (&from)[2], const Strided (&to)[2], const char* const (&name)[4],
+                           Shared* shared) {
     const int size = size_of(x.dtype), n[2] = {x.heads, x.kv_heads};
     const Place f0{name[0], from[0], x.rows, n[0], x.head_dim, size}, f1{name[1], from[1], x.rows, n[1], x.head_dim, size};
     const Place t0{name[2], to[0], x.rows, n[0], x.head_dim, size}, t1{name[3], to[1], x.rows, n[1], x.head_dim, size};
-    auto same = [](const Place& a, const Place& b) {
-        return a.at() == b.at() && (a.rows == 1 || a.t.row == b.t.row) && (a.heads == 1 || a.t.head == b.t.head);
+    auto same = [&](int i) {
+        return from[i].p == to[i].p && (x.rows == 1 || from[i].row == to[i].row) && (n[i] == 1 || from[i].head == to[i].head);
     };
     OK_OR_RETURN(check_apart(who, t0, {&f1, &t1}));
     OK_OR_RETURN(check_apart(who, t1, {&f0}));
-    if (!same(t0, f0)) OK_OR_RETURN(check_apart(who, t0, {&f0}));
-    if (!same(t1, f1)) OK_OR_RETURN(check_apart(who, t1, {&f1}));
+    if (!same(0)) OK_OR_RETURN(check_apart(who, t0, {&f0}));
+    if (!same(1)) OK_OR_RETURN(check_apart(who, t1, {&f1}));
+    const int64_t table = (int64_t)x.n_positions * (x.head_dim / 2) * 4, gain = (int64_t)x.head_dim * 4;
+    const Place c{"cos", x.cosv, table}, s{"sin", x.sinv, table}, p{"positions", x.positions, x.rows * 4};
+    const Place g0{"q_gain", x.q_gain, gain}, g1{"k_gain", x.k_gain, gain};
+    for (const Place* t : {&t0, &t1}) shared->look(*t, {&c, &s, &p, &g0, &g1});
     return DPTM_OK;
 }
 
@@ -632,10 +699,11 @@ int dptm_qk_norm_rope_forward(const dptm_norm_rope_args* x) try {
     OK_OR_RETURN(norm_rope_args(who, x, &a));
     OK_OR_RETURN(check_rows(who, "q_out", x->q_out, x->heads ? x->rows : 0, x->heads, x->head_dim, x->dtype, true, &a.y[0]));
     OK_OR_RETURN(check_rows(who, "k_out", x->k_out, x->kv_heads ? x->rows : 0, x->kv_heads, x->head_dim, x->dtype, true, &a.y[1]));
-    OK_OR_RETURN(norm_rope_apart(who, *x, a.x, a.y, {"q", "k", "q_out", "k_out"}));
+    Shared shared;
+    OK_OR_RETURN(norm_rope_apart(who, *x, a.x, a.y, {"q", "k", "q_out", "k_out"}, &shared));
     if (x->rows == 0) return DPTM_OK;
     const OnDevice on(x->device);
-    if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
+    OK_OR_RETURN(shared.check(who, on.ok));
     return hip_result(who, norm_rope_forward(a, x->dtype, static_cast<hipStream_t>(x->stream)));
 } catch (...) {
     return on_exception("dptm_qk_norm_rope_forward");
@@ -658,16 +726,32 @@ int dptm_qk_norm_rope_backward(const dptm_norm_rope_args* x) try {
     OK_OR_RETURN(check_rows(who, "dk", x->dk, rk, x->kv_heads, x->head_dim, x->dtype, true, &a.dx[1]));
     if ((x->q_gain && !x->dq_gain) || (x->k_gain && !x->dk_gain))
         return fail(DPTM_EINVAL, std::string(who) + ": gain without a buffer for its gradient");
+    if ((reinterpret_cast<uintptr_t>(x->dq_gain) & 3) || (reinterpret_cast<uintptr_t>(x->dk_gain) & 3))
+        return fail(DPTM_EINVAL, std::string(who) + ": gradients of gains must be aligned to their elements");
     const int64_t half = dptm_qk_norm_rope_workspace(x) / 2;
     if ((x->q_gain || x->k_gain) && (!x->workspace || x->workspace_bytes < (size_t)half * 2 || (reinterpret_cast<uintptr_t>(x->workspace) & 255)))
         return fail(DPTM_EINVAL, std::string(who) + ": workspace of " + std::to_string(half * 2) + " bytes, 256-byte aligned, needed");
-    OK_OR_RETURN(norm_rope_apart(who, *x, a.dy, a.dx, {"dq_out", "dk_out", "dq", "dk"}));
-    OK_OR_RETURN(norm_rope_apart(who, *x, a.x, a.dx, {"q", "k", "dq", "dk"}));
+    Shared shared;
+    OK_OR_RETURN(norm_rope_apart(who, *x, a.dy, a.dx, {"dq_out", "dk_out", "dq", "dk"}, &shared));
+    OK_OR_RETURN(norm_rope_apart(who, *x, a.x, a.dx, {"q", "k", "dq", "dk"}, &shared));
+    if (x->q_gain || x->k_gain) {
+        const int size = size_of(x->dtype), dim = x->head_dim;
+        const int64_t table = (int64_t)x->n_positions * (dim / 2) * 4;
+        const Place q{"q", a.x[0], x->rows, x->heads, dim, size}, k{"k", a.x[1], x->rows, x->kv_heads, dim, size};
+        const Place gq{"dq_out", a.dy[0], x->rows, x->heads, dim, size}, gk{"dk_out", a.dy[1], x->rows, x->kv_heads, dim, size};
+        const Place dq{"dq", a.dx[0], x->rows, x->heads, dim, size}, dk{"dk", a.dx[1], x->rows, x->kv_heads, dim, size};
+        const Place c{"cos", x->cosv, table}, s{"sin", x->sinv, table}, p{"positions", x->positions, x->rows * 4};
+        const Place g0{"q_gain", x->q_gain, dim * 4}, g1{"k_gain", x->k_gain, dim * 4}, w{"workspace", x->workspace, half * 2};
+        const Place d0{"dq_gain", x->q_gain ? x->dq_gain : nullptr, dim * 4}, d1{"dk_gain", x->k_gain ? x->dk_gain : nullptr, dim * 4};
+        shared.look(d0, {&q, &k, &gq, &gk, &dq, &dk, &c, &s, &p, &g0, &g1, &d1, &w});
+        shared.look(d1, {&q, &k, &gq, &gk, &dq, &dk, &c, &s, &p, &g0, &g1, &w});
+        shared.look(w, {&q, &k, &gq, &gk, &dq, &dk, &c, &s, &p, &g0, &g1});
+    }
     a.part[0] = static_cast<float*>(x->workspace);
     a.part[1] = x->workspace ? reinterpret_cast<float*>(static_cast<char*>(x->workspace) + half) : nullptr;
     a.dgain[0] = x->dq_gain, a.dgain[1] = x->dk_gain;
     const OnDevice on(x->device);
-    if (!on.ok) return fail(DPTM_EINVAL, std::string(who) + ": no such device");
+    OK_OR_RETURN(shared.check(who, on.ok));
     return hip_result(who, norm_rope_backward(a, x->dtype, static_cast<hipStream_t>(x->stream)));
 } catch (...) {
     return on_exception("dptm_qk_norm_rope_backward");

@@ -435,8 +435,8 @@ int64_t dptm_attention_plan(const dptm_attention_desc* d, const int32_t* q_len, 
  *   workspace        dptm_attention_workspace bytes, 256-byte aligned, contents of no meaning before or after
  *   dout .. dtable   the backward call only; dtable [n_buckets][heads] with a bias
  *   scale            of the scores, 2^-64..2^64
- * What a call writes (out; dq, dk, dv) lies apart from what it reads and from what else it writes; columns of one packed
- * tensor do.  Row strides are below 32 MiB */
+ * What a call writes (out, lse; dq, dk, dv, dtable; the workspace) lies apart from what it reads and from what else it writes, and is
+ * refused otherwise; columns of one packed tensor do.  Row strides are below 32 MiB */
 typedef struct dptm_attention_args {
     const int32_t* plan;
     const int32_t* plan_dev;

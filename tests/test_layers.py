@@ -410,3 +410,103 @@ def test_keys_out_of_reach_of_a_window_without_limit_are_refused():
         w = layers.AttentionPlan([1], [100], q_positions=[position], window=window, **ok).words
         assert [int(x) for x in w[w[13] + 4:w[13] + 6]] == [0, keys] and w[12] == 1
     assert layers.AttentionPlan([0, 1], [far - 1, 4], window=(-1, -1), **ok).k_rows == far + 3
+
+
+def test_shared_memory_is_found_byte_by_byte():
+    """Random layouts -- head-major, packed, repeated, larger or smaller than each other -- against the sets of their bytes."""
+    lib = _native.load_library()
+    rng = np.random.default_rng(7)
+    base, seen = 1 << 24, {True: 0, False: 0}
+
+    def layout(rows, heads):
+        kind = rng.integers(0, 5)
+        gap = lambda most: 8 * int(rng.integers(0, most))                       # elements of two bytes, steps of 16 bytes  # noqa: E731
+        if kind < 2:
+            head = 16 + gap(8)
+            return heads * head + gap(8), head
+        if kind < 4:
+            row = 16 + gap(8)
+            return row, rows * row + gap(8)
+        return [(0, 16), (16, 0), (8, 24), (0, 0)][rng.integers(0, 4)]          # for what is read alone
+
+    def touched(at, rows, heads, row, head):
+        return {at + 2 * (i * row + j * head) + b for i in range(rows) for j in range(heads) for b in range(0, 32, 16)}
+
+    for _ in range(4000):
+        nq, nk, heads, kv = int(rng.integers(1, 5)), int(rng.integers(1, 6)), 2, int(rng.integers(1, 3))
+        plan = layers.AttentionPlan([nq], [nk], heads=heads, kv_heads=kv, head_dim=16, device=None)
+        P = plan.words.ctypes.data
+        (orow, ohead), (krow, khead) = layout(nq, heads), layout(nk, kv)
+        out, k = base, base + 16 * int(rng.integers(-30, 30))
+        far = _native.Rows(1 << 26, 8, 64, 16)
+        x = _native.AttentionArgs(plan=P, plan_dev=P, q=far, k=_native.Rows(k, nk, krow, khead), v=far, out=_native.Rows(out, nq, orow, ohead), lse=1 << 27,
+                                  dtype=1, scale=0.1, device=4096, workspace=1 << 28, workspace_bytes=1 << 20)
+        rc, said = lib.dptm_attention_forward(C.addressof(x)), lib.dptm_layer_last_error().decode()
+        assert rc == _native.DPTM_EINVAL
+        if "overlap" in said:
+            continue                                                            # no layout for what is written
+        shared = bool(touched(out, nq, heads, orow, ohead) & touched(k, nk, kv, krow, khead))
+        seen[shared] += 1
+        assert ("out shares memory with k" in said) == shared and ("no such device" in said) != shared, (said, nq, nk, kv, orow, ohead, krow, khead, k - out)
+    assert min(seen.values()) > 300
+
+
+def test_every_buffer_that_a_call_writes_lies_apart():
+    """Head-major tensors, lse, tables, gradients of tables and gains, and the workspace."""
+    lib = _native.load_library()
+    plan = layers.AttentionPlan([10, 300], heads=2, head_dim=64, device=None)
+    P, n, u = plan.words.ctypes.data, 310, 1 << 22
+    at = {name: (i + 4) * u for i, name in enumerate("q k v out dout dq dk dv lse table buckets dtable ws".split())}
+
+    def said(call, **moved):
+        a = {**at, **moved}
+        r = {x: _native.Rows(a[x], n, 64, n * 64) for x in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")}      # [heads][rows][64]
+        x = _native.AttentionArgs(plan=P, plan_dev=P, lse=a["lse"], table=a["table"], buckets=a["buckets"], dtable=a["dtable"], workspace=a["ws"], workspace_bytes=u,
+                                  dtype=1, scale=0.1, device=4096, n_buckets=8, max_distance=20, **r)
+        assert call(C.addressof(x)) == _native.DPTM_EINVAL
+        return lib.dptm_layer_last_error().decode()
+
+    fwd, bwd = lib.dptm_attention_forward, lib.dptm_attention_backward
+    need = [lib.dptm_attention_workspace(P, 8, 20, b) for b in (0, 1)]
+    apart = "no such device"                   # at the end of what is said, the last check before anything runs
+    assert said(fwd).endswith(apart) and said(bwd).endswith(apart) and need[1] > 1000
+    head = n * 64 * 2
+    assert "out shares memory with q" in said(fwd, out=at["q"] + head)                  # one head on
+    assert "out shares memory with q" in said(fwd, out=at["q"] + 128)
+    assert said(fwd, out=at["q"] + 2 * head).endswith(apart)
+    assert "lse" in said(fwd, lse=at["q"] + 256) and "lse" in said(fwd, lse=at["out"] + 256)
+    assert "out shares memory with table" in said(fwd, table=at["out"] + 64) and "buckets" in said(fwd, buckets=at["out"] + 2 * head - 4)
+    assert said(fwd, buckets=at["out"] + 2 * head).endswith(apart)
+    assert "out shares memory with plan" in said(fwd, out=(P + 15) // 16 * 16)
+    for other in ("q", "k", "v", "out", "dout", "lse", "table", "buckets", "dtable", "ws", "dk"):
+        assert f"dq shares memory with {'workspace' if other == 'ws' else other}" in said(bwd, dq=at[other])
+        if other not in ("dtable", "dk"):
+            assert "dtable shares memory with" in said(bwd, dtable=at[other])
+        if other not in ("ws", "dk", "dtable"):
+            assert f"workspace shares memory with {other}" in said(bwd, ws=at[other])
+    assert "workspace shares memory with q" in said(bwd, ws=(at["q"] - need[1]) // 256 * 256 + 256)
+    assert said(bwd, ws=(at["q"] - need[1]) // 256 * 256).endswith(apart)
+
+    def norm(back, **moved):
+        names = "q k q_out k_out dq_out dk_out dq dk".split()
+        a = {x: (i + 4) * u for i, x in enumerate(names + "q_gain k_gain cosv sinv positions dq_gain dk_gain workspace".split())}
+        a.update(moved)
+        x = _native.NormRopeArgs(**{**a, **{x: _native.Rows(a[x], 40, 64, 40 * 64) for x in names}}, workspace_bytes=u, rows=40, dtype=1, device=4096, head_dim=64,
+                                 heads=2, kv_heads=2, n_positions=40, eps=1e-6)
+        assert (lib.dptm_qk_norm_rope_backward if back else lib.dptm_qk_norm_rope_forward)(C.addressof(x)) == _native.DPTM_EINVAL
+        return lib.dptm_layer_last_error().decode()
+
+    assert norm(False).endswith(apart) and norm(True).endswith(apart)
+    assert norm(False, q_out=4 * u).endswith(apart) and norm(True, dq=4 * u).endswith(apart) and norm(True, dq=8 * u).endswith(apart)
+    assert "q_out shares memory with q" in norm(False, q_out=4 * u + 40 * 128)
+    for x in ("q_gain", "k_gain", "cosv", "sinv", "positions"):
+        assert "q_out shares memory" in norm(False, **{x: 6 * u + 128}) and "dk shares memory" in norm(True, **{x: 11 * u + 2 * 40 * 128 - 16})
+    for x in ("dq_gain", "dk_gain", "workspace"):
+        for y in range(4, 17):
+            if y not in (6, 7):                                                         # q_out, k_out: the forward call's
+                assert "shares memory with" in norm(True, **{x: y * u}), (x, y)
+    assert "dq_gain shares memory with dk_gain" in norm(True, dq_gain=18 * u) and "aligned" in norm(True, dq_gain=17 * u + 2)
+    # the same memory in another order is not in place
+    x = _native.NormRopeArgs(q=_native.Rows(u, 40, 64, 40 * 64), q_out=_native.Rows(u, 40, 128, 64), cosv=2 * u, sinv=3 * u, rows=40, dtype=1, device=4096,
+                             head_dim=64, heads=2, kv_heads=0, n_positions=40, eps=1e-6)
+    assert lib.dptm_qk_norm_rope_forward(C.addressof(x)) == _native.DPTM_EINVAL and b"q_out shares memory with q" in lib.dptm_layer_last_error()
