@@ -12,8 +12,9 @@ strides of rows and heads do, if addresses and strides are multiples of 16 bytes
 elements are adjacent.  What a call writes shares no memory with what it reads, except where it says so.  Types are float32,
 bfloat16 and float16.  Calls go out on the current stream of the tensors' GPU and wait for nothing; what they need
 besides their results they take from torch's allocator, so calls on several streams and captured graphs do not share
-memory.  A plan may be dropped while calls on any stream still run; a captured graph needs its plans kept as it needs its inputs.  Gradients are explicit calls, as everywhere in this package: a tensor that requires grad is refused while autograd
-records.
+memory.  A plan may be dropped while calls on any stream still run; a captured graph needs its plans kept as it needs its
+inputs.  Gradients are explicit calls, as everywhere in this package: a tensor that requires grad is refused while autograd
+records, and so is one with a tangent of forward-mode differentiation.
 """
 from __future__ import annotations
 
@@ -24,6 +25,7 @@ from typing import Optional, Sequence, Tuple
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _native
 
@@ -99,6 +101,12 @@ def _refuse(t, what: str, name: str, dtype, device: int):
         raise ValueError(f"{what}: {name} is on {t.device}, not on cuda:{device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: {name} requires grad, and this call does not record; detach it or use no_grad")
+
+
+def _refuse_tangents(what: str, **tensors):
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{what}: {name} carries a tangent of forward-mode differentiation, which this call would lose")
 
 
 def _rows(t, what: str, name: str, dtype, device: int, heads: int, dim: int, rows: int):
@@ -269,6 +277,8 @@ def attention(q, k, v, plan: AttentionPlan, *, scale: Optional[float] = None, ta
     ``-inf``; a table entry at or below ``-2^100`` hides the pairs of its bucket.  ``out`` and ``lse`` may be given; rows of ``out`` behind the plan's are left as they are."""
     lib, what, dim = _native.load_library(), "attention", plan.head_dim
     code, device = _first(q, what)
+    if _forward_ad._current_level >= 0:         # inside dual_level: asking every tensor takes microseconds
+        _refuse_tangents(what, q=q, k=k, v=v, table=table, out=out, lse=lse)
     dtype, heads, nq, nk = q.dtype, plan.heads, plan.q_rows, plan.k_rows
     stream = _stream(device)
     host, dev = plan._words(what, device, stream)
@@ -298,6 +308,8 @@ def attention_backward(dout, q, k, v, out, lse, plan: AttentionPlan, *, scale: O
     Nothing is added through atomics: equal calls give equal bits."""
     lib, what, dim = _native.load_library(), "attention_backward", plan.head_dim
     code, device = _first(q, what)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents(what, dout=dout, q=q, k=k, v=v, out=out, lse=lse, table=table, dq=dq, dk=dk, dv=dv)
     dtype, heads, kv_heads, nq, nk = q.dtype, plan.heads, plan.kv_heads, plan.q_rows, plan.k_rows
     stream = _stream(device)
     host, dev = plan._words(what, device, stream)
@@ -348,6 +360,8 @@ def qk_norm_rope(q, k, cos, sin, *, q_gain=None, k_gain=None, positions=None, ep
     row NaN.  ``q_out`` / ``k_out`` may be given, also as the inputs themselves."""
     lib, what = _native.load_library(), "qk_norm_rope"
     code, device = _first(q, what)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents(what, q=q, k=k, cos=cos, sin=sin, q_gain=q_gain, k_gain=k_gain, q_out=q_out, k_out=k_out)
     dtype = q.dtype
     n, heads, kv_heads, dim, n_pos, shared = _norm_rope(what, q, k, cos, sin, q_gain, k_gain, positions, code, device)
     q_out, q_out_rows = _result(q_out, q, what, "q_out", device, heads, dim, n)
@@ -370,6 +384,8 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, cos, sin, *, q_gain=None, k_gain
     rows need a position inside the table too: one outside makes the gains' gradients NaN with its row."""
     lib, what = _native.load_library(), "qk_norm_rope_backward"
     code, device = _first(q, what)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents(what, dq_out=dq_out, dk_out=dk_out, q=q, k=k, cos=cos, sin=sin, q_gain=q_gain, k_gain=k_gain, dq=dq, dk=dk)
     dtype = q.dtype
     n, heads, kv_heads, dim, n_pos, shared = _norm_rope(what, q, k, cos, sin, q_gain, k_gain, positions, code, device)
     dq, dq_rows = _result(dq, q, what, "dq", device, heads, dim, n)

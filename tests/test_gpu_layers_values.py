@@ -200,6 +200,32 @@ def test_float16_gradients_far_from_one(lens, k_lens, dim, given, size, size_v, 
         assert off <= 1.04 * most, f"{name}: {off / most:.3g} of what is left to it"
 
 
+def test_tensors_of_forward_mode_differentiation_are_refused():
+    """Their tangents would be lost without a word."""
+    import torch.autograd.forward_ad as fwad
+
+    rng = np.random.default_rng(94)
+    q, k, v = (tensor(rng, "f32", 40, 2, 32) for _ in range(3))
+    plan = layers.AttentionPlan([40], heads=2, head_dim=32)
+    cos, sin = layers.rotary_table(40, 32)
+    gain = torch.ones(32, device="cuda")
+    want, _ = layers.attention(q, k, v, plan)
+    with fwad.dual_level():
+        got, _ = layers.attention(q, k, v, plan)             # nothing to lose
+        assert torch.equal(got, want)
+        dual = fwad.make_dual(v, torch.ones_like(v))
+        with pytest.raises(ValueError, match="tangent"):
+            layers.attention(q, k, dual, plan)
+        with pytest.raises(ValueError, match="tangent"):
+            layers.qk_norm_rope(dual, k, cos, sin)
+        with pytest.raises(ValueError, match="tangent"):
+            layers.qk_norm_rope(q, k, cos, sin, q_gain=fwad.make_dual(gain, gain))
+        with pytest.raises(ValueError, match="tangent"):
+            layers.attention_backward(dual, q, k, v, got, torch.zeros(2, 40, device="cuda"), plan)
+        with pytest.raises(ValueError, match="tangent"):
+            layers.qk_norm_rope_backward(q, dual, q, k, cos, sin)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("rows,keys,heads,dim", [(1500, 1500, 2, 32), (130, 400, 2, 64), (53, 2100, 4, 64), (300, 300, 48, 128)])
 def test_bias_gradient_of_listed_positions(dtype, rows, keys, heads, dim):
