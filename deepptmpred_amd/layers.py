@@ -155,6 +155,24 @@ def _lengths(a, name: str) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=np.int32)
 
 
+def _whole(x, what: str, name: str, least: int = -2 ** 31, most: int = 2 ** 31 - 1) -> int:
+    """``x`` as a whole number of 32 bits (a ctypes field would drop the bits above them)."""
+    try:
+        n = int(x)
+    except (TypeError, ValueError, OverflowError):
+        n = None
+    if n is None or n != x or not least <= n <= most:
+        raise ValueError(f"{what}: {name} must be a whole number in {least}..{most}, got {x!r}")
+    return n
+
+
+def _f32(x, what: str, name: str) -> float:
+    """``x``, which an argument block holds in 32 bits."""
+    if not abs(x) < 3.4e38:
+        raise ValueError(f"{what}: {name} must be a number that float32 holds, got {x!r}")
+    return x
+
+
 class AttentionPlan:
     """The layout of one batch: lengths, window, heads, and the work list made from them.  Kept and used for every
     layer and step of that batch; it only holds what it was made with, so any number of calls may use it at once.
@@ -179,9 +197,18 @@ class AttentionPlan:
             pos = _lengths(q_positions, "q_positions")
             if len(pos) != int(q.sum(dtype=np.int64)):
                 raise ValueError(f"AttentionPlan: {len(pos)} positions for {int(q.sum(dtype=np.int64))} query rows")
-        left, right = window
-        d = _native.AttentionDesc(heads, kv_heads if kv_heads is not None else heads, head_dim, max(-1, min(int(left), 2 ** 31 - 1)),
-                                  max(-1, min(int(right), 2 ** 31 - 1)), sinks, 1 if training else 0)
+        what, far = "AttentionPlan", 2 ** 31 - 1
+        try:
+            left, right = window
+        except TypeError:
+            raise ValueError(f"{what}: window must be a pair (left, right), got {window!r}") from None
+        left, right = (max(-1, min(_whole(w, what, "window", -2 ** 63, 2 ** 63), far)) for w in (left, right))
+        d = _native.AttentionDesc(_whole(heads, what, "heads"), _whole(heads if kv_heads is None else kv_heads, what, "kv_heads"),
+                                  _whole(head_dim, what, "head_dim"), left, right, min(_whole(sinks, what, "sinks", most=2 ** 63), far), 1 if training else 0)
+        if device is not None:
+            device = _device(device)
+            if device.type != "cuda":
+                raise ValueError(f"{what}: device must be a GPU, or None for a plan that stays on the host, not {device}")
         words = np.empty(4096, dtype=np.int32)
         while True:
             n = _check(lib.dptm_attention_plan(C.byref(d), q.ctypes.data, k.ctypes.data, None if pos is None else pos.ctypes.data,
@@ -190,10 +217,10 @@ class AttentionPlan:
                 break
             words = np.empty(n, dtype=np.int32)
         self.words = words[:n]
-        self.heads, self.kv_heads, self.head_dim = d.heads, d.kv_heads, head_dim
+        self.heads, self.kv_heads, self.head_dim = d.heads, d.kv_heads, d.head_dim
         self.q_rows, self.k_rows = int(q.sum(dtype=np.int64)), int(k.sum(dtype=np.int64))
         self.training = bool(training)
-        self.device = None if device is None else _device(device)
+        self.device = device
         self.device_words = None if device is None else torch.from_numpy(self.words).to(self.device)
         self._at = None if device is None else (self.words.ctypes.data, self.device_words.data_ptr())
         self._streams = set() if device is None else {_stream(self.device.index)}
@@ -224,6 +251,7 @@ def relative_buckets(n_buckets: int, max_distance: int, bidirectional: bool = Tr
     distance each, the others by the logarithm of the distance up to ``max_distance``; ``bidirectional``: the upper half of
     the buckets for keys behind the query, otherwise those count as distance 0.  Borders are found in whole numbers.
     ``device=None``: a NumPy array."""
+    n_buckets, max_distance = (_whole(x, "relative_buckets", name) for x, name in ((n_buckets, "n_buckets"), (max_distance, "max_distance")))
     side = n_buckets // 2 if bidirectional else n_buckets
     near = side // 2
     if near < 1 or n_buckets > 64 or (bidirectional and n_buckets % 2):
@@ -246,8 +274,9 @@ def relative_buckets(n_buckets: int, max_distance: int, bidirectional: bool = Tr
 
 def rotary_table(n_positions: int, head_dim: int, base: float = 10000.0, device=0):
     """Cosine and sine of ``position * base^(-2 i / head_dim)``, float32 ``[n_positions, head_dim / 2]`` each; angles in 64 bits."""
-    if n_positions < 0 or head_dim < 2 or head_dim % 2:
-        raise ValueError("rotary_table: bad sizes")
+    n_positions, head_dim = _whole(n_positions, "rotary_table", "n_positions"), _whole(head_dim, "rotary_table", "head_dim")
+    if n_positions < 0 or head_dim < 2 or head_dim % 2 or not 0 < base < float("inf"):
+        raise ValueError("rotary_table: bad sizes, or a base that is not positive and finite")
     angle = np.arange(n_positions, dtype=np.float64)[:, None] * float(base) ** (-np.arange(0, head_dim, 2, dtype=np.float64) / head_dim)
     cos, sin = np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
     return torch.from_numpy(cos).to(_device(device)), torch.from_numpy(sin).to(_device(device))
@@ -294,7 +323,7 @@ def attention(q, k, v, plan: AttentionPlan, *, scale: Optional[float] = None, ta
         *_rows(k, what, "k", dtype, device, plan.kv_heads, dim, nk), *_rows(v, what, "v", dtype, device, plan.kv_heads, dim, nk),
         *out_rows, _flat(lse, what, "lse", (heads, nq), torch.float32, device),
         table_at, buckets_at, hold.data_ptr() if n else 0, n, stream, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0,
-        code, device, n_buckets, reach, dim ** -0.5 if scale is None else scale)
+        code, device, n_buckets, reach, dim ** -0.5 if scale is None else _f32(scale, what, "scale"))
     rc = lib.dptm_attention_forward(block.attention_at)
     if rc:
         _check(rc, what)
@@ -327,7 +356,7 @@ def attention_backward(dout, q, k, v, out, lse, plan: AttentionPlan, *, scale: O
         *_rows(out, what, "out", dtype, device, heads, dim, nq), _flat(lse, what, "lse", (heads, nq), torch.float32, device),
         table_at, buckets_at, hold.data_ptr() if n else 0, n, stream,
         *_rows(dout, what, "dout", dtype, device, heads, dim, nq), *dq_rows, *dk_rows, *dv_rows,
-        dtable.data_ptr() if n_buckets else 0, code, device, n_buckets, reach, dim ** -0.5 if scale is None else scale)
+        dtable.data_ptr() if n_buckets else 0, code, device, n_buckets, reach, dim ** -0.5 if scale is None else _f32(scale, what, "scale"))
     rc = lib.dptm_attention_backward(block.attention_at)
     if rc:
         _check(rc, what)
@@ -370,7 +399,7 @@ def qk_norm_rope(q, k, cos, sin, *, q_gain=None, k_gain=None, positions=None, ep
     _NORM_ROPE.pack_into(
         block.norm_rope, 0, *_rows(q, what, "q", dtype, device, heads, dim, n), *_rows(k, what, "k", dtype, device, kv_heads, dim, n),
         *q_out_rows, *k_out_rows, *shared, _stream(device), *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0, 0, 0, n, code, device, dim, heads, kv_heads, n_pos,
-        1 if interleaved else 0, eps)
+        1 if interleaved else 0, _f32(eps, what, "eps"))
     rc = lib.dptm_qk_norm_rope_forward(block.norm_rope_at)
     if rc:
         _check(rc, what)
@@ -399,7 +428,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, cos, sin, *, q_gain=None, k_gain
             *_NO_ROWS, *_NO_ROWS, *shared, _stream(device),
             *_rows(dq_out, what, "dq_out", dtype, device, heads, dim, n), *_rows(dk_out, what, "dk_out", dtype, device, kv_heads, dim, n),
             *dq_rows, *dk_rows, 0 if dq_gain is None else dq_gain.data_ptr(), 0 if dk_gain is None else dk_gain.data_ptr(), at, size, n, code, device, dim,
-            heads, kv_heads, n_pos, 1 if interleaved else 0, eps)
+            heads, kv_heads, n_pos, 1 if interleaved else 0, _f32(eps, what, "eps"))
 
     size, hold = 0, None
     if dq_gain is not None or dk_gain is not None:

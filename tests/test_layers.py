@@ -510,3 +510,29 @@ def test_every_buffer_that_a_call_writes_lies_apart():
     x = _native.NormRopeArgs(q=_native.Rows(u, 40, 64, 40 * 64), q_out=_native.Rows(u, 40, 128, 64), cosv=2 * u, sinv=3 * u, rows=40, dtype=1, device=4096,
                              head_dim=64, heads=2, kv_heads=0, n_positions=40, eps=1e-6)
     assert lib.dptm_qk_norm_rope_forward(C.addressof(x)) == _native.DPTM_EINVAL and b"q_out shares memory with q" in lib.dptm_layer_last_error()
+
+
+def test_numbers_that_the_argument_blocks_do_not_hold():
+    """Sizes are refused, not cut to 32 bits; more first tokens, or a wider window, than any sequence is long are all of them."""
+    ok = dict(heads=4, head_dim=64, device=None)
+    for bad in (dict(heads=2 ** 32 + 4), dict(kv_heads=2 ** 32 + 4), dict(head_dim=2 ** 32 + 64), dict(heads=2.5), dict(sinks=1.5), dict(sinks=-2 ** 40),
+                dict(window=(1.5, 0)), dict(window=(float("inf"), 0)), dict(window=3), dict(window=(None, 0)), dict(heads=None), dict(device="cpu")):
+        with pytest.raises(ValueError, match="AttentionPlan"):
+            layers.AttentionPlan([5], **{**ok, **bad})
+    every = layers.AttentionPlan([500], window=(3, 0), sinks=500, **ok).words
+    for many in (2 ** 32 + 1, 2 ** 31, 10 ** 6):
+        w = layers.AttentionPlan([500], window=(3, 0), sinks=many, **ok).words
+        assert np.array_equal(w[w[13]:w[18]], every[every[13]:every[18]]) and w[7] >= 500
+    w = layers.AttentionPlan([5], window=(2 ** 40, -2 ** 40), **ok).words
+    assert list(w[5:7]) == [2 ** 29] * 2
+    assert layers.AttentionPlan([5], **{**ok, "heads": np.int64(4), "window": (np.int32(2), 2.0)}).words[5] == 2
+    for bad in ((32.5, 128), (32, 128.5), (2 ** 40, 128), (32, "x")):
+        with pytest.raises(ValueError):
+            layers.relative_buckets(*bad, device=None)
+    for bad in ((5.5, 64, 1e4), (5, 64.5, 1e4), (5, 64, -3.0), (5, 64, 0.0), (5, 64, float("nan"))):
+        with pytest.raises(ValueError):
+            layers.rotary_table(*bad, device="cpu")
+    for bad in (1e39, -1e39, float("inf"), float("nan"), 10 ** 400):
+        with pytest.raises(ValueError, match="eps"):
+            layers._f32(bad, "qk_norm_rope", "eps")
+    assert layers._f32(np.float32(0.125), "attention", "scale") == 0.125
