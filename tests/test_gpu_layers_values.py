@@ -7,7 +7,7 @@ torch = pytest.importorskip("torch")
 
 from deepptmpred_amd import layers  # noqa: E402
 from oracle import layers_ref as R  # noqa: E402
-from test_gpu_layers import host, tensor, within  # noqa: E402
+from test_gpu_layers import attend, host, tensor, within  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -247,3 +247,66 @@ def test_bias_gradient_of_listed_positions(dtype, rows, keys, heads, dim):
     alone, off = (np.sqrt(np.mean((x - value) ** 2)) for x in (rounded, host(got[3])))
     print(f"dtable: {off / alone:.3f} times the error of rounding it")
     assert off <= 1.05 * alone
+
+
+# five sequences of 64 heads fill the card: tiles of 128 rows in the forward kernel, four wavefronts in both backward ones; fewer heads take
+# tiles of 64 and two wavefronts
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("buckets", [None, (16, 50, True)])
+@pytest.mark.parametrize("heads,kinds", [(64, (0, 4, 4)), (20, (1, 2, 2))])
+def test_kernels_that_large_batches_take(dtype, dim, buckets, heads, kinds):
+    """The plan says which kernels ran; rows in order, ragged lengths, a window with first tokens."""
+    plan = attend(dtype, dim, [256, 250, 199, 128, 1], heads=heads, kv_heads=heads, window=(90, 40), sinks=2, buckets=buckets, seed=97, packed=True)
+    assert tuple(int(x) for x in plan.words[[11, 19, 22]]) == kinds
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_kernels_that_large_batches_take_with_shared_heads(dtype, dim):
+    plan = attend(dtype, dim, [256] * 4, heads=128, kv_heads=64, window=(-1, 0), buckets=(16, 50, False), seed=98)
+    assert tuple(int(x) for x in plan.words[[11, 19, 22]]) == (0, 4, 4)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lens,heads,kinds", [([256, 250, 199, 128, 1], 64, (0, 4, 4)), ([200, 190], 40, (1, 2, 2))])
+def test_hidden_places_in_the_kernels_that_large_batches_take(dtype, lens, heads, kinds):
+    """Keys, values, queries and gradients of NaN and infinity reach what sees them and nothing else."""
+    rng = np.random.default_rng(99)
+    n, window = sum(lens), (9, 4)
+    q, k, v, dout = (tensor(rng, dtype, n, heads, 64) for _ in range(4))
+    plan = layers.AttentionPlan(lens, heads=heads, head_dim=64, window=window)
+    assert tuple(int(x) for x in plan.words[[11, 19, 22]]) == kinds
+    out, lse = layers.attention(q, k, v, plan)
+    want = R.attention(host(q), host(k), host(v), lens, lens, window, dout=host(dout), kernel_out=host(out), dtype=dtype)
+    start = np.repeat(np.cumsum([0] + lens[:-1]), lens)
+    p, j = np.arange(n)[:, None], np.arange(n)[None]
+    see = (j <= p + window[1]) & (j >= p - window[0]) & (start[:, None] == start[None])
+    # keys and values; 140 and 131 lie in a tile with rows that do not see them
+    k2, v2 = k.clone(), v.clone()
+    k2[140], v2[131, :, 3] = NAN, INF
+    out2, lse2 = layers.attention(q, k2, v2, plan)
+    dq, dk, dv, _ = layers.attention_backward(dout, q, k2, v2, out2, lse2, plan)
+    met = see[:, [140, 131]].any(1)
+    for t, name in ((out2, "out"), (dq, "dq")):
+        rows_within(t, want, name, ~met)
+        assert not np.isfinite(host(t)[met]).all(axis=(1, 2)).any()
+    rows_within(lse2.T, {"lse": (want["lse"][0].T, want["lse"][1].T)}, "lse", ~see[:, 140])
+    rows_within(dk, want, "dk", ~see[met].any(0))
+    rows_within(dv, want, "dv", ~see[see[:, 140]].any(0))
+    # a row
+    q2, dout2 = q.clone(), dout.clone()
+    q2[150], dout2[150] = NAN, INF
+    out3, lse3 = layers.attention(q2, k, v, plan)
+    dq, dk, dv, _ = layers.attention_backward(dout2, q2, k, v, out3, lse3, plan)
+    rows_within(out3, want, "out", np.arange(n) != 150)
+    rows_within(dq, want, "dq", np.arange(n) != 150)
+    for t, name in ((dk, "dk"), (dv, "dv")):
+        rows_within(t, want, name, ~see[150])
+        assert not np.isfinite(host(t)[see[150]]).any()
+
+
+def test_kernels_that_large_batches_take_with_the_most_shared_memory():
+    """fp32 heads of 128 with the largest bias and four wavefronts in both backward kernels, rows in order."""
+    plan = attend("f32", 128, [256] * 4, heads=64, kv_heads=64, window=(200, 100), buckets=(64, 1024, True), seed=100)
+    assert tuple(int(x) for x in plan.words[[11, 19, 22]]) == (0, 4, 4)
