@@ -304,9 +304,10 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, POS>)) void attn_dq_kernel
         }
     }
     if (redo) {
-        float t[16 * DT];
-        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, &over, item, head, rowc, rw.pos, delta, bias, h);
+        float t[16 * DT], sum;       // `over` itself would live in memory from the start
+        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, &sum, item, head, rowc, rw.pos, delta, bias, h);
         take<DT>(acc, t);
+        over = sum;
         lift = 0;
     }
     if constexpr (sizeof(T) == 2) {
@@ -638,13 +639,20 @@ __global__ __launch_bounds__(NW * 64, D * sizeof(T) <= 128 || PART != kBoth ? 2 
                     }
                     if constexpr (SUMS) {
                         if (near) {
-                            f32x16_a d = p;
-                            if (Lift<T>::kOn && lift.moved) Lift<T>::down(d, lift.e - Lift<T>::kFirst);     // keys meet in a sum
-                            float* mine = shear + 32 + (lane & 31) * kShearRow + 4 * h;
+                            auto put_sheared = [&](const f32x16_a& d) {
+                                float* mine = shear + 32 + (lane & 31) * kShearRow + 4 * h;
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) {
-                                const V4<float> y{d[4 * x], d[4 * x + 1], d[4 * x + 2], d[4 * x + 3]};
-                                *reinterpret_cast<V4<float>*>(mine + 8 * x) = y;
+                                for (int x = 0; x < 4; ++x) {
+                                    const V4<float> y{d[4 * x], d[4 * x + 1], d[4 * x + 2], d[4 * x + 3]};
+                                    *reinterpret_cast<V4<float>*>(mine + 8 * x) = y;
+                                }
+                            };
+                            if (Lift<T>::kOn && lift.moved) {     // keys meet in a sum
+                                f32x16_a d = p;
+                                Lift<T>::down(d, lift.e - Lift<T>::kFirst);
+                                put_sheared(d);
+                            } else {
+                                put_sheared(p);
                             }
                         } else {
                             float sum = 0.f;
