@@ -192,8 +192,10 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs a, int
     }
     if constexpr (GRAD) {
         // the block's threads with one chunk: kThreads / D threads a column for every so many of them, in order of their index
-        // (one thread a column walks over 4096 / D of them: at heads of 32 two thirds of a short call's last 3 us)
-        __shared__ float sums[kThreads * 17], some[kThreads];
+        // (one thread a column walks over 4096 / D of them: at heads of 32 two thirds of a short call's last 3 us).  In 64 bits: in 32
+        // the gains' gradients were 1.7 times as far off as those of elementary operations (now 1.3: a thread's own sums)
+        __shared__ float sums[kThreads * 17];
+        __shared__ double some[kThreads];
         constexpr int kSplit = kThreads / D;
         const int col = threadIdx.x % D, c = col % (D / 2) / 8, at = col % 8 + (col < D / 2 ? 0 : 8);
 #pragma unroll
@@ -206,15 +208,15 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs a, int
                 sums[threadIdx.x * 17 + 8 + e] = d1[t][e];
             }
             __syncthreads();
-            float x = 0.f;
+            double x = 0.0;
 #pragma unroll 8
-            for (int i = c + L * (threadIdx.x / D); i < kThreads; i += L * kSplit) x += sums[i * 17 + at];
+            for (int i = c + L * (threadIdx.x / D); i < kThreads; i += L * kSplit) x += (double)sums[i * 17 + at];
             some[threadIdx.x] = x;
             __syncthreads();
             if (threadIdx.x < D) {
 #pragma unroll
                 for (int k = 1; k < kSplit; ++k) x += some[k * D + col];
-                (t ? a.part[1] : a.part[0])[(int64_t)blockIdx.x * D + col] = x;
+                (t ? a.part[1] : a.part[0])[(int64_t)blockIdx.x * D + col] = (float)x;
             }
         }
     }
