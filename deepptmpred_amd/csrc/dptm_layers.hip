@@ -434,6 +434,7 @@ int make_plan(const dptm_attention_desc& d, const int32_t* q_len, const int32_t*
 
 int check_plan(const char* who, const int32_t* plan, const int32_t* plan_dev) {
     if (!plan || !plan_dev) return fail(DPTM_EINVAL, std::string(who) + ": NULL plan");
+    if ((reinterpret_cast<uintptr_t>(plan) | reinterpret_cast<uintptr_t>(plan_dev)) & 3) return fail(DPTM_EINVAL, std::string(who) + ": plan must be 4-byte aligned");
     if (plan[kPlanMagicAt] != kPlanMagic || plan[kPlanCheck] != (int32_t)header_sum(plan))
         return fail(DPTM_EINVAL, std::string(who) + ": not a plan of dptm_attention_plan");
     return DPTM_OK;
@@ -709,10 +710,12 @@ int dptm_qk_norm_rope_forward(const dptm_norm_rope_args* x) try {
     return on_exception("dptm_qk_norm_rope_forward");
 }
 
-int64_t dptm_qk_norm_rope_workspace(const dptm_norm_rope_args* x) {
-    if (!x || !good_dim(x->head_dim) || x->rows < 0 || x->heads < 0 || x->kv_heads < 0)
+int64_t dptm_qk_norm_rope_workspace(const dptm_norm_rope_args* x) try {
+    if (!x || !good_dim(x->head_dim) || x->rows < 0 || x->rows > INT32_MAX || x->heads < 0 || x->heads > 4096 || x->kv_heads < 0 || x->kv_heads > 4096)
         return fail(DPTM_EINVAL, "dptm_qk_norm_rope_workspace: bad sizes");
     return (int64_t)norm_rope_blocks(x->rows, x->heads + x->kv_heads, x->head_dim) * x->head_dim * 2 * 4;
+} catch (...) {
+    return on_exception("dptm_qk_norm_rope_workspace");
 }
 
 int dptm_qk_norm_rope_backward(const dptm_norm_rope_args* x) try {

@@ -431,7 +431,7 @@ int64_t dptm_attention_plan(const dptm_attention_desc* d, const int32_t* q_len, 
  *                    ([n_buckets][heads], of the tensors' type) that is added to the scaled score of a key d = j - p_i away,
  *                    distances beyond max_distance counting as it.  1 to 64 buckets, max_distance 0 to 1024; an entry outside
  *                    0..n_buckets-1 is clamped into it.  A table entry at or below -2^100 (-inf, or the lowest value of
- *                    float32 and bfloat16) hides the pairs of its bucket
+ *                    float32 and bfloat16) hides the pairs of its bucket; the others, divided by the scale, have to lie in float32's range
  *   workspace        dptm_attention_workspace bytes, 256-byte aligned, contents of no meaning before or after
  *   dout .. dtable   the backward call only; dtable [n_buckets][heads] with a bias
  *   scale            of the scores, 2^-64..2^64

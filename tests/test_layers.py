@@ -536,3 +536,22 @@ def test_numbers_that_the_argument_blocks_do_not_hold():
         with pytest.raises(ValueError, match="eps"):
             layers._f32(bad, "qk_norm_rope", "eps")
     assert layers._f32(np.float32(0.125), "attention", "scale") == 0.125
+
+
+def test_c_sizes_and_addresses_at_their_limits():
+    """Sizes that no call takes have no workspace, and a plan at an odd address is no plan."""
+    lib = _native.load_library()
+
+    def workspace(**more):
+        x = _native.NormRopeArgs(**{**dict(rows=100, heads=4, kv_heads=4, head_dim=64), **more})
+        return lib.dptm_qk_norm_rope_workspace(C.addressof(x))
+
+    assert workspace() > 0 and workspace(rows=0) > 0 and workspace(rows=2 ** 31 - 1) == 1536 * 64 * 8
+    for bad in (dict(rows=2 ** 31), dict(rows=2 ** 62), dict(heads=2 ** 31 - 1), dict(kv_heads=4097), dict(head_dim=48)):
+        assert workspace(**bad) == _native.DPTM_EINVAL and b"sizes" in lib.dptm_layer_last_error()
+    plan = layers.AttentionPlan([10], heads=2, head_dim=64, device=None)
+    P = plan.words.ctypes.data
+    good = rows_of(10, 2, 64)
+    x = _native.AttentionArgs(plan=P, plan_dev=P + 2, q=good, k=good, v=good, out=rows_of(10, 2, 64, at=1 << 24), lse=1 << 25, dtype=1, scale=0.1, device=4096,
+                              workspace=1 << 26, workspace_bytes=1 << 20)
+    assert lib.dptm_attention_forward(C.addressof(x)) == _native.DPTM_EINVAL and b"aligned" in lib.dptm_layer_last_error()
