@@ -122,18 +122,37 @@ struct Tile {
 template <typename T> __device__ __forceinline__ void after_reads() {
     if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
 }
+// the row fragments of one lane.  Left to itself the compiler keeps the places of all steps over the loop around them: eight registers
+// with 16-bit heads of 128, whose kernels spill operands for them.  There they are formed from one, which it cannot see through.
+template <typename T, int D>
+struct RowFrags {
+    static constexpr bool kFresh = sizeof(T) == 2 && D == 128;
+    int row, h;
+    unsigned place = 0;
+    __device__ __forceinline__ RowFrags(int row, int h) : row(row), h(h) {
+        if constexpr (kFresh) {
+            place = row * (D * (int)sizeof(T)) + ((h ^ Tile<T, D>::swz(row)) << 4);      // of step 0; step s flips bits 5 to 7
+            asm volatile("" : "+v"(place));
+        }
+    }
+    __device__ __forceinline__ V8<T> get(const char* t, int step) const {
+        if constexpr (kFresh) return *reinterpret_cast<const V8<T>*>(t + (place ^ (unsigned)(step << 5)));
+        else return Tile<T, D>::row_frag(t, row, step, h);
+    }
+};
 // c0 += A0 B0 and c1 += A1 B1 over the whole head dimension, A rows row0 .. row0 + 31 of two tiles; MOST steps at a time
 template <typename T, int D, int MOST>
 __device__ __forceinline__ void row_products(f32x16_a& c0, f32x16_a& c1, const char* t0, const char* t1, int row0, const V8<T> (&b0)[D / 16],
                                              const V8<T> (&b1)[D / 16], int lane) {
     constexpr int G = D / 16 < MOST ? D / 16 : MOST;
+    const RowFrags<T, D> rows(row0 + (lane & 31), lane >> 5);
 #pragma unroll
     for (int g = 0; g < D / 16; g += G) {
         V8<T> f0[G], f1[G];
 #pragma unroll
         for (int s = 0; s < G; ++s) {
-            f0[s] = Tile<T, D>::row_frag(t0, row0 + (lane & 31), g + s, lane >> 5);
-            f1[s] = Tile<T, D>::row_frag(t1, row0 + (lane & 31), g + s, lane >> 5);
+            f0[s] = rows.get(t0, g + s);
+            f1[s] = rows.get(t1, g + s);
         }
         after_reads<T>();
 #pragma unroll
@@ -147,11 +166,12 @@ __device__ __forceinline__ void row_products(f32x16_a& c0, f32x16_a& c1, const c
 template <typename T, int D, int MOST>
 __device__ __forceinline__ void row_product(f32x16_a& c0, const char* t0, int row0, const V8<T> (&b0)[D / 16], int lane) {
     constexpr int G = D / 16 < MOST ? D / 16 : MOST;
+    const RowFrags<T, D> rows(row0 + (lane & 31), lane >> 5);
 #pragma unroll
     for (int g = 0; g < D / 16; g += G) {
         V8<T> f0[G];
 #pragma unroll
-        for (int s = 0; s < G; ++s) f0[s] = Tile<T, D>::row_frag(t0, row0 + (lane & 31), g + s, lane >> 5);
+        for (int s = 0; s < G; ++s) f0[s] = rows.get(t0, g + s);
         after_reads<T>();
 #pragma unroll
         for (int s = 0; s < G; ++s) mma(c0, f0[s], b0[g + s]);

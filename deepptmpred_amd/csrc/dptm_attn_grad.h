@@ -66,16 +66,16 @@ template <typename T> struct Lift {
     }
 };
 
-// A wavefront's rows of dq once more, pair by pair (see Stage::not_finite); *over: the sum of a row's dS.
+// A wavefront's rows of dq once more, pair by pair (see Stage::not_finite); `mend`: the row's delta takes on the sum of its dS.
 template <typename T, int D, int DT, bool BIAS>
-DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, float* over, int item, int head, int row, int pos, float delta, const float* bias, int h) {
+DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, bool mend, int item, int head, int row, int pos, const float* bias, int h) {
     const QItem& it = reinterpret_cast<const QItem*>(a.plan + a.items_at)[item];
     const Window win{a.left, a.right, a.sinks};
     const int hk = head / a.group;
     const int64_t qr = (int64_t)it.q0 + row;
     const T* q = row_ptr<T>(a.q, qr, head);
     const T* g = row_ptr<T>(a.dout, qr, head);
-    const float ref = lse_log2(a.lse[(int64_t)head * a.q_rows + qr]);
+    const float ref = lse_log2(a.lse[(int64_t)head * a.q_rows + qr]), delta = a.delta[(int64_t)head * a.q_rows + qr];
 #pragma unroll 1
     for (int i = 0; i < 16 * DT; ++i) acc[i] = 0.f;
     float sum = 0.f;
@@ -91,7 +91,7 @@ DPTM_COLD void dq_by_pairs(const AttnArgs& a, float* acc, float* over, int item,
 #pragma unroll 1
         for (int i = 0; i < 16 * DT; ++i) acc[i] += see ? ds * (float)k[reg_col<D>(i >> 4, i & 15, h)] : 0.f;
     }
-    *over = sum;
+    if (mend) a.delta[(int64_t)head * a.q_rows + qr] = delta + sum;
 }
 
 // rows of a tile in LDS: fewer than in the forward pass where a wavefront's own operands and sums take the registers
@@ -295,6 +295,10 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, POS>)) void attn_dq_kernel
         if (walk.more()) fetch(walk);
     }
     over = off(over), below = off(below), above = off(above);
+    // this lane's row once more, from the lane's number: kept over the loop it would take the place of operands (heads of 128)
+    const int mine = 32 * w + (__lane_id() & 31);
+    const bool first_half = __lane_id() < 32;
+    float* const delta_at = a.delta + (int64_t)head * a.q_rows + it.q0 + mine;
     bool redo = __syncthreads_or((int)odd);
     if constexpr (BIAS || Lift<T>::kOn) {
         const bool lost = !finite(over + sum_of_all(acc));
@@ -303,19 +307,19 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, POS>)) void attn_dq_kernel
             if constexpr (BIAS) redo |= table_hides<T>(a.bias, a.heads, head, 1);
         }
     }
-    if (redo) {
-        float t[16 * DT], sum;       // `over` itself would live in memory from the start
-        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, &sum, item, head, rowc, rw.pos, delta, bias, h);
+    if (__builtin_expect(redo, 0)) {
+        float t[16 * DT];
+        const int i = min(mine, it.nq - 1);
+        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, sizeof(T) == 2 && first_half && mine < it.nq, item, head, i,
+                                    row_position(a.plan, a.has_pos, a.pos_at, it.pos0, it.q0, i), bias, first_half ? 0 : 1);
         take<DT>(acc, t);
-        over = sum;
         lift = 0;
+    } else if (sizeof(T) == 2 && first_half && mine < it.nq) {
+        *delta_at = delta + over;
     }
-    if constexpr (sizeof(T) == 2) {
-        if (h == 0 && row < it.nq) a.delta[(int64_t)head * a.q_rows + qr] = delta + over;
-    }
-    if (row < it.nq) {
+    if (mine < it.nq) {
         const float by = off(a.scale);
-        T* o = const_cast<T*>(row_ptr<T>(a.dq, (int64_t)it.q0 + row, head));
+        T* o = const_cast<T*>(row_ptr<T>(a.dq, (int64_t)it.q0 + mine, head)) + (first_half ? 0 : 4);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -323,7 +327,7 @@ __global__ __launch_bounds__(NW * 64, (kDqWaves<T, D, POS>)) void attn_dq_kernel
                 V4<T> y;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[e] = (T)(acc[d][4 * x + e] * by);
-                *reinterpret_cast<V4<T>*>(o + 32 * d + 8 * x + 4 * h) = y;
+                *reinterpret_cast<V4<T>*>(o + 32 * d + 8 * x) = y;
             }
     }
     if constexpr (POS) {

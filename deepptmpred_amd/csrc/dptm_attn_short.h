@@ -102,15 +102,19 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
     V8<T> kf[ST], vf[ST];
 #pragma unroll
     for (int s = 0; s < ST; ++s) vf[s] = global_frag<T>(vrow, s, h);
-    if constexpr (BIAS) load_bias<T>(bias, a.bias, 1.f / a.scale, a.heads, head, tid, NT);
+    bool hides = false;                                     // the table hides a bucket of this head
+    if constexpr (BIAS) {
+        hides = table_hides<T>(a.bias, a.heads, head, 1);
+        load_bias<T>(bias, a.bias, 1.f / a.scale, a.heads, head, tid, NT);
+    }
     sq.store(qt, tid);
     sg.store(gt, tid);
     sk.store(kt, tid);
     unsigned odd = 0;
     const bool whole = Sight(win, pos0, pos0 + nq - 1).all(0, nk);
-    if (BIAS | !whole) odd = sq.not_finite() | sg.not_finite() | sk.not_finite();
+    if (hides | !whole) odd = sq.not_finite() | sg.not_finite() | sk.not_finite();
     if (h == 0) rowref[mine] = mine < nq ? lse_log2(lse) * (kLseLast<T> ? -1.f : -1.f / c) : kMinusInf;      // rows behind the last weigh nothing
-    bool redo = __syncthreads_or((int)odd) && (!BIAS || !whole || table_hides<T>(a.bias, a.heads, head, 1));
+    bool redo = __syncthreads_or((int)odd);
     auto delta_of_out = [&] { return dot_rows<T, D>(row_ptr<T>(a.dout, qr, head), row_ptr<T>(a.out, qr, head)); };
     if (redo) {
         if (h == 0 && mine < nq) a.delta[(int64_t)head * a.q_rows + qr] = delta_of_out();
@@ -139,9 +143,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
     auto row_sums = [&](const f32x16_a& x, int u) {
         const float sum = Lift<T>::off_first(lane_sums(x, lane));
         if ((lane & 16) == 0) rowdelta[kRows * w + 32 * u + reg_row(lane & 15) + 4 * h] = sum;
-        return sum;
     };
-    bool lost = false;                                      // a row's delta is not finite
     f32x16_a dk[DT], dv[DT], weight[N], d_s[N];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -188,15 +190,16 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
             cols.read(gt, r0, lane);
             cols.product(dv, s);
         }
-        lost |= !finite(row_sums(p, u));
+        row_sums(p, u);
     }
-    // (a value row of NaN, say): what it is multiplied with is zero where pairs are hidden, but the product is not
-    lost = __syncthreads_or((int)lost);
-    Lift<T> lift_k, lift_q;      // of dk and dq; weight and d_s hold what is lifted by the first power, and so do dv's sums
-    bool hides = false;
+    __syncthreads();
+    // A row's delta is not finite (a value row of NaN, say): what it is multiplied with is zero where pairs are hidden, but the product
+    // is not.  All wavefronts read the same sums, so they agree
+    const int of_row = min(lane, kRows - 1);
+    const bool lost = __ballot(!finite(rowdelta[of_row] + (N == 2 ? rowdelta[kRows + of_row] : 0.f)));
     if constexpr (BIAS) {
-        if (lost && table_hides<T>(a.bias, a.heads, head, 1)) {
-            hides = true;
+        if (lost & hides) {
+            __syncthreads();
 #pragma unroll
             for (int u = 0; u < N; ++u) {
                 hide_buckets(weight[u], u);
@@ -208,6 +211,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
             __syncthreads();
         }
     }
+    Lift<T> lift_k, lift_q;      // of dk and dq; weight and d_s hold what is lifted by the first power, and so do dv's sums
 #pragma unroll
     for (int u = 0; u < N; ++u)
         if ((32 * w < nk) & (32 * u < nq)) {
@@ -220,7 +224,7 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
                 for (int e = 0; e < 4; ++e) d_s[u][4 * x + e] = fmaf(-y[e], weight[u][4 * x + e], d_s[u][4 * x + e]);
             }
             if (lost) hide_rows(d_s[u], u);
-            if (hides) hide_buckets(d_s[u], u);
+            if (lost & hides) hide_buckets(d_s[u], u);
             Cols<T, D> cols;
             cols.read(qt, 32 * u, lane);
             f32x16_a x = d_s[u];
@@ -295,8 +299,8 @@ __global__ __launch_bounds__(64 * N, 2) void attn_short_grad_kernel(AttnArgs a, 
     }
     float dq_by = lift_q.off(a.scale);
     if (redo) {
-        float t[16 * DT], over;
-        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, &over, item, head, rowc, pos0 + rowc, a.delta[(int64_t)head * a.q_rows + qr], bias, h);
+        float t[16 * DT];
+        dq_by_pairs<T, D, DT, BIAS>(kernel_args(), t, false, item, head, rowc, pos0 + rowc, bias, h);
         take<DT>(dq, t);
         dq_by = a.scale;
     }
