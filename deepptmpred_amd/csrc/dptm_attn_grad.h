@@ -8,9 +8,11 @@
 // added through atomics: results do not depend on the order in which workgroups run.  P and dS are rounded to the tensors'
 // type for the products that sum them; everything else stays in 32 bits.
 //
-// Bound by instructions, vector and matrix together (they do not run side by side on this hardware): 48 proteins of up to 1,024
-// residues, 20 heads of 64, with a bias 175 us for dq and 291 for dk, dv and the bias; 32,768 rows in sequences of 4,096 without one
-// 621 TFLOP/s by the five products that count, heads of 128 520.
+// The kernel that owns queries is bound by instructions, vector and matrix together (51 and 29 % of the busy cycles; they do not run side
+// by side on this hardware).  The one that owns keys is not: 33 and 19 %, the rest of its time its two wavefronts a SIMD wait, for the most
+// part for fragments from LDS, of which it reads twice as many to a vector instruction.  48 proteins of up to 1,024 residues, 20 heads of 64,
+// with a bias: 172 us for dq, 286 for dk, dv and the bias.  32,768 rows in sequences of 4,096 without one: 605 TFLOP/s by the five products
+// that count, heads of 128 510.
 #pragma once
 #include "dptm_attn_kernels.h"
 
@@ -25,7 +27,7 @@ __device__ __forceinline__ float lse_log2(float lse) { return lse == kMinusInf ?
 // For float16 alone both are therefore formed larger by a power of two, which is part of the exponent that exp2 takes.
 //   dk, dv and short sequences: 2^13.  What rounding a pair then takes away is 2^-38 at least, and the results' own rounding 2^-25.  A
 // lane -- a key -- that meets a |dS| above 2^14 so lifted goes on with a smaller power of two, and its sums move along: eight three-way
-// maxima a tile (16,001 rows, window of 512, with the bias: 161 -> 172 us).
+// maxima a tile (16,001 rows, window of 512, with the bias: 162 -> 172 us, or 192 from memory).
 //   dq: a lane is a query, and its dout says how large dS is, so that no tile has to be looked at: the power takes the largest |dout| to
 // 2^4.  P of 2^-20 still keeps all bits then; rows whose sums come out infinite (|dP - delta| of thousands of times |dout|, values in the
 // hundreds or thousands) are done over pair by pair.
@@ -441,7 +443,7 @@ DPTM_COLD void dkv_by_pairs(const AttnArgs& a, float* dk, float* dv, int items_a
 
 // Heads of 128 of the 16-bit types take two launches, one for dk and one for dv (8 products then, the scores a third time):
 // together their operands and sums leave room for one wavefront a SIMD, and the two launches took 2,392 us where the one took
-// 3,018 (32,768 rows in sequences of 2,048, 20 heads).
+// 3,018 (32,768 rows in sequences of 2,048, 20 heads); the two take 2,160 now.
 //
 // Tiles of 64 rows with heads of 64: the 32 that one barrier's second half works on are a loop of its own and columns are read
 // when they are needed, which keeps the sums of the bias gradient (SUMS) out of scratch: 48 proteins 291 us; unrolled with early

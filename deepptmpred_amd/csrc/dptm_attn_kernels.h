@@ -6,9 +6,10 @@
 // One pass over the keys with a running maximum m and sum l per query, in units of log2 and in 32 bits.  The weights are
 // rounded to the tensors' type for the second product (fp32: not at all), l sums them unrounded.
 //
-// What bounds them.  Long sequences in 16 bits: the vector unit, which works on a tile's softmax for half as long again as its
-// matrix instructions take at heads of 64 (32,768 rows, 20 heads, bf16: 620 TFLOP/s in sequences of 1,024, 708 of 4,096; heads
-// of 128 704 and 812; a large plain product reaches 1,228).  Few queries over long keys: memory (64 new tokens over caches of up to
+// What bounds them.  Long sequences in 16 bits: vector and matrix instructions, which do not overlap here, and at heads of 128 the LDS
+// reads between them.  Heads of 64 with a bias: the vector unit works on a tile's softmax for twice as long as its matrix instructions take
+// (46 and 23 % of the busy cycles); heads of 128: 33 and 41 %, a quarter is waiting.  32,768 rows, 20 heads, bf16: 550 TFLOP/s in
+// sequences of 1,024, 710 of 4,096; heads of 128 700 and 810; a large plain product reaches 1,228.  Few queries over long keys: memory (64 new tokens over caches of up to
 // 4,099 keys, 8 key heads of 128: 839 MB in 164 us, 5.1 TB/s; a large copy reaches 5.05).  One short protein: the way of a tile
 // from memory through two products and a join in LDS (482 rows, 20 heads: 12.8 us for 5 MB).
 #pragma once

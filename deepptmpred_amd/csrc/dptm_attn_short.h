@@ -12,7 +12,7 @@
 // Backward pass of 1,000 windows, 8 heads, with a bias, this kernel against those two, in us: 51 rows, bf16 heads of 64 144 : 280,
 // of 32 75 : 154, f16 heads of 16 61 : 137, fp32 heads of 64 323 : 695; 33 rows, fp32 heads of 32 149 : 251; 21 rows, bf16 heads of 64
 // 51 : 161, fp32 heads of 16 47 : 120; one window 25 : 27.  Of 2,048 windows of 51 rows with 4 fp32 heads of 16 the bytes take
-// 29 us, the matrix instructions 65 (products that end in the head's 16 columns fill half of each), the kernel 122: the rest is a
+// 29 us, the matrix instructions 65 (products that end in the head's 16 columns fill half of each), the kernel 125: the rest is a
 // workgroup's way from memory through five barriers back.  Heads of 128 would leave one wavefront a SIMD, and heads that
 // share keys would need a sum over workgroups: both take the two kernels.
 #pragma once

@@ -7,7 +7,7 @@
 // half, so both kinds of pairs are its own, the loads are 16 bytes wide, and the sum over the head is at most three
 // exchanges.  A thread keeps the angles and gains of its elements in registers over the heads of a row that it takes.
 // All arithmetic is fp32; results are rounded once to the tensors' type.  65,539 rows of 40 heads of 64, bf16: forward 125 us for
-// 671 MB (5.4 TB/s), backward 219 + 6 us for 1,007 MB (4.5 TB/s; a large copy reaches 5.05); 482 rows 4.3 us, the launch.
+// 671 MB (5.4 TB/s), backward 228 + 5 us for 1,007 MB (4.4 TB/s; a large copy reaches 5.05); 482 rows 4.4 us, the launch.
 #include "dptm_layers.h"
 
 namespace dptm {
