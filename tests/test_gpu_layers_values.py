@@ -137,7 +137,9 @@ def test_lse_of_rows_whose_scores_are_nan(dtype, lens, k_lens, heads, kv_heads):
 FAR_GRADIENTS = [([2048], [2048], 64, False, 1.0, 1.0, 1e-3), ([2048], [2048], 128, False, 1.0, 1.0, 1e-4), ([1500], [1500], 32, True, 1.0, 1.0, 1e-4),
                  ([64], [20000], 64, False, 1.0, 1.0, 100.0), ([51] * 8, [51] * 8, 32, False, 1.0, 1.0, 1e-5),
                  ([51] * 8, [51] * 8, 64, False, 0.01, 100.0, 3000.0), ([700], [700], 64, False, 0.01, 100.0, 10000.0),
-                 ([300], [300], 64, False, 2.0, 3000.0, 0.01), ([300], [300], 64, True, 2.0, 3000.0, 0.01)]
+                 ([300], [300], 64, False, 2.0, 3000.0, 0.01), ([300], [300], 64, True, 2.0, 3000.0, 0.01),
+                 ([300], [300], 64, False, 2.0, 1.0, 30.0), ([300], [300], 16, False, 2.0, 1.0, 30.0), ([300, 90], [200, 90], 128, False, 2.0, 1.0, 30.0),
+                 ([64, 40], [64, 30], 32, False, 2.0, 1.0, 30.0)]
 
 
 def rounding_of_pairs(q, k, v, dout, out, lens, k_lens, positions, table, buckets):
